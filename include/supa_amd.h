@@ -800,6 +800,128 @@ int supa_amd_fused_sgd(int32_t ntensors, void* const* params, void* const* grads
                        const float* lr_ptr, double dampening, int nesterov, int maximize, int is_first_step,
                        const float* grad_scale, const float* found_inf, void* stream);
 
+/* ------------------------------- gated residual with the norms around it
+ * Of each row of `width` elements (x the output of a block, residual the
+ * stream it is added to):
+ *   u = N_post(x)                    (post_norm NONE: x)
+ *   h = residual_scale residual + gate u      (no gate: + u)
+ *   y = N(h)                         (norm NONE: no y)
+ * with N of kind RMS, v / sqrt(mean(v^2) + eps) weight, or LAYER,
+ * (v - mean(v)) / sqrt(var(v) + eps) weight + bias (var over width).  y is the
+ * norm of h before h is rounded to its type.  Everything is computed in
+ * float32.  No reference counterpart: a program of the reference writes it as
+ * var_mean, rsqrt, mul and add. */
+#define SUPA_AMD_NORM_NONE 0
+#define SUPA_AMD_NORM_RMS 1
+#define SUPA_AMD_NORM_LAYER 2
+#define SUPA_AMD_RESIDUAL_NORM_MAX_WIDTH 16384
+
+typedef struct supa_amd_residual_norm_desc {
+  int64_t rows;              /* fewer than 2^31 */
+  int64_t width;             /* 1 .. SUPA_AMD_RESIDUAL_NORM_MAX_WIDTH */
+  int64_t x_stride;          /* elements from one row of x to the next; elements of a row are contiguous */
+  int64_t residual_stride;   /* the same of residual */
+  int64_t gate_period;       /* consecutive rows that share a row of the gate (a divisor of rows); unused without a gate */
+  int32_t dtype;             /* of x and y: f32, bf16 or f16 */
+  int32_t residual_dtype;    /* of residual and h: dtype or f32 */
+  int32_t param_dtype;       /* of gate, weights and biases: dtype or f32 */
+  int32_t post_norm, norm;   /* SUPA_AMD_NORM_* */
+  int32_t reserved;
+  double residual_scale, eps;
+  const void* x;
+  const void* residual;
+  const void* gate;          /* contiguous [rows / gate_period, width], or NULL */
+  const void* post_weight;   /* [width], or NULL for ones */
+  const void* post_bias;     /* LAYER only: [width], or NULL for zeros */
+  const void* weight;
+  const void* bias;
+} supa_amd_residual_norm_desc;
+
+/* h ([rows, width] of residual_dtype) and y ([rows, width] of dtype; NULL
+ * exactly when norm is NONE), both contiguous.  stats, when given, receives
+ * four floats a row for the backward: the post norm's mean and reciprocal
+ * deviation, then the norm's (0 for a mean or a norm that is not there). */
+int supa_amd_residual_norm_forward(const supa_amd_residual_norm_desc* d, void* h, void* y, float* stats, void* stream);
+
+/* The gradients from grad_h ([rows, width] of residual_dtype, or NULL for
+ * zeros) and grad_y ([rows, width] of dtype, or NULL), contiguous, and the
+ * forward's stats.  Every output may be NULL.  grad_x is of dtype,
+ * grad_residual of residual_dtype, both contiguous; grad_gate, grad_post_weight,
+ * grad_post_bias, grad_weight and grad_bias of param_dtype in their
+ * parameter's shape, summed in float32 in an order that only the sizes fix.
+ * h, when given, is the forward's h and takes the place of x and residual
+ * (which are then not read): for a call without post norm and gate.  x is read
+ * for those two, residual only when there is a norm. */
+int64_t supa_amd_residual_norm_backward_workspace_bytes(const supa_amd_residual_norm_desc* d);
+int supa_amd_residual_norm_backward(const supa_amd_residual_norm_desc* d, const void* h, const void* grad_h,
+                                    const void* grad_y, const float* stats, void* grad_x, void* grad_residual,
+                                    void* grad_gate, void* grad_post_weight, void* grad_post_bias, void* grad_weight,
+                                    void* grad_bias, void* workspace, int64_t ws_bytes, void* stream);
+
+/* --------------------------------------------------------- rotary positions
+ * The pairs of the first `rotary` elements of every head of q and k turned by
+ * the angle position * frequency, and multiplied by `scale`:
+ *   (a, b) -> scale (a cos - b sin, b cos + a sin)
+ * INTERLEAVED pairs neighbours (2i, 2i + 1); HALF pairs (i, i + rotary / 2).  The
+ * elements past `rotary` are copied.  `inverse` turns by the negative angles
+ * (with the same scale: the gradient of the forward call).  Angles are formed
+ * in 64 bits, their sine and cosine and the rotation in float32.  q and k are
+ * [batch, seq, heads, dim] with element strides for the first three dims
+ * and contiguous dim; an output may be its own input (the elements past `rotary`
+ * are then left alone), but must not overlap it otherwise.  No reference
+ * counterpart. */
+#define SUPA_AMD_ROTARY_HALF 0
+#define SUPA_AMD_ROTARY_INTERLEAVED 1
+
+typedef struct supa_amd_rotary_tensor {
+  const void* in;            /* NULL: no such tensor */
+  void* out;
+  int64_t heads;
+  int64_t in_strides[3];     /* batch, seq, heads */
+  int64_t out_strides[3];
+} supa_amd_rotary_tensor;
+
+typedef struct supa_amd_rotary_desc {
+  int64_t batch, seq;
+  int64_t dim, rotary;       /* rotary even, 0 < rotary <= dim */
+  int32_t dtype;             /* of q and k: f32, bf16 or f16 */
+  int32_t layout;            /* SUPA_AMD_ROTARY_* */
+  int32_t inverse;
+  int32_t position_dtype;    /* I64 or I32 */
+  double scale;
+  const double* frequencies; /* [rotary / 2], contiguous */
+  const void* positions;     /* element (b, s) at b position_strides[0] + s position_strides[1]; NULL: offset + s */
+  int64_t position_strides[2];
+  int64_t offset;            /* added to every position */
+  supa_amd_rotary_tensor q, k;
+} supa_amd_rotary_desc;
+
+int supa_amd_rotary(const supa_amd_rotary_desc* d, void* stream);
+
+/* ------------------------------------- global gradient norm and clipping
+ * norm = the ord-norm (1, 2 or inf) of all elements of ntensors device
+ * tensors together (contiguous, numel[i] elements of dtypes[i]: f32, bf16, f16
+ * or f64), summed in float64 in an order that only the sizes fix; then
+ *   tensor *= min(1, max_norm / (norm + 1e-6))
+ * in place, rounded once to the tensor's type.  A factor of 1 writes nothing.
+ * A NaN norm makes every element NaN, an infinite one zero (and the infinite
+ * elements NaN).  norm_out is one element of norm_dtype (f32 or f64).  The
+ * tensors must not overlap.
+ * supa_amd_grad_norm writes the norm alone, supa_amd_grad_scale scales by a
+ * norm that the former left in the same workspace; supa_amd_clip_grad_norm is
+ * the two together.  Replaces the reference's _foreach_norm, stack,
+ * linalg_vector_norm, clamp and _foreach_mul_.Tensor of clip_grad_norm_ (upstream
+ * ForeachReduceOp.cu, ForeachBinaryOpScalarTensor.cu). */
+int64_t supa_amd_grad_norm_workspace_bytes(int32_t ntensors, const int64_t* numel, const int32_t* dtypes);
+int supa_amd_grad_norm(int32_t ntensors, const void* const* tensors, const int64_t* numel, const int32_t* dtypes,
+                       double ord, void* norm_out, int32_t norm_dtype, void* workspace, int64_t ws_bytes,
+                       void* stream);
+int supa_amd_grad_scale(int32_t ntensors, void* const* tensors, const int64_t* numel, const int32_t* dtypes,
+                        double max_norm, const void* workspace, int64_t ws_bytes, void* stream);
+int supa_amd_clip_grad_norm(int32_t ntensors, void* const* tensors, const int64_t* numel, const int32_t* dtypes,
+                            double ord, double max_norm, void* norm_out, int32_t norm_dtype, void* workspace,
+                            int64_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,642 @@
+// Operators of the `supa` namespace: what a transformer does between its
+// matrix products and before its optimizer step.  They have no aten schema;
+// torch.supa.residual_norm, rotary_embedding(_) and clip_grad_norm_ call them
+// (torch_supa/supa/transformer.py).  Arguments are checked here; the device
+// work is the C ABI's, on the tensors' device and its current stream, with
+// workspaces from the caching allocator.
+#include <ATen/MemoryOverlap.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/library.h>
+
+#include <algorithm>
+#include <cmath>
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "common.h"
+
+namespace supa {
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<at::Tensor>;
+
+bool is_float16_or_32(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
+bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+OptTensor maybe(const at::Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
+const void* ptr(const OptTensor& t) { return given(t) ? t->data_ptr() : nullptr; }
+
+void check_on(const char* op, const char* name, const at::Tensor& t, const at::Tensor& like) {
+  TORCH_CHECK(t.device() == like.device(), op, ": ", name, " is on ", t.device(), ", expected ", like.device());
+}
+
+// ------------------------------------------------------------ residual_norm
+// x or residual as rows at one distance, elements contiguous; a copy where a
+// view has no such form.
+struct Rows {
+  at::Tensor t;
+  int64_t stride;
+};
+Rows rows_of(const at::Tensor& t) {
+  const int64_t nd = t.dim(), width = t.size(-1);
+  bool ok = width == 1 || t.stride(-1) == 1;
+  int64_t stride = width, next = -1;  // next: the distance of a step in the dim before
+  for (int64_t i = nd - 2; i >= 0 && ok; --i) {
+    if (t.size(i) == 1) continue;
+    if (next < 0) stride = t.stride(i);
+    else ok = t.stride(i) == next;
+    next = t.stride(i) * t.size(i);
+  }
+  if (!ok) return {t.contiguous(), width};
+  return {t, stride};
+}
+
+struct NormArgs {
+  double scale, eps;
+  int64_t post, norm, period;
+};
+
+// The consecutive rows that share a row of the gate: the gate's leading dims are
+// x's first ones, and 1 (or nothing) from there on.
+int64_t gate_period(const at::Tensor& gate, const at::Tensor& x) {
+  const int64_t nd = x.dim(), shift = nd - gate.dim();
+  bool ok = gate.dim() >= 1 && shift >= 0 && gate.size(-1) == x.size(-1);
+  int64_t period = 1;
+  bool shared = false;  // walking back from the last leading dim: no longer shared
+  for (int64_t i = nd - 2; i >= 0 && ok; --i) {
+    const int64_t g = i >= shift ? gate.size(i - shift) : 1;
+    if (x.size(i) == 1 && g == 1) continue;
+    if (g == 1 && !shared) period *= x.size(i);
+    else if (g == x.size(i)) shared = true;
+    else ok = false;
+  }
+  TORCH_CHECK(ok, "residual_norm: a gate of shape ", gate.sizes(), " does not fit x of shape ", x.sizes(),
+              ": its last dim is x's, its leading dims are x's first ones and then 1");
+  return period;
+}
+
+void check_residual_norm(const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate, NormArgs& a,
+                         const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& weight,
+                         const OptTensor& bias) {
+  constexpr const char* op = "residual_norm";
+  TORCH_CHECK(x.device().type() == kSupa, op, ": expected supa tensors, got x on ", x.device());
+  check_on(op, "residual", residual, x);
+  TORCH_CHECK(is_float16_or_32(x.scalar_type()), op, ": expected float32, bfloat16 or float16, got x of ",
+              x.scalar_type());
+  TORCH_CHECK(x.dim() >= 1, op, ": expected x with a last dim to normalise, got a scalar");
+  TORCH_CHECK(x.sizes() == residual.sizes(), op, ": x is of shape ", x.sizes(), ", residual of ", residual.sizes());
+  TORCH_CHECK(residual.scalar_type() == x.scalar_type() || residual.scalar_type() == at::kFloat, op,
+              ": expected residual of x's dtype (", x.scalar_type(), ") or float32, got ", residual.scalar_type());
+  const int64_t width = x.size(-1);
+  TORCH_CHECK(width >= 1 && width <= SUPA_AMD_RESIDUAL_NORM_MAX_WIDTH, op, ": the last dim holds ", width,
+              " elements, expected 1 to ", SUPA_AMD_RESIDUAL_NORM_MAX_WIDTH);
+  TORCH_CHECK(x.numel() / width < (int64_t(1) << 31), op, ": expected fewer than 2^31 rows");
+  TORCH_CHECK(std::isfinite(a.eps) && a.eps >= 0, op, ": expected eps >= 0, got ", a.eps);
+  std::optional<at::ScalarType> param;
+  const auto check_param = [&](const char* name, const OptTensor& t) {
+    if (!given(t)) return;
+    check_on(op, name, *t, x);
+    const at::ScalarType p = t->scalar_type();
+    TORCH_CHECK(p == x.scalar_type() || p == at::kFloat, op, ": expected ", name, " of x's dtype (", x.scalar_type(),
+                ") or float32, got ", p);
+    TORCH_CHECK(!param || *param == p, op, ": gate, weights and biases are of one dtype, got ", *param, " and ", p);
+    param = p;
+  };
+  const auto check_vector = [&](const char* name, const OptTensor& t, bool allowed, const char* when) {
+    if (!given(t)) return;
+    TORCH_CHECK(allowed, op, ": ", name, " is given ", when);
+    TORCH_CHECK(t->dim() == 1 && t->size(0) == width, op, ": expected ", name, " of shape [", width, "], got ",
+                t->sizes());
+    check_param(name, t);
+  };
+  check_vector("post_weight", post_weight, a.post != SUPA_AMD_NORM_NONE, "without a post norm");
+  check_vector("post_bias", post_bias, a.post == SUPA_AMD_NORM_LAYER, "with a post norm that is not a layer norm");
+  check_vector("weight", weight, a.norm != SUPA_AMD_NORM_NONE, "without a norm");
+  check_vector("bias", bias, a.norm == SUPA_AMD_NORM_LAYER, "with a norm that is not a layer norm");
+  check_param("gate", gate);
+  a.period = given(gate) ? gate_period(*gate, x) : 1;
+}
+
+OptTensor contiguous(const OptTensor& t) { return given(t) ? OptTensor(t->contiguous()) : std::nullopt; }
+
+supa_amd_residual_norm_desc norm_desc(const Rows& x, const Rows& residual, const OptTensor& gate, const NormArgs& a,
+                                      const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& weight,
+                                      const OptTensor& bias) {
+  supa_amd_residual_norm_desc d{};
+  d.width = x.t.size(-1);
+  d.rows = x.t.numel() / d.width;
+  d.x_stride = x.stride;
+  d.residual_stride = residual.stride;
+  d.gate_period = a.period;
+  d.dtype = dtype_code(x.t.scalar_type());
+  d.residual_dtype = dtype_code(residual.t.scalar_type());
+  d.param_dtype = d.dtype;
+  for (const OptTensor* t : {&gate, &post_weight, &post_bias, &weight, &bias})
+    if (given(*t)) d.param_dtype = dtype_code((*t)->scalar_type());
+  d.post_norm = (int32_t)a.post;
+  d.norm = (int32_t)a.norm;
+  d.residual_scale = a.scale;
+  d.eps = a.eps;
+  d.x = x.t.data_ptr();
+  d.residual = residual.t.data_ptr();
+  d.gate = ptr(gate);
+  d.post_weight = ptr(post_weight);
+  d.post_bias = ptr(post_bias);
+  d.weight = ptr(weight);
+  d.bias = ptr(bias);
+  return d;
+}
+
+struct NormResult {
+  at::Tensor h, y, stats;
+};
+NormResult residual_norm_forward(const Rows& x, const Rows& residual, const OptTensor& gate, const NormArgs& a,
+                                 const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& weight,
+                                 const OptTensor& bias, bool want_stats) {
+  const auto dev = x.t.device().index();
+  NormResult r;
+  r.h = empty_supa(x.t.sizes(), residual.t.scalar_type(), dev);
+  if (a.norm != SUPA_AMD_NORM_NONE) r.y = empty_supa(x.t.sizes(), x.t.scalar_type(), dev);
+  if (x.t.numel() == 0) return r;
+  const supa_amd_residual_norm_desc d = norm_desc(x, residual, gate, a, post_weight, post_bias, weight, bias);
+  if (want_stats && (a.post != SUPA_AMD_NORM_NONE || a.norm != SUPA_AMD_NORM_NONE))
+    r.stats = empty_supa({d.rows, 4}, at::kFloat, dev);
+  check_status(supa_amd_residual_norm_forward(&d, r.h.data_ptr(), r.y.defined() ? r.y.data_ptr() : nullptr,
+                                              r.stats.defined() ? r.stats.data_ptr<float>() : nullptr,
+                                              current_stream(dev)),
+               "residual_norm");
+  return r;
+}
+
+std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate,
+                                                 double residual_scale, int64_t post_norm, const OptTensor& post_weight,
+                                                 const OptTensor& post_bias, int64_t norm, const OptTensor& weight,
+                                                 const OptTensor& bias, double eps) {
+  NormArgs a{residual_scale, eps, post_norm, norm, 1};
+  check_residual_norm(x, residual, gate, a, post_weight, post_bias, weight, bias);
+  const c10::DeviceGuard guard(x.device());
+  NormResult r = residual_norm_forward(rows_of(x), rows_of(residual), contiguous(gate), a, contiguous(post_weight),
+                                       contiguous(post_bias), contiguous(weight), contiguous(bias), false);
+  return {r.h, r.y};
+}
+
+// x and residual are saved for the backward, which forms h from them again;
+// without post norm and gate h alone is enough, as long as it is not rounded
+// more coarsely than the weight's gradient it enters.
+class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual,
+                               const OptTensor& gate, double scale, int64_t post, const OptTensor& post_weight,
+                               const OptTensor& post_bias, int64_t norm, const OptTensor& weight, const OptTensor& bias,
+                               double eps) {
+    NormArgs a{scale, eps, post, norm, 1};
+    check_residual_norm(x, residual, gate, a, post_weight, post_bias, weight, bias);
+    const c10::DeviceGuard guard(x.device());
+    ctx->set_materialize_grads(false);
+    const Rows xr = rows_of(x), rr = rows_of(residual);
+    const OptTensor g = contiguous(gate), pw = contiguous(post_weight), pb = contiguous(post_bias),
+                    w = contiguous(weight), b = contiguous(bias);
+    NormResult r = residual_norm_forward(xr, rr, g, a, pw, pb, w, b, true);
+    const bool wide = given(weight) && weight->scalar_type() == at::kFloat;
+    const bool from_h = !given(gate) && post == SUPA_AMD_NORM_NONE &&
+                        (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat || !wide);
+    const bool needs_h = norm != SUPA_AMD_NORM_NONE;
+    ctx->save_for_backward({from_h ? at::Tensor() : xr.t, from_h || !needs_h ? at::Tensor() : rr.t,
+                            from_h && needs_h ? r.h : at::Tensor(), r.stats, g.value_or(at::Tensor()),
+                            pw.value_or(at::Tensor()), pb.value_or(at::Tensor()), w.value_or(at::Tensor()),
+                            b.value_or(at::Tensor())});
+    ctx->saved_data["scalars"] = std::vector<double>{scale, eps};
+    ctx->saved_data["ints"] = std::vector<int64_t>{post, norm, a.period, xr.stride, rr.stride, from_h,
+                                                   (int64_t)residual.scalar_type(), (int64_t)x.scalar_type()};
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["gate_shape"] = given(gate) ? gate->sizes().vec() : std::vector<int64_t>{};
+    return r.y.defined() ? variable_list{r.h, r.y} : variable_list{r.h};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(),
+                "residual_norm: the gradient has no gradient of its own (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &x = saved[0], &residual = saved[1], &h = saved[2], &stats = saved[3];
+    const OptTensor gate = maybe(saved[4]), pw = maybe(saved[5]), pb = maybe(saved[6]), w = maybe(saved[7]),
+                    b = maybe(saved[8]);
+    const auto scalars = ctx->saved_data["scalars"].toDoubleVector();
+    const auto ints = ctx->saved_data["ints"].toIntVector();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    const at::Tensor gh = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
+    const at::Tensor gy = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
+    variable_list out(11);
+    if (!gh.defined() && !gy.defined()) return out;
+    const auto xt = (at::ScalarType)ints[7], rt = (at::ScalarType)ints[6];
+    const c10::Device device = gh.defined() ? gh.device() : gy.device();
+    const c10::DeviceGuard guard(device);
+    const auto dev = device.index();
+
+    supa_amd_residual_norm_desc d{};
+    d.width = shape.back();
+    d.rows = 1;
+    for (size_t i = 0; i + 1 < shape.size(); ++i) d.rows *= shape[i];
+    d.x_stride = ints[3];
+    d.residual_stride = ints[4];
+    d.gate_period = ints[2];
+    d.dtype = dtype_code(xt);
+    d.residual_dtype = dtype_code(rt);
+    d.param_dtype = d.dtype;
+    for (const OptTensor* t : {&gate, &pw, &pb, &w, &b})
+      if (given(*t)) d.param_dtype = dtype_code((*t)->scalar_type());
+    d.post_norm = (int32_t)ints[0];
+    d.norm = (int32_t)ints[1];
+    d.residual_scale = scalars[0];
+    d.eps = scalars[1];
+    d.x = x.defined() ? x.data_ptr() : nullptr;
+    d.residual = residual.defined() ? residual.data_ptr() : nullptr;
+    d.gate = ptr(gate);
+    d.post_weight = ptr(pw);
+    d.post_bias = ptr(pb);
+    d.weight = ptr(w);
+    d.bias = ptr(b);
+
+    // the edges are the tensors that the forward was given, in its order
+    size_t edge = 0;
+    const auto wanted = [&](bool present) { return present && ctx->needs_input_grad(edge++); };
+    if (wanted(true)) out[0] = empty_supa(shape, xt, dev);
+    if (wanted(true)) out[1] = empty_supa(shape, rt, dev);
+    if (wanted(given(gate))) out[2] = empty_supa(ctx->saved_data["gate_shape"].toIntVector(), gate->scalar_type(), dev);
+    const std::pair<int, const OptTensor*> vectors[] = {{5, &pw}, {6, &pb}, {8, &w}, {9, &b}};
+    for (const auto& [at, t] : vectors)
+      if (wanted(given(*t))) out[at] = empty_supa({d.width}, (*t)->scalar_type(), dev);
+    if (d.rows == 0) {
+      for (auto& t : out)
+        if (t.defined()) t.zero_();
+      return out;
+    }
+    const auto data = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
+    const int64_t ws_bytes = supa_amd_residual_norm_backward_workspace_bytes(&d);
+    TORCH_CHECK(ws_bytes >= 0, "residual_norm: ", supa_amd_status_string((int)ws_bytes));
+    const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
+    check_status(supa_amd_residual_norm_backward(&d, data(h), data(gh), data(gy),
+                                                 stats.defined() ? stats.data_ptr<float>() : nullptr, data(out[0]),
+                                                 data(out[1]), data(out[2]), data(out[5]), data(out[6]), data(out[8]),
+                                                 data(out[9]), ws.data_ptr(), ws_bytes, current_stream(dev)),
+                 "residual_norm (backward)");
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(const at::Tensor& x, const at::Tensor& residual,
+                                                          const OptTensor& gate, double scale, int64_t post,
+                                                          const OptTensor& post_weight, const OptTensor& post_bias,
+                                                          int64_t norm, const OptTensor& weight, const OptTensor& bias,
+                                                          double eps) {
+  bool needs = x.requires_grad() || residual.requires_grad();
+  for (const OptTensor* t : {&gate, &post_weight, &post_bias, &weight, &bias})
+    needs = needs || (given(*t) && (*t)->requires_grad());
+  if (!needs || !at::GradMode::is_enabled()) {
+    const at::AutoDispatchBelowAutograd below;
+    return residual_norm(x, residual, gate, scale, post, post_weight, post_bias, norm, weight, bias, eps);
+  }
+  const variable_list r =
+      ResidualNorm::apply(x, residual, gate, scale, post, post_weight, post_bias, norm, weight, bias, eps);
+  return {r[0], r.size() > 1 ? r[1] : at::Tensor()};
+}
+
+// --------------------------------------------------------- rotary_embedding
+struct RotaryArgs {
+  at::Tensor frequencies;  // contiguous float64
+  OptTensor positions;
+  int64_t offset;
+  bool interleaved;
+  double scale;
+  bool inverse;
+};
+
+// [seq, heads, dim] or [batch, seq, heads, dim].
+struct RotaryShape {
+  int64_t batch, seq, heads, dim;
+};
+RotaryShape rotary_shape(const char* op, const char* name, const at::Tensor& t) {
+  TORCH_CHECK(t.dim() == 3 || t.dim() == 4, op, ": expected ", name,
+              " of shape [seq, heads, dim] or [batch, seq, heads, dim], got ", t.sizes());
+  return {t.dim() == 4 ? t.size(0) : 1, t.size(-3), t.size(-2), t.size(-1)};
+}
+
+RotaryArgs check_rotary(const char* op, const at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies,
+                        const OptTensor& positions, int64_t offset, bool interleaved, double scale, bool inverse) {
+  TORCH_CHECK(q.device().type() == kSupa, op, ": expected supa tensors, got q on ", q.device());
+  TORCH_CHECK(is_float16_or_32(q.scalar_type()), op, ": expected float32, bfloat16 or float16, got q of ",
+              q.scalar_type());
+  const RotaryShape s = rotary_shape(op, "q", q);
+  if (given(k)) {
+    check_on(op, "k", *k, q);
+    TORCH_CHECK(k->scalar_type() == q.scalar_type(), op, ": q is of ", q.scalar_type(), ", k of ", k->scalar_type());
+    const RotaryShape r = rotary_shape(op, "k", *k);
+    TORCH_CHECK(k->dim() == q.dim() && r.batch == s.batch && r.seq == s.seq && r.dim == s.dim, op,
+                ": q and k differ in more than their heads: ", q.sizes(), " and ", k->sizes());
+  }
+  check_on(op, "frequencies", frequencies, q);
+  TORCH_CHECK(frequencies.dim() == 1 && at::isFloatingType(frequencies.scalar_type()), op,
+              ": expected frequencies as a vector of floats, got ", frequencies.scalar_type(), " of shape ",
+              frequencies.sizes());
+  const int64_t rotary = 2 * frequencies.size(0);
+  TORCH_CHECK(rotary >= 2 && rotary <= s.dim && rotary <= 1024, op, ": ", frequencies.size(0),
+              " frequencies rotate ", rotary, " elements of a head; expected 2 to ", std::min<int64_t>(s.dim, 1024));
+  TORCH_CHECK(!frequencies.requires_grad(), op, ": frequencies have no gradient");
+  TORCH_CHECK(std::isfinite(scale), op, ": expected a finite scale, got ", scale);
+  if (given(positions)) {
+    check_on(op, "positions", *positions, q);
+    TORCH_CHECK(positions->scalar_type() == at::kLong || positions->scalar_type() == at::kInt, op,
+                ": expected int64 or int32 positions, got ", positions->scalar_type());
+    const bool ok = (positions->dim() == 1 && positions->size(0) == s.seq) ||
+                    (positions->dim() == 2 && q.dim() == 4 && positions->size(1) == s.seq &&
+                     (positions->size(0) == s.batch || positions->size(0) == 1));
+    TORCH_CHECK(ok, op, ": expected positions of shape [", s.seq, "]", q.dim() == 4 ? " or [batch, seq]" : "",
+                ", got ", positions->sizes());
+  }
+  TORCH_CHECK(s.batch * s.seq < (int64_t(1) << 31), op, ": expected fewer than 2^31 tokens");
+  // frequencies of another type are widened, not formed anew
+  return {frequencies.to(at::kDouble).contiguous(), positions, offset, interleaved, scale, inverse};
+}
+
+supa_amd_rotary_tensor rotary_tensor(const at::Tensor& in, const at::Tensor& out) {
+  supa_amd_rotary_tensor t{};
+  t.in = in.data_ptr();
+  t.out = out.data_ptr();
+  t.heads = in.size(-2);
+  for (int i = 0; i < 3; ++i) {
+    const int64_t dim = in.dim() - 4 + i;
+    t.in_strides[i] = dim < 0 ? 0 : in.stride(dim);
+    t.out_strides[i] = dim < 0 ? 0 : out.stride(dim);
+  }
+  return t;
+}
+
+void launch_rotary(const char* op, const at::Tensor& q, const at::Tensor& q_out, const at::Tensor& k,
+                   const at::Tensor& k_out, const RotaryArgs& a) {
+  const RotaryShape s = rotary_shape(op, "q", q);
+  supa_amd_rotary_desc d{};
+  d.batch = s.batch;
+  d.seq = s.seq;
+  d.dim = s.dim;
+  d.rotary = 2 * a.frequencies.size(0);
+  d.dtype = dtype_code(q.scalar_type());
+  d.layout = a.interleaved ? SUPA_AMD_ROTARY_INTERLEAVED : SUPA_AMD_ROTARY_HALF;
+  d.inverse = a.inverse;
+  d.position_dtype = SUPA_AMD_I64;
+  d.scale = a.scale;
+  d.frequencies = a.frequencies.data_ptr<double>();
+  d.offset = a.offset;
+  if (given(a.positions)) {
+    const at::Tensor& p = *a.positions;
+    d.positions = p.data_ptr();
+    d.position_dtype = dtype_code(p.scalar_type());
+    d.position_strides[0] = p.dim() == 2 && p.size(0) > 1 ? p.stride(0) : 0;
+    d.position_strides[1] = p.stride(-1);
+  }
+  if (q.numel() > 0) d.q = rotary_tensor(q, q_out);
+  if (k.defined() && k.numel() > 0) d.k = rotary_tensor(k, k_out);
+  if (!d.q.in && !d.k.in) return;
+  check_status(supa_amd_rotary(&d, current_stream(q.device().index())), op);
+}
+
+at::Tensor heads_contiguous(const at::Tensor& t) {
+  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const OptTensor& k,
+                                                    const at::Tensor& frequencies, const OptTensor& positions,
+                                                    int64_t offset, bool interleaved, double scale, bool inverse) {
+  constexpr const char* op = "rotary_embedding";
+  const c10::OptionalDeviceGuard guard(q.device());
+  const RotaryArgs a = check_rotary(op, q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  // the outputs keep their inputs' order of dims where these are dense
+  const at::Tensor qi = heads_contiguous(q), ki = given(k) ? heads_contiguous(*k) : at::Tensor();
+  const at::Tensor qo = at::empty_like(qi), ko = ki.defined() ? at::empty_like(ki) : at::Tensor();
+  launch_rotary(op, qi, qo, ki, ko, a);
+  return {qo, ko};
+}
+
+// Whether q and k, which interleave in memory, share no element: k's part of
+// every token (or of every sample) lies beside q's.
+bool beside(const at::Tensor& q, const at::Tensor& k) {
+  const int64_t nd = q.dim();
+  // elements from the first to behind the last, over the dims from `from` on
+  const auto extent = [&](const at::Tensor& t, int64_t from) {
+    int64_t e = 1;
+    for (int64_t i = from; i < nd; ++i) e += (t.size(i) - 1) * t.stride(i);
+    return e;
+  };
+  const int64_t apart = (static_cast<const char*>(k.data_ptr()) - static_cast<const char*>(q.data_ptr())) /
+                        (int64_t)q.element_size();
+  for (int64_t from = 0; from <= nd - 2; ++from) {  // the dims before `from` step alike
+    bool alike = true;
+    int64_t step = INT64_MAX;
+    for (int64_t i = 0; i < from; ++i) {
+      if (q.size(i) == 1) continue;
+      alike = alike && q.stride(i) == k.stride(i);
+      step = std::min(step, q.stride(i));
+    }
+    const int64_t first = apart >= 0 ? extent(q, from) : extent(k, from);
+    const int64_t second = apart >= 0 ? extent(k, from) : extent(q, from);
+    const int64_t gap = std::abs(apart);
+    if (alike && first <= gap && (step == INT64_MAX || gap + second <= step)) return true;
+  }
+  return false;
+}
+
+void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies, const OptTensor& positions,
+                       int64_t offset, bool interleaved, double scale, bool inverse) {
+  constexpr const char* op = "rotary_embedding_";
+  const c10::OptionalDeviceGuard guard(q.device());
+  const RotaryArgs a = check_rotary(op, q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  for (const at::Tensor* t : {(const at::Tensor*)&q, given(k) ? &*k : nullptr}) {
+    if (!t || t->numel() == 0) continue;
+    TORCH_CHECK(t->size(-1) == 1 || t->stride(-1) == 1, op, ": expected heads whose elements are contiguous");
+    at::assert_no_internal_overlap(*t);
+  }
+  if (given(k) && q.numel() > 0 && k->numel() > 0)
+    TORCH_CHECK(beside(q, *k), op, ": q and k overlap in memory");
+  launch_rotary(op, q, q, given(k) ? *k : at::Tensor(), given(k) ? *k : at::Tensor(), a);
+}
+
+class RotaryEmbedding : public torch::autograd::Function<RotaryEmbedding> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k,
+                               const at::Tensor& frequencies, const OptTensor& positions, int64_t offset,
+                               bool interleaved, double scale, bool inverse) {
+    ctx->set_materialize_grads(false);
+    auto [qo, ko] = rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+    ctx->save_for_backward({frequencies, given(positions) ? *positions : at::Tensor()});
+    ctx->saved_data["offset"] = offset;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["inverse"] = inverse;
+    return ko.defined() ? variable_list{qo, ko} : variable_list{qo};
+  }
+
+  // The rotation back, by the same call: it has a gradient of its own.
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool second = grads.size() > 1;
+    const at::Tensor gq = ctx->needs_input_grad(0) ? grads[0] : at::Tensor();
+    const at::Tensor gk = second && ctx->needs_input_grad(1) ? grads[1] : at::Tensor();
+    variable_list out(8);
+    if (!gq.defined() && !gk.defined()) return out;
+    static const auto call =
+        c10::Dispatcher::singleton()
+            .findSchemaOrThrow("supa::rotary_embedding", "")
+            .typed<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const OptTensor&, const at::Tensor&,
+                                                      const OptTensor&, int64_t, bool, double, bool)>();
+    const bool both = gq.defined() && gk.defined();
+    auto [a, b] = call.call(gq.defined() ? gq : gk, both ? OptTensor(gk) : std::nullopt, saved[0], maybe(saved[1]),
+                            ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(),
+                            ctx->saved_data["scale"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    if (gq.defined()) out[0] = a;
+    if (gk.defined()) out[1] = both ? b : a;
+    return out;
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q, const OptTensor& k,
+                                                             const at::Tensor& frequencies, const OptTensor& positions,
+                                                             int64_t offset, bool interleaved, double scale,
+                                                             bool inverse) {
+  const bool needs = q.requires_grad() || (given(k) && k->requires_grad());
+  TORCH_CHECK(!frequencies.requires_grad(), "rotary_embedding: frequencies have no gradient");
+  if (!needs || !at::GradMode::is_enabled()) {
+    const at::AutoDispatchBelowAutograd below;
+    return rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  }
+  const variable_list r =
+      RotaryEmbedding::apply(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  return {r[0], r.size() > 1 ? r[1] : at::Tensor()};
+}
+
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void rotary_embedding_autograd_(at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies,
+                                const OptTensor& positions, int64_t offset, bool interleaved, double scale,
+                                bool inverse) {
+  TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || (given(k) && k->requires_grad())),
+              "rotary_embedding_: the call in place has no gradient; use rotary_embedding");
+  const at::AutoDispatchBelowAutograd below;
+  rotary_embedding_(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  written(q);
+  if (given(k)) written(*k);
+}
+
+// ----------------------------------------------------------- clip_grad_norm_
+at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bool error_if_nonfinite) {
+  constexpr const char* op = "clip_grad_norm_";
+  TORCH_CHECK(!grads.empty(), op, ": expected at least one tensor");
+  TORCH_CHECK(max_norm >= 0, op, ": expected max_norm >= 0, got ", max_norm);
+  TORCH_CHECK(ord == 1.0 || ord == 2.0 || ord == HUGE_VAL, op, ": expected the norm 1, 2 or inf, got ", ord);
+  const c10::Device device = grads[0].device();
+  const size_t n = grads.size();
+  std::vector<at::Tensor> copies;  // of tensors that are not dense, in the list's order
+  std::vector<void*> p(n);
+  std::vector<int64_t> numel(n);
+  std::vector<int32_t> dtypes(n);
+  std::vector<std::pair<const char*, const char*>> spans;
+  spans.reserve(n);
+  at::ScalarType norm_type = at::kFloat;
+  const c10::OptionalDeviceGuard guard(device);
+  for (size_t i = 0; i < n; ++i) {
+    const at::Tensor& g = grads[i];
+    TORCH_CHECK(g.device().type() == kSupa && g.layout() == at::kStrided, op,
+                ": expected dense supa tensors, got one of layout ", g.layout(), " on ", g.device());
+    TORCH_CHECK(g.device() == device, op, ": the tensors are on ", device, " and ", g.device(), ", expected one device");
+    const at::ScalarType t = g.scalar_type();
+    TORCH_CHECK(is_float16_or_32(t) || t == at::kDouble, op, ": expected floating tensors, got one of ", t);
+    if (t == at::kDouble) norm_type = at::kDouble;
+    at::Tensor x = g;
+    if (!g.is_non_overlapping_and_dense()) {
+      at::assert_no_internal_overlap(g);
+      x = g.contiguous();
+      copies.push_back(x);
+    } else if (g.numel() > 0) {
+      const char* at = static_cast<const char*>(g.data_ptr());
+      spans.emplace_back(at, at + g.numel() * (int64_t)g.element_size());
+    }
+    p[i] = x.data_ptr();
+    numel[i] = x.numel();
+    dtypes[i] = dtype_code(t);
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i - 1].second <= spans[i].first, op, ": two of the tensors share memory");
+  const auto dev = device.index();
+  const int64_t ws_bytes = supa_amd_grad_norm_workspace_bytes((int32_t)n, numel.data(), dtypes.data());
+  TORCH_CHECK(ws_bytes >= 0, op, ": ", supa_amd_status_string((int)ws_bytes));
+  const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
+  at::Tensor norm = empty_supa({}, norm_type, dev);
+  const hipStream_t st = current_stream(dev);
+  if (error_if_nonfinite) {  // reads the norm back before anything is scaled
+    check_status(supa_amd_grad_norm((int32_t)n, p.data(), numel.data(), dtypes.data(), ord, norm.data_ptr(),
+                                    dtype_code(norm_type), ws.data_ptr(), ws_bytes, st),
+                 op);
+    const double v = norm.item().toDouble();
+    TORCH_CHECK(std::isfinite(v), "The total norm of order ", ord, " for gradients from `parameters` is non-finite, so "
+                "it cannot be clipped. To disable this error and scale the gradients by the non-finite norm anyway, "
+                "set `error_if_nonfinite=False`");
+    check_status(supa_amd_grad_scale((int32_t)n, p.data(), numel.data(), dtypes.data(), max_norm, ws.data_ptr(),
+                                     ws_bytes, st),
+                 op);
+  } else {
+    check_status(supa_amd_clip_grad_norm((int32_t)n, p.data(), numel.data(), dtypes.data(), ord, max_norm,
+                                         norm.data_ptr(), dtype_code(norm_type), ws.data_ptr(), ws_bytes, st),
+                 op);
+  }
+  size_t c = 0;
+  for (size_t i = 0; i < n && c < copies.size(); ++i) {
+    if (grads[i].is_non_overlapping_and_dense()) continue;
+    grads[i].copy_(copies[c++]);
+  }
+  return norm;
+}
+
+at::Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double ord, bool error_if_nonfinite) {
+  for (const at::Tensor& g : grads)
+    TORCH_CHECK(!(at::GradMode::is_enabled() && g.requires_grad()), "clip_grad_norm_: a tensor of the list needs a "
+                "gradient; the scaling in place has none");
+  const at::AutoDispatchBelowAutograd below;
+  at::Tensor norm = clip_grad_norm_(grads, max_norm, ord, error_if_nonfinite);
+  for (const at::Tensor& g : grads) written(g);
+  return norm;
+}
+
+}  // namespace
+}  // namespace supa
+
+TORCH_LIBRARY(supa, m) {
+  m.def(
+      "residual_norm(Tensor x, Tensor residual, Tensor? gate, float residual_scale, int post_norm, Tensor? post_weight, "
+      "Tensor? post_bias, int norm, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
+  m.def(
+      "rotary_embedding(Tensor q, Tensor? k, Tensor frequencies, Tensor? positions, int offset, bool interleaved, "
+      "float scale, bool inverse) -> (Tensor, Tensor)");
+  m.def(
+      "rotary_embedding_(Tensor(a!) q, Tensor(b!)? k, Tensor frequencies, Tensor? positions, int offset, "
+      "bool interleaved, float scale, bool inverse) -> ()");
+  m.def("clip_grad_norm_(Tensor(a!)[] grads, float max_norm, float ord, bool error_if_nonfinite) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(supa, PrivateUse1, m) {
+  using namespace supa;
+  m.impl("residual_norm", TORCH_FN(residual_norm));
+  m.impl("rotary_embedding", TORCH_FN(rotary_embedding));
+  m.impl("rotary_embedding_", TORCH_FN(rotary_embedding_));
+  m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_));
+}
+
+TORCH_LIBRARY_IMPL(supa, AutogradPrivateUse1, m) {
+  using namespace supa;
+  m.impl("residual_norm", TORCH_FN(residual_norm_autograd));
+  m.impl("rotary_embedding", TORCH_FN(rotary_embedding_autograd));
+  m.impl("rotary_embedding_", TORCH_FN(rotary_embedding_autograd_));
+  m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_autograd_));
+}

@@ -1,0 +1,234 @@
+// The norm of a list of tensors together, and their scaling to a largest norm:
+// what clip_grad_norm_ does to a model's gradients before the optimizer step.
+//
+// HBM-bound: a read of every gradient, then, where the norm exceeds the limit, a
+// read and a write (a factor of 1 ends a workgroup before it reads anything).
+// The tensors travel in the kernel arguments (mta.h); a workgroup reduces one
+// chunk to a partial in float64 -- no square of a float32 overflows or
+// underflows there, and a sum over 10^9 terms keeps its digits -- and one
+// workgroup adds the partials in their order, so the norm does not depend on
+// timing.
+#include "mta.h"
+
+namespace sa {
+
+constexpr int kClipTensors = 128;  // tensors a launch; the table takes 2.9 KiB of kernel arguments
+constexpr int kClipBlock = 256;
+constexpr int kClipVecs = 4;       // 16-byte vectors a thread
+
+struct ClipTable {
+  void* p[kClipTensors];
+  int64_t numel[kClipTensors];
+  uint32_t chunk_start[kClipTensors + 1];
+  int32_t ntensors;
+  uint32_t bucket_shift;
+  MtaBucket bucket[kMtaBuckets];
+};
+
+template <typename T> constexpr int64_t clip_chunk() { return (int64_t)kClipBlock * kClipVecs * (16 / (int64_t)sizeof(T)); }
+
+constexpr int kOrdInf = 0;
+template <int ORD> __device__ __forceinline__ double clip_term(double acc, double x) {
+  if constexpr (ORD == 2) return fma(x, x, acc);
+  else if constexpr (ORD == 1) return acc + fabs(x);
+  else return (acc != acc || acc > fabs(x)) ? acc : fabs(x);  // NaN stays
+}
+template <int ORD> __device__ __forceinline__ double clip_join(double a, double b) {
+  if constexpr (ORD == kOrdInf) return (a != a || a > b) ? a : b;
+  else return a + b;
+}
+// Over the workgroup, in thread 0.
+template <int ORD, int BS> __device__ __forceinline__ double clip_block(double v) {
+  __shared__ double part[BS / 64];
+  for (int off = 32; off > 0; off >>= 1) v = clip_join<ORD>(v, __shfl_xor(v, off, 64));
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < BS / 64; ++w) v = clip_join<ORD>(v, part[w]);
+  }
+  return v;
+}
+
+template <typename T, int ORD>
+__global__ void __launch_bounds__(kClipBlock) k_clip_partial(ClipTable tab, double* __restrict__ part) {
+  constexpr int V = 16 / sizeof(T);
+  const MtaRange r = mta_range<clip_chunk<T>()>(tab);
+  const T* x = static_cast<const T*>(tab.p[r.k]);
+  double acc = 0.0;
+  int64_t start = r.lo;
+  if (aligned(x, 16)) {
+    const int64_t nv = (r.hi - r.lo) / V;
+    for (int64_t v = threadIdx.x; v < nv; v += kClipBlock) {
+      const Vec<T, V> w = ld_stream(reinterpret_cast<const Vec<T, V>*>(x + r.lo + v * V));
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc = clip_term<ORD>(acc, (double)to_arith(w.v[i]));
+    }
+    start = r.lo + nv * V;
+  }
+  for (int64_t e = start + threadIdx.x; e < r.hi; e += kClipBlock) acc = clip_term<ORD>(acc, (double)to_arith(x[e]));
+  acc = clip_block<ORD, kClipBlock>(acc);
+  if (threadIdx.x == 0) part[blockIdx.x] = acc;
+}
+
+// The norm of all partials, to ws[0] and to `out`.
+constexpr int kClipFinal = 1024;
+template <int ORD>
+__global__ void __launch_bounds__(kClipFinal)
+k_clip_norm(double* __restrict__ ws, int64_t parts, void* __restrict__ out, int out_f64) {
+  double acc = fold_strided<8>(
+      0.0, (int64_t)threadIdx.x, kClipFinal, parts, [&](int64_t i) { return ws[1 + i]; },
+      [](double a, double b) { return clip_join<ORD>(a, b); });
+  acc = clip_block<ORD, kClipFinal>(acc);
+  if (threadIdx.x == 0) {
+    const double norm = ORD == 2 ? sqrt(acc) : acc;
+    ws[0] = norm;
+    if (out_f64) *static_cast<double*>(out) = norm;
+    else *static_cast<float*>(out) = (float)norm;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kClipBlock)
+k_clip_scale(ClipTable tab, const double* __restrict__ norm, double max_norm) {
+  using A = opmath_t<T>;
+  constexpr int V = 16 / sizeof(T);
+  const double q = max_norm / (*norm + 1e-6);
+  if (q >= 1.0) return;  // a NaN goes on
+  const A c = (A)q;
+  const MtaRange r = mta_range<clip_chunk<T>()>(tab);
+  T* x = static_cast<T*>(tab.p[r.k]);
+  int64_t start = r.lo;
+  if (aligned(x, 16)) {
+    const int64_t nv = (r.hi - r.lo) / V;
+    for (int64_t v = threadIdx.x; v < nv; v += kClipBlock) {
+      Vec<T, V>* at = reinterpret_cast<Vec<T, V>*>(x + r.lo + v * V);
+      Vec<T, V> w = ld_stream(at);
+#pragma unroll
+      for (int i = 0; i < V; ++i) w.v[i] = from_arith<T>((A)to_arith(w.v[i]) * c);
+      st_stream(at, w);
+    }
+    start = r.lo + nv * V;
+  }
+  for (int64_t e = start + threadIdx.x; e < r.hi; e += kClipBlock) x[e] = from_arith<T>((A)to_arith(x[e]) * c);
+}
+
+// Calls fn(tab, chunks, T*) for tables of at most kClipTensors tensors, those
+// of one dtype together; empty tensors are left out.
+template <typename F>
+int clip_tables(int32_t n, void* const* p, const int64_t* numel, const int32_t* dtypes, F&& fn) {
+  for (const int dtype : {SUPA_AMD_F32, SUPA_AMD_BF16, SUPA_AMD_F16, SUPA_AMD_F64}) {
+    const int rc = with_mta_storage(dtype, [&](auto* tag) -> int {
+      using T = std::remove_pointer_t<decltype(tag)>;
+      int i = 0;
+      while (i < n) {
+        ClipTable tab{};
+        int64_t chunks = 0;
+        int nt = 0;
+        for (; i < n && nt < kClipTensors; ++i) {
+          if (dtypes[i] != dtype || numel[i] == 0) continue;
+          const int64_t c = (numel[i] + clip_chunk<T>() - 1) / clip_chunk<T>();
+          if (c >= (int64_t(1) << 24)) return SUPA_AMD_ELAYOUT;
+          if (chunks + c >= (int64_t(1) << 24)) break;  // HIP: fewer than 2^32 threads a launch
+          tab.p[nt] = p ? p[i] : nullptr;
+          tab.numel[nt] = numel[i];
+          tab.chunk_start[nt++] = (uint32_t)chunks;
+          chunks += c;
+        }
+        if (nt == 0) continue;
+        tab.chunk_start[nt] = (uint32_t)chunks;
+        tab.ntensors = nt;
+        mta_index(tab, (uint32_t)chunks);
+        const int r = fn(tab, (uint32_t)chunks, tag);
+        if (r) return r;
+      }
+      return SUPA_AMD_OK;
+    });
+    if (rc) return rc;
+  }
+  return SUPA_AMD_OK;
+}
+
+int clip_check(int32_t n, const void* const* p, const int64_t* numel, const int32_t* dtypes) {
+  if (n < 0 || (n > 0 && (!p || !numel || !dtypes))) return SUPA_AMD_EINVAL;
+  for (int32_t i = 0; i < n; ++i) {
+    if (numel[i] < 0 || (numel[i] > 0 && !p[i])) return SUPA_AMD_EINVAL;
+    if (!dtype_is_floating(dtypes[i])) return SUPA_AMD_EDTYPE;
+  }
+  return SUPA_AMD_OK;
+}
+
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" {
+
+int64_t supa_amd_grad_norm_workspace_bytes(int32_t n, const int64_t* numel, const int32_t* dtypes) {
+  if (n < 0 || (n > 0 && (!numel || !dtypes))) return SUPA_AMD_EINVAL;
+  for (int32_t i = 0; i < n; ++i) {
+    if (numel[i] < 0) return SUPA_AMD_EINVAL;
+    if (!dtype_is_floating(dtypes[i])) return SUPA_AMD_EDTYPE;
+  }
+  int64_t parts = 0;
+  const int rc = clip_tables(n, nullptr, numel, dtypes, [&](const ClipTable&, uint32_t chunks, auto*) {
+    parts += chunks;
+    return SUPA_AMD_OK;
+  });
+  return rc ? rc : (1 + parts) * 8;
+}
+
+int supa_amd_grad_norm(int32_t n, const void* const* tensors, const int64_t* numel, const int32_t* dtypes, double ord,
+                       void* norm_out, int32_t norm_dtype, void* workspace, int64_t ws_bytes, void* stream) {
+  const int rc = clip_check(n, tensors, numel, dtypes);
+  if (rc) return rc;
+  if (!norm_out || (ord != 1.0 && ord != 2.0 && ord != HUGE_VAL)) return SUPA_AMD_EINVAL;
+  if (norm_dtype != SUPA_AMD_F32 && norm_dtype != SUPA_AMD_F64) return SUPA_AMD_EDTYPE;
+  const int64_t need = supa_amd_grad_norm_workspace_bytes(n, numel, dtypes);
+  if (need < 0) return (int)need;
+  if (!workspace || ws_bytes < need) return SUPA_AMD_EWORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  double* ws = static_cast<double*>(workspace);
+  auto go = [&](auto O) -> int {
+    int64_t parts = 0;
+    const int r = clip_tables(n, const_cast<void* const*>(tensors), numel, dtypes,
+                              [&](const ClipTable& tab, uint32_t chunks, auto* tag) -> int {
+                                using T = std::remove_pointer_t<decltype(tag)>;
+                                k_clip_partial<T, O.value><<<chunks, kClipBlock, 0, st>>>(tab, ws + 1 + parts);
+                                parts += chunks;
+                                return launch_status();
+                              });
+    if (r) return r;
+    k_clip_norm<O.value><<<1, kClipFinal, 0, st>>>(ws, parts, norm_out, norm_dtype == SUPA_AMD_F64);
+    return launch_status();
+  };
+  if (ord == 2.0) return go(std::integral_constant<int, 2>{});
+  if (ord == 1.0) return go(std::integral_constant<int, 1>{});
+  return go(std::integral_constant<int, kOrdInf>{});
+}
+
+int supa_amd_grad_scale(int32_t n, void* const* tensors, const int64_t* numel, const int32_t* dtypes, double max_norm,
+                        const void* workspace, int64_t ws_bytes, void* stream) {
+  const int rc = clip_check(n, tensors, numel, dtypes);
+  if (rc) return rc;
+  if (!(max_norm >= 0.0)) return SUPA_AMD_EINVAL;
+  if (!workspace || ws_bytes < 8) return SUPA_AMD_EWORKSPACE;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return clip_tables(n, tensors, numel, dtypes, [&](const ClipTable& tab, uint32_t chunks, auto* tag) -> int {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    k_clip_scale<T><<<chunks, kClipBlock, 0, st>>>(tab, static_cast<const double*>(workspace), max_norm);
+    return launch_status();
+  });
+}
+
+int supa_amd_clip_grad_norm(int32_t n, void* const* tensors, const int64_t* numel, const int32_t* dtypes, double ord,
+                            double max_norm, void* norm_out, int32_t norm_dtype, void* workspace, int64_t ws_bytes,
+                            void* stream) {
+  if (!(max_norm >= 0.0)) return SUPA_AMD_EINVAL;
+  const int rc = supa_amd_grad_norm(n, const_cast<const void* const*>(tensors), numel, dtypes, ord, norm_out, norm_dtype,
+                                    workspace, ws_bytes, stream);
+  if (rc) return rc;
+  return supa_amd_grad_scale(n, tensors, numel, dtypes, max_norm, workspace, ws_bytes, stream);
+}
+
+}  // extern "C"

@@ -12,6 +12,13 @@ from __future__ import annotations
 import torch
 
 from .. import _C
+from .transformer import (  # noqa: F401
+    clip_grad_norm_,
+    residual_norm,
+    rotary_embedding,
+    rotary_embedding_,
+    rotary_frequencies,
+)
 
 
 def is_available() -> bool:
