@@ -38,56 +38,61 @@ struct RnArgs {
   float scale, eps, inv_width;
 };
 
-// VW elements of a parameter vector; `fill` where there is none.
-template <typename T, int VW>
-__device__ __forceinline__ void rn_param(const void* p, int pf32, int64_t at, int col, int width, float fill,
-                                         float (&f)[VW]) {
+// A vector of a parameter (the row at p + at); `fill` where there is none.
+template <typename T, int G, int NV, int VW>
+__device__ __forceinline__ void rn_param(const RowSlots<G, NV, VW>& c, const void* p, int pf32, int64_t at, int j,
+                                         float fill, float (&f)[VW], bool on = true) {
   if (p == nullptr) {
 #pragma unroll
     for (int k = 0; k < VW; ++k) f[k] = fill;
   } else if (std::is_same<T, float>::value || pf32) {
-    const auto r = row_load<false, VW>(static_cast<const float*>(p) + at, col, width);
+    const auto r = c.template load<false>(static_cast<const float*>(p) + at, j, on);
 #pragma unroll
     for (int k = 0; k < VW; ++k) f[k] = row_elem<float, VW>(r, k);
   } else {
-    const auto r = row_load<false, VW>(static_cast<const T*>(p) + at, col, width);
+    const auto r = c.template load<false>(static_cast<const T*>(p) + at, j, on);
 #pragma unroll
     for (int k = 0; k < VW; ++k) f[k] = row_elem<T, VW>(r, k);
   }
 }
-template <typename T, int VW>
-__device__ __forceinline__ void rn_param_store(void* p, int pf32, int64_t at, int col, int width,
-                                               const float (&f)[VW]) {
-  if (std::is_same<T, float>::value || pf32) row_store<float, VW>(static_cast<float*>(p) + at, col, width, f);
-  else row_store<T, VW>(static_cast<T*>(p) + at, col, width, f);
+template <typename T, int G, int NV, int VW>
+__device__ __forceinline__ void rn_param_store(const RowSlots<G, NV, VW>& c, void* p, int pf32, int64_t at, int j,
+                                               const float (&f)[VW], bool on = true) {
+  if (std::is_same<T, float>::value || pf32) c.store(static_cast<float*>(p) + at, j, f, on);
+  else c.store(static_cast<T*>(p) + at, j, f, on);
 }
 
-// Mean and reciprocal deviation of a row's values (zeros past its end).
+// Mean and reciprocal deviation of a row's values.
 template <int G, int NV, int VW>
-__device__ __forceinline__ float2 rn_stats(const float (&v)[NV][VW], int l, const RnArgs& a, bool layer, float* lds0,
-                                           float* lds1) {
+__device__ __forceinline__ float2 rn_stats(const float (&v)[NV][VW], const RowSlots<G, NV, VW>& c, const RnArgs& a,
+                                           bool layer, float* lds0, float* lds1) {
   float mean = 0.f;
   if (layer) {
     float s[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
-      for (int k = 0; k < VW; ++k) s[0] += v[j][k];
+      for (int k = 0; k < VW; ++k) s[0] += c.mine(j, k) ? v[j][k] : 0.f;
     group_sum<G>(s, lds0);
     mean = s[0] * a.inv_width;
   }
   float q[1] = {0.f};
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int col = (l + j * G) * VW;
 #pragma unroll
     for (int k = 0; k < VW; ++k) {
-      const float d = col + k < a.width ? v[j][k] - mean : 0.f;
+      const float d = c.mine(j, k) ? v[j][k] - mean : 0.f;
       q[0] = fmaf(d, d, q[0]);
     }
   }
   group_sum<G>(q, lds1);
   return make_float2(mean, rsqrtf(fmaf(q[0], a.inv_width, a.eps)));
+}
+
+// The group of a row in the workgroup, as a scalar where a wavefront has one row.
+template <int G> __device__ __forceinline__ int rn_group() {
+  const int g = threadIdx.x / G;
+  return G >= 64 ? __builtin_amdgcn_readfirstlane(g) : g;
 }
 
 template <typename T, typename R, int G, int EPT>
@@ -97,16 +102,17 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
   constexpr int VW = 16 / (int)sizeof(T), NV = EPT / VW;
   __shared__ float lds[4][BS / 64];
   const int l = threadIdx.x & (G - 1);
-  const int64_t row = a.row0 + (int64_t)blockIdx.x * (BS / G) + threadIdx.x / G;
+  const int64_t row = a.row0 + (int64_t)blockIdx.x * (BS / G) + rn_group<G>();
   if (row >= a.rows) return;  // G above 64: a row a workgroup, all of them there
+  const RowSlots<G, NV, VW> c(l, a.width);
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const R* res = static_cast<const R*>(a.res) + row * a.res_stride;
   RowVec<T, VW> xq[NV];
   RowVec<R, VW> rq[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) xq[j] = row_load<true, VW>(x, (l + j * G) * VW, a.width);
+  for (int j = 0; j < NV; ++j) xq[j] = c.template load<true>(x, j);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) rq[j] = row_load<true, VW>(res, (l + j * G) * VW, a.width);
+  for (int j = 0; j < NV; ++j) rq[j] = c.template load<true>(res, j);
   float v[NV][VW];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -114,14 +120,14 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
     for (int k = 0; k < VW; ++k) v[j][k] = row_elem<T, VW>(xq[j], k);
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
   if (a.post != kNone) {
-    const float2 m = rn_stats<G>(v, l, a, a.post == kLayer, lds[0], lds[1]);
+    const float2 m = rn_stats(v, c, a, a.post == kLayer, lds[0], lds[1]);
     st.x = m.x;
     st.y = m.y;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float w[VW], b[VW];
-      rn_param<T, VW>(a.pw, a.pf32, 0, (l + j * G) * VW, a.width, 1.f, w);
-      rn_param<T, VW>(a.pb, a.pf32, 0, (l + j * G) * VW, a.width, 0.f, b);
+      rn_param<T>(c, a.pw, a.pf32, 0, j, 1.f, w);
+      rn_param<T>(c, a.pb, a.pf32, 0, j, 0.f, b);
 #pragma unroll
       for (int k = 0; k < VW; ++k) v[j][k] = fmaf((v[j][k] - m.x) * m.y, w[k], b[k]);
     }
@@ -129,35 +135,28 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
   const int64_t gate_at = a.gate ? (int64_t)((uint32_t)row / a.period) * a.width : 0;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int col = (l + j * G) * VW;
     if (a.gate) {
       float g[VW];
-      rn_param<T, VW>(a.gate, a.pf32, gate_at, col, a.width, 1.f, g);
+      rn_param<T>(c, a.gate, a.pf32, gate_at, j, 1.f, g);
 #pragma unroll
       for (int k = 0; k < VW; ++k) v[j][k] *= g[k];
     }
 #pragma unroll
     for (int k = 0; k < VW; ++k) v[j][k] = fmaf(a.scale, row_elem<R, VW>(rq[j], k), v[j][k]);
-    row_store<R, VW>(h_out + row * a.width, col, a.width, v[j]);
+    c.store(h_out + row * a.width, j, v[j]);
   }
   if (a.norm != kNone) {
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int k = 0; k < VW; ++k)  // a post bias has filled the columns past the row
-        if ((l + j * G) * VW + k >= a.width) v[j][k] = 0.f;
-    const float2 m = rn_stats<G>(v, l, a, a.norm == kLayer, lds[2], lds[3]);
+    const float2 m = rn_stats(v, c, a, a.norm == kLayer, lds[2], lds[3]);
     st.z = m.x;
     st.w = m.y;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      const int col = (l + j * G) * VW;
       float w[VW], b[VW];
-      rn_param<T, VW>(a.w, a.pf32, 0, col, a.width, 1.f, w);
-      rn_param<T, VW>(a.b, a.pf32, 0, col, a.width, 0.f, b);
+      rn_param<T>(c, a.w, a.pf32, 0, j, 1.f, w);
+      rn_param<T>(c, a.b, a.pf32, 0, j, 0.f, b);
 #pragma unroll
       for (int k = 0; k < VW; ++k) v[j][k] = fmaf((v[j][k] - m.x) * m.y, w[k], b[k]);
-      row_store<T, VW>(y_out + row * a.width, col, a.width, v[j]);
+      c.store(y_out + row * a.width, j, v[j]);
     }
   }
   if (stats && l == 0) stats[row] = st;
@@ -177,6 +176,17 @@ struct RnGrads {
   int32_t want_gate, want_pw, want_pb, want_w, want_b;  // want_gate 1: a sum a section, 2: a value an element
 };
 
+// A row's operands of the backward as loaded.
+template <typename T, typename R, int NV, int VW> struct RnRaw {
+  RowVec<T, VW> x[NV], gy[NV];
+  RowVec<R, VW> r[NV], gh[NV];
+  float4 st;
+};
+
+// The operands of the next row are requested as soon as this row's are
+// widened, before its sums are joined: the parameters stay in registers
+// (loads return in order, and one made later would wait for the row requested
+// before it).
 template <typename T, typename R, int G, int EPT, bool POST>
 __global__ void __launch_bounds__(rn_bwd_block(G))
 k_residual_norm_backward(RnArgs a, RnGrads o) {
@@ -184,18 +194,30 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
   constexpr int VW = 16 / (int)sizeof(T), NV = EPT / VW;
   __shared__ float lds[2][2][2 * BS / 64];
   __shared__ float fold[ROWS > 1 ? BS * EPT : 1];
-  const int l = threadIdx.x & (G - 1), grp = threadIdx.x / G;
-  const bool need_x = POST || (a.gate != nullptr && o.want_gate);
+  const int l = threadIdx.x & (G - 1), grp = rn_group<G>();
+  const RowSlots<G, NV, VW> c(l, a.width);
   const bool has_norm = a.norm != kNone && o.gy != nullptr;
+  const bool need_x = POST || o.want_gate || (has_norm && !o.h);
   float ag[NV][VW] = {}, aw[NV][VW] = {}, ab[NV][VW] = {};
   float apw[POST ? NV : 1][VW] = {}, apb[POST ? NV : 1][VW] = {};
+  float w[NV][VW], gate[NV][VW], pw[POST ? NV : 1][VW], pb[POST ? NV : 1][VW];
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    rn_param<T>(c, a.w, a.pf32, 0, j, 1.f, w[j]);
+#pragma unroll
+    for (int k = 0; k < VW; ++k) gate[j][k] = 1.f;
+    if constexpr (POST) {
+      rn_param<T>(c, a.pw, a.pf32, 0, j, 1.f, pw[j]);
+      rn_param<T>(c, a.pb, a.pf32, 0, j, 0.f, pb[j]);
+    }
+  }
 
   // Adds a column sum over the workgroup's groups of rows and hands each
   // thread of the first group its columns' totals.
   auto folded = [&](const float (&s)[NV][VW], auto&& put) {
     if constexpr (ROWS == 1) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) put((l + j * G) * VW, s[j]);
+      for (int j = 0; j < NV; ++j) put(j, s[j]);
     } else {
       __syncthreads();
 #pragma unroll
@@ -206,19 +228,37 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
       if (grp == 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int col = (l + j * G) * VW;
+          const int at = (l + j * G) * VW;
           float t[VW];
 #pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            t[k] = s[j][k];
-            for (int g = 1; g < ROWS; ++g) t[k] += fold[g * (G * EPT) + col + k];
+          for (int k = 0; k < VW; ++k) t[k] = s[j][k];
+#pragma unroll 1
+          for (int g = 1; g < ROWS; ++g) {
+#pragma unroll
+            for (int k = 0; k < VW; ++k) t[k] += fold[g * (G * EPT) + at + k];
           }
-          put(col, t);
+          put(j, t);
         }
       }
     }
   };
   float* part = o.part + (int64_t)blockIdx.x * o.sums * a.width;
+
+  const R* r_rows = static_cast<const R*>(o.h ? o.h : a.res);
+  const int64_t r_stride = o.h ? (int64_t)a.width : a.res_stride;
+  RnRaw<T, R, NV, VW> q;
+  auto request = [&](int64_t row, bool active) {
+    q.st = active && o.stats ? o.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (need_x) q.x[j] = c.template load<true>(static_cast<const T*>(a.x) + row * a.x_stride, j, active);
+      if (has_norm) {
+        q.r[j] = c.template load<true>(r_rows + row * r_stride, j, active);
+        q.gy[j] = c.template load<true>(static_cast<const T*>(o.gy) + row * a.width, j, active);
+      }
+      if (o.gh) q.gh[j] = c.template load<true>(static_cast<const R*>(o.gh) + row * a.width, j, active);
+    }
+  };
 
   int parity = 0;
   const int64_t sec0 = (int64_t)(blockIdx.x / (uint32_t)o.cuts) * o.per;
@@ -227,71 +267,49 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
     const int64_t r0 = sec * o.section + (int64_t)(blockIdx.x % (uint32_t)o.cuts) * o.run;
     const int64_t end = (sec + 1) * o.section < a.rows ? (sec + 1) * o.section : a.rows;
     const int64_t r1 = r0 + o.run < end ? r0 + o.run : end;
+    if (a.gate && a.period != 1) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        rn_param<T>(c, a.gate, a.pf32, (int64_t)((uint32_t)r0 / a.period) * a.width, j, 1.f, gate[j]);
+    }
+    request(r0 + grp, r0 + grp < r1);
     for (int64_t base = r0; base < r1; base += ROWS, parity ^= 1) {
       const int64_t row = base + grp;
-      const bool active = row < r1;
-      const int width = active ? a.width : 0;  // loads give zeros, stores nothing
-      RowVec<T, VW> xq[NV], yq[NV];
-      RowVec<R, VW> rq[NV], hq[NV];
-      const float4 st = active && o.stats ? o.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
+      const bool active = row < r1;  // no row: nothing added, nothing stored
+      if (a.gate && a.period == 1) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int col = (l + j * G) * VW;
-        if (need_x || (has_norm && !o.h)) xq[j] = row_load<true, VW>(static_cast<const T*>(a.x) + row * a.x_stride, col, width);
-        if (has_norm) {
-          rq[j] = o.h ? row_load<true, VW>(static_cast<const R*>(o.h) + row * a.width, col, width)
-                      : row_load<true, VW>(static_cast<const R*>(a.res) + row * a.res_stride, col, width);
-          yq[j] = row_load<true, VW>(static_cast<const T*>(o.gy) + row * a.width, col, width);
-        }
-        if (o.gh) hq[j] = row_load<true, VW>(static_cast<const R*>(o.gh) + row * a.width, col, width);
+        for (int j = 0; j < NV; ++j)
+          rn_param<T>(c, a.gate, a.pf32, row * a.width, j, 1.f, gate[j], active);
       }
-      const int64_t gate_at = a.gate && active ? (int64_t)((uint32_t)row / a.period) * a.width : 0;
-      float xn[NV][VW], gate[NV][VW], dH[NV][VW];
+      const float4 st = q.st;
+      float xn[NV][VW], dH[NV][VW], n[NV][VW], da[NV][VW], s[2] = {0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        rn_param<T, VW>(a.gate, a.pf32, gate_at, (l + j * G) * VW, width, 1.f, gate[j]);
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
-          xn[j][k] = need_x || (has_norm && !o.h) ? row_elem<T, VW>(xq[j], k) : 0.f;
+          xn[j][k] = need_x ? row_elem<T, VW>(q.x[j], k) : 0.f;
           if constexpr (POST) xn[j][k] = (xn[j][k] - st.x) * st.y;
-          dH[j][k] = o.gh ? row_elem<R, VW>(hq[j], k) : 0.f;
-        }
-      }
-      auto post_out = [&](int j, float (&u)[VW]) {
-        if constexpr (POST) {
-          float w[VW], b[VW];
-          rn_param<T, VW>(a.pw, a.pf32, 0, (l + j * G) * VW, width, 1.f, w);
-          rn_param<T, VW>(a.pb, a.pf32, 0, (l + j * G) * VW, width, 0.f, b);
-#pragma unroll
-          for (int k = 0; k < VW; ++k) u[k] = fmaf(xn[j][k], w[k], b[k]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < VW; ++k) u[k] = xn[j][k];
-        }
-      };
-      if (has_norm) {
-        float n[NV][VW], da[NV][VW], s[2] = {0.f, 0.f};
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-          const int col = (l + j * G) * VW;
-          float u[VW], w[VW];
-          post_out(j, u);
-          rn_param<T, VW>(a.w, a.pf32, 0, col, width, 1.f, w);
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            const float r = row_elem<R, VW>(rq[j], k);
-            const float h = o.h ? r : fmaf(a.scale, r, u[k] * gate[j][k]);
-            const float dy = row_elem<T, VW>(yq[j], k);
+          dH[j][k] = o.gh ? row_elem<R, VW>(q.gh[j], k) : 0.f;
+          if (has_norm) {
+            float u = xn[j][k];
+            if constexpr (POST) u = fmaf(u, pw[j][k], pb[j][k]);
+            const float r = row_elem<R, VW>(q.r[j], k);
+            const float h = o.h ? r : fmaf(a.scale, r, u * gate[j][k]);
+            const float dy = row_elem<T, VW>(q.gy[j], k);
             n[j][k] = (h - st.z) * st.w;
-            da[j][k] = dy * w[k];
-            if (col + k < width) {
-              s[0] += da[j][k];
-              s[1] = fmaf(da[j][k], n[j][k], s[1]);
+            da[j][k] = dy * w[j][k];
+            if (active) {
+              const float d = c.mine(j, k) ? da[j][k] : 0.f;
+              s[0] += d;
+              s[1] = fmaf(d, n[j][k], s[1]);
               aw[j][k] = fmaf(dy, n[j][k], aw[j][k]);
               ab[j][k] += dy;
             }
           }
         }
+      }
+      if (base + ROWS < r1) request(row + ROWS, row + ROWS < r1);
+      if (has_norm) {
         group_sum<G>(s, lds[parity][0]);
         const float c0 = a.norm == kLayer ? s[0] * a.inv_width : 0.f, c1 = s[1] * a.inv_width;
 #pragma unroll
@@ -299,42 +317,44 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
 #pragma unroll
           for (int k = 0; k < VW; ++k) dH[j][k] = fmaf(st.w, fmaf(-n[j][k], c1, da[j][k] - c0), dH[j][k]);
       }
-      float du[NV][VW], s[2] = {0.f, 0.f};
+      s[0] = s[1] = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        const int col = (l + j * G) * VW;
         float t[VW];
         if (o.gres) {
 #pragma unroll
           for (int k = 0; k < VW; ++k) t[k] = a.scale * dH[j][k];
-          row_store<R, VW>(static_cast<R*>(o.gres) + row * a.width, col, width, t);
+          c.store(static_cast<R*>(o.gres) + row * a.width, j, t, active);
         }
         if (o.want_gate) {
           float u[VW];
-          post_out(j, u);
+#pragma unroll
+          for (int k = 0; k < VW; ++k) {
+            u[k] = xn[j][k];
+            if constexpr (POST) u[k] = fmaf(u[k], pw[j][k], pb[j][k]);
+          }
           if (o.want_gate == 2) {
 #pragma unroll
             for (int k = 0; k < VW; ++k) t[k] = u[k] * dH[j][k];
-            rn_param_store<T, VW>(o.ggate, a.pf32, gate_at, col, width, t);
+            rn_param_store<T>(c, o.ggate, a.pf32, row * a.width, j, t, active);
           } else {
 #pragma unroll
             for (int k = 0; k < VW; ++k)
-              if (col + k < width) ag[j][k] = fmaf(u[k], dH[j][k], ag[j][k]);
+              if (active) ag[j][k] = fmaf(u[k], dH[j][k], ag[j][k]);
           }
         }
 #pragma unroll
-        for (int k = 0; k < VW; ++k) du[j][k] = gate[j][k] * dH[j][k];
+        for (int k = 0; k < VW; ++k) dH[j][k] *= gate[j][k];  // du from here on
         if constexpr (POST) {
-          float w[VW];
-          rn_param<T, VW>(a.pw, a.pf32, 0, col, width, 1.f, w);
 #pragma unroll
           for (int k = 0; k < VW; ++k) {
-            if (col + k < width) {
-              apw[j][k] = fmaf(du[j][k], xn[j][k], apw[j][k]);
-              apb[j][k] += du[j][k];
-              du[j][k] *= w[k];
-              s[0] += du[j][k];
-              s[1] = fmaf(du[j][k], xn[j][k], s[1]);
+            if (active) {
+              apw[j][k] = fmaf(dH[j][k], xn[j][k], apw[j][k]);
+              apb[j][k] += dH[j][k];
+              dH[j][k] *= pw[j][k];
+              const float d = c.mine(j, k) ? dH[j][k] : 0.f;
+              s[0] += d;
+              s[1] = fmaf(d, xn[j][k], s[1]);
             }
           }
         }
@@ -345,18 +365,18 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int k = 0; k < VW; ++k) du[j][k] = st.y * fmaf(-xn[j][k], c1, du[j][k] - c0);
+          for (int k = 0; k < VW; ++k) dH[j][k] = st.y * fmaf(-xn[j][k], c1, dH[j][k] - c0);
       }
       if (o.gx) {
 #pragma unroll
         for (int j = 0; j < NV; ++j)
-          row_store<T, VW>(static_cast<T*>(o.gx) + row * a.width, (l + j * G) * VW, width, du[j]);
+          c.store(static_cast<T*>(o.gx) + row * a.width, j, dH[j], active);
       }
     }
     if (o.want_gate == 1) {
-      folded(ag, [&](int col, const float (&t)[VW]) {
-        if (o.cuts > 1) row_store<float, VW>(part, col, a.width, t);
-        else rn_param_store<T, VW>(o.ggate, a.pf32, sec * a.width, col, a.width, t);
+      folded(ag, [&](int j, const float (&t)[VW]) {
+        if (o.cuts > 1) c.store(part, j, t);
+        else rn_param_store<T>(c, o.ggate, a.pf32, sec * a.width, j, t);
       });
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -367,7 +387,7 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
   if (o.want_gate == 1 && o.cuts > 1) part += a.width;
   auto put = [&](int want, const float (&s)[NV][VW]) {
     if (!want) return;
-    folded(s, [&](int col, const float (&t)[VW]) { row_store<float, VW>(part, col, a.width, t); });
+    folded(s, [&](int j, const float (&t)[VW]) { c.store(part, j, t); });
     part += a.width;
   };
   if constexpr (POST) {

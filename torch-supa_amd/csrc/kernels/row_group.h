@@ -1,5 +1,5 @@
 // Rows held in the registers of a group of threads: G threads (16, a
-// wavefront, or several) share a row, thread l owning the vectors l, l + G, ...
+// wavefront, or several) share a row, thread l holding the vectors l, l + G, ...
 // of VW elements, at any element alignment.
 #pragma once
 
@@ -45,6 +45,65 @@ __device__ __forceinline__ void row_store(S* __restrict__ row, int col, int widt
       if (col + k < width) row[col + k] = from_arith<S>(f[k]);
   }
 }
+
+// Where a thread's NV vectors lie in a row of `width` elements, the same for
+// every row.  The vector that would run past the row's end is moved back
+// to it: it computes and stores some elements a second time, with the values
+// that the vector before has for them, and only sums along the row leave them
+// out.  So every access is a whole vector, and one instruction; a row
+// narrower than a vector, in groups of 16, goes element by element.
+template <int G, int NV, int VW> struct RowSlots {
+  static constexpr bool kWhole = G > 16;  // callers use them for rows of more than 16 vectors
+  uint32_t col[NV];
+  int32_t skip[NV];  // elements that another vector holds; VW: no vector here
+  int32_t width;
+
+  __device__ __forceinline__ RowSlots(int l, int w) : width(w) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int c = (l + j * G) * VW;
+      const int past = c + VW - w;
+      col[j] = (uint32_t)c;
+      skip[j] = 0;
+      if constexpr (kWhole) {
+        if (past > 0) {
+          skip[j] = past < VW ? past : VW;
+          col[j] = past < VW ? (uint32_t)(w - VW) : 0u;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ bool live(int j) const { return !kWhole || skip[j] < VW; }
+  __device__ __forceinline__ bool mine(int j, int k) const {
+    return kWhole ? k >= skip[j] : (int)col[j] + k < width;
+  }
+  // Vector j of the row at p; zeros where there is none.
+  template <bool STREAM, typename S>
+  __device__ __forceinline__ RowVec<S, VW> load(const S* __restrict__ p, int j, bool on = true) const {
+    if constexpr (kWhole) {
+      RowVec<S, VW> r{};
+      if (on && live(j)) {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(r.q) / 16); ++i) {
+          const char* at = reinterpret_cast<const char*>(p) + (col[j] * (uint32_t)sizeof(S) + 16u * i);
+          r.q[i] = STREAM ? ld_any_stream(at) : ld_any(at);
+        }
+      }
+      return r;
+    } else {
+      return row_load<STREAM, VW>(p, (int)col[j], on ? width : 0);
+    }
+  }
+  template <typename S>
+  __device__ __forceinline__ void store(S* __restrict__ p, int j, const float (&f)[VW], bool on = true) const {
+    if constexpr (kWhole) {
+      if (on && live(j))
+        store_any<S, VW>(reinterpret_cast<S*>(reinterpret_cast<char*>(p) + col[j] * (uint32_t)sizeof(S)), f);
+    } else {
+      row_store<S, VW>(p, (int)col[j], on ? width : 0, f);
+    }
+  }
+};
 
 // Sums over 16 lanes by four lane permutations within the row of 16, in every
 // lane: neighbours, pairs, then the two mirrors (a mirror pairs lanes that
