@@ -70,21 +70,17 @@ __device__ __forceinline__ float2 rn_stats(const float (&v)[NV][VW], const RowSl
   if (layer) {
     float s[1] = {0.f};
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int k = 0; k < VW; ++k) s[0] += c.mine(j, k) ? v[j][k] : 0.f;
+    for (int j = 0; j < NV; ++j) c.each(j, [&](int k) { s[0] += v[j][k]; });
     group_sum<G>(s, lds0);
     mean = s[0] * a.inv_width;
   }
   float q[1] = {0.f};
 #pragma unroll
-  for (int j = 0; j < NV; ++j) {
-#pragma unroll
-    for (int k = 0; k < VW; ++k) {
-      const float d = c.mine(j, k) ? v[j][k] - mean : 0.f;
+  for (int j = 0; j < NV; ++j)
+    c.each(j, [&](int k) {
+      const float d = v[j][k] - mean;
       q[0] = fmaf(d, d, q[0]);
-    }
-  }
+    });
   group_sum<G>(q, lds1);
   return make_float2(mean, rsqrtf(fmaf(q[0], a.inv_width, a.eps)));
 }
@@ -181,41 +177,153 @@ template <typename T, typename R, int NV, int VW> struct RnRaw {
   RowVec<T, VW> x[NV], gy[NV];
   RowVec<R, VW> r[NV], gh[NV];
   float4 st;
+  // keeps the compiler from holding on to floats formed before this
+  __device__ __forceinline__ void hide() {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      opaque(x[j].q);
+      opaque(gy[j].q);
+      opaque(r[j].q);
+      opaque(gh[j].q);
+    }
+  }
+};
+
+// Where the backward keeps what a column needs for all rows.  Up to 8 elements
+// a thread parameters and sums fit the registers beside two rows.  With 16, the
+// parameters lie in LDS (in global memory their loads, which return in order,
+// would wait for the row requested before them); and a workgroup of 1024
+// threads, with half the registers each, has the two sums that are always there
+// in LDS instead, requests a row when it begins, and reads the parameters again.
+template <int G, int EPT> struct RnKeep {
+  static constexpr bool kRegParams = EPT == 8;
+  static constexpr bool kLdsParams = EPT == 16 && G == 512;
+  static constexpr bool kLdsSums = EPT == 16 && G == 1024;
+  static constexpr bool kAhead = !kLdsSums;
+  // bytes of LDS beside the static ones
+  static constexpr int bytes(bool post, bool bias) {
+    return kLdsSums ? 2 * G * EPT * 4 : kLdsParams ? (2 + post + (post && bias)) * G * EPT * 4 : 0;
+  }
+};
+
+// A vector of a thread in LDS: its groups of four floats lie G NV vectors
+// apart, so that neighbouring threads read neighbouring 16 bytes.
+template <int G, int NV, int VW> struct RnLds {
+  float4* p;
+  __device__ __forceinline__ void get(int l, int j, float (&f)[VW]) const {
+#pragma unroll
+    for (int i = 0; i < VW / 4; ++i) {
+      const float4 v = p[i * (G * NV) + l + j * G];
+      f[4 * i] = v.x;
+      f[4 * i + 1] = v.y;
+      f[4 * i + 2] = v.z;
+      f[4 * i + 3] = v.w;
+    }
+  }
+  __device__ __forceinline__ void put(int l, int j, const float (&f)[VW]) const {
+#pragma unroll
+    for (int i = 0; i < VW / 4; ++i)
+      p[i * (G * NV) + l + j * G] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+  }
 };
 
 // The operands of the next row are requested as soon as this row's are
-// widened, before its sums are joined: the parameters stay in registers
-// (loads return in order, and one made later would wait for the row requested
-// before it).
-template <typename T, typename R, int G, int EPT, bool POST>
+// widened, before its sums are joined.
+template <typename T, typename R, int G, int EPT, bool POST, bool BIAS>
 __global__ void __launch_bounds__(rn_bwd_block(G))
 k_residual_norm_backward(RnArgs a, RnGrads o) {
   constexpr int BS = rn_bwd_block(G), ROWS = BS / G;
   constexpr int VW = 16 / (int)sizeof(T), NV = EPT / VW;
+  using Keep = RnKeep<G, EPT>;
+  using Lds = RnLds<G, NV, VW>;
+  constexpr int kReg = Keep::kRegParams ? NV : 1;
+  extern __shared__ float4 keep[];
+  // parameters (kLdsParams), or the sums of dw and dgate (kLdsSums)
+  const Lds lw{keep}, lgate{keep + G * EPT / 4}, lpw{keep + G * EPT / 2}, lpb{keep + 3 * (G * EPT / 4)};
   __shared__ float lds[2][2][2 * BS / 64];
   __shared__ float fold[ROWS > 1 ? BS * EPT : 1];
   const int l = threadIdx.x & (G - 1), grp = rn_group<G>();
-  const RowSlots<G, NV, VW> c(l, a.width);
+  RowSlots<G, NV, VW> c(l, a.width);
   const bool has_norm = a.norm != kNone && o.gy != nullptr;
   const bool need_x = POST || o.want_gate || (has_norm && !o.h);
-  float ag[NV][VW] = {}, aw[NV][VW] = {}, ab[NV][VW] = {};
-  float apw[POST ? NV : 1][VW] = {}, apb[POST ? NV : 1][VW] = {};
-  float w[NV][VW], gate[NV][VW], pw[POST ? NV : 1][VW], pb[POST ? NV : 1][VW];
+  constexpr int kSums = Keep::kLdsSums ? 1 : NV;
+  float ag[kSums][VW] = {}, aw[kSums][VW] = {};
+  float ab[BIAS ? NV : 1][VW] = {}, apw[POST ? NV : 1][VW] = {}, apb[POST && BIAS ? NV : 1][VW] = {};
+  float rw[kReg][VW], rgate[kReg][VW], rpw[kReg][VW], rpb[kReg][VW];
+  // vector j of the gate's row (where several rows share it)
+  auto set_gate = [&](int64_t at) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      float f[VW];
+      rn_param<T>(c, a.gate, a.pf32, at, j, 1.f, f);
+      if constexpr (Keep::kLdsParams) {
+        lgate.put(l, j, f);
+      } else if constexpr (Keep::kRegParams) {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) rgate[j][k] = f[k];
+      }
+    }
+  };
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    rn_param<T>(c, a.w, a.pf32, 0, j, 1.f, w[j]);
+    float f[VW];
+    rn_param<T>(c, a.w, a.pf32, 0, j, 1.f, f);
+    if constexpr (Keep::kRegParams) {
 #pragma unroll
-    for (int k = 0; k < VW; ++k) gate[j][k] = 1.f;
+      for (int k = 0; k < VW; ++k) rw[j][k] = f[k];
+    } else if constexpr (Keep::kLdsParams) {
+      lw.put(l, j, f);
+    }
     if constexpr (POST) {
-      rn_param<T>(c, a.pw, a.pf32, 0, j, 1.f, pw[j]);
-      rn_param<T>(c, a.pb, a.pf32, 0, j, 0.f, pb[j]);
+      rn_param<T>(c, a.pw, a.pf32, 0, j, 1.f, f);
+      if constexpr (Keep::kRegParams) {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) rpw[j][k] = f[k];
+      } else if constexpr (Keep::kLdsParams) {
+        lpw.put(l, j, f);
+      }
+    }
+    if constexpr (POST && BIAS) {
+      rn_param<T>(c, a.pb, a.pf32, 0, j, 0.f, f);
+      if constexpr (Keep::kRegParams) {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) rpb[j][k] = f[k];
+      } else if constexpr (Keep::kLdsParams) {
+        lpb.put(l, j, f);
+      }
+    }
+    if constexpr (Keep::kLdsSums) {
+      const float zero[VW] = {};
+      lw.put(l, j, zero);
+      lgate.put(l, j, zero);
     }
   }
+  if (!a.gate) set_gate(0);  // ones
+
+  // vector j of a parameter: every thread reads back what it has kept itself
+  auto get = [&](const float (&reg)[kReg][VW], const Lds& lds_at, const void* p, int64_t at, int j, float fill,
+                 float (&f)[VW]) {
+    if constexpr (Keep::kRegParams) {
+#pragma unroll
+      for (int k = 0; k < VW; ++k) f[k] = reg[j][k];
+    } else if constexpr (Keep::kLdsParams) {
+      lds_at.get(l, j, f);
+    } else {
+      rn_param<T>(c, p, a.pf32, at, j, fill, f);
+    }
+  };
 
   // Adds a column sum over the workgroup's groups of rows and hands each
   // thread of the first group its columns' totals.
-  auto folded = [&](const float (&s)[NV][VW], auto&& put) {
-    if constexpr (ROWS == 1) {
+  auto folded = [&](const auto& s, const Lds& at, auto&& put) {
+    if constexpr (sizeof(s) < sizeof(float) * NV * VW) {  // kept in LDS, by each thread its own
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float t[VW];
+        at.get(l, j, t);
+        put(j, t);
+      }
+    } else if constexpr (ROWS == 1) {
 #pragma unroll
       for (int j = 0; j < NV; ++j) put(j, s[j]);
     } else {
@@ -228,14 +336,14 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
       if (grp == 0) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int at = (l + j * G) * VW;
+          const int first = (l + j * G) * VW;
           float t[VW];
 #pragma unroll
           for (int k = 0; k < VW; ++k) t[k] = s[j][k];
 #pragma unroll 1
           for (int g = 1; g < ROWS; ++g) {
 #pragma unroll
-            for (int k = 0; k < VW; ++k) t[k] += fold[g * (G * EPT) + at + k];
+            for (int k = 0; k < VW; ++k) t[k] += fold[g * (G * EPT) + first + k];
           }
           put(j, t);
         }
@@ -244,19 +352,20 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
   };
   float* part = o.part + (int64_t)blockIdx.x * o.sums * a.width;
 
+  // h alone in the place of x and residual: the same sum with factors 1 and 0
   const R* r_rows = static_cast<const R*>(o.h ? o.h : a.res);
   const int64_t r_stride = o.h ? (int64_t)a.width : a.res_stride;
+  const float r_scale = o.h ? 1.f : a.scale;
   RnRaw<T, R, NV, VW> q;
+  // What a row does not have, or a group without a row, is zeros.
   auto request = [&](int64_t row, bool active) {
     q.st = active && o.stats ? o.stats[row] : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (need_x) q.x[j] = c.template load<true>(static_cast<const T*>(a.x) + row * a.x_stride, j, active);
-      if (has_norm) {
-        q.r[j] = c.template load<true>(r_rows + row * r_stride, j, active);
-        q.gy[j] = c.template load<true>(static_cast<const T*>(o.gy) + row * a.width, j, active);
-      }
-      if (o.gh) q.gh[j] = c.template load<true>(static_cast<const R*>(o.gh) + row * a.width, j, active);
+      q.x[j] = c.template load<true>(static_cast<const T*>(a.x) + row * a.x_stride, j, active && need_x);
+      q.r[j] = c.template load<true>(r_rows + row * r_stride, j, active && has_norm);
+      q.gy[j] = c.template load<true>(static_cast<const T*>(o.gy) + row * a.width, j, active && has_norm);
+      q.gh[j] = c.template load<true>(static_cast<const R*>(o.gh) + row * a.width, j, active && o.gh);
     }
   };
 
@@ -267,105 +376,188 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
     const int64_t r0 = sec * o.section + (int64_t)(blockIdx.x % (uint32_t)o.cuts) * o.run;
     const int64_t end = (sec + 1) * o.section < a.rows ? (sec + 1) * o.section : a.rows;
     const int64_t r1 = r0 + o.run < end ? r0 + o.run : end;
-    if (a.gate && a.period != 1) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        rn_param<T>(c, a.gate, a.pf32, (int64_t)((uint32_t)r0 / a.period) * a.width, j, 1.f, gate[j]);
-    }
-    request(r0 + grp, r0 + grp < r1);
+    const int64_t gate_at = a.gate ? (int64_t)((uint32_t)r0 / a.period) * a.width : 0;
+    if (a.gate && a.period != 1) set_gate(gate_at);
+    if constexpr (Keep::kAhead) request(r0 + grp, r0 + grp < r1);
     for (int64_t base = r0; base < r1; base += ROWS, parity ^= 1) {
+      c.renew();
       const int64_t row = base + grp;
-      const bool active = row < r1;  // no row: nothing added, nothing stored
-      if (a.gate && a.period == 1) {
-#pragma unroll
-        for (int j = 0; j < NV; ++j)
-          rn_param<T>(c, a.gate, a.pf32, row * a.width, j, 1.f, gate[j], active);
-      }
+      const bool active = ROWS == 1 || row < r1;  // no row: zeros are added and nothing is stored
+      if constexpr (!Keep::kAhead) request(row, active);
+      const bool own_gate = a.gate && a.period == 1;
+      auto gate_of = [&](int j, float (&f)[VW]) {
+        if (own_gate) rn_param<T>(c, a.gate, a.pf32, row * a.width, j, 1.f, f, active);
+        else get(rgate, lgate, a.gate, gate_at, j, 1.f, f);
+      };
       const float4 st = q.st;
-      float xn[NV][VW], dH[NV][VW], n[NV][VW], da[NV][VW], s[2] = {0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
+      // The row as floats: kept while the next row is on its way into q, or
+      // (kAhead false, registers for one of the two) formed from q each time.
+      constexpr int kRow = Keep::kAhead ? NV : 1;
+      float xs[kRow][VW], ns[kRow][VW], das[kRow][VW], dH[NV][VW], s[2] = {0.f, 0.f};
+      auto normalised_x = [&](int j, float (&x)[VW]) {
 #pragma unroll
         for (int k = 0; k < VW; ++k) {
-          xn[j][k] = need_x ? row_elem<T, VW>(q.x[j], k) : 0.f;
-          if constexpr (POST) xn[j][k] = (xn[j][k] - st.x) * st.y;
-          dH[j][k] = o.gh ? row_elem<R, VW>(q.gh[j], k) : 0.f;
-          if (has_norm) {
-            float u = xn[j][k];
-            if constexpr (POST) u = fmaf(u, pw[j][k], pb[j][k]);
-            const float r = row_elem<R, VW>(q.r[j], k);
-            const float h = o.h ? r : fmaf(a.scale, r, u * gate[j][k]);
-            const float dy = row_elem<T, VW>(q.gy[j], k);
-            n[j][k] = (h - st.z) * st.w;
-            da[j][k] = dy * w[j][k];
-            if (active) {
-              const float d = c.mine(j, k) ? da[j][k] : 0.f;
-              s[0] += d;
-              s[1] = fmaf(d, n[j][k], s[1]);
-              aw[j][k] = fmaf(dy, n[j][k], aw[j][k]);
-              ab[j][k] += dy;
-            }
-          }
+          x[k] = row_elem<T, VW>(q.x[j], k);
+          if constexpr (POST) x[k] = (x[k] - st.x) * st.y;
         }
-      }
-      if (base + ROWS < r1) request(row + ROWS, row + ROWS < r1);
-      if (has_norm) {
-        group_sum<G>(s, lds[parity][0]);
-        const float c0 = a.norm == kLayer ? s[0] * a.inv_width : 0.f, c1 = s[1] * a.inv_width;
+      };
+      auto x_of = [&](int j, float (&x)[VW]) {
+        if constexpr (Keep::kAhead) {
+#pragma unroll
+          for (int k = 0; k < VW; ++k) x[k] = xs[j][k];
+        } else {
+          normalised_x(j, x);
+        }
+      };
+      // u from the normalised x
+      auto post_out = [&](int j, const float (&x)[VW], float (&u)[VW]) {
+        float pw[VW], pb[VW];
+        if constexpr (POST) get(rpw, lpw, a.pw, 0, j, 1.f, pw);
+        if constexpr (POST && BIAS) get(rpb, lpb, a.pb, 0, j, 0.f, pb);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          u[k] = x[k];
+          if constexpr (POST && BIAS) u[k] = fmaf(u[k], pw[k], pb[k]);
+          else if constexpr (POST) u[k] *= pw[k];
+        }
+      };
+      // n = (h - mean) rstd and a = dy w of vector j
+      auto normalised_h = [&](int j, float (&n)[VW], float (&da)[VW], float (&dy)[VW]) {
+        float x[VW], u[VW], w[VW], gate[VW];
+        x_of(j, x);
+        post_out(j, x, u);
+        gate_of(j, gate);
+        get(rw, lw, a.w, 0, j, 1.f, w);
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          const float h = fmaf(r_scale, row_elem<R, VW>(q.r[j], k), u[k] * gate[k]);
+          dy[k] = row_elem<T, VW>(q.gy[j], k);
+          n[k] = (h - st.z) * st.w;
+          da[k] = dy[k] * w[k];
+        }
+      };
+      if constexpr (Keep::kAhead) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) normalised_x(j, xs[j]);
 #pragma unroll
         for (int j = 0; j < NV; ++j)
 #pragma unroll
-          for (int k = 0; k < VW; ++k) dH[j][k] = fmaf(st.w, fmaf(-n[j][k], c1, da[j][k] - c0), dH[j][k]);
+          for (int k = 0; k < VW; ++k) dH[j][k] = row_elem<R, VW>(q.gh[j], k);
       }
-      s[0] = s[1] = 0.f;
+      if (has_norm) {
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        float t[VW];
-        if (o.gres) {
+        for (int j = 0; j < NV; ++j) {
+          float n[VW], da[VW], dy[VW], sum[VW];
+          normalised_h(j, n, da, dy);
+          if constexpr (Keep::kLdsSums) lw.get(l, j, sum);
+#pragma unroll
+          for (int k = 0; k < VW; ++k) {
+            if constexpr (Keep::kLdsSums) sum[k] = fmaf(dy[k], n[k], sum[k]);
+            else aw[j][k] = fmaf(dy[k], n[k], aw[j][k]);
+            if constexpr (BIAS) ab[j][k] += dy[k];
+            if constexpr (Keep::kAhead) {
+              ns[j][k] = n[k];
+              das[j][k] = da[k];
+            }
+          }
+          if constexpr (Keep::kLdsSums) lw.put(l, j, sum);
+          c.each(j, [&](int k) {
+            s[0] += da[k];
+            s[1] = fmaf(da[k], n[k], s[1]);
+          });
+        }
+        if constexpr (Keep::kAhead) {
+          if (base + ROWS < r1) request(row + ROWS, row + ROWS < r1);
+        }
+        group_sum<G>(s, lds[parity][0]);
+        if constexpr (!Keep::kAhead) q.hide(), c.renew();
+        const float c0 = a.norm == kLayer ? s[0] * a.inv_width : 0.f, c1 = s[1] * a.inv_width;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          if constexpr (Keep::kAhead) {
+#pragma unroll
+            for (int k = 0; k < VW; ++k) dH[j][k] = fmaf(st.w, fmaf(-ns[j][k], c1, das[j][k] - c0), dH[j][k]);
+          } else {
+            float n[VW], da[VW], dy[VW];
+            normalised_h(j, n, da, dy);
+#pragma unroll
+            for (int k = 0; k < VW; ++k)
+              dH[j][k] = fmaf(st.w, fmaf(-n[k], c1, da[k] - c0), row_elem<R, VW>(q.gh[j], k));
+          }
+        }
+      } else if constexpr (Keep::kAhead) {
+        if (base + ROWS < r1) request(row + ROWS, row + ROWS < r1);
+      } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+          for (int k = 0; k < VW; ++k) dH[j][k] = row_elem<R, VW>(q.gh[j], k);
+      }
+      if (o.gres) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+          float t[VW];
 #pragma unroll
           for (int k = 0; k < VW; ++k) t[k] = a.scale * dH[j][k];
           c.store(static_cast<R*>(o.gres) + row * a.width, j, t, active);
         }
-        if (o.want_gate) {
-          float u[VW];
+      }
+      if (o.want_gate) {
 #pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            u[k] = xn[j][k];
-            if constexpr (POST) u[k] = fmaf(u[k], pw[j][k], pb[j][k]);
-          }
+        for (int j = 0; j < NV; ++j) {
+          float x[VW], u[VW], sum[VW];
+          x_of(j, x);
+          post_out(j, x, u);
           if (o.want_gate == 2) {
 #pragma unroll
-            for (int k = 0; k < VW; ++k) t[k] = u[k] * dH[j][k];
-            rn_param_store<T>(c, o.ggate, a.pf32, row * a.width, j, t, active);
+            for (int k = 0; k < VW; ++k) u[k] *= dH[j][k];
+            rn_param_store<T>(c, o.ggate, a.pf32, row * a.width, j, u, active);
+          } else if constexpr (Keep::kLdsSums) {
+            lgate.get(l, j, sum);
+#pragma unroll
+            for (int k = 0; k < VW; ++k) sum[k] = fmaf(u[k], dH[j][k], sum[k]);
+            lgate.put(l, j, sum);
           } else {
 #pragma unroll
-            for (int k = 0; k < VW; ++k)
-              if (active) ag[j][k] = fmaf(u[k], dH[j][k], ag[j][k]);
-          }
-        }
-#pragma unroll
-        for (int k = 0; k < VW; ++k) dH[j][k] *= gate[j][k];  // du from here on
-        if constexpr (POST) {
-#pragma unroll
-          for (int k = 0; k < VW; ++k) {
-            if (active) {
-              apw[j][k] = fmaf(dH[j][k], xn[j][k], apw[j][k]);
-              apb[j][k] += dH[j][k];
-              dH[j][k] *= pw[j][k];
-              const float d = c.mine(j, k) ? dH[j][k] : 0.f;
-              s[0] += d;
-              s[1] = fmaf(d, xn[j][k], s[1]);
-            }
+            for (int k = 0; k < VW; ++k) ag[j][k] = fmaf(u[k], dH[j][k], ag[j][k]);
           }
         }
       }
+      s[0] = s[1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        float x[VW], gate[VW], pw[VW];
+        gate_of(j, gate);
+        if constexpr (POST) {
+          x_of(j, x);
+          get(rpw, lpw, a.pw, 0, j, 1.f, pw);
+        }
+#pragma unroll
+        for (int k = 0; k < VW; ++k) {
+          dH[j][k] *= gate[k];  // du from here on
+          if constexpr (POST) {
+            apw[j][k] = fmaf(dH[j][k], x[k], apw[j][k]);
+            if constexpr (BIAS) apb[j][k] += dH[j][k];
+            dH[j][k] *= pw[k];
+          }
+        }
+        if constexpr (POST)
+          c.each(j, [&](int k) {
+            s[0] += dH[j][k];
+            s[1] = fmaf(dH[j][k], x[k], s[1]);
+          });
+      }
       if constexpr (POST) {
         group_sum<G>(s, lds[parity][1]);
+        if constexpr (!Keep::kAhead) q.hide(), c.renew();
         const float c0 = a.post == kLayer ? s[0] * a.inv_width : 0.f, c1 = s[1] * a.inv_width;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+          float x[VW];
+          x_of(j, x);
 #pragma unroll
-          for (int k = 0; k < VW; ++k) dH[j][k] = st.y * fmaf(-xn[j][k], c1, dH[j][k] - c0);
+          for (int k = 0; k < VW; ++k) dH[j][k] = st.y * fmaf(-x[k], c1, dH[j][k] - c0);
+        }
       }
       if (o.gx) {
 #pragma unroll
@@ -374,28 +566,31 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
       }
     }
     if (o.want_gate == 1) {
-      folded(ag, [&](int j, const float (&t)[VW]) {
+      folded(ag, lgate, [&](int j, const float (&t)[VW]) {
         if (o.cuts > 1) c.store(part, j, t);
         else rn_param_store<T>(c, o.ggate, a.pf32, sec * a.width, j, t);
       });
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+      for (int j = 0; j < kSums; ++j)
 #pragma unroll
         for (int k = 0; k < VW; ++k) ag[j][k] = 0.f;
+      if constexpr (Keep::kLdsSums) {
+        const float zero[VW] = {};
+#pragma unroll
+        for (int j = 0; j < NV; ++j) lgate.put(l, j, zero);
+      }
     }
   }
   if (o.want_gate == 1 && o.cuts > 1) part += a.width;
-  auto put = [&](int want, const float (&s)[NV][VW]) {
+  auto put = [&](int want, const auto& s, const Lds& at) {
     if (!want) return;
-    folded(s, [&](int j, const float (&t)[VW]) { c.store(part, j, t); });
+    folded(s, at, [&](int j, const float (&t)[VW]) { c.store(part, j, t); });
     part += a.width;
   };
-  if constexpr (POST) {
-    put(o.want_pw, apw);
-    put(o.want_pb, apb);
-  }
-  put(o.want_w, aw);
-  put(o.want_b, ab);
+  if constexpr (POST) put(o.want_pw, apw, Lds{nullptr});
+  if constexpr (POST && BIAS) put(o.want_pb, apb, Lds{nullptr});
+  put(o.want_w, aw, lw);
+  if constexpr (BIAS) put(o.want_b, ab, Lds{nullptr});
 }
 
 // Adds the partials: block (x, y) the columns [64 x, 64 x + 64) of sum y.  The
@@ -446,6 +641,16 @@ template <typename F> int rn_shape(int64_t width, F&& go) {
   if (width <= 4096) return go(integral_constant<int, 512>{}, E8{});
   if (width <= 8192) return go(integral_constant<int, 1024>{}, E8{});
   return go(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
+}
+// The same for the backward, whose threads need more registers: 512 threads up
+// to 8192 elements.
+template <typename F> int rn_bwd_shape(int64_t width, F&& go) {
+  if (width > 4096 && width <= 8192)
+    return go(std::integral_constant<int, 512>{}, std::integral_constant<int, 16>{});
+  return rn_shape(width, [&](auto G, auto E) -> int {
+    if constexpr (G.value == 1024 && E.value == 8) return SUPA_AMD_EINVAL;  // taken above
+    else return go(G, E);
+  });
 }
 
 template <typename F> int rn_types(int dtype, int residual, F&& go) {
@@ -505,7 +710,7 @@ struct RnPlan {
 RnPlan rn_plan(const supa_amd_residual_norm_desc& d) {
   RnPlan p{};
   int64_t at_once = 1;
-  rn_shape(d.width, [&](auto G, auto) {
+  rn_bwd_shape(d.width, [&](auto G, auto) {
     at_once = rn_bwd_block(G.value) / G.value;
     return 0;
   });
@@ -605,12 +810,22 @@ int supa_amd_residual_norm_backward(const supa_amd_residual_norm_desc* d, const 
   return rn_types(d->dtype, d->residual_dtype, [&](auto* t, auto* r) -> int {
     using T = std::remove_pointer_t<decltype(t)>;
     using R = std::remove_pointer_t<decltype(r)>;
-    const int rl = rn_shape(d->width, [&](auto G, auto E) -> int {
-      if (post)
-        k_residual_norm_backward<T, R, G.value, E.value, true><<<(unsigned)p.parts, rn_bwd_block(G.value), 0, st>>>(a, o);
-      else
-        k_residual_norm_backward<T, R, G.value, E.value, false><<<(unsigned)p.parts, rn_bwd_block(G.value), 0, st>>>(a, o);
-      return launch_status();
+    const int rl = rn_bwd_shape(d->width, [&](auto G, auto E) -> int {
+      auto go = [&](auto post_c, auto bias_c) -> int {
+        constexpr auto kernel = k_residual_norm_backward<T, R, G.value, E.value, post_c.value, bias_c.value>;
+        constexpr int lds = RnKeep<G.value, E.value>::bytes(post_c.value, bias_c.value);
+        if constexpr (lds > 0) {  // past the 64 KiB that a launch has without asking
+          static const hipError_t allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                                hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+          if (allowed != hipSuccess) return (int)allowed;
+        }
+        kernel<<<(unsigned)p.parts, rn_bwd_block(G.value), lds, st>>>(a, o);
+        return launch_status();
+      };
+      using std::bool_constant;
+      const bool bias = d->post_bias || d->bias || grad_post_bias || grad_bias;
+      if (post) return bias ? go(bool_constant<true>{}, bool_constant<true>{}) : go(bool_constant<true>{}, bool_constant<false>{});
+      return bias ? go(bool_constant<false>{}, bool_constant<true>{}) : go(bool_constant<false>{}, bool_constant<false>{});
     });
     if (rl || o.sums == 0) return rl;
     RnSums f{};

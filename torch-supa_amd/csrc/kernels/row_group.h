@@ -73,9 +73,31 @@ template <int G, int NV, int VW> struct RowSlots {
       }
     }
   }
+  // At the top of a loop over rows: keeps the compiler from forming every
+  // operand's 64-bit addresses ahead of the loop (and spilling them), where a
+  // scalar row address and these 32-bit offsets do.
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(col[j]));
+  }
   __device__ __forceinline__ bool live(int j) const { return !kWhole || skip[j] < VW; }
-  __device__ __forceinline__ bool mine(int j, int k) const {
-    return kWhole ? k >= skip[j] : (int)col[j] + k < width;
+  // f(k) for the elements of vector j that are the row's and no other vector's.
+  // The vector that was moved back is one thread's, and takes a branch of its own.
+  template <typename F> __device__ __forceinline__ void each(int j, F&& f) const {
+    if constexpr (kWhole) {
+      if (skip[j] == 0) {
+#pragma unroll
+        for (int k = 0; k < VW; ++k) f(k);
+      } else if (skip[j] < VW) {
+#pragma unroll
+        for (int k = 0; k < VW; ++k)
+          if (k >= skip[j]) f(k);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < VW; ++k)
+        if ((int)col[j] + k < width) f(k);
+    }
   }
   // Vector j of the row at p; zeros where there is none.
   template <bool STREAM, typename S>
