@@ -111,16 +111,17 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
   __shared__ float lds[4][BS / 64];
   const int l = threadIdx.x & (G - 1);
   const int64_t row = a.row0 + (int64_t)blockIdx.x * (BS / G) + rn_group<G>();
-  if (row >= a.rows) return;  // G above 64: a row a workgroup, all of them there
+  const bool on = row < a.rows;
+  if (G <= 64 && !on) return;  // above 64, every thread joins the barriers
   const RowSlots<G, NV, VW> c(l, a.width);
   const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
   const R* res = static_cast<const R*>(a.res) + row * a.res_stride;
   RowVec<T, VW> xq[NV];
   RowVec<R, VW> rq[NV];
 #pragma unroll
-  for (int j = 0; j < NV; ++j) xq[j] = c.template load<true>(x, j);
+  for (int j = 0; j < NV; ++j) xq[j] = c.template load<true>(x, j, on);
 #pragma unroll
-  for (int j = 0; j < NV; ++j) rq[j] = c.template load<true>(res, j);
+  for (int j = 0; j < NV; ++j) rq[j] = c.template load<true>(res, j, on);
   float v[NV][VW];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
@@ -145,13 +146,13 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
   for (int j = 0; j < NV; ++j) {
     if (a.gate) {
       float g[VW];
-      rn_param<T>(c, a.gate, a.pf32, gate_at, j, 1.f, g);
+      rn_param<T>(c, a.gate, a.pf32, gate_at, j, 1.f, g, on);
 #pragma unroll
       for (int k = 0; k < VW; ++k) v[j][k] *= g[k];
     }
 #pragma unroll
     for (int k = 0; k < VW; ++k) v[j][k] = fmaf(a.scale, row_elem<R, VW>(rq[j], k), v[j][k]);
-    c.store(h_out + row * a.width, j, v[j]);
+    c.store(h_out + row * a.width, j, v[j], on);
   }
   if (a.norm != kNone) {
     const float2 m = rn_stats(v, c, a, a.norm == kLayer, lds[2], lds[3]);
@@ -164,10 +165,10 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
       rn_param<T>(c, a.b, a.pf32, 0, j, 0.f, b);
 #pragma unroll
       for (int k = 0; k < VW; ++k) v[j][k] = fmaf((v[j][k] - m.x) * m.y, w[k], b[k]);
-      c.store(y_out + row * a.width, j, v[j]);
+      c.store(y_out + row * a.width, j, v[j], on);
     }
   }
-  if (stats && l == 0) stats[row] = st;
+  if (stats && l == 0 && on) stats[row] = st;
 }
 
 // The backward's outputs and how its rows are shared out: `sections` of
@@ -725,7 +726,9 @@ template <typename F> int rn_shape(int64_t width, F&& go) {
   using std::integral_constant;
   using E8 = integral_constant<int, 8>;
   if (width <= 128) return go(integral_constant<int, 16>{}, E8{});
+  if (width <= 256) return go(integral_constant<int, 32>{}, E8{});
   if (width <= 512) return go(integral_constant<int, 64>{}, E8{});
+  if (width <= 1024) return go(integral_constant<int, 128>{}, E8{});
   if (width <= 2048) return go(integral_constant<int, 256>{}, E8{});
   if (width <= 4096) return go(integral_constant<int, 512>{}, E8{});
   if (width <= 8192) return go(integral_constant<int, 1024>{}, E8{});
@@ -740,7 +743,9 @@ template <int esize, typename F> int rn_bwd_shape(int64_t width, F&& go) {
   using V1 = integral_constant<int, E>;
   using E16 = integral_constant<int, 16>;
   if (width <= 16 * E) return go(integral_constant<int, 16>{}, V1{});
+  if (width <= 32 * E) return go(integral_constant<int, 32>{}, V1{});
   if (width <= 64 * E) return go(integral_constant<int, 64>{}, V1{});
+  if (width <= 128 * E) return go(integral_constant<int, 128>{}, V1{});
   if (width <= 256 * E) return go(integral_constant<int, 256>{}, V1{});
   if (width <= 512 * E) return go(integral_constant<int, 512>{}, V1{});
   if constexpr (esize == 4) {

@@ -154,6 +154,12 @@ template <int G, int N> __device__ __forceinline__ void group_sum(float (&v)[N],
   if constexpr (G == 16) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = sum16(v[i]);
+  } else if constexpr (G == 32) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = sum16(v[i]);
+      v[i] += __shfl_xor(v[i], 16, 64);
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = sum64(v[i]);
