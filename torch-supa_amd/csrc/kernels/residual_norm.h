@@ -75,11 +75,11 @@ __device__ __forceinline__ void rn_param_store(const RowSlots<G, NV, VW>& c, voi
 }
 
 // Mean and reciprocal deviation of a row's values.
-template <int G, int NV, int VW>
+template <bool LAYER, int G, int NV, int VW>
 __device__ __forceinline__ float2 rn_stats(const float (&v)[NV][VW], const RowSlots<G, NV, VW>& c, const RnArgs& a,
                                            bool layer, float* lds0, float* lds1) {
   float mean = 0.f;
-  if (layer) {
+  if (LAYER && layer) {
     float s[1] = {0.f};
 #pragma unroll
     for (int j = 0; j < NV; ++j) c.each(j, [&](int k) { s[0] += v[j][k]; });
@@ -90,7 +90,7 @@ __device__ __forceinline__ float2 rn_stats(const float (&v)[NV][VW], const RowSl
 #pragma unroll
   for (int j = 0; j < NV; ++j)
     c.each(j, [&](int k) {
-      const float d = v[j][k] - mean;
+      const float d = LAYER ? v[j][k] - mean : v[j][k];
       q[0] = fmaf(d, d, q[0]);
     });
   group_sum<G>(q, lds1);
@@ -103,7 +103,12 @@ template <int G> __device__ __forceinline__ int rn_group() {
   return G >= 64 ? __builtin_amdgcn_readfirstlane(g) : g;
 }
 
-template <typename T, typename R, int G, int EPT>
+// P is the parameters' type, LAYER as in the backward.  Parameters are asked for
+// before the row's sums, which hide their time ([8192, 8192] bf16 101 -> 96 us,
+// [12000, 2560] 53 -> 46); not where float32 ones would cost a workgroup its
+// place on the CU ([8192, 6144] bf16 on a float32 stream, layer norm: 115 us, 133
+// with them early; [16384, 8192] 287, 294).
+template <typename T, typename R, typename P, int G, int EPT, bool LAYER>
 __global__ void __launch_bounds__(G > 256 ? G : 256)
 k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* __restrict__ stats) {
   constexpr int BS = G > 256 ? G : 256;
@@ -118,55 +123,82 @@ k_residual_norm(RnArgs a, R* __restrict__ h_out, T* __restrict__ y_out, float4* 
   const R* res = static_cast<const R*>(a.res) + row * a.res_stride;
   RowVec<T, VW> xq[NV];
   RowVec<R, VW> rq[NV];
+  constexpr bool kEarly = !(sizeof(P) == 4 && (LAYER || G == 1024));
+  RowVec<P, VW> pwq[NV], pbq[NV], gq[NV], wq[NV], bq[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) xq[j] = c.template load<true>(x, j, on);
 #pragma unroll
   for (int j = 0; j < NV; ++j) rq[j] = c.template load<true>(res, j, on);
+  const int64_t gate_at = a.gate ? (int64_t)((uint32_t)row / a.period) * a.width : 0;
+  auto ask = [&](RowVec<P, VW> (&to)[NV], const void* p, int64_t at) {
+    if (!p) return;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) to[j] = c.template load<false>(static_cast<const P*>(p) + at, j, on);
+  };
+  auto ask_post = [&]() {
+    ask(pwq, a.pw, 0);
+    if (LAYER) ask(pbq, a.pb, 0);
+    ask(gq, a.gate, gate_at);
+  };
+  auto ask_norm = [&]() {
+    ask(wq, a.w, 0);
+    if (LAYER) ask(bq, a.b, 0);
+  };
+  if (kEarly) ask_post(), ask_norm();
   float v[NV][VW];
 #pragma unroll
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int k = 0; k < VW; ++k) v[j][k] = row_elem<T, VW>(xq[j], k);
+  // v from its row's mean and deviation
+  auto normalise = [&](float2 m, const void* w, const RowVec<P, VW> (&wv)[NV], const void* b,
+                       const RowVec<P, VW> (&bv)[NV]) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) v[j][k] = (LAYER ? v[j][k] - m.x : v[j][k]) * m.y;
+    if (w) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) v[j][k] *= row_elem<P, VW>(wv[j], k);
+    }
+    if (LAYER && b) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int k = 0; k < VW; ++k) v[j][k] += row_elem<P, VW>(bv[j], k);
+    }
+  };
   float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
   if (a.post != kNone) {
-    const float2 m = rn_stats(v, c, a, a.post == kLayer, lds[0], lds[1]);
+    const float2 m = rn_stats<LAYER>(v, c, a, a.post == kLayer, lds[0], lds[1]);
     st.x = m.x;
     st.y = m.y;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float w[VW], b[VW];
-      rn_param<T>(c, a.pw, a.pf32, 0, j, 1.f, w);
-      rn_param<T>(c, a.pb, a.pf32, 0, j, 0.f, b);
-#pragma unroll
-      for (int k = 0; k < VW; ++k) v[j][k] = fmaf((v[j][k] - m.x) * m.y, w[k], b[k]);
-    }
+    if (!kEarly) ask_post();
+    normalise(m, a.pw, pwq, a.pb, pbq);
   }
-  const int64_t gate_at = a.gate ? (int64_t)((uint32_t)row / a.period) * a.width : 0;
+  if (!kEarly && a.post == kNone) ask_post();
+  if (a.gate) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int k = 0; k < VW; ++k) v[j][k] *= row_elem<P, VW>(gq[j], k);
+  }
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    if (a.gate) {
-      float g[VW];
-      rn_param<T>(c, a.gate, a.pf32, gate_at, j, 1.f, g, on);
-#pragma unroll
-      for (int k = 0; k < VW; ++k) v[j][k] *= g[k];
-    }
 #pragma unroll
     for (int k = 0; k < VW; ++k) v[j][k] = fmaf(a.scale, row_elem<R, VW>(rq[j], k), v[j][k]);
     c.store(h_out + row * a.width, j, v[j], on);
   }
   if (a.norm != kNone) {
-    const float2 m = rn_stats(v, c, a, a.norm == kLayer, lds[2], lds[3]);
+    const float2 m = rn_stats<LAYER>(v, c, a, a.norm == kLayer, lds[2], lds[3]);
     st.z = m.x;
     st.w = m.y;
+    if (!kEarly) ask_norm();
+    normalise(m, a.w, wq, a.b, bq);
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      float w[VW], b[VW];
-      rn_param<T>(c, a.w, a.pf32, 0, j, 1.f, w);
-      rn_param<T>(c, a.b, a.pf32, 0, j, 0.f, b);
-#pragma unroll
-      for (int k = 0; k < VW; ++k) v[j][k] = fmaf((v[j][k] - m.x) * m.y, w[k], b[k]);
-      c.store(y_out + row * a.width, j, v[j], on);
-    }
+    for (int j = 0; j < NV; ++j) c.store(y_out + row * a.width, j, v[j], on);
   }
   if (stats && l == 0 && on) stats[row] = st;
 }
@@ -848,8 +880,18 @@ int rn_forward_t(const supa_amd_residual_norm_desc* d, const RnArgs& a, void* h,
       RnArgs s = a;
       s.row0 = r0;
       s.rows = std::min(d->rows, r0 + kSlab);
-      k_residual_norm<T, R, G.value, E.value><<<(unsigned)((s.rows - r0 + PER - 1) / PER), BS, 0, st>>>(
-          s, static_cast<R*>(h), static_cast<T*>(y), reinterpret_cast<float4*>(stats));
+      auto go = [&](auto* p, auto layer) {
+        using P = std::remove_pointer_t<decltype(p)>;
+        k_residual_norm<T, R, P, G.value, E.value, layer.value>
+            <<<(unsigned)((s.rows - r0 + PER - 1) / PER), BS, 0, st>>>(s, static_cast<R*>(h), static_cast<T*>(y),
+                                                                      reinterpret_cast<float4*>(stats));
+      };
+      auto typed = [&](auto layer) {
+        if (a.pf32) go((float*)nullptr, layer);
+        else go((T*)nullptr, layer);
+      };
+      if (rn_layer(*d)) typed(std::true_type{});
+      else typed(std::false_type{});
       const int rl = launch_status();
       if (rl) return rl;
     }
