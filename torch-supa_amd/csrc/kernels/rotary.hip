@@ -4,9 +4,12 @@
 //
 // HBM-bound: q and k are read and written once, together in one launch; the
 // angles cost 20 bytes a token.  Every head of a token turns by the same
-// angles, so a workgroup takes whole tokens: its threads form the sine and
-// cosine of each angle once, in LDS, while the first vectors of q and k are on
-// their way.  position * frequency is formed in 64 bits and reduced to a
+// angles, so a workgroup takes a tile of tokens and heads: its threads form the
+// sine and cosine of each angle once, in LDS, while the first vectors of q and k
+// are on their way.  Where a token's heads are neighbours in memory the tile is
+// all heads of one token (or of a few, if they are small); where a head's tokens
+// are, it is a run of tokens of some heads, so that a workgroup reads and writes
+// long pieces of memory and shares few lines with others.  position * frequency is formed in 64 bits and reduced to a
 // fraction of a turn there: a float32 angle is off by 0.03 rad at position
 // 500 000.  The fraction, its sine and cosine and the rotation are float32.
 #include "row_group.h"
@@ -16,6 +19,10 @@ namespace sa {
 constexpr int kRotBlock = 512;       // most threads of a workgroup
 constexpr int kRotMaxPairs = 512;    // most pairs a head
 constexpr int kRotTable = 1024;      // angles a workgroup holds
+// Units that a thread has on their way at once: two where their rotation needs
+// little else ([4, 2048, 40, 128] bf16 HALF: 31.5 us with one, 29.4 with two; INTERLEAVED
+// the same with both).
+constexpr int rot_units(bool half) { return half ? 2 : 1; }
 
 struct RotTensor {
   const void* in;
@@ -32,46 +39,63 @@ struct RotArgs {
   int64_t ps[2], offset;
   int32_t first, tokens;   // the tokens [first, tokens)
   int32_t dim, rotary;
-  int32_t per;             // tokens a workgroup
+  int32_t per, heads;      // tokens and heads (of q, then k) of a workgroup's tile
   int32_t slots;           // heads of q and k together
+  int32_t head_major;      // a tile's vectors go head by head, not token by token
   int32_t turn_units;      // vectors (HALF: pairs of vectors) of a head's rotated part
   int32_t units;           // and with those of its copied part
   int32_t pos64, inverse;
   float scale;
-  FastDiv seq, by_token, by_unit;  // token -> (batch, seq); thread's unit -> token, head, unit of the head
+  FastDiv seq, by_unit, by_inner;  // token -> (batch, seq); a thread's vector -> its place in a head, token and head
 };
 
-// One unit of a head: V elements of the rotated part (HALF: V pairs), or of the copied part.
-template <typename T, bool HALF> struct RotUnit {
+// One unit of a head: V elements of the rotated part (HALF: V pairs), or of the
+// copied part.  A part's last vector is moved back to its end and does some
+// elements twice, with the same values; in place, where another thread may have
+// written them before, it goes element by element, as does a part shorter than a
+// vector.
+template <typename T, bool HALF, typename OFF> struct RotUnit {
   static constexpr int V = 16 / (int)sizeof(T);
   const T* in;
   T* out;
   int col, part;  // first element; the part's end
+  int tk;         // token of the tile
   bool turn, live;
   RowVec<T, V> a, b;
 
-  __device__ __forceinline__ void find(const RotArgs& g, uint32_t unit, int32_t token0) {
-    uint32_t tk, rest, slot, u;
-    g.by_token.divmod(unit, tk, rest);
-    g.by_unit.divmod(rest, slot, u);
+  __device__ __forceinline__ void find(const RotArgs& g, uint32_t unit, int32_t token0, int32_t slot0) {
+    uint32_t outer, inner, v, u;
+    g.by_unit.divmod(unit, v, u);
+    g.by_inner.divmod(v, outer, inner);
+    tk = (int)(g.head_major ? inner : outer);
+    const int32_t slot = slot0 + (int32_t)(g.head_major ? outer : inner);
     const int64_t token = (int64_t)token0 + tk;
-    live = (int)tk < g.per && token < g.tokens;
-    const bool second = (int)slot >= g.t[0].heads;
-    const RotTensor& t = g.t[second ? 1 : 0];
-    const int64_t head = (int64_t)slot - (second ? g.t[0].heads : 0);
+    const bool second = slot >= g.t[0].heads;
+    // chosen value by value: an indexed pointer would not be known to be global memory
+    auto of = [&](auto q, auto k) { return second ? k : q; };
+    const RotTensor &q = g.t[0], &k = g.t[1];
+    const OFF head = slot - (second ? q.heads : 0);
+    auto step = [&](int64_t sq, int64_t sk) { return second ? (OFF)sk : (OFF)sq; };
     turn = (int)u < g.turn_units;
-    live = live && (turn || t.copy);
+    live = token < g.tokens && slot < g.slots && (turn || of(q.copy, k.copy));
     uint32_t bi, si;
     g.seq.divmod((uint32_t)token, bi, si);
-    in = static_cast<const T*>(t.in) + bi * t.is[0] + si * t.is[1] + head * t.is[2];
-    out = static_cast<T*>(t.out) + bi * t.os[0] + si * t.os[1] + head * t.os[2];
+    const OFF ob = (OFF)bi, os = (OFF)si;
+    in = static_cast<const T*>(of(q.in, k.in)) +
+         (ob * step(q.is[0], k.is[0]) + os * step(q.is[1], k.is[1]) + head * step(q.is[2], k.is[2]));
+    out = static_cast<T*>(of(q.out, k.out)) +
+          (ob * step(q.os[0], k.os[0]) + os * step(q.os[1], k.os[1]) + head * step(q.os[2], k.os[2]));
+    int first;
     if (turn) {
+      first = 0;
       col = (int)u * V;
       part = HALF ? g.rotary / 2 : g.rotary;
     } else {
+      first = g.rotary;
       col = g.rotary + ((int)u - g.turn_units) * V;
       part = g.dim;
     }
+    if (col + V > part && part - first >= V && in != out) col = part - V;
   }
   __device__ __forceinline__ void load(const RotArgs& g) {
     if (!live) return;
@@ -107,18 +131,28 @@ template <typename T, bool HALF> struct RotUnit {
   }
 };
 
-template <typename T, bool HALF>
+// OFF: the type of offsets within a tensor.  A 64-bit product is four 32-bit ones, each
+// of a quarter of the rate; with six of them a vector they bounded the kernel
+// ([2, 4096, 64, 192] bf16, interleaved: 103 us, 79 with 32-bit offsets).
+template <typename T, bool HALF, typename OFF>
 __global__ void __launch_bounds__(kRotBlock) k_rotary(RotArgs g) {
   __shared__ float2 cs[kRotTable];
   const int32_t token0 = g.first + (int32_t)blockIdx.x * g.per;
-  const uint32_t all = (uint32_t)(g.per * g.slots * g.units);
+  const int32_t slot0 = (int32_t)blockIdx.y * g.heads;
+  const uint32_t all = (uint32_t)(g.per * g.heads * g.units);
   const int pairs = g.rotary / 2;
-  RotUnit<T, HALF> w;
+  constexpr int U = rot_units(HALF);
+  RotUnit<T, HALF, OFF> w[U];
   uint32_t unit = threadIdx.x;
-  if (unit < all) {
-    w.find(g, unit, token0);
-    w.load(g);
-  }
+  auto request = [&]() {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      w[i].find(g, unit + i * blockDim.x, token0, slot0);
+      if (U > 1) w[i].live = w[i].live && unit + i * blockDim.x < all;
+      w[i].load(g);
+    }
+  };
+  if (unit < all) request();
   for (int i = threadIdx.x; i < g.per * pairs; i += blockDim.x) {
     const int tk = i / pairs;
     const int32_t token = token0 + tk;
@@ -137,15 +171,11 @@ __global__ void __launch_bounds__(kRotBlock) k_rotary(RotArgs g) {
     }
   }
   __syncthreads();
-  for (; unit < all; ) {
-    uint32_t tk, rest;
-    g.by_token.divmod(unit, tk, rest);
-    w.store(g, cs + tk * pairs);
-    unit += blockDim.x;
-    if (unit < all) {
-      w.find(g, unit, token0);
-      w.load(g);
-    }
+  while (unit < all) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) w[i].store(g, cs + w[i].tk * pairs);
+    unit += U * blockDim.x;
+    if (unit < all) request();
   }
 }
 
@@ -187,23 +217,54 @@ template <typename T> int rot_launch(const supa_amd_rotary_desc& d, hipStream_t 
   a.scale = (float)d.scale;
   const int64_t per_token = slots * a.units;
   if (per_token >= (int64_t(1) << 31)) return SUPA_AMD_ELAYOUT;
-  // tokens of few heads share a workgroup of 256 threads; a token of many takes
-  // up to 512 threads, as many rounds of them as it needs, evenly filled
-  const int64_t fit = std::min<int64_t>(256 / per_token, kRotTable / (d.rotary / 2));
-  a.per = (int32_t)std::max<int64_t>(1, std::min<int64_t>(fit, a.tokens));
-  const int64_t all = a.per * per_token, rounds = (all + kRotBlock - 1) / kRotBlock;
-  const int block = (int)((((all + rounds - 1) / rounds) + 63) / 64 * 64);
+  const int64_t table = kRotTable / (d.rotary / 2);  // tokens whose angles fit
+  // by the larger tensor's output: its tokens lie closer together than its heads
+  const RotTensor& large = a.t[a.t[1].heads > a.t[0].heads ? 1 : 0];
+  a.head_major = large.heads > 1 && d.seq > 1 && large.os[1] < large.os[2];
+  if (a.head_major) {
+    // a run of tokens, and as many heads as fill four steps of 512 threads:
+    // [4, 40, 2048, 128] bf16 38 -> 33 us
+    a.per = (int32_t)std::min<int64_t>({table, 32, a.tokens});
+    a.heads = (int32_t)std::min<int64_t>(slots, std::max<int64_t>(1, 4 * kRotBlock / (a.per * a.units)));
+  } else {
+    // tokens of few heads share a workgroup of 256 threads
+    a.per = (int32_t)std::max<int64_t>(1, std::min<int64_t>({256 / per_token, table, a.tokens}));
+    a.heads = (int32_t)slots;
+  }
+  // up to 512 threads, evenly filled
+  const int64_t all = (int64_t)a.per * a.heads * a.units, each = (all + rot_units(half) - 1) / rot_units(half);
+  const int64_t steps = (each + kRotBlock - 1) / kRotBlock;
+  const int block = (int)((((each + steps - 1) / steps) + 63) / 64 * 64);
   a.seq = FastDiv((uint32_t)d.seq);
-  a.by_token = FastDiv((uint32_t)per_token);
   a.by_unit = FastDiv((uint32_t)a.units);
-  const int64_t slab = (int64_t(1) << 31) / kRotBlock * a.per;  // HIP: fewer than 2^32 threads a launch
+  a.by_inner = FastDiv((uint32_t)(a.head_major ? a.per : a.heads));
+  // whether every offset of q and k, and those formed of the tile's places past
+  // the last token or head, fits 32 bits
+  bool narrow = true;
+  for (const RotTensor& t : a.t)
+    for (const int64_t* step : {t.is, t.os}) {
+      const double most = std::fabs((double)step[0]) * (double)(d.batch + a.per) +
+                          std::fabs((double)step[1]) * (double)d.seq +
+                          std::fabs((double)step[2]) * (double)(t.heads + a.heads);
+      narrow = narrow && most < 2147483648.0;
+    }
+  const unsigned groups = (unsigned)((slots + a.heads - 1) / a.heads);
+  if (groups > 65535) return SUPA_AMD_ELAYOUT;
+  const int64_t slab = (int64_t(1) << 31) / kRotBlock / groups * a.per;  // HIP: fewer than 2^32 threads a launch
   const int64_t tokens = a.tokens;
   for (int64_t first = 0; first < tokens; first += slab) {
     a.first = (int32_t)first;
     a.tokens = (int32_t)std::min(tokens, first + slab);
     const unsigned blocks = (unsigned)((a.tokens - first + a.per - 1) / a.per);
-    if (half) k_rotary<T, true><<<blocks, block, 0, st>>>(a);
-    else k_rotary<T, false><<<blocks, block, 0, st>>>(a);
+    auto go = [&](auto h, auto* off) {
+      k_rotary<T, h.value, std::remove_pointer_t<decltype(off)>><<<dim3(blocks, groups), block, 0, st>>>(a);
+    };
+    auto offsets = [&](auto h) {
+      if (narrow) go(h, (int32_t*)nullptr);
+      else go(h, (int64_t*)nullptr);
+    };
+    if (half) offsets(std::true_type{});
+    else offsets(std::false_type{});
     const int rc = launch_status();
     if (rc) return rc;
   }
