@@ -850,12 +850,14 @@ inline RnPlan rn_plan(const supa_amd_residual_norm_desc& d) {
   p.section = d.gate && !p.elementwise ? d.gate_period : d.rows;
   p.sections = d.rows / p.section;
   const int64_t steps = (p.section + at_once - 1) / at_once;
-  p.cuts = (int32_t)std::min<int64_t>(steps, (kRnParts + p.sections - 1) / p.sections);
-  // Rows of whole 128-byte lines are dealt out in turn, so that the chip works on
-  // neighbouring rows at any time ([8192, 8192] bf16 164 -> 151 us, [8192, 4096] 89 ->
-  // 85); of others a workgroup takes consecutive ones, whose shared lines it
-  // writes itself ([6006, 2047] float32 72 us, dealt out 95).
-  if (d.width * dtype_size(d.dtype) % 128 == 0) {
+  // no more workgroups than CUs where that can be: one left over would run alone
+  // ([6, 1024, 2048] float32 in 258 workgroups 84 us, in 252 67)
+  p.cuts = (int32_t)std::min<int64_t>(steps, std::max<int64_t>(1, kRnParts / p.sections));
+  // Rows of one section are dealt out in turn, so that the chip works on
+  // neighbouring rows at any time ([8192, 8192] bf16 170 -> 151 us, [8192, 4096] 82 ->
+  // 79, [20000, 1500] float32 127 -> 109); of several sections, which lie apart in any case, a
+  // workgroup takes consecutive rows ([8, 1024, 4096] bf16 86 us, dealt out 92).
+  if (p.sections == 1) {
     p.first = at_once;
     p.step = p.cuts * at_once;
     p.span = p.section;
