@@ -600,10 +600,7 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
 }
 
 at::Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double ord, bool error_if_nonfinite) {
-  for (const at::Tensor& g : grads)
-    TORCH_CHECK(!(at::GradMode::is_enabled() && g.requires_grad()), "clip_grad_norm_: a tensor of the list needs a "
-                "gradient; the scaling in place has none");
-  const at::AutoDispatchBelowAutograd below;
+  const at::AutoDispatchBelowAutograd below;  // the scaling is no part of a graph, as under no_grad
   at::Tensor norm = clip_grad_norm_(grads, max_norm, ord, error_if_nonfinite);
   for (const at::Tensor& g : grads) written(g);
   return norm;

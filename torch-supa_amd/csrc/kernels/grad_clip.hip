@@ -28,9 +28,12 @@ constexpr int kClipBlock = 256;
 constexpr int kClipNormVecs = 16, kClipScaleVecs = 8;
 constexpr int64_t kClipFold = 512;  // most partials that the scaling adds itself
 
+// Tensors of every type share a table: the type, in the low bits of `sized`, is
+// one for a workgroup (bfloat16 matrices beside float32 vectors: two launches of five
+// less, 50 us -> 43).
 struct ClipTable {
   void* p[kClipTensors];
-  int64_t numel[kClipTensors];
+  int64_t sized[kClipTensors];  // elements x 4 + clip_type
   uint32_t chunk_start[kClipTensors + 1];
   int32_t ntensors;
   uint32_t bucket_shift;
@@ -38,6 +41,27 @@ struct ClipTable {
 };
 
 template <typename T> constexpr int64_t clip_chunk(int vecs) { return (int64_t)kClipBlock * vecs * (16 / (int64_t)sizeof(T)); }
+
+inline int clip_type(int dtype) {
+  return dtype == SUPA_AMD_F32 ? 0 : dtype == SUPA_AMD_BF16 ? 1 : dtype == SUPA_AMD_F16 ? 2 : 3;
+}
+
+// fn(tensor, lo, hi) for the workgroup's chunk, with the tensor's type.
+template <int VECS, typename F> __device__ __forceinline__ void clip_chunk_of(const ClipTable& tab, F&& fn) {
+  const int k = find_tensor(tab, blockIdx.x);
+  const int64_t c = blockIdx.x - tab.chunk_start[k], n = tab.sized[k] >> 2;
+  auto go = [&](auto* x) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    const int64_t lo = c * clip_chunk<T>(VECS);
+    fn(x, lo, lo + clip_chunk<T>(VECS) < n ? lo + clip_chunk<T>(VECS) : n);
+  };
+  switch (tab.sized[k] & 3) {
+    case 0: return go(static_cast<float*>(tab.p[k]));
+    case 1: return go(static_cast<bf16*>(tab.p[k]));
+    case 2: return go(static_cast<f16*>(tab.p[k]));
+    default: return go(static_cast<double*>(tab.p[k]));
+  }
+}
 
 constexpr int kOrdInf = 0;
 template <int ORD> __device__ __forceinline__ double clip_term(double acc, double x) {
@@ -62,24 +86,25 @@ template <int ORD, int BS> __device__ __forceinline__ double clip_block(double v
   return v;
 }
 
-template <typename T, int ORD>
+template <int ORD>
 __global__ void __launch_bounds__(kClipBlock) k_clip_partial(ClipTable tab, double* __restrict__ part) {
-  constexpr int V = 16 / sizeof(T);
-  const MtaRange r = mta_range<clip_chunk<T>(kClipNormVecs)>(tab);
-  const T* x = static_cast<const T*>(tab.p[r.k]);
   double acc = 0.0;
-  int64_t start = r.lo;
-  if (aligned(x, 16)) {
-    const int64_t nv = (r.hi - r.lo) / V;
+  clip_chunk_of<kClipNormVecs>(tab, [&](auto* x, int64_t lo, int64_t hi) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    constexpr int V = 16 / sizeof(T);
+    int64_t start = lo;
+    if (aligned(x, 16)) {
+      const int64_t nv = (hi - lo) / V;
 #pragma unroll 4
-    for (int64_t v = threadIdx.x; v < nv; v += kClipBlock) {
-      const Vec<T, V> w = ld_stream(reinterpret_cast<const Vec<T, V>*>(x + r.lo + v * V));
+      for (int64_t v = threadIdx.x; v < nv; v += kClipBlock) {
+        const Vec<T, V> w = ld_stream(reinterpret_cast<const Vec<T, V>*>(x + lo + v * V));
 #pragma unroll
-      for (int i = 0; i < V; ++i) acc = clip_term<ORD>(acc, (double)to_arith(w.v[i]));
+        for (int i = 0; i < V; ++i) acc = clip_term<ORD>(acc, (double)to_arith(w.v[i]));
+      }
+      start = lo + nv * V;
     }
-    start = r.lo + nv * V;
-  }
-  for (int64_t e = start + threadIdx.x; e < r.hi; e += kClipBlock) acc = clip_term<ORD>(acc, (double)to_arith(x[e]));
+    for (int64_t e = start + threadIdx.x; e < hi; e += kClipBlock) acc = clip_term<ORD>(acc, (double)to_arith(x[e]));
+  });
   acc = clip_block<ORD, kClipBlock>(acc);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
 }
@@ -119,11 +144,9 @@ struct ClipNorm {
 };
 
 constexpr int kOrdGiven = 3;  // the norm is in ws[0]
-template <typename T, int ORD>
+template <int ORD>
 __global__ void __launch_bounds__(kClipBlock)
 k_clip_scale(ClipTable tab, ClipNorm from, double max_norm) {
-  using A = opmath_t<T>;
-  constexpr int V = 16 / sizeof(T), U = kClipScaleVecs;
   double norm;
   if constexpr (ORD == kOrdGiven) {
     norm = from.ws[0];
@@ -139,63 +162,65 @@ k_clip_scale(ClipTable tab, ClipNorm from, double max_norm) {
   }
   const double q = max_norm / (norm + 1e-6);
   if (q >= 1.0) return;  // a NaN goes on
-  const A c = (A)q;
-  const MtaRange r = mta_range<clip_chunk<T>(U)>(tab);
-  T* x = static_cast<T*>(tab.p[r.k]);
-  auto scaled = [&](Vec<T, V> w) {
+  clip_chunk_of<kClipScaleVecs>(tab, [&](auto* x, int64_t lo, int64_t hi) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    using A = opmath_t<T>;
+    constexpr int V = 16 / sizeof(T), U = kClipScaleVecs;
+    const A c = (A)q;
+    auto scaled = [&](Vec<T, V> w) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) w.v[i] = from_arith<T>((A)to_arith(w.v[i]) * c);
-    return w;
-  };
-  int64_t start = r.lo;
-  if (aligned(x, 16)) {
-    Vec<T, V>* at = reinterpret_cast<Vec<T, V>*>(x + r.lo) + threadIdx.x;
-    if (r.hi - r.lo == clip_chunk<T>(U)) {
-      Vec<T, V> w[U];
+      for (int i = 0; i < V; ++i) w.v[i] = from_arith<T>((A)to_arith(w.v[i]) * c);
+      return w;
+    };
+    int64_t start = lo;
+    if (aligned(x, 16)) {
+      Vec<T, V>* at = reinterpret_cast<Vec<T, V>*>(x + lo) + threadIdx.x;
+      if (hi - lo == clip_chunk<T>(U)) {
+        Vec<T, V> w[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = ld_stream(at + u * kClipBlock);
+        for (int u = 0; u < U; ++u) w[u] = ld_stream(at + u * kClipBlock);
 #pragma unroll
-      for (int u = 0; u < U; ++u) st_stream(at + u * kClipBlock, scaled(w[u]));
-      return;
+        for (int u = 0; u < U; ++u) st_stream(at + u * kClipBlock, scaled(w[u]));
+        return;
+      }
+      const int64_t nv = (hi - lo) / V;
+      for (int64_t v = threadIdx.x; v < nv; v += kClipBlock, at += kClipBlock) st_stream(at, scaled(ld_stream(at)));
+      start = lo + nv * V;
     }
-    const int64_t nv = (r.hi - r.lo) / V;
-    for (int64_t v = threadIdx.x; v < nv; v += kClipBlock, at += kClipBlock) st_stream(at, scaled(ld_stream(at)));
-    start = r.lo + nv * V;
-  }
-  for (int64_t e = start + threadIdx.x; e < r.hi; e += kClipBlock) x[e] = from_arith<T>((A)to_arith(x[e]) * c);
+    for (int64_t e = start + threadIdx.x; e < hi; e += kClipBlock) x[e] = from_arith<T>((A)to_arith(x[e]) * c);
+  });
 }
 
-// Calls fn(tab, chunks, T*) for tables of at most kClipTensors tensors, those
-// of one dtype together, in chunks of `vecs` vectors a thread; empty tensors are left out.
+// Chunks of a tensor, of `vecs` vectors a thread.
+inline int64_t clip_chunks(int64_t numel, int dtype, int vecs) {
+  const int64_t chunk = (int64_t)kClipBlock * vecs * (16 / dtype_size(dtype));
+  return (numel + chunk - 1) / chunk;
+}
+
+// Calls fn(tab, chunks) for tables of at most kClipTensors tensors; empty
+// tensors are left out.
 template <typename F>
 int clip_tables(int vecs, int32_t n, void* const* p, const int64_t* numel, const int32_t* dtypes, F&& fn) {
-  for (const int dtype : {SUPA_AMD_F32, SUPA_AMD_BF16, SUPA_AMD_F16, SUPA_AMD_F64}) {
-    const int rc = with_mta_storage(dtype, [&](auto* tag) -> int {
-      using T = std::remove_pointer_t<decltype(tag)>;
-      int i = 0;
-      while (i < n) {
-        ClipTable tab{};
-        int64_t chunks = 0;
-        int nt = 0;
-        for (; i < n && nt < kClipTensors; ++i) {
-          if (dtypes[i] != dtype || numel[i] == 0) continue;
-          const int64_t c = (numel[i] + clip_chunk<T>(vecs) - 1) / clip_chunk<T>(vecs);
-          if (c >= (int64_t(1) << 24)) return SUPA_AMD_ELAYOUT;
-          if (chunks + c >= (int64_t(1) << 24)) break;  // HIP: fewer than 2^32 threads a launch
-          tab.p[nt] = p ? p[i] : nullptr;
-          tab.numel[nt] = numel[i];
-          tab.chunk_start[nt++] = (uint32_t)chunks;
-          chunks += c;
-        }
-        if (nt == 0) continue;
-        tab.chunk_start[nt] = (uint32_t)chunks;
-        tab.ntensors = nt;
-        mta_index(tab, (uint32_t)chunks);
-        const int r = fn(tab, (uint32_t)chunks, tag);
-        if (r) return r;
-      }
-      return SUPA_AMD_OK;
-    });
+  int i = 0;
+  while (i < n) {
+    ClipTable tab{};
+    int64_t chunks = 0;
+    int nt = 0;
+    for (; i < n && nt < kClipTensors; ++i) {
+      const int64_t c = clip_chunks(numel[i], dtypes[i], vecs);
+      if (c == 0) continue;
+      if (c >= (int64_t(1) << 24)) return SUPA_AMD_ELAYOUT;
+      if (chunks + c >= (int64_t(1) << 24)) break;  // HIP: fewer than 2^32 threads a launch
+      tab.p[nt] = p[i];
+      tab.sized[nt] = numel[i] * 4 + clip_type(dtypes[i]);
+      tab.chunk_start[nt++] = (uint32_t)chunks;
+      chunks += c;
+    }
+    if (nt == 0) continue;
+    tab.chunk_start[nt] = (uint32_t)chunks;
+    tab.ntensors = nt;
+    mta_index(tab, (uint32_t)chunks);
+    const int rc = fn(tab, (uint32_t)chunks);
     if (rc) return rc;
   }
   return SUPA_AMD_OK;
@@ -228,9 +253,8 @@ template <typename F> int clip_ord(double ord, F&& go) {
 
 template <int ORD> int clip_partials(const ClipList& l, int64_t& parts) {
   parts = 0;
-  return clip_tables(kClipNormVecs, l.n, l.p, l.numel, l.dtypes, [&](const ClipTable& tab, uint32_t chunks, auto* tag) -> int {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    k_clip_partial<T, ORD><<<chunks, kClipBlock, 0, l.st>>>(tab, l.ws + 1 + parts);
+  return clip_tables(kClipNormVecs, l.n, l.p, l.numel, l.dtypes, [&](const ClipTable& tab, uint32_t chunks) -> int {
+    k_clip_partial<ORD><<<chunks, kClipBlock, 0, l.st>>>(tab, l.ws + 1 + parts);
     parts += chunks;
     return launch_status();
   });
@@ -242,9 +266,8 @@ template <int ORD> int clip_norm(const ClipList& l, int64_t parts, void* out, in
 }
 
 template <int ORD> int clip_scale(const ClipList& l, ClipNorm from, double max_norm) {
-  return clip_tables(kClipScaleVecs, l.n, l.p, l.numel, l.dtypes, [&](const ClipTable& tab, uint32_t chunks, auto* tag) -> int {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    k_clip_scale<T, ORD><<<chunks, kClipBlock, 0, l.st>>>(tab, from, max_norm);
+  return clip_tables(kClipScaleVecs, l.n, l.p, l.numel, l.dtypes, [&](const ClipTable& tab, uint32_t chunks) -> int {
+    k_clip_scale<ORD><<<chunks, kClipBlock, 0, l.st>>>(tab, from, max_norm);
     from.out = nullptr;  // the first launch writes it
     return launch_status();
   });
@@ -274,8 +297,7 @@ int64_t supa_amd_grad_norm_workspace_bytes(int32_t n, const int64_t* numel, cons
   for (int32_t i = 0; i < n; ++i) {
     if (numel[i] < 0) return SUPA_AMD_EINVAL;
     if (!dtype_is_floating(dtypes[i])) return SUPA_AMD_EDTYPE;
-    const int64_t chunk = (int64_t)kClipBlock * kClipNormVecs * (16 / dtype_size(dtypes[i]));
-    const int64_t c = (numel[i] + chunk - 1) / chunk;
+    const int64_t c = clip_chunks(numel[i], dtypes[i], kClipNormVecs);
     if (c >= (int64_t(1) << 24)) return SUPA_AMD_ELAYOUT;
     parts += c;
   }

@@ -161,5 +161,4 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    with torch.no_grad():
-        return torch.ops.supa.clip_grad_norm_(grads, float(max_norm), float(norm_type), bool(error_if_nonfinite))
+    return torch.ops.supa.clip_grad_norm_(grads, float(max_norm), float(norm_type), bool(error_if_nonfinite))
