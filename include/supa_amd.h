@@ -838,15 +838,15 @@ typedef struct supa_amd_residual_norm_desc {
 } supa_amd_residual_norm_desc;
 
 /* h ([rows, width] of residual_dtype) and y ([rows, width] of dtype; NULL
- * exactly when norm is NONE), both contiguous.  stats, when given, receives
- * four floats a row for the backward: the post norm's mean and reciprocal
+ * exactly when norm is NONE), both contiguous, neither overlapping an input.  stats, when given, receives
+ * four floats a row (16-byte aligned) for the backward: the post norm's mean and reciprocal
  * deviation, then the norm's (0 for a mean or a norm that is not there). */
 int supa_amd_residual_norm_forward(const supa_amd_residual_norm_desc* d, void* h, void* y, float* stats, void* stream);
 
 /* The gradients from grad_h ([rows, width] of residual_dtype, or NULL for
  * zeros) and grad_y ([rows, width] of dtype, or NULL), contiguous, and the
  * forward's stats.  Every output may be NULL.  grad_x is of dtype,
- * grad_residual of residual_dtype, both contiguous; grad_gate, grad_post_weight,
+ * grad_residual of residual_dtype, both contiguous, no output overlapping an input; grad_gate, grad_post_weight,
  * grad_post_bias, grad_weight and grad_bias of param_dtype in their
  * parameter's shape, summed in float32 in an order that only the sizes fix.
  * h, when given, is the forward's h and takes the place of x and residual
@@ -906,7 +906,7 @@ int supa_amd_rotary(const supa_amd_rotary_desc* d, void* stream);
  * in place, rounded once to the tensor's type.  A factor of 1 writes nothing.
  * A NaN norm makes every element NaN, an infinite one zero (and the infinite
  * elements NaN).  norm_out is one element of norm_dtype (f32 or f64).  The
- * tensors must not overlap.
+ * tensors must not overlap; the workspace is 8-byte aligned.
  * supa_amd_grad_norm writes the norm alone, supa_amd_grad_scale scales by a
  * norm that the former left in the same workspace; supa_amd_clip_grad_norm is
  * the two together.  Replaces the reference's _foreach_norm, stack,

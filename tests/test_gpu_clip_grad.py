@@ -152,7 +152,7 @@ def test_refusals(supa):
     for grads, args, text in [
         ([x], (-1.0, 2.0, False), "max_norm"), ([x], (math.nan, 2.0, False), "max_norm"), ([x], (1.0, 3.0, False), "norm"),
         ([x, x], (1.0, 2.0, False), "share memory"), ([x[0], x.reshape(-1)[3:]], (1.0, 2.0, False), "share memory"),
-        ([x, x.cpu()], (1.0, 2.0, False), "supa"), ([x.long()], (1.0, 2.0, False), "floating"),
+        ([x[:, :2], x[:, :2]], (1.0, 2.0, False), "share memory"), ([x, x.cpu()], (1.0, 2.0, False), "supa"), ([x.long()], (1.0, 2.0, False), "floating"),
         ([x[:1].expand(4, 4)], (1.0, 2.0, False), None),
     ]:
         before = x.cpu()

@@ -211,6 +211,8 @@ def test_refusals(supa):
         put(q[:, :, :2], q[:, :, 1:], f)
     with pytest.raises(RuntimeError, match="overlap"):
         put(q[:, :4], q[:, 1:], f)
+    with pytest.raises(RuntimeError, match="overlap"):  # windows that slide over each other
+        put(torch.ones(100, device="supa").as_strided((4, 5, 1, 8), (10, 11, 8, 1)), None, f)
     with pytest.raises(RuntimeError, match="contiguous"):
         put(torch.ones(2, 5, 8, 3, device="supa").transpose(2, 3), None, f)
     with pytest.raises(RuntimeError):

@@ -79,6 +79,8 @@ def test_residual_norm_other_refusals(lib):
         return bwd(ctypes.byref(desc), vp(h), vp(FAKE), vp(FAKE), vp(stats), vp(FAKE), vp(FAKE), vp(gate), vp(pw), vp(pb),
                    vp(w), vp(b), vp(ws), i64(size), None)
 
+    assert back(stats=FAKE + 8) == EINVAL and back(ws=FAKE + 2) == EINVAL  # alignment
+    assert fwd(ctypes.byref(d), vp(FAKE), vp(FAKE), vp(FAKE + 4), None) == EINVAL
     assert back(ws=None) == EWORKSPACE and back(size=need - 1) == EWORKSPACE
     assert back(stats=None) == EINVAL and back(gate=FAKE) == EINVAL and back(pw=FAKE) == EINVAL
     assert back(b=FAKE) == EINVAL  # the bias of an RMS norm
@@ -126,6 +128,7 @@ def test_clip_refuses(lib):
     assert call(order=3.0) == EINVAL and call(limit=-1.0) == EINVAL and call(limit=math.nan) == EINVAL
     assert call(out=None) == EINVAL and call(out_type=BF16) == EDTYPE and call(count=-1) == EINVAL
     assert call(ptrs=(vp * 2)(FAKE, None)) == EINVAL and call(dtypes=(i32 * 2)(F32, I64)) == EDTYPE
+    assert call(ws=FAKE + 4) == EINVAL and lib.supa_amd_grad_scale(2, p, n, t, dbl(1.0), vp(FAKE + 4), i64(8), None) == EINVAL
     assert call(ws=None) == EWORKSPACE and call(size=need - 1) == EWORKSPACE
     assert lib.supa_amd_grad_scale(2, p, n, t, dbl(-1.0), vp(FAKE), i64(8), None) == EINVAL
     assert lib.supa_amd_grad_scale(2, p, n, t, dbl(1.0), None, i64(8), None) == EWORKSPACE

@@ -418,8 +418,23 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const O
   return {qo, ko};
 }
 
-// Whether q and k, which interleave in memory, share no element: k's part of
-// every token (or of every sample) lies beside q's.
+// Whether blocks of `block` elements, one at every index of the dims before
+// `dims`, keep apart: each dim steps over all that the smaller steps reach.
+bool apart(const at::Tensor& t, int64_t dims, int64_t block) {
+  std::vector<std::pair<int64_t, int64_t>> steps;  // stride, size
+  for (int64_t i = 0; i < dims; ++i)
+    if (t.size(i) > 1) steps.emplace_back(t.stride(i), t.size(i));
+  std::sort(steps.begin(), steps.end());
+  for (const auto& [stride, size] : steps) {
+    if (stride < block) return false;
+    block += (size - 1) * stride;
+  }
+  return true;
+}
+
+// Whether q and k share no element: over some of the trailing dims k lies beside
+// q, and the dims before step alike from one such pair to the next (q and k of
+// a packed projection, token by token or sample by sample).
 bool beside(const at::Tensor& q, const at::Tensor& k) {
   const int64_t nd = q.dim();
   // elements from the first to behind the last, over the dims from `from` on
@@ -428,20 +443,14 @@ bool beside(const at::Tensor& q, const at::Tensor& k) {
     for (int64_t i = from; i < nd; ++i) e += (t.size(i) - 1) * t.stride(i);
     return e;
   };
-  const int64_t apart = (static_cast<const char*>(k.data_ptr()) - static_cast<const char*>(q.data_ptr())) /
+  const int64_t shift = (static_cast<const char*>(k.data_ptr()) - static_cast<const char*>(q.data_ptr())) /
                         (int64_t)q.element_size();
-  for (int64_t from = 0; from <= nd - 2; ++from) {  // the dims before `from` step alike
+  const int64_t gap = std::abs(shift);
+  for (int64_t from = 0; from <= nd - 2; ++from) {
     bool alike = true;
-    int64_t step = INT64_MAX;
-    for (int64_t i = 0; i < from; ++i) {
-      if (q.size(i) == 1) continue;
-      alike = alike && q.stride(i) == k.stride(i);
-      step = std::min(step, q.stride(i));
-    }
-    const int64_t first = apart >= 0 ? extent(q, from) : extent(k, from);
-    const int64_t second = apart >= 0 ? extent(k, from) : extent(q, from);
-    const int64_t gap = std::abs(apart);
-    if (alike && first <= gap && (step == INT64_MAX || gap + second <= step)) return true;
+    for (int64_t i = 0; i < from; ++i) alike = alike && (q.size(i) == 1 || q.stride(i) == k.stride(i));
+    const int64_t first = extent(shift >= 0 ? q : k, from), second = extent(shift >= 0 ? k : q, from);
+    if (alike && first <= gap && apart(q, from, gap + second)) return true;
   }
   return false;
 }
@@ -454,7 +463,7 @@ void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& freq
   for (const at::Tensor* t : {(const at::Tensor*)&q, given(k) ? &*k : nullptr}) {
     if (!t || t->numel() == 0) continue;
     TORCH_CHECK(t->size(-1) == 1 || t->stride(-1) == 1, op, ": expected heads whose elements are contiguous");
-    at::assert_no_internal_overlap(*t);
+    TORCH_CHECK(apart(*t, t->dim() - 1, t->size(-1)), op, ": expected a tensor whose heads do not overlap in memory");
   }
   if (given(k) && q.numel() > 0 && k->numel() > 0)
     TORCH_CHECK(beside(q, *k), op, ": q and k overlap in memory");
@@ -537,7 +546,8 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   TORCH_CHECK(ord == 1.0 || ord == 2.0 || ord == HUGE_VAL, op, ": expected the norm 1, 2 or inf, got ", ord);
   const c10::Device device = grads[0].device();
   const size_t n = grads.size();
-  std::vector<at::Tensor> copies;  // of tensors that are not dense, in the list's order
+  std::vector<at::Tensor> copies;         // of tensors that are not dense, in the list's order
+  std::vector<const void*> copied;        // and where those begin
   std::vector<void*> p(n);
   std::vector<int64_t> numel(n);
   std::vector<int32_t> dtypes(n);
@@ -558,6 +568,7 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
       at::assert_no_internal_overlap(g);
       x = g.contiguous();
       copies.push_back(x);
+      copied.push_back(g.data_ptr());
     } else if (g.numel() > 0) {
       const char* at = static_cast<const char*>(g.data_ptr());
       spans.emplace_back(at, at + g.numel() * (int64_t)g.element_size());
@@ -569,6 +580,9 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)
     TORCH_CHECK(spans[i - 1].second <= spans[i].first, op, ": two of the tensors share memory");
+  std::sort(copied.begin(), copied.end());
+  TORCH_CHECK(std::adjacent_find(copied.begin(), copied.end()) == copied.end(), op,
+              ": two of the tensors share memory");
   const auto dev = device.index();
   const int64_t ws_bytes = supa_amd_grad_norm_workspace_bytes((int32_t)n, numel.data(), dtypes.data());
   TORCH_CHECK(ws_bytes >= 0, op, ": ", supa_amd_status_string((int)ws_bytes));

@@ -278,6 +278,7 @@ int clip_norm_check(int32_t n, const void* const* tensors, const int64_t* numel,
                     const void* norm_out, int32_t norm_dtype, const void* workspace, int64_t ws_bytes) {
   const int rc = clip_check(n, tensors, numel, dtypes);
   if (rc) return rc;
+  if (!aligned(workspace, 8)) return SUPA_AMD_EINVAL;
   if (!norm_out || (ord != 1.0 && ord != 2.0 && ord != HUGE_VAL)) return SUPA_AMD_EINVAL;
   if (norm_dtype != SUPA_AMD_F32 && norm_dtype != SUPA_AMD_F64) return SUPA_AMD_EDTYPE;
   const int64_t need = supa_amd_grad_norm_workspace_bytes(n, numel, dtypes);
@@ -321,7 +322,7 @@ int supa_amd_grad_scale(int32_t n, void* const* tensors, const int64_t* numel, c
                         const void* workspace, int64_t ws_bytes, void* stream) {
   const int rc = clip_check(n, tensors, numel, dtypes);
   if (rc) return rc;
-  if (!(max_norm >= 0.0)) return SUPA_AMD_EINVAL;
+  if (!(max_norm >= 0.0) || !aligned(workspace, 8)) return SUPA_AMD_EINVAL;
   if (!workspace || ws_bytes < 8) return SUPA_AMD_EWORKSPACE;
   const ClipList l{n, tensors, numel, dtypes, nullptr, static_cast<hipStream_t>(stream)};
   return clip_scale<kOrdGiven>(l, ClipNorm{static_cast<const double*>(workspace), 0, nullptr, 0}, max_norm);

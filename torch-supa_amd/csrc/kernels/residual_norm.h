@@ -753,21 +753,28 @@ __global__ void __launch_bounds__(64 * kRnSumWaves) k_residual_norm_sums(RnSums 
   }
 }
 
-// The threads a row and the elements a thread: the fewest threads that hold the row.
-template <typename F> int rn_shape(int64_t width, F&& go) {
+// The threads a row and the elements a thread, for an x of esize bytes an
+// element: the fewest threads that hold the row with 8 elements each; of float32
+// twice as many with one vector each where that helped ([6006, 2047] layer norms 41.6
+// us with two vectors, 39.3 with one; [8192, 4096] 86, 87; [262144, 72] 70, 76).
+template <int esize, typename F> int rn_fwd_shape(int64_t width, F&& go) {
   using std::integral_constant;
+  using E4 = integral_constant<int, 4>;
   using E8 = integral_constant<int, 8>;
   if (width <= 128) return go(integral_constant<int, 16>{}, E8{});
   if (width <= 256) return go(integral_constant<int, 32>{}, E8{});
   if (width <= 512) return go(integral_constant<int, 64>{}, E8{});
+  if constexpr (esize == 4) {
+    if (width <= 1024) return go(integral_constant<int, 256>{}, E4{});
+    if (width <= 2048) return go(integral_constant<int, 512>{}, E4{});
+  }
   if (width <= 1024) return go(integral_constant<int, 128>{}, E8{});
   if (width <= 2048) return go(integral_constant<int, 256>{}, E8{});
   if (width <= 4096) return go(integral_constant<int, 512>{}, E8{});
   if (width <= 8192) return go(integral_constant<int, 1024>{}, E8{});
   return go(integral_constant<int, 1024>{}, integral_constant<int, 16>{});
 }
-// The same for the backward of an x of esize bytes an element, whose threads need
-// more registers: one vector a thread up to 4096 elements ([16384, 1024] float32
+// The same for the backward, whose threads need more registers: one vector a thread up to 4096 elements ([16384, 1024] float32
 // 82 us with two, 73 with one), then 512 threads of 16 elements up to 8192.
 template <int esize, typename F> int rn_bwd_shape(int64_t width, F&& go) {
   using std::integral_constant;
@@ -850,8 +857,9 @@ inline RnPlan rn_plan(const supa_amd_residual_norm_desc& d) {
   p.section = d.gate && !p.elementwise ? d.gate_period : d.rows;
   p.sections = d.rows / p.section;
   const int64_t steps = (p.section + at_once - 1) / at_once;
-  // no more workgroups than CUs where that can be: one left over would run alone
-  // ([6, 1024, 2048] float32 in 258 workgroups 84 us, in 252 67)
+  // No more workgroups than CUs: one left over would run alone ([6, 1024, 2048] float32
+  // in 258 workgroups 84 us, in 252 67), and 160 CUs come near the memory's rate
+  // ([160, 64, 2048] bf16 in 160 workgroups 60 us, in 480 74).
   p.cuts = (int32_t)std::min<int64_t>(steps, std::max<int64_t>(1, kRnParts / p.sections));
   // Rows of one section are dealt out in turn, so that the chip works on
   // neighbouring rows at any time ([8192, 8192] bf16 170 -> 151 us, [8192, 4096] 82 ->
@@ -875,7 +883,7 @@ inline RnPlan rn_plan(const supa_amd_residual_norm_desc& d) {
 // The launches for one pair of types (residual_norm_*.hip).
 template <typename T, typename R>
 int rn_forward_t(const supa_amd_residual_norm_desc* d, const RnArgs& a, void* h, void* y, float* stats, hipStream_t st) {
-  return rn_shape(d->width, [&](auto G, auto E) -> int {
+  return rn_fwd_shape<sizeof(T)>(d->width, [&](auto G, auto E) -> int {
     constexpr int BS = G.value > 256 ? G.value : 256, PER = BS / G.value;
     constexpr int64_t kSlab = (int64_t(1) << 31) / BS * PER;  // HIP: fewer than 2^32 threads a launch
     for (int64_t r0 = 0; r0 < d->rows; r0 += kSlab) {

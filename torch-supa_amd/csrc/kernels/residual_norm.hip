@@ -44,6 +44,7 @@ int supa_amd_residual_norm_forward(const supa_amd_residual_norm_desc* d, void* h
   if (rc) return rc;
   if (d->rows == 0) return SUPA_AMD_OK;
   if (!d->x || !d->residual || !h || (d->norm != SUPA_AMD_NORM_NONE) != (y != nullptr)) return SUPA_AMD_EINVAL;
+  if (!aligned(stats, 16)) return SUPA_AMD_EINVAL;
   const RnArgs a = rn_args(*d);
   hipStream_t st = static_cast<hipStream_t>(stream);
   return rn_with(*d, [&](auto fns) { return fns.forward(d, a, h, y, stats, st); });
@@ -67,7 +68,7 @@ int supa_amd_residual_norm_backward(const supa_amd_residual_norm_desc* d, const 
   if ((post || d->gate) && h) return SUPA_AMD_EINVAL;
   if ((post || grad_gate || (norm && !h)) && !d->x) return SUPA_AMD_EINVAL;
   if (norm && !h && !d->residual) return SUPA_AMD_EINVAL;
-  if ((post || norm) && !stats) return SUPA_AMD_EINVAL;
+  if (((post || norm) && !stats) || !aligned(stats, 16) || !aligned(workspace, 4)) return SUPA_AMD_EINVAL;
   if ((!d->gate && grad_gate) || (!post && (grad_post_weight || grad_post_bias)) || (!norm && (grad_weight || grad_bias)))
     return SUPA_AMD_EINVAL;
   if ((d->post_norm != SUPA_AMD_NORM_LAYER && grad_post_bias) || (d->norm != SUPA_AMD_NORM_LAYER && grad_bias))

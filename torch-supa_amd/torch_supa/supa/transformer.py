@@ -11,6 +11,11 @@ import math
 
 import torch
 
+_residual_norm = torch.ops.supa.residual_norm.default
+_rotary_embedding = torch.ops.supa.rotary_embedding.default
+_rotary_embedding_ = torch.ops.supa.rotary_embedding_.default
+_clip_grad_norm_ = torch.ops.supa.clip_grad_norm_.default
+
 _NORMS = {None: 0, "none": 0, "rms": 1, "layer": 2}
 _LAYOUTS = {"half": False, "interleaved": True}
 
@@ -47,8 +52,8 @@ def residual_norm(x, residual, *, gate=None, residual_scale=1.0, post_norm=None,
 
     Differentiable (once) in every tensor.
     """
-    return torch.ops.supa.residual_norm(x, residual, gate, residual_scale, _norm_kind("post_norm", post_norm),
-                                        post_weight, post_bias, _norm_kind("norm", norm), weight, bias, eps)
+    return _residual_norm(x, residual, gate, residual_scale, _norm_kind("post_norm", post_norm), post_weight, post_bias,
+                          _norm_kind("norm", norm), weight, bias, eps)
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, original_length=None, slow=1.0,
@@ -132,7 +137,7 @@ def rotary_embedding(q, k, frequencies, positions=0, *, layout="half", scale=1.0
 
     Angles are formed in 64 bits.  Differentiable in q and k.  Returns (q, k)."""
     at, offset, interleaved = _rotary_args("rotary_embedding", positions, layout)
-    return torch.ops.supa.rotary_embedding(q, k, frequencies, at, offset, interleaved, scale, False)
+    return _rotary_embedding(q, k, frequencies, at, offset, interleaved, scale, False)
 
 
 def rotary_embedding_(q, k, frequencies, positions=0, *, layout="half", scale=1.0):
@@ -140,7 +145,7 @@ def rotary_embedding_(q, k, frequencies, positions=0, *, layout="half", scale=1.
     one projection (its heads contiguous in their last dim), and the elements
     that do not turn are not touched.  Returns (q, k)."""
     at, offset, interleaved = _rotary_args("rotary_embedding_", positions, layout)
-    torch.ops.supa.rotary_embedding_(q, k, frequencies, at, offset, interleaved, scale, False)
+    _rotary_embedding_(q, k, frequencies, at, offset, interleaved, scale, False)
     return q, k
 
 
@@ -161,4 +166,4 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.tensor(0.0)
-    return torch.ops.supa.clip_grad_norm_(grads, float(max_norm), float(norm_type), bool(error_if_nonfinite))
+    return _clip_grad_norm_(grads, float(max_norm), float(norm_type), bool(error_if_nonfinite))
