@@ -247,8 +247,8 @@ template <typename T, typename R, int NV, int VW, bool OWN> struct RnRaw {
 // the next one's operands.  With 16, the factors lie in LDS (in global memory
 // their loads, which return in order, would wait for the row requested before
 // them); and a workgroup of 1024 threads, with half the registers each, has two
-// of the sums in LDS instead, requests a row when it begins, and reads the
-// factors again.
+// of the sums in LDS instead and those of the post norm's parameters with its
+// partials, requests a row when it begins, and reads the factors again.
 template <int G, int EPT> struct RnKeep {
   static constexpr bool kRegs = EPT <= 8;
   static constexpr bool kLdsFactors = EPT == 16 && G <= 512;
@@ -291,8 +291,9 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
   constexpr int VW = 16 / (int)sizeof(T), NV = EPT / VW;
   using Keep = RnKeep<G, EPT>;
   using Lds = RnLds<G, NV, VW>;
-  constexpr int kReg = Keep::kRegs ? NV : 1, kSums = Keep::kLdsSums ? 1 : NV, kPost = POST ? NV : 1;
-  constexpr int kBias = LAYER ? NV : 1, kPostBias = POST && LAYER ? NV : 1;
+  constexpr int kReg = Keep::kRegs ? NV : 1, kSums = Keep::kLdsSums ? 1 : NV;
+  constexpr bool kTotals = POST && !Keep::kLdsSums;  // else kept with the partials, section by section
+  constexpr int kPost = kTotals ? NV : 1, kPostBias = kTotals && LAYER ? NV : 1, kBias = LAYER ? NV : 1;
   constexpr int NS = LAYER ? 2 : 1;  // sums along a row: a n (and a)
   __shared__ float lds[2][2][NS * BS / 64];
   __shared__ float fold[ROWS > 1 ? BS * EPT : 1];
@@ -307,7 +308,7 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
 
   float aw[kSums][VW] = {}, at[kSums][VW] = {};            // dw; dH xn since the gate's row began
   float ab[kBias][VW] = {}, av[kBias][VW] = {};            // db; dH
-  float apw[kPost][VW] = {}, apb[kPostBias][VW] = {};      // g times those
+  float apw[kPost][VW] = {}, apb[kPostBias][VW] = {};      // g times those, of all sections
   float rw[kReg][VW], rp[kReg][VW], rq[kReg][VW];
 
   // factors of vector j from memory, with the gate's row at `at` (none: 1)
@@ -591,14 +592,24 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
             for (int k = 0; k < VW; ++k) u[k] = (POST && LAYER ? fmaf(x[k], p[k], b[k]) : x[k] * p[k]) * dH[j][k];
             rn_param_store<T>(c, o.ggate, a.pf32, row * a.width, j, u, active);
           }
-          if constexpr (POST) {
-            if constexpr (!Keep::kAhead) rn_param<T>(c, a.gate, a.pf32, row * a.width, j, 1.f, g, active);
+          if constexpr (kTotals) {
 #pragma unroll
             for (int k = 0; k < VW; ++k) {
-              const float du = dH[j][k] * (Keep::kAhead ? gs[Keep::kAhead ? j : 0][k] : g[k]);
+              const float du = dH[j][k] * gs[Keep::kAhead ? j : 0][k];
               apw[j][k] = fmaf(du, x[k], apw[j][k]);
               if constexpr (LAYER) apb[j][k] += du;
             }
+          } else if constexpr (POST) {
+            float sum[VW];
+            rn_param<T>(c, a.gate, a.pf32, row * a.width, j, 1.f, g, active);
+            lp.get(l, j, sum);
+#pragma unroll
+            for (int k = 0; k < VW; ++k) {
+              const float du = dH[j][k] * g[k];
+              sum[k] = fmaf(du, x[k], sum[k]);
+              if constexpr (LAYER) av[j][k] += du;
+            }
+            lp.put(l, j, sum);
           }
         }
       } else if (sum_xn) {
@@ -667,12 +678,27 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
             at[j][k] = 0.f;
           }
         }
-        if constexpr (POST) {
-          rn_param<T>(c, a.gate, a.pf32, gate_at, j, 1.f, g);
+        if constexpr (POST) rn_param<T>(c, a.gate, a.pf32, gate_at, j, 1.f, g);
+        if constexpr (kTotals) {
 #pragma unroll
           for (int k = 0; k < VW; ++k) {
             apw[j][k] = fmaf(g[k], t[k], apw[j][k]);
             if constexpr (LAYER) apb[j][k] = fmaf(g[k], av[j][k], apb[j][k]);
+          }
+        } else if constexpr (POST) {
+          float* total = part + (o.want_gate == 1 && o.cuts > 1 ? a.width : 0);
+          auto add = [&](const auto& s) {  // to the total that this thread wrote at the last section's end
+            RowVec<float, VW> old{};
+            if (sec > sec0) old = c.template load<false>(total, j);
+            float f[VW];
+#pragma unroll
+            for (int k = 0; k < VW; ++k) f[k] = fmaf(g[k], s[k], sec > sec0 ? row_elem<float, VW>(old, k) : 0.f);
+            c.store(total, j, f);
+            total += a.width;
+          };
+          if (o.want_pw) add(t);
+          if constexpr (LAYER) {
+            if (o.want_pb) add(av[j]);
           }
         }
         if (o.want_gate) {
@@ -708,8 +734,15 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
       for (int k = 0; k < VW; ++k) t[k] = s[j][k];
     };
   };
-  if constexpr (POST) put(o.want_pw, from(apw));
-  if constexpr (POST && LAYER) put(o.want_pb, from(apb));
+  if constexpr (kTotals) {
+    put(o.want_pw, from(apw));
+    if constexpr (LAYER) put(o.want_pb, from(apb));
+  } else if constexpr (POST && OWN) {
+    put(o.want_pw, [&](int j, float (&t)[VW]) { lp.get(l, j, t); });
+    if constexpr (LAYER) put(o.want_pb, from(av));
+  } else if constexpr (POST) {  // written at the sections' ends
+    part += (o.want_pw + (LAYER ? o.want_pb : 0)) * (int64_t)a.width;
+  }
   if constexpr (Keep::kLdsSums) put(o.want_w, [&](int j, float (&t)[VW]) { lw.get(l, j, t); });
   else put(o.want_w, from(aw));
   if constexpr (LAYER) put(o.want_b, from(ab));
