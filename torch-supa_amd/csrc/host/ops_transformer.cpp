@@ -6,7 +6,9 @@
 // workspaces from the caching allocator.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -20,7 +22,7 @@
 namespace supa {
 namespace {
 
-using torch::autograd::AutogradContext;
+using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<at::Tensor>;
 
@@ -183,107 +185,73 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::
   return {r.h, r.y};
 }
 
-// x and residual are saved for the backward, which forms h from them again;
-// without post norm and gate h alone is enough, as long as it is not rounded
-// more coarsely than the weight's gradient it enters.
-class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
- public:
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& residual,
-                               const OptTensor& gate, double scale, int64_t post, const OptTensor& post_weight,
-                               const OptTensor& post_bias, int64_t norm, const OptTensor& weight, const OptTensor& bias,
-                               double eps) {
-    NormArgs a{scale, eps, post, norm, 1};
-    check_residual_norm(x, residual, gate, a, post_weight, post_bias, weight, bias);
-    const c10::DeviceGuard guard(x.device());
-    ctx->set_materialize_grads(false);
-    const Rows xr = rows_of(x), rr = rows_of(residual);
-    const OptTensor g = contiguous(gate), pw = contiguous(post_weight), pb = contiguous(post_bias),
-                    w = contiguous(weight), b = contiguous(bias);
-    NormResult r = residual_norm_forward(xr, rr, g, a, pw, pb, w, b, true);
-    const bool wide = given(weight) && weight->scalar_type() == at::kFloat;
-    const bool from_h = !given(gate) && post == SUPA_AMD_NORM_NONE &&
-                        (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat || !wide);
-    const bool needs_h = norm != SUPA_AMD_NORM_NONE;
-    ctx->save_for_backward({from_h ? at::Tensor() : xr.t, from_h || !needs_h ? at::Tensor() : rr.t,
-                            from_h && needs_h ? r.h : at::Tensor(), r.stats, g.value_or(at::Tensor()),
-                            pw.value_or(at::Tensor()), pb.value_or(at::Tensor()), w.value_or(at::Tensor()),
-                            b.value_or(at::Tensor())});
-    ctx->saved_data["scalars"] = std::vector<double>{scale, eps};
-    ctx->saved_data["ints"] = std::vector<int64_t>{post, norm, a.period, xr.stride, rr.stride, from_h,
-                                                   (int64_t)residual.scalar_type(), (int64_t)x.scalar_type()};
-    ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->saved_data["gate_shape"] = given(gate) ? gate->sizes().vec() : std::vector<int64_t>{};
-    return r.y.defined() ? variable_list{r.h, r.y} : variable_list{r.h};
+// A node of its own, with plain fields, instead of a custom Function: the small
+// calls of training are bound by the host, and it takes 6 us off a pass.  x and
+// residual are saved for the backward, which forms h from them again; without
+// post norm and gate h alone is enough, as long as it is not rounded more
+// coarsely than the weight's gradient it enters.
+struct ResidualNormBackward final : public torch::autograd::Node {
+  // the inputs' places, in the order of the edges
+  enum { kX, kResidual, kGate, kPostWeight, kPostBias, kWeight, kBias, kInputs };
+
+  std::string name() const override { return "ResidualNormBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    x.reset_data();
+    residual.reset_data();
+    h.reset_data();
+    stats.reset_data();
+    for (SavedVariable& p : params) p.reset_data();
   }
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+  variable_list apply(variable_list&& grads) override {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "residual_norm: the gradient has no gradient of its own (create_graph)");
-    const auto saved = ctx->get_saved_variables();
-    const at::Tensor &x = saved[0], &residual = saved[1], &h = saved[2], &stats = saved[3];
-    const OptTensor gate = maybe(saved[4]), pw = maybe(saved[5]), pb = maybe(saved[6]), w = maybe(saved[7]),
-                    b = maybe(saved[8]);
-    const auto scalars = ctx->saved_data["scalars"].toDoubleVector();
-    const auto ints = ctx->saved_data["ints"].toIntVector();
-    const auto shape = ctx->saved_data["shape"].toIntVector();
+    variable_list out(kInputs);
+    if (!grads[0].defined() && !(grads.size() > 1 && grads[1].defined())) return out;
+    std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor gh = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
     const at::Tensor gy = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
-    variable_list out(11);
-    if (!gh.defined() && !gy.defined()) return out;
-    const auto xt = (at::ScalarType)ints[7], rt = (at::ScalarType)ints[6];
+    const at::Tensor xt = x.unpack(), rt = residual.unpack(), ht = h.unpack(shared_from_this()), st = stats.unpack();
+    at::Tensor p[kInputs];
+    for (int i = kGate; i < kInputs; ++i) p[i] = params[i].unpack();
     const c10::Device device = gh.defined() ? gh.device() : gy.device();
     const c10::DeviceGuard guard(device);
     const auto dev = device.index();
+    const auto data = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
 
-    supa_amd_residual_norm_desc d{};
-    d.width = shape.back();
-    d.rows = 1;
-    for (size_t i = 0; i + 1 < shape.size(); ++i) d.rows *= shape[i];
-    d.x_stride = ints[3];
-    d.residual_stride = ints[4];
-    d.gate_period = ints[2];
-    d.dtype = dtype_code(xt);
-    d.residual_dtype = dtype_code(rt);
-    d.param_dtype = d.dtype;
-    for (const OptTensor* t : {&gate, &pw, &pb, &w, &b})
-      if (given(*t)) d.param_dtype = dtype_code((*t)->scalar_type());
-    d.post_norm = (int32_t)ints[0];
-    d.norm = (int32_t)ints[1];
-    d.residual_scale = scalars[0];
-    d.eps = scalars[1];
-    d.x = x.defined() ? x.data_ptr() : nullptr;
-    d.residual = residual.defined() ? residual.data_ptr() : nullptr;
-    d.gate = ptr(gate);
-    d.post_weight = ptr(pw);
-    d.post_bias = ptr(pb);
-    d.weight = ptr(w);
-    d.bias = ptr(b);
-
-    // the edges are the tensors that the forward was given, in its order
-    size_t edge = 0;
-    const auto wanted = [&](bool present) { return present && ctx->needs_input_grad(edge++); };
-    if (wanted(true)) out[0] = empty_supa(shape, xt, dev);
-    if (wanted(true)) out[1] = empty_supa(shape, rt, dev);
-    if (wanted(given(gate))) out[2] = empty_supa(ctx->saved_data["gate_shape"].toIntVector(), gate->scalar_type(), dev);
-    const std::pair<int, const OptTensor*> vectors[] = {{5, &pw}, {6, &pb}, {8, &w}, {9, &b}};
-    for (const auto& [at, t] : vectors)
-      if (wanted(given(*t))) out[at] = empty_supa({d.width}, (*t)->scalar_type(), dev);
+    d.x = data(xt);
+    d.residual = data(rt);
+    d.gate = data(p[kGate]);
+    d.post_weight = data(p[kPostWeight]);
+    d.post_bias = data(p[kPostBias]);
+    d.weight = data(p[kWeight]);
+    d.bias = data(p[kBias]);
+    if (task_should_compute_output(kX)) out[kX] = empty_supa(shape, (at::ScalarType)d.dtype, dev);
+    if (task_should_compute_output(kResidual)) out[kResidual] = empty_supa(shape, (at::ScalarType)d.residual_dtype, dev);
+    for (int i = kGate; i < kInputs; ++i)
+      if (p[i].defined() && task_should_compute_output(i))
+        out[i] = empty_supa(i == kGate ? c10::IntArrayRef(gate_shape) : p[i].sizes(), p[i].scalar_type(), dev);
     if (d.rows == 0) {
       for (auto& t : out)
         if (t.defined()) t.zero_();
       return out;
     }
-    const auto data = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
     const int64_t ws_bytes = supa_amd_residual_norm_backward_workspace_bytes(&d);
     TORCH_CHECK(ws_bytes >= 0, "residual_norm: ", supa_amd_status_string((int)ws_bytes));
     const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
-    check_status(supa_amd_residual_norm_backward(&d, data(h), data(gh), data(gy),
-                                                 stats.defined() ? stats.data_ptr<float>() : nullptr, data(out[0]),
-                                                 data(out[1]), data(out[2]), data(out[5]), data(out[6]), data(out[8]),
-                                                 data(out[9]), ws.data_ptr(), ws_bytes, current_stream(dev)),
+    check_status(supa_amd_residual_norm_backward(&d, data(ht), data(gh), data(gy),
+                                                 st.defined() ? st.data_ptr<float>() : nullptr, data(out[kX]),
+                                                 data(out[kResidual]), data(out[kGate]), data(out[kPostWeight]),
+                                                 data(out[kPostBias]), data(out[kWeight]), data(out[kBias]),
+                                                 ws.data_ptr(), ws_bytes, current_stream(dev)),
                  "residual_norm (backward)");
     return out;
   }
+
+  SavedVariable x, residual, h, stats, params[kInputs];
+  supa_amd_residual_norm_desc d{};  // its pointers are set from the saved tensors
+  std::vector<int64_t> shape, gate_shape;
 };
 
 std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(const at::Tensor& x, const at::Tensor& residual,
@@ -298,9 +266,41 @@ std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(const at::Tensor& x, c
     const at::AutoDispatchBelowAutograd below;
     return residual_norm(x, residual, gate, scale, post, post_weight, post_bias, norm, weight, bias, eps);
   }
-  const variable_list r =
-      ResidualNorm::apply(x, residual, gate, scale, post, post_weight, post_bias, norm, weight, bias, eps);
-  return {r[0], r.size() > 1 ? r[1] : at::Tensor()};
+  NormArgs a{scale, eps, post, norm, 1};
+  check_residual_norm(x, residual, gate, a, post_weight, post_bias, weight, bias);
+  auto node = std::shared_ptr<ResidualNormBackward>(new ResidualNormBackward(), torch::autograd::deleteNode);
+  using Node = ResidualNormBackward;
+  const auto edge = [](const OptTensor& t) {
+    return given(t) ? torch::autograd::impl::gradient_edge(*t) : torch::autograd::Edge();
+  };
+  node->set_next_edges({torch::autograd::impl::gradient_edge(x), torch::autograd::impl::gradient_edge(residual),
+                        edge(gate), edge(post_weight), edge(post_bias), edge(weight), edge(bias)});
+  NormResult r;
+  {
+    const at::AutoDispatchBelowAutograd below;
+    const c10::DeviceGuard guard(x.device());
+    const Rows xr = rows_of(x), rr = rows_of(residual);
+    const OptTensor g = contiguous(gate), pw = contiguous(post_weight), pb = contiguous(post_bias),
+                    w = contiguous(weight), b = contiguous(bias);
+    r = residual_norm_forward(xr, rr, g, a, pw, pb, w, b, true);
+    node->d = norm_desc(xr, rr, g, a, pw, pb, w, b);
+    const bool wide = given(weight) && weight->scalar_type() == at::kFloat;
+    const bool from_h = !given(gate) && post == SUPA_AMD_NORM_NONE &&
+                        (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat || !wide);
+    const bool needs_h = norm != SUPA_AMD_NORM_NONE;
+    if (!from_h) node->x = SavedVariable(xr.t, false);
+    if (!from_h && needs_h) node->residual = SavedVariable(rr.t, false);
+    if (r.stats.defined()) node->stats = SavedVariable(r.stats, false);
+    const OptTensor* saved[] = {nullptr, nullptr, &g, &pw, &pb, &w, &b};
+    for (int i = Node::kGate; i < Node::kInputs; ++i)
+      if (given(*saved[i])) node->params[i] = SavedVariable(**saved[i], false);
+    node->shape = x.sizes().vec();
+    if (given(gate)) node->gate_shape = gate->sizes().vec();
+    torch::autograd::set_history(r.h, node);
+    if (r.y.defined()) torch::autograd::set_history(r.y, node);
+    if (from_h && needs_h) node->h = SavedVariable(r.h, true);
+  }
+  return {r.h, r.y};
 }
 
 // --------------------------------------------------------- rotary_embedding
@@ -470,42 +470,43 @@ void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& freq
   launch_rotary(op, q, q, given(k) ? *k : at::Tensor(), given(k) ? *k : at::Tensor(), a);
 }
 
-class RotaryEmbedding : public torch::autograd::Function<RotaryEmbedding> {
- public:
-  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const OptTensor& k,
-                               const at::Tensor& frequencies, const OptTensor& positions, int64_t offset,
-                               bool interleaved, double scale, bool inverse) {
-    ctx->set_materialize_grads(false);
-    auto [qo, ko] = rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
-    ctx->save_for_backward({frequencies, given(positions) ? *positions : at::Tensor()});
-    ctx->saved_data["offset"] = offset;
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["scale"] = scale;
-    ctx->saved_data["inverse"] = inverse;
-    return ko.defined() ? variable_list{qo, ko} : variable_list{qo};
-  }
+std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q, const OptTensor& k,
+                                                             const at::Tensor& frequencies, const OptTensor& positions,
+                                                             int64_t offset, bool interleaved, double scale,
+                                                             bool inverse);
 
-  // The rotation back, by the same call: it has a gradient of its own.
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const auto saved = ctx->get_saved_variables();
-    const bool second = grads.size() > 1;
-    const at::Tensor gq = ctx->needs_input_grad(0) ? grads[0] : at::Tensor();
-    const at::Tensor gk = second && ctx->needs_input_grad(1) ? grads[1] : at::Tensor();
-    variable_list out(8);
+// The rotation back.  Under create_graph by the same call, which has a gradient
+// of its own.
+struct RotaryEmbeddingBackward final : public torch::autograd::Node {
+  std::string name() const override { return "RotaryEmbeddingBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    frequencies.reset_data();
+    positions.reset_data();
+  }
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(2);
+    const at::Tensor gq = task_should_compute_output(0) ? grads[0] : at::Tensor();
+    const at::Tensor gk = grads.size() > 1 && task_should_compute_output(1) ? grads[1] : at::Tensor();
     if (!gq.defined() && !gk.defined()) return out;
-    static const auto call =
-        c10::Dispatcher::singleton()
-            .findSchemaOrThrow("supa::rotary_embedding", "")
-            .typed<std::tuple<at::Tensor, at::Tensor>(const at::Tensor&, const OptTensor&, const at::Tensor&,
-                                                      const OptTensor&, int64_t, bool, double, bool)>();
+    std::lock_guard<std::mutex> lock(mutex_);
     const bool both = gq.defined() && gk.defined();
-    auto [a, b] = call.call(gq.defined() ? gq : gk, both ? OptTensor(gk) : std::nullopt, saved[0], maybe(saved[1]),
-                            ctx->saved_data["offset"].toInt(), ctx->saved_data["interleaved"].toBool(),
-                            ctx->saved_data["scale"].toDouble(), !ctx->saved_data["inverse"].toBool());
+    const at::Tensor& first = gq.defined() ? gq : gk;
+    const OptTensor second = both ? OptTensor(gk) : std::nullopt;
+    const at::Tensor f = frequencies.unpack();
+    const OptTensor p = maybe(positions.unpack());
+    auto [a, b] = at::GradMode::is_enabled()
+                      ? rotary_embedding_autograd(first, second, f, p, offset, interleaved, scale, !inverse)
+                      : rotary_embedding(first, second, f, p, offset, interleaved, scale, !inverse);
     if (gq.defined()) out[0] = a;
     if (gk.defined()) out[1] = both ? b : a;
     return out;
   }
+
+  SavedVariable frequencies, positions;
+  int64_t offset;
+  bool interleaved, inverse;
+  double scale;
 };
 
 std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q, const OptTensor& k,
@@ -518,9 +519,22 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q
     const at::AutoDispatchBelowAutograd below;
     return rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
   }
-  const variable_list r =
-      RotaryEmbedding::apply(q, k, frequencies, positions, offset, interleaved, scale, inverse);
-  return {r[0], r.size() > 1 ? r[1] : at::Tensor()};
+  auto node = std::shared_ptr<RotaryEmbeddingBackward>(new RotaryEmbeddingBackward(), torch::autograd::deleteNode);
+  torch::autograd::edge_list edges{torch::autograd::impl::gradient_edge(q)};
+  if (given(k)) edges.push_back(torch::autograd::impl::gradient_edge(*k));
+  else edges.emplace_back();
+  node->set_next_edges(std::move(edges));
+  node->offset = offset;
+  node->interleaved = interleaved;
+  node->inverse = inverse;
+  node->scale = scale;
+  const at::AutoDispatchBelowAutograd below;
+  auto [qo, ko] = rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  node->frequencies = SavedVariable(frequencies, false);
+  if (given(positions)) node->positions = SavedVariable(*positions, false);
+  torch::autograd::set_history(qo, node);
+  if (ko.defined()) torch::autograd::set_history(ko, node);
+  return {qo, ko};
 }
 
 void written(const at::Tensor& t) {
