@@ -54,7 +54,7 @@ struct RotArgs {
 // elements twice, with the same values; in place, where another thread may have
 // written them before, it goes element by element, as does a part shorter than a
 // vector.
-template <typename T, bool HALF, typename OFF> struct RotUnit {
+template <typename T, bool HALF, bool ONE, typename OFF> struct RotUnit {
   static constexpr int V = 16 / (int)sizeof(T);
   const T* in;
   T* out;
@@ -64,11 +64,16 @@ template <typename T, bool HALF, typename OFF> struct RotUnit {
   RowVec<T, V> a, b;
 
   __device__ __forceinline__ void find(const RotArgs& g, uint32_t unit, int32_t token0, int32_t slot0) {
-    uint32_t outer, inner, v, u;
+    uint32_t v, u;
     g.by_unit.divmod(unit, v, u);
-    g.by_inner.divmod(v, outer, inner);
-    tk = (int)(g.head_major ? inner : outer);
-    const int32_t slot = slot0 + (int32_t)(g.head_major ? outer : inner);
+    int32_t slot = slot0 + (int32_t)v;
+    tk = 0;
+    if constexpr (!ONE) {
+      uint32_t outer, inner;
+      g.by_inner.divmod(v, outer, inner);
+      tk = (int)(g.head_major ? inner : outer);
+      slot = slot0 + (int32_t)(g.head_major ? outer : inner);
+    }
     const int64_t token = (int64_t)token0 + tk;
     const bool second = slot >= g.t[0].heads;
     // chosen value by value: an indexed pointer would not be known to be global memory
@@ -81,10 +86,16 @@ template <typename T, bool HALF, typename OFF> struct RotUnit {
     uint32_t bi, si;
     g.seq.divmod((uint32_t)token, bi, si);
     const OFF ob = (OFF)bi, os = (OFF)si;
-    in = static_cast<const T*>(of(q.in, k.in)) +
-         (ob * step(q.is[0], k.is[0]) + os * step(q.is[1], k.is[1]) + head * step(q.is[2], k.is[2]));
-    out = static_cast<T*>(of(q.out, k.out)) +
-          (ob * step(q.os[0], k.os[0]) + os * step(q.os[1], k.os[1]) + head * step(q.os[2], k.os[2]));
+    OFF in_at, out_at;
+    if constexpr (ONE) {  // the token is the workgroup's: scalar products
+      in_at = of((OFF)(ob * (OFF)q.is[0] + os * (OFF)q.is[1]), (OFF)(ob * (OFF)k.is[0] + os * (OFF)k.is[1]));
+      out_at = of((OFF)(ob * (OFF)q.os[0] + os * (OFF)q.os[1]), (OFF)(ob * (OFF)k.os[0] + os * (OFF)k.os[1]));
+    } else {
+      in_at = ob * step(q.is[0], k.is[0]) + os * step(q.is[1], k.is[1]);
+      out_at = ob * step(q.os[0], k.os[0]) + os * step(q.os[1], k.os[1]);
+    }
+    in = static_cast<const T*>(of(q.in, k.in)) + (in_at + head * step(q.is[2], k.is[2]));
+    out = static_cast<T*>(of(q.out, k.out)) + (out_at + head * step(q.os[2], k.os[2]));
     int first;
     if (turn) {
       first = 0;
@@ -107,34 +118,41 @@ template <typename T, bool HALF, typename OFF> struct RotUnit {
     float f[V], h[V];
 #pragma unroll
     for (int k = 0; k < V; ++k) f[k] = row_elem<T, V>(a, k);
-    if (turn) {
+    auto rotated = [&](auto whole) {
+      // the angles of a whole vector are neighbours; past a part's end, any will do
+      auto angle = [&](int pair, int e) { return cs[whole.value || e < part ? pair : 0]; };
       if constexpr (HALF) {
 #pragma unroll
         for (int k = 0; k < V; ++k) {
-          const float2 w = cs[col + k < part ? col + k : 0];
+          const float2 w = angle(col + k, col + k);
           const float y = row_elem<T, V>(b, k);
           h[k] = fmaf(y, w.x, f[k] * w.y);
           f[k] = fmaf(f[k], w.x, -(y * w.y));
         }
         row_store<T, V>(out + g.rotary / 2, col, part, h);
       } else {
+        const int first = col / 2;
 #pragma unroll
         for (int k = 0; k < V; k += 2) {
-          const float2 w = cs[col + k < part ? (col + k) / 2 : 0];
+          const float2 w = angle(first + k / 2, col + k);
           const float x = f[k], y = f[k + 1];
           f[k] = fmaf(x, w.x, -(y * w.y));
           f[k + 1] = fmaf(y, w.x, x * w.y);
         }
       }
+    };
+    if (turn) {
+      if (col + V <= part) rotated(std::true_type{});
+      else rotated(std::false_type{});
     }
     row_store<T, V>(out, col, part, f);
   }
 };
 
-// OFF: the type of offsets within a tensor.  A 64-bit product is four 32-bit ones, each
+// ONE: a workgroup's tile is one token.  OFF: the type of offsets within a tensor.  A 64-bit product is four 32-bit ones, each
 // of a quarter of the rate; with six of them a vector they bounded the kernel
 // ([2, 4096, 64, 192] bf16, interleaved: 103 us, 79 with 32-bit offsets).
-template <typename T, bool HALF, typename OFF>
+template <typename T, bool HALF, bool ONE, typename OFF>
 __global__ void __launch_bounds__(kRotBlock) k_rotary(RotArgs g) {
   __shared__ float2 cs[kRotTable];
   const int32_t token0 = g.first + (int32_t)blockIdx.x * g.per;
@@ -142,7 +160,7 @@ __global__ void __launch_bounds__(kRotBlock) k_rotary(RotArgs g) {
   const uint32_t all = (uint32_t)(g.per * g.heads * g.units);
   const int pairs = g.rotary / 2;
   constexpr int U = rot_units(HALF);
-  RotUnit<T, HALF, OFF> w[U];
+  RotUnit<T, HALF, ONE, OFF> w[U];
   uint32_t unit = threadIdx.x;
   auto request = [&]() {
 #pragma unroll
@@ -256,15 +274,19 @@ template <typename T> int rot_launch(const supa_amd_rotary_desc& d, hipStream_t 
     a.first = (int32_t)first;
     a.tokens = (int32_t)std::min(tokens, first + slab);
     const unsigned blocks = (unsigned)((a.tokens - first + a.per - 1) / a.per);
-    auto go = [&](auto h, auto* off) {
-      k_rotary<T, h.value, std::remove_pointer_t<decltype(off)>><<<dim3(blocks, groups), block, 0, st>>>(a);
+    auto go = [&](auto h, auto one, auto* off) {
+      k_rotary<T, h.value, one.value, std::remove_pointer_t<decltype(off)>><<<dim3(blocks, groups), block, 0, st>>>(a);
     };
-    auto offsets = [&](auto h) {
-      if (narrow) go(h, (int32_t*)nullptr);
-      else go(h, (int64_t*)nullptr);
+    auto offsets = [&](auto h, auto one) {
+      if (narrow) go(h, one, (int32_t*)nullptr);
+      else go(h, one, (int64_t*)nullptr);
     };
-    if (half) offsets(std::true_type{});
-    else offsets(std::false_type{});
+    auto tile = [&](auto h) {
+      if (a.per == 1 && !a.head_major) offsets(h, std::true_type{});
+      else offsets(h, std::false_type{});
+    };
+    if (half) tile(std::true_type{});
+    else tile(std::false_type{});
     const int rc = launch_status();
     if (rc) return rc;
   }
