@@ -15,9 +15,17 @@
 //   dw = sum dy n, db = sum dy, dw_post = sum du xn, db_post = sum du
 // The statistics come from the forward (four floats a row); h is formed again
 // from x and r, not taken rounded.  The sums run down the columns: a
-// workgroup takes consecutive rows and keeps its columns' sums in registers,
+// workgroup stays for many rows and keeps its columns' sums in registers,
 // writes them as one row of partials, and a second launch adds the partials in
 // a fixed order.
+//
+// Measured on MI355X (a device copy by torch: 5.0 TB/s): bf16 [8192, 4096] with
+// both norms and a gate 47 us forward (5.7 TB/s), 75 + 5 backward (5.4 of its own
+// bytes, 0.43 GB with the partials); float32 [6006, 2047], layer norms, a gate a
+// sample: 40 us (4.9; rows at 4-byte alignment) and 65 + 5; bf16 on a float32 stream
+// [16384, 8192], no gate: 288 us (5.6) and 385 + 5 (5.6).  Rows of more than 8192
+// elements with layer norms on both sides spill registers in the backward
+// ([4096, 16384] bf16 540 us, RMS norms 232).
 #pragma once
 
 #include <atomic>
