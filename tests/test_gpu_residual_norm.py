@@ -142,6 +142,9 @@ CASES = [
     ((64, 96), "bf16", "bf16", "bf16", None, None, None, 0.5),
     ((4097,), "f32", "f32", "f32", "channel", "layer", "layer", 1.0),
     ((270, 2, 8200), "bf16", "bf16", "bf16", "sample", "layer", "layer", 1.0),
+    ((270, 2, 8201), "bf16", "bf16", "bf16", "sample", "layer", "layer", 1.0),
+    ((300, 2, 8195), "f32", "f32", "f32", "sample", "rms", "rms", 1.0),
+    ((261, 3, 4099), "bf16", "f32", "f32", "sample", "layer", "rms", 1.0),
     ((3, 40, 9001), "f32", "f32", "f32", "sample", "rms", "rms", 1.0),
     ((160, 24, 520), "bf16", "bf16", "bf16", "sample", "layer", "layer", 1.0),
     ((300, 9, 260), "f32", "f32", "f32", "sample", "rms", "layer", 1.0),

@@ -695,13 +695,22 @@ k_residual_norm_backward(RnArgs a, RnGrads o) {
           }
         } else if constexpr (POST) {
           float* total = part + (o.want_gate == 1 && o.cuts > 1 ? a.width : 0);
-          auto add = [&](const auto& s) {  // to the total that this thread wrote at the last section's end
-            RowVec<float, VW> old{};
-            if (sec > sec0) old = c.template load<false>(total, j);
-            float f[VW];
+          // to the total that this thread wrote at the last section's end; of the vector
+          // that was moved back its own elements alone, as another thread adds the others
+          auto add = [&](const auto& s) {
+            if (c.whole(j)) {
+              RowVec<float, VW> old{};
+              if (sec > sec0) old = c.template load<false>(total, j);
+              float f[VW];
 #pragma unroll
-            for (int k = 0; k < VW; ++k) f[k] = fmaf(g[k], s[k], sec > sec0 ? row_elem<float, VW>(old, k) : 0.f);
-            c.store(total, j, f);
+              for (int k = 0; k < VW; ++k) f[k] = fmaf(g[k], s[k], row_elem<float, VW>(old, k));
+              c.store(total, j, f);
+            } else {
+              c.each(j, [&](int k) {
+                float* at = total + c.col[j] + k;
+                *at = fmaf(g[k], s[k], sec > sec0 ? *at : 0.f);
+              });
+            }
             total += a.width;
           };
           if (o.want_pw) add(t);

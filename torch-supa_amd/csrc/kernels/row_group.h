@@ -49,9 +49,10 @@ __device__ __forceinline__ void row_store(S* __restrict__ row, int col, int widt
 // Where a thread's NV vectors lie in a row of `width` elements, the same for
 // every row.  The vector that would run past the row's end is moved back
 // to it: it computes and stores some elements a second time, with the values
-// that the vector before has for them, and only sums along the row leave them
-// out.  So every access is a whole vector, and one instruction; a row
-// narrower than a vector, in groups of 16, goes element by element.
+// that the vector before has for them; sums along the row leave them out, and
+// what is read, changed and written back has to.  So every access is a whole
+// vector, and one instruction; a row narrower than a vector, in groups of 16,
+// goes element by element.
 template <int G, int NV, int VW> struct RowSlots {
   static constexpr bool kWhole = G > 16;  // callers use them for rows of more than 16 vectors
   uint32_t col[NV];
@@ -80,6 +81,8 @@ template <int G, int NV, int VW> struct RowSlots {
 #pragma unroll
     for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(col[j]));
   }
+  // Vector j is there and all its elements are its own.
+  __device__ __forceinline__ bool whole(int j) const { return kWhole && skip[j] == 0; }
   __device__ __forceinline__ bool live(int j) const { return !kWhole || skip[j] < VW; }
   // f(k) for the elements of vector j that are the row's and no other vector's.
   // The vector that was moved back is one thread's, and takes a branch of its own.
