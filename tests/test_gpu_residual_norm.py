@@ -256,6 +256,50 @@ def test_views_and_strides(no_fallback):
     assert torch.equal(h.cpu(), (row.cpu() * 2)) and torch.equal(y[0].cpu(), y[8].cpu())
 
 
+def test_saved_tensors_come_back_otherwise(no_fallback):
+    """Hooks that keep what the backward needs elsewhere give it back with other
+    strides (a slice of a wider projection contiguous, a contiguous tensor as
+    every second row): the same gradients, bit for bit; another shape or type
+    raises."""
+    g = torch.Generator().manual_seed(6)
+    wide = torch.randn(40, 700, generator=g).to("supa")
+    w = torch.randn(260, generator=g).to("supa").requires_grad_()
+    apart = lambda t: torch.stack((t, t), -2)[..., 0, :] if t.dim() > 1 else torch.stack((t, t), -1)[..., 0]  # noqa: E731
+
+    def grads(unpack):
+        x = wide[:, 13:273].detach().requires_grad_()
+        r = wide[:, 300:560].detach().requires_grad_()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach(), unpack):
+            h, y = torch.supa.residual_norm(x, r, post_norm="rms", post_weight=w, weight=w)
+        return [t.cpu() for t in torch.autograd.grad(h.sum() + y.sum(), [x, r, w])]
+
+    want = grads(lambda t: t)
+    for unpack in (torch.Tensor.contiguous, apart, lambda t: t.cpu().to("supa")):
+        assert all(torch.equal(a, b) for a, b in zip(grads(unpack), want))
+    for unpack in (torch.Tensor.half, lambda t: t[:1], torch.Tensor.cpu):
+        with pytest.raises(RuntimeError, match="saved tensor came back"):
+            grads(unpack)
+
+
+def test_changed_or_used_twice(no_fallback):
+    """A saved tensor that was written since, and a second backward, raise."""
+    x = torch.ones(4, 64, device="supa", requires_grad=True)
+    w = torch.ones(64, device="supa", requires_grad=True)
+    r = torch.ones(4, 64, device="supa")
+    h, y = torch.supa.residual_norm(x, r, weight=w, gate=torch.ones(64, device="supa"))
+    y.sum().backward()
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward()
+    h, y = torch.supa.residual_norm(x, r, weight=w, gate=torch.ones(64, device="supa"))
+    r.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    h, y = torch.supa.residual_norm(x, r, weight=w)  # keeps h
+    h.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_zero_nan_and_infinite_rows(no_fallback):
     d, gh, gy = make((6, 1000), "bf16", "bf16", "bf16", "channel", "rms", "rms", 9)
     dev = {k: t.to("supa") for k, t in d.items()}

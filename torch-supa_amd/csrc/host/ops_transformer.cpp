@@ -212,11 +212,29 @@ struct ResidualNormBackward final : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     const at::Tensor gh = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
     const at::Tensor gy = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
-    const at::Tensor xt = x.unpack(), rt = residual.unpack(), ht = h.unpack(shared_from_this()), st = stats.unpack();
-    at::Tensor p[kInputs];
-    for (int i = kGate; i < kInputs; ++i) p[i] = params[i].unpack();
     const c10::Device device = gh.defined() ? gh.device() : gy.device();
     const c10::DeviceGuard guard(device);
+    // hooks on saved tensors (offloading, recomputation) may give them back with other strides
+    const auto back = [&](const SavedVariable& v, int32_t dtype, c10::IntArrayRef sizes) {
+      const at::Tensor t = v.unpack(shared_from_this());
+      TORCH_CHECK(!t.defined() || (t.device() == device && dtype_code(t.scalar_type()) == dtype && t.sizes() == sizes),
+                  "residual_norm: a saved tensor came back as ", t.scalar_type(), " of shape ", t.sizes(), " on ",
+                  t.device(), ", expected shape ", sizes, " on ", device);
+      return t;
+    };
+    const int64_t width[] = {d.width}, rows[] = {d.rows, 4};
+    at::Tensor xt = back(x, d.dtype, shape), rt = back(residual, d.residual_dtype, shape);
+    for (auto [t, stride] : {std::pair(&xt, &d.x_stride), std::pair(&rt, &d.residual_stride)}) {
+      if (!t->defined() || t->numel() == 0) continue;
+      const Rows r = rows_of(*t);
+      *t = r.t;
+      *stride = r.stride;
+    }
+    const auto dense = [](const at::Tensor& t) { return t.defined() ? t.contiguous() : t; };
+    const at::Tensor ht = dense(back(h, d.residual_dtype, shape)), st = dense(back(stats, SUPA_AMD_F32, rows));
+    at::Tensor p[kInputs];
+    for (int i = kGate; i < kInputs; ++i)
+      p[i] = dense(back(params[i], d.param_dtype, i == kGate ? c10::IntArrayRef(gate_shape) : c10::IntArrayRef(width)));
     const auto dev = device.index();
     const auto data = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
 
