@@ -882,8 +882,8 @@ typedef struct supa_amd_rotary_tensor {
 } supa_amd_rotary_tensor;
 
 typedef struct supa_amd_rotary_desc {
-  int64_t batch, seq;
-  int64_t dim, rotary;       /* rotary even, 0 < rotary <= dim */
+  int64_t batch, seq;        /* batch * seq fewer than 2^31 */
+  int64_t dim, rotary;       /* rotary even, 0 < rotary <= dim, at most 1024; dim below 2^24 */
   int32_t dtype;             /* of q and k: f32, bf16 or f16 */
   int32_t layout;            /* SUPA_AMD_ROTARY_* */
   int32_t inverse;

@@ -137,6 +137,29 @@ def test_positions_far_out(no_fallback):
     assert torch.equal(one.cpu(), got[3:4].cpu())
 
 
+def test_offsets_past_32_bits(no_fallback):
+    """Samples that lie 2^31 elements apart, and almost 2^31 tokens: the same
+    bits as the same rows close together."""
+    g = torch.Generator().manual_seed(8)
+    f = torch.tensor([1.0, 0.01], dtype=torch.float64, device="supa")
+    near = torch.randn(2, 3, 2, 5, generator=g).half().to("supa")
+    room = torch.empty(2 ** 31 + 64, dtype=torch.half, device="supa")
+    far = room.as_strided((2, 3, 2, 5), (2 ** 31, 10, 5, 1), 7)
+    far.copy_(near)
+    for layout in ("half", "interleaved"):
+        want, _ = torch.supa.rotary_embedding(near, None, f, 9, layout=layout)
+        assert torch.equal(torch.supa.rotary_embedding(far, None, f, 9, layout=layout)[0].cpu(), want.cpu())
+    torch.supa.rotary_embedding_(far, None, f, 9, layout="interleaved")
+    assert torch.equal(far.cpu(), want.cpu())
+    del far, room
+    n, last = 2 ** 31 - 3, 700
+    row = torch.tensor([[[0.5, -1.5]]], device="supa", dtype=torch.bfloat16)
+    got, _ = torch.supa.rotary_embedding(row.expand(n, 1, 2), None, f[1:])
+    for at in (0, 2 ** 30 - 300, n - last):
+        want, _ = torch.supa.rotary_embedding(row.expand(last, 1, 2), None, f[1:], at)
+        assert torch.equal(got[at: at + last].cpu(), want.cpu())
+
+
 def test_second_derivative_and_difference(no_fallback):
     q = torch.randn(4, 2, 16, generator=torch.Generator().manual_seed(5)).to("supa").requires_grad_()
     f, scale = torch.supa.rotary_frequencies(12, scaling="yarn", factor=4.0, original_length=64)

@@ -103,7 +103,7 @@ def rotary_desc(**kw):
     (dict(batch=-1), EINVAL), (dict(layout=2), EINVAL), (dict(position_dtype=F32), EDTYPE), (dict(dtype=F64), EDTYPE),
     (dict(frequencies=None), EINVAL), (dict(q=RotaryTensor(data_in=FAKE, heads=2)), EINVAL),
     (dict(q=RotaryTensor(data_in=FAKE, out=FAKE, heads=-1)), EINVAL), (dict(dim=2048, rotary=1026), ELAYOUT),
-    (dict(batch=1 << 16, seq=1 << 16), ELAYOUT),
+    (dict(batch=1 << 16, seq=1 << 16), ELAYOUT), (dict(dim=1 << 24), ELAYOUT),
     (dict(q=RotaryTensor()), 0), (dict(seq=0), 0), (dict(batch=0), 0),  # nothing to do
 ])
 def test_rotary_refuses(lib, kw, want):

@@ -374,6 +374,7 @@ RotaryArgs check_rotary(const char* op, const at::Tensor& q, const OptTensor& k,
                 ", got ", positions->sizes());
   }
   TORCH_CHECK(s.batch * s.seq < (int64_t(1) << 31), op, ": expected fewer than 2^31 tokens");
+  TORCH_CHECK(s.dim < (int64_t(1) << 24), op, ": expected heads of fewer than 2^24 elements, got ", s.dim);
   // frequencies of another type are widened, not formed anew
   return {frequencies.to(at::kDouble).contiguous(), positions, offset, interleaved, scale, inverse};
 }

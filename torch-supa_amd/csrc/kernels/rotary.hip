@@ -178,8 +178,8 @@ __global__ void __launch_bounds__(kRotBlock) k_rotary(RotArgs g) {
   if (unit < all) request();
   for (int i = threadIdx.x; i < g.per * pairs; i += blockDim.x) {
     const int tk = i / pairs;
-    const int32_t token = token0 + tk;
-    if (token < g.tokens) {
+    if (tk < g.tokens - token0) {  // token0 + tk may pass 2^31
+      const int32_t token = token0 + tk;
       uint32_t bi, si;
       g.seq.divmod((uint32_t)token, bi, si);
       int64_t p = si;
@@ -310,7 +310,7 @@ extern "C" int supa_amd_rotary(const supa_amd_rotary_desc* d, void* stream) {
   if (!d->frequencies) return SUPA_AMD_EINVAL;
   for (const supa_amd_rotary_tensor* t : {&d->q, &d->k})
     if (t->in && (!t->out || t->heads < 0)) return SUPA_AMD_EINVAL;
-  if (d->rotary > 2 * kRotMaxPairs || d->dim >= (int64_t(1) << 30) || d->q.heads >= (int64_t(1) << 30) ||
+  if (d->rotary > 2 * kRotMaxPairs || d->dim >= (int64_t(1) << 24) || d->q.heads >= (int64_t(1) << 30) ||
       d->k.heads >= (int64_t(1) << 30) ||
       (d->batch > 0 && d->seq >= (int64_t(1) << 31) / d->batch))
     return SUPA_AMD_ELAYOUT;
