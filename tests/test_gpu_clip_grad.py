@@ -134,6 +134,17 @@ def test_layouts(no_fallback):
     assert torch.equal(dbig.cpu().reshape(-1)[:3], big.reshape(-1)[:3]) and torch.equal(dbig.cpu().reshape(-1)[4004:], big.reshape(-1)[4004:])
 
 
+def test_more_than_2_31_elements(no_fallback):
+    """The last elements of a long tensor count and are scaled."""
+    x = torch.zeros(2 ** 31 + 77, dtype=BF16, device="supa")
+    x[-3:] = 4.0
+    x[2 ** 31 - 1] = 1.0
+    n = torch.supa.clip_grad_norm_(as_params([x]), 3.5)
+    assert float(n) == 7.0
+    # a factor of 3.5 / 7.000001, off from a half by 2^-22 of it: to the nearest bfloat16, a half
+    assert (x[-3:].cpu() == 2.0).all() and float(x[2 ** 31 - 1]) == 0.5 and float(x[2 ** 31]) == 0.0
+
+
 def test_argument_forms(no_fallback):
     p = torch.ones(3, device="supa")
     assert float(torch.supa.clip_grad_norm_(p, 1.0)) == 0.0  # no gradient

@@ -300,6 +300,22 @@ def test_changed_or_used_twice(no_fallback):
         y.sum().backward()
 
 
+def test_offsets_past_32_bits(no_fallback):
+    """Rows that lie 2^30 elements apart: the same bits as from close ones."""
+    g = torch.Generator().manual_seed(12)
+    near = torch.randn(3, 300, generator=g).bfloat16().to("supa")
+    room = torch.empty(2 ** 31 + 400, dtype=torch.bfloat16, device="supa")
+    far = room.as_strided((3, 300), (2 ** 30, 1), 5)
+    far.copy_(near)
+    w = torch.randn(300, generator=g).bfloat16().to("supa").requires_grad_()
+    outs = []
+    for t in (near, far):
+        x, r = t.detach().requires_grad_(), t.detach().requires_grad_()
+        h, y = torch.supa.residual_norm(x, r, post_norm="layer", post_weight=w, weight=w)
+        outs.append([o.detach().cpu() for o in (h, y, *torch.autograd.grad(h.sum() + y.sum(), [x, r, w]))])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
 def test_zero_nan_and_infinite_rows(no_fallback):
     d, gh, gy = make((6, 1000), "bf16", "bf16", "bf16", "channel", "rms", "rms", 9)
     dev = {k: t.to("supa") for k, t in d.items()}
