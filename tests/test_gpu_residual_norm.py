@@ -392,3 +392,8 @@ def test_refusals(supa):
     y = f(xg, x)[1]
     with pytest.raises(RuntimeError, match="create_graph"):
         torch.autograd.grad(y.sum(), xg, create_graph=True)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w, w)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            f(x, x, weight=dual)
+        assert f(x, x, weight=w)[0].shape == x.shape

@@ -242,3 +242,8 @@ def test_refusals(supa):
         put(torch.ones(1, 5, 3, 8, device="supa").expand(2, 5, 3, 8), None, f)
     with pytest.raises(RuntimeError, match="no gradient"):
         put(q.clone().requires_grad_(), None, f)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(q, q.clone())
+        for call in (rot, put):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual, None, f)

@@ -31,6 +31,17 @@ bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 OptTensor maybe(const at::Tensor& t) { return t.defined() ? OptTensor(t) : std::nullopt; }
 const void* ptr(const OptTensor& t) { return given(t) ? t->data_ptr() : nullptr; }
 
+// Values of forward-mode differentiation would be dropped without a word.
+void check_no_tangent(const char* op, std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), op,
+                                ": no forward-mode derivative");
+}
+const at::Tensor& tensor(const OptTensor& t) {
+  static const at::Tensor none;
+  return given(t) ? *t : none;
+}
+
 void check_on(const char* op, const char* name, const at::Tensor& t, const at::Tensor& like) {
   TORCH_CHECK(t.device() == like.device(), op, ": ", name, " is on ", t.device(), ", expected ", like.device());
 }
@@ -277,6 +288,8 @@ std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(const at::Tensor& x, c
                                                           const OptTensor& post_weight, const OptTensor& post_bias,
                                                           int64_t norm, const OptTensor& weight, const OptTensor& bias,
                                                           double eps) {
+  check_no_tangent("residual_norm", {&x, &residual, &tensor(gate), &tensor(post_weight), &tensor(post_bias),
+                                     &tensor(weight), &tensor(bias)});
   bool needs = x.requires_grad() || residual.requires_grad();
   for (const OptTensor* t : {&gate, &post_weight, &post_bias, &weight, &bias})
     needs = needs || (given(*t) && (*t)->requires_grad());
@@ -532,6 +545,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q
                                                              const at::Tensor& frequencies, const OptTensor& positions,
                                                              int64_t offset, bool interleaved, double scale,
                                                              bool inverse) {
+  check_no_tangent("rotary_embedding", {&q, &tensor(k), &frequencies});
   const bool needs = q.requires_grad() || (given(k) && k->requires_grad());
   TORCH_CHECK(!frequencies.requires_grad(), "rotary_embedding: frequencies have no gradient");
   if (!needs || !at::GradMode::is_enabled()) {
@@ -565,6 +579,7 @@ void rotary_embedding_autograd_(at::Tensor& q, const OptTensor& k, const at::Ten
                                 bool inverse) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || (given(k) && k->requires_grad())),
               "rotary_embedding_: the call in place has no gradient; use rotary_embedding");
+  check_no_tangent("rotary_embedding_", {&q, &tensor(k), &frequencies});
   const at::AutoDispatchBelowAutograd below;
   rotary_embedding_(q, k, frequencies, positions, offset, interleaved, scale, inverse);
   written(q);
