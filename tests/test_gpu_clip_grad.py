@@ -145,6 +145,25 @@ def test_more_than_2_31_elements(no_fallback):
     assert (x[-3:].cpu() == 2.0).all() and float(x[2 ** 31 - 1]) == 0.5 and float(x[2 ** 31]) == 0.0
 
 
+def test_columns_of_one_buffer(no_fallback):
+    """Tensors that reach over each other's memory without sharing any of it; two
+    that share some are refused with nothing written."""
+    host = torch.randn(40, 30, generator=torch.Generator().manual_seed(4))
+    dev = host.to("supa")
+    parts = lambda t: [t[:, :7], t[:, 20:], t[:, 7:20]]  # noqa: E731
+    norm = norm_of([host], 2)
+    assert float(torch.supa.clip_grad_norm_(as_params(parts(dev)), norm / 2)) == pytest.approx(norm, rel=1e-6)
+    torch.testing.assert_close(dev.cpu(), host * 0.5, rtol=4 * 2.0 ** -24 + 1e-6 / norm, atol=0)
+    line = torch.ones(9, device="supa")
+    assert float(torch.supa.clip_grad_norm_(as_params([line[::2], line[1::2]]), 1.0)) == 3.0
+    before = dev.cpu()
+    for pair in ([dev[:, :8], dev[:, 7:20]], [dev, dev[:, 3:9]], [dev[:, 3:9], dev[3]], [dev[:, 3:9], dev[:, 5:9].t()],
+                 [dev[:20, :4], dev[19:, :4]]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            torch.supa.clip_grad_norm_(as_params(pair), 0.1)
+    assert torch.equal(dev.cpu(), before)
+
+
 def test_argument_forms(no_fallback):
     p = torch.ones(3, device="supa")
     assert float(torch.supa.clip_grad_norm_(p, 1.0)) == 0.0  # no gradient

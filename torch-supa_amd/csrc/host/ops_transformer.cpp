@@ -451,11 +451,14 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const O
 }
 
 // Whether blocks of `block` elements, one at every index of the dims before
-// `dims`, keep apart: each dim steps over all that the smaller steps reach.
-bool apart(const at::Tensor& t, int64_t dims, int64_t block) {
+// `dims`, keep apart: each dim steps over all that the smaller steps reach.  The
+// dims are as long as t's or, if there is one, the other tensor's, the longer.
+bool apart(const at::Tensor& t, int64_t dims, int64_t block, const at::Tensor& other = {}) {
   std::vector<std::pair<int64_t, int64_t>> steps;  // stride, size
-  for (int64_t i = 0; i < dims; ++i)
-    if (t.size(i) > 1) steps.emplace_back(t.stride(i), t.size(i));
+  for (int64_t i = 0; i < dims; ++i) {
+    const int64_t size = other.defined() ? std::max(t.size(i), other.size(i)) : t.size(i);
+    if (size > 1) steps.emplace_back(t.stride(i), size);
+  }
   std::sort(steps.begin(), steps.end());
   for (const auto& [stride, size] : steps) {
     if (stride < block) return false;
@@ -464,9 +467,10 @@ bool apart(const at::Tensor& t, int64_t dims, int64_t block) {
   return true;
 }
 
-// Whether q and k share no element: over some of the trailing dims k lies beside
-// q, and the dims before step alike from one such pair to the next (q and k of
-// a packed projection, token by token or sample by sample).
+// Whether q and k, of one type and number of dims, share no element: over some of
+// the trailing dims (or none) k lies beside q, and the dims before step alike from
+// one such pair to the next (q and k of a packed projection, token by token or
+// sample by sample).
 bool beside(const at::Tensor& q, const at::Tensor& k) {
   const int64_t nd = q.dim();
   // elements from the first to behind the last, over the dims from `from` on
@@ -478,11 +482,11 @@ bool beside(const at::Tensor& q, const at::Tensor& k) {
   const int64_t shift = (static_cast<const char*>(k.data_ptr()) - static_cast<const char*>(q.data_ptr())) /
                         (int64_t)q.element_size();
   const int64_t gap = std::abs(shift);
-  for (int64_t from = 0; from <= nd - 2; ++from) {
+  for (int64_t from = 0; from <= nd; ++from) {
     bool alike = true;
-    for (int64_t i = 0; i < from; ++i) alike = alike && (q.size(i) == 1 || q.stride(i) == k.stride(i));
+    for (int64_t i = 0; i < from; ++i) alike = alike && ((q.size(i) == 1 && k.size(i) == 1) || q.stride(i) == k.stride(i));
     const int64_t first = extent(shift >= 0 ? q : k, from), second = extent(shift >= 0 ? k : q, from);
-    if (alike && first <= gap && apart(q, from, gap + second)) return true;
+    if (alike && first <= gap && apart(q, from, gap + second, k)) return true;
   }
   return false;
 }
@@ -595,11 +599,11 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   const c10::Device device = grads[0].device();
   const size_t n = grads.size();
   std::vector<at::Tensor> copies;         // of tensors that are not dense, in the list's order
-  std::vector<const void*> copied;        // and where those begin
   std::vector<void*> p(n);
   std::vector<int64_t> numel(n);
   std::vector<int32_t> dtypes(n);
-  std::vector<std::pair<const char*, const char*>> spans;
+  // the memory from a tensor's first element to behind its last, and the tensor
+  std::vector<std::tuple<const char*, const char*, size_t>> spans;
   spans.reserve(n);
   at::ScalarType norm_type = at::kFloat;
   const c10::OptionalDeviceGuard guard(device);
@@ -616,21 +620,27 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
       at::assert_no_internal_overlap(g);
       x = g.contiguous();
       copies.push_back(x);
-      copied.push_back(g.data_ptr());
-    } else if (g.numel() > 0) {
+    }
+    if (g.numel() > 0) {
+      int64_t last = 0;
+      for (int64_t d = 0; d < g.dim(); ++d) last += (g.size(d) - 1) * g.stride(d);
       const char* at = static_cast<const char*>(g.data_ptr());
-      spans.emplace_back(at, at + g.numel() * (int64_t)g.element_size());
+      spans.emplace_back(at, at + (last + 1) * (int64_t)g.element_size(), i);
     }
     p[i] = x.data_ptr();
     numel[i] = x.numel();
     dtypes[i] = dtype_code(t);
   }
+  // two that reach over each other have to lie beside each other, as the columns of a matrix do
   std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
-    TORCH_CHECK(spans[i - 1].second <= spans[i].first, op, ": two of the tensors share memory");
-  std::sort(copied.begin(), copied.end());
-  TORCH_CHECK(std::adjacent_find(copied.begin(), copied.end()) == copied.end(), op,
-              ": two of the tensors share memory");
+  for (size_t i = 0; i < spans.size(); ++i) {
+    const auto& [at, end, one] = spans[i];
+    for (size_t j = i + 1; j < spans.size() && std::get<0>(spans[j]) < end; ++j) {
+      const at::Tensor &a = grads[one], &b = grads[std::get<2>(spans[j])];
+      TORCH_CHECK(a.scalar_type() == b.scalar_type() && a.dim() == b.dim() && beside(a, b), op,
+                  ": two of the tensors share memory");
+    }
+  }
   const auto dev = device.index();
   const int64_t ws_bytes = supa_amd_grad_norm_workspace_bytes((int32_t)n, numel.data(), dtypes.data());
   TORCH_CHECK(ws_bytes >= 0, op, ": ", supa_amd_status_string((int)ws_bytes));
