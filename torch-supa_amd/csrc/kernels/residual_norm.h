@@ -968,7 +968,8 @@ int rn_backward_t(const supa_amd_residual_norm_desc* d, const RnArgs& a, const R
       constexpr auto kernel = k_residual_norm_backward<T, R, G.value, E.value, post.value, layer.value, own.value>;
       constexpr int lds = RnKeep<G.value, E.value>::bytes(layer.value);
       constexpr int block = rn_bwd_block(G.value, rn_light(sizeof(T), E.value, post.value, layer.value, own.value));
-      if constexpr (lds > 65536) {  // more than a launch has without asking; once a device
+      // with the static part it may take more than a launch has without asking; once a device
+      if constexpr (lds > 32768) {
         static std::atomic<uint64_t> asked{0};
         int dev = 0;
         const hipError_t e = hipGetDevice(&dev);
