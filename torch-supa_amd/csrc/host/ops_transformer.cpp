@@ -393,6 +393,7 @@ RotaryArgs check_rotary(const char* op, const at::Tensor& q, const OptTensor& k,
 }
 
 supa_amd_rotary_tensor rotary_tensor(const at::Tensor& in, const at::Tensor& out) {
+  TORCH_INTERNAL_ASSERT(in.stride(-1) == 1 && out.stride(-1) == 1);
   supa_amd_rotary_tensor t{};
   t.in = in.data_ptr();
   t.out = out.data_ptr();
@@ -433,8 +434,13 @@ void launch_rotary(const char* op, const at::Tensor& q, const at::Tensor& q_out,
   check_status(supa_amd_rotary(&d, current_stream(q.device().index())), op);
 }
 
-at::Tensor heads_contiguous(const at::Tensor& t) {
-  return t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+at::Tensor heads_contiguous(const at::Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+
+// An output in t's order of dims.  Of windows that slide over each other the strides
+// do not say which dim is innermost, and empty_like may take another than the last.
+at::Tensor rotated_like(const at::Tensor& t) {
+  const at::Tensor out = at::empty_like(t);
+  return out.stride(-1) == 1 ? out : at::empty_like(t, at::MemoryFormat::Contiguous);
 }
 
 std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const OptTensor& k,
@@ -443,9 +449,8 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const O
   constexpr const char* op = "rotary_embedding";
   const c10::OptionalDeviceGuard guard(q.device());
   const RotaryArgs a = check_rotary(op, q, k, frequencies, positions, offset, interleaved, scale, inverse);
-  // the outputs keep their inputs' order of dims where these are dense
   const at::Tensor qi = heads_contiguous(q), ki = given(k) ? heads_contiguous(*k) : at::Tensor();
-  const at::Tensor qo = at::empty_like(qi), ko = ki.defined() ? at::empty_like(ki) : at::Tensor();
+  const at::Tensor qo = rotated_like(qi), ko = ki.defined() ? rotated_like(ki) : at::Tensor();
   launch_rotary(op, qi, qo, ki, ko, a);
   return {qo, ko};
 }
@@ -498,7 +503,7 @@ void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& freq
   const RotaryArgs a = check_rotary(op, q, k, frequencies, positions, offset, interleaved, scale, inverse);
   for (const at::Tensor* t : {(const at::Tensor*)&q, given(k) ? &*k : nullptr}) {
     if (!t || t->numel() == 0) continue;
-    TORCH_CHECK(t->size(-1) == 1 || t->stride(-1) == 1, op, ": expected heads whose elements are contiguous");
+    TORCH_CHECK(t->stride(-1) == 1, op, ": expected heads whose elements are contiguous");
     TORCH_CHECK(apart(*t, t->dim() - 1, t->size(-1)), op, ": expected a tensor whose heads do not overlap in memory");
   }
   if (given(k) && q.numel() > 0 && k->numel() > 0)
