@@ -199,8 +199,11 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::
 // A node of its own, with plain fields, instead of a custom Function: the small
 // calls of training are bound by the host, and it takes 6 us off a pass.  x and
 // residual are saved for the backward, which forms h from them again; without
-// post norm and gate h alone is enough, as long as it is not rounded more
-// coarsely than the weight's gradient it enters.
+// post norm and gate h alone is enough where it is float32.  A 16-bit h, once rounded,
+// is off by half a step of its own, which a layer norm magnifies by mean / deviation
+// of the row ([3, 11, 520] bf16, mean 8, deviation 0.25: gradients off by 6 half steps
+// of theirs); forming it again costs a read ([8192, 4096] bf16, RMS norm, both ways:
+// 118 us, from the rounded h 107; [16384, 8192] 452, 397).
 struct ResidualNormBackward final : public torch::autograd::Node {
   // the inputs' places, in the order of the edges
   enum { kX, kResidual, kGate, kPostWeight, kPostBias, kWeight, kBias, kInputs };
@@ -315,9 +318,8 @@ std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(const at::Tensor& x, c
                     w = contiguous(weight), b = contiguous(bias);
     r = residual_norm_forward(xr, rr, g, a, pw, pb, w, b, true);
     node->d = norm_desc(xr, rr, g, a, pw, pb, w, b);
-    const bool wide = given(weight) && weight->scalar_type() == at::kFloat;
     const bool from_h = !given(gate) && post == SUPA_AMD_NORM_NONE &&
-                        (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat || !wide);
+                        (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat);
     const bool needs_h = norm != SUPA_AMD_NORM_NONE;
     if (!from_h) node->x = SavedVariable(xr.t, false);
     if (!from_h && needs_h) node->residual = SavedVariable(rr.t, false);

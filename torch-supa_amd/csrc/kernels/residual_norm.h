@@ -3,7 +3,7 @@
 // (N an RMS or layer norm, or absent), and its gradients.
 //
 // HBM-bound: the forward reads x and r and writes h and y, once each; the
-// backward reads x, r (or h alone where neither gate nor post norm needs x), dh
+// backward reads x, r (or a float32 h alone where neither gate nor post norm needs x), dh
 // and dy and writes dx and dr.  A row stays in the registers of the G threads
 // that share it (row_group.h), as float32, so that its statistics are taken in
 // two passes over registers: the mean, then the deviations from it.
