@@ -4,7 +4,14 @@
 // (torch_supa/supa/transformer.py).  Arguments are checked here; the device
 // work is the C ABI's, on the tensors' device and its current stream, with
 // workspaces from the caching allocator.
+//
+// Every call goes through the dispatcher below autograd, forward and backward, so
+// that dispatch modes see it and tensors that wrap others (fake tensors, those of
+// function transforms) reach a kernel that knows them; Meta kernels give the
+// results' shapes.
 #include <ATen/MemoryOverlap.h>
+#include <ATen/core/LegacyTypeDispatch.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -12,6 +19,7 @@
 #include <torch/library.h>
 
 #include <algorithm>
+#include <array>
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -40,6 +48,17 @@ void check_no_tangent(const char* op, std::initializer_list<const at::Tensor*> t
 const at::Tensor& tensor(const OptTensor& t) {
   static const at::Tensor none;
   return given(t) ? *t : none;
+}
+
+// The operator of this schema name, called through the dispatcher.
+template <typename F> c10::TypedOperatorHandle<F> find_op(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<F>();
+}
+
+// Meta tensors stand for supa ones.
+bool is_supa(const at::Tensor& t) { return t.device().type() == kSupa || t.is_meta(); }
+at::Tensor empty_beside(const at::Tensor& t, c10::IntArrayRef sizes, at::ScalarType dtype) {
+  return t.is_meta() ? at::empty(sizes, t.options().dtype(dtype)) : empty_supa(sizes, dtype, t.device().index());
 }
 
 void check_on(const char* op, const char* name, const at::Tensor& t, const at::Tensor& like) {
@@ -91,32 +110,33 @@ int64_t gate_period(const at::Tensor& gate, const at::Tensor& x) {
   return period;
 }
 
-void check_residual_norm(const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate, NormArgs& a,
-                         const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& weight,
-                         const OptTensor& bias) {
-  constexpr const char* op = "residual_norm";
-  TORCH_CHECK(x.device().type() == kSupa, op, ": expected supa tensors, got x on ", x.device());
-  check_on(op, "residual", residual, x);
-  TORCH_CHECK(is_float16_or_32(x.scalar_type()), op, ": expected float32, bfloat16 or float16, got x of ",
-              x.scalar_type());
-  TORCH_CHECK(x.dim() >= 1, op, ": expected x with a last dim to normalise, got a scalar");
-  TORCH_CHECK(x.sizes() == residual.sizes(), op, ": x is of shape ", x.sizes(), ", residual of ", residual.sizes());
-  TORCH_CHECK(residual.scalar_type() == x.scalar_type() || residual.scalar_type() == at::kFloat, op,
-              ": expected residual of x's dtype (", x.scalar_type(), ") or float32, got ", residual.scalar_type());
-  const int64_t width = x.size(-1);
+// What a call has beside x and residual.
+struct NormParams {
+  OptTensor gate, post_weight, post_bias, weight, bias;
+};
+
+// Sizes, types, norms and parameters, forward and backward; `like` has x's shape.
+void check_norm(const char* op, const at::Tensor& like, at::ScalarType dtype, at::ScalarType residual_dtype, NormArgs& a,
+                const NormParams& p) {
+  TORCH_CHECK(is_float16_or_32(dtype), op, ": expected float32, bfloat16 or float16, got x of ", dtype);
+  TORCH_CHECK(like.dim() >= 1, op, ": expected x with a last dim to normalise, got a scalar");
+  TORCH_CHECK(residual_dtype == dtype || residual_dtype == at::kFloat, op, ": expected residual of x's dtype (", dtype,
+              ") or float32, got ", residual_dtype);
+  const int64_t width = like.size(-1);
   TORCH_CHECK(width >= 1 && width <= SUPA_AMD_RESIDUAL_NORM_MAX_WIDTH, op, ": the last dim holds ", width,
               " elements, expected 1 to ", SUPA_AMD_RESIDUAL_NORM_MAX_WIDTH);
-  TORCH_CHECK(x.numel() / width < (int64_t(1) << 31), op, ": expected fewer than 2^31 rows");
+  TORCH_CHECK(like.numel() / width < (int64_t(1) << 31), op, ": expected fewer than 2^31 rows");
   TORCH_CHECK(std::isfinite(a.eps) && a.eps >= 0, op, ": expected eps >= 0, got ", a.eps);
+  for (int64_t n : {a.post, a.norm})
+    TORCH_CHECK(n >= SUPA_AMD_NORM_NONE && n <= SUPA_AMD_NORM_LAYER, op, ": no norm has number ", n);
   std::optional<at::ScalarType> param;
   const auto check_param = [&](const char* name, const OptTensor& t) {
     if (!given(t)) return;
-    check_on(op, name, *t, x);
-    const at::ScalarType p = t->scalar_type();
-    TORCH_CHECK(p == x.scalar_type() || p == at::kFloat, op, ": expected ", name, " of x's dtype (", x.scalar_type(),
-                ") or float32, got ", p);
-    TORCH_CHECK(!param || *param == p, op, ": gate, weights and biases are of one dtype, got ", *param, " and ", p);
-    param = p;
+    check_on(op, name, *t, like);
+    const at::ScalarType s = t->scalar_type();
+    TORCH_CHECK(s == dtype || s == at::kFloat, op, ": expected ", name, " of x's dtype (", dtype, ") or float32, got ", s);
+    TORCH_CHECK(!param || *param == s, op, ": gate, weights and biases are of one dtype, got ", *param, " and ", s);
+    param = s;
   };
   const auto check_vector = [&](const char* name, const OptTensor& t, bool allowed, const char* when) {
     if (!given(t)) return;
@@ -125,75 +145,196 @@ void check_residual_norm(const at::Tensor& x, const at::Tensor& residual, const 
                 t->sizes());
     check_param(name, t);
   };
-  check_vector("post_weight", post_weight, a.post != SUPA_AMD_NORM_NONE, "without a post norm");
-  check_vector("post_bias", post_bias, a.post == SUPA_AMD_NORM_LAYER, "with a post norm that is not a layer norm");
-  check_vector("weight", weight, a.norm != SUPA_AMD_NORM_NONE, "without a norm");
-  check_vector("bias", bias, a.norm == SUPA_AMD_NORM_LAYER, "with a norm that is not a layer norm");
-  check_param("gate", gate);
-  a.period = given(gate) ? gate_period(*gate, x) : 1;
+  check_vector("post_weight", p.post_weight, a.post != SUPA_AMD_NORM_NONE, "without a post norm");
+  check_vector("post_bias", p.post_bias, a.post == SUPA_AMD_NORM_LAYER, "with a post norm that is not a layer norm");
+  check_vector("weight", p.weight, a.norm != SUPA_AMD_NORM_NONE, "without a norm");
+  check_vector("bias", p.bias, a.norm == SUPA_AMD_NORM_LAYER, "with a norm that is not a layer norm");
+  check_param("gate", p.gate);
+  a.period = given(p.gate) ? gate_period(*p.gate, like) : 1;
+}
+
+void check_residual_norm(const at::Tensor& x, const at::Tensor& residual, NormArgs& a, const NormParams& p) {
+  constexpr const char* op = "residual_norm";
+  TORCH_CHECK(is_supa(x), op, ": expected supa tensors, got x on ", x.device());
+  check_on(op, "residual", residual, x);
+  TORCH_CHECK(x.sizes() == residual.sizes(), op, ": x is of shape ", x.sizes(), ", residual of ", residual.sizes());
+  check_norm(op, x, x.scalar_type(), residual.scalar_type(), a, p);
 }
 
 OptTensor contiguous(const OptTensor& t) { return given(t) ? OptTensor(t->contiguous()) : std::nullopt; }
 
-supa_amd_residual_norm_desc norm_desc(const Rows& x, const Rows& residual, const OptTensor& gate, const NormArgs& a,
-                                      const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& weight,
-                                      const OptTensor& bias) {
+NormParams contiguous(const NormParams& p) {
+  return {contiguous(p.gate), contiguous(p.post_weight), contiguous(p.post_bias), contiguous(p.weight),
+          contiguous(p.bias)};
+}
+
+supa_amd_residual_norm_desc norm_desc(int64_t rows, int64_t width, at::ScalarType dtype, at::ScalarType residual_dtype,
+                                      const NormArgs& a, const NormParams& p) {
   supa_amd_residual_norm_desc d{};
-  d.width = x.t.size(-1);
-  d.rows = x.t.numel() / d.width;
-  d.x_stride = x.stride;
-  d.residual_stride = residual.stride;
+  d.width = width;
+  d.rows = rows;
+  d.x_stride = d.residual_stride = width;
   d.gate_period = a.period;
-  d.dtype = dtype_code(x.t.scalar_type());
-  d.residual_dtype = dtype_code(residual.t.scalar_type());
+  d.dtype = dtype_code(dtype);
+  d.residual_dtype = dtype_code(residual_dtype);
   d.param_dtype = d.dtype;
-  for (const OptTensor* t : {&gate, &post_weight, &post_bias, &weight, &bias})
+  for (const OptTensor* t : {&p.gate, &p.post_weight, &p.post_bias, &p.weight, &p.bias})
     if (given(*t)) d.param_dtype = dtype_code((*t)->scalar_type());
   d.post_norm = (int32_t)a.post;
   d.norm = (int32_t)a.norm;
   d.residual_scale = a.scale;
   d.eps = a.eps;
-  d.x = x.t.data_ptr();
-  d.residual = residual.t.data_ptr();
-  d.gate = ptr(gate);
-  d.post_weight = ptr(post_weight);
-  d.post_bias = ptr(post_bias);
-  d.weight = ptr(weight);
-  d.bias = ptr(bias);
+  d.gate = ptr(p.gate);
+  d.post_weight = ptr(p.post_weight);
+  d.post_bias = ptr(p.post_bias);
+  d.weight = ptr(p.weight);
+  d.bias = ptr(p.bias);
   return d;
 }
 
-struct NormResult {
-  at::Tensor h, y, stats;
-};
-NormResult residual_norm_forward(const Rows& x, const Rows& residual, const OptTensor& gate, const NormArgs& a,
-                                 const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& weight,
-                                 const OptTensor& bias, bool want_stats) {
-  const auto dev = x.t.device().index();
-  NormResult r;
-  r.h = empty_supa(x.t.sizes(), residual.t.scalar_type(), dev);
-  if (a.norm != SUPA_AMD_NORM_NONE) r.y = empty_supa(x.t.sizes(), x.t.scalar_type(), dev);
-  if (x.t.numel() == 0) return r;
-  const supa_amd_residual_norm_desc d = norm_desc(x, residual, gate, a, post_weight, post_bias, weight, bias);
+// Outputs of a forward call: h, y (undefined without a norm), the rows' statistics
+// (if wanted and there is a norm).
+using NormResult = std::tuple<at::Tensor, at::Tensor, at::Tensor>;
+NormResult norm_outputs(const at::Tensor& x, const at::Tensor& residual, const NormArgs& a, bool want_stats) {
+  const int64_t rows[] = {x.numel() / x.size(-1), 4};
+  at::Tensor h = empty_beside(x, x.sizes(), residual.scalar_type()), y, stats;
+  if (a.norm != SUPA_AMD_NORM_NONE) y = empty_beside(x, x.sizes(), x.scalar_type());
   if (want_stats && (a.post != SUPA_AMD_NORM_NONE || a.norm != SUPA_AMD_NORM_NONE))
-    r.stats = empty_supa({d.rows, 4}, at::kFloat, dev);
-  check_status(supa_amd_residual_norm_forward(&d, r.h.data_ptr(), r.y.defined() ? r.y.data_ptr() : nullptr,
-                                              r.stats.defined() ? r.stats.data_ptr<float>() : nullptr,
-                                              current_stream(dev)),
+    stats = empty_beside(x, rows, at::kFloat);
+  return {h, y, stats};
+}
+
+NormResult norm_forward(const at::Tensor& x, const at::Tensor& residual, NormArgs a, const NormParams& params,
+                        bool want_stats) {
+  check_residual_norm(x, residual, a, params);
+  const c10::DeviceGuard guard(x.device());
+  const NormResult r = norm_outputs(x, residual, a, want_stats);
+  const auto& [h, y, stats] = r;
+  if (x.numel() == 0) return r;
+  const Rows xr = rows_of(x), rr = rows_of(residual);
+  const NormParams p = contiguous(params);
+  supa_amd_residual_norm_desc d =
+      norm_desc(x.numel() / x.size(-1), x.size(-1), x.scalar_type(), residual.scalar_type(), a, p);
+  d.x = xr.t.data_ptr();
+  d.x_stride = xr.stride;
+  d.residual = rr.t.data_ptr();
+  d.residual_stride = rr.stride;
+  check_status(supa_amd_residual_norm_forward(&d, h.data_ptr(), y.defined() ? y.data_ptr() : nullptr,
+                                              stats.defined() ? stats.data_ptr<float>() : nullptr,
+                                              current_stream(x.device().index())),
                "residual_norm");
   return r;
 }
 
-std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::Tensor& residual, const OptTensor& gate,
-                                                 double residual_scale, int64_t post_norm, const OptTensor& post_weight,
-                                                 const OptTensor& post_bias, int64_t norm, const OptTensor& weight,
-                                                 const OptTensor& bias, double eps) {
-  NormArgs a{residual_scale, eps, post_norm, norm, 1};
-  check_residual_norm(x, residual, gate, a, post_weight, post_bias, weight, bias);
-  const c10::DeviceGuard guard(x.device());
-  NormResult r = residual_norm_forward(rows_of(x), rows_of(residual), contiguous(gate), a, contiguous(post_weight),
-                                       contiguous(post_bias), contiguous(weight), contiguous(bias), false);
-  return {r.h, r.y};
+#define SUPA_NORM_PARAMS                                                                                             \
+  const at::Tensor &x, const at::Tensor &residual, const OptTensor &gate, double scale, int64_t post,                \
+      const OptTensor &post_weight, const OptTensor &post_bias, int64_t norm, const OptTensor &weight,               \
+      const OptTensor &bias, double eps
+
+std::tuple<at::Tensor, at::Tensor> residual_norm(SUPA_NORM_PARAMS) {
+  auto [h, y, stats] = norm_forward(x, residual, {scale, eps, post, norm, 1},
+                                    {gate, post_weight, post_bias, weight, bias}, false);
+  return {h, y};
+}
+NormResult residual_norm_forward(SUPA_NORM_PARAMS) {
+  return norm_forward(x, residual, {scale, eps, post, norm, 1}, {gate, post_weight, post_bias, weight, bias}, true);
+}
+
+std::tuple<at::Tensor, at::Tensor> residual_norm_meta(SUPA_NORM_PARAMS) {
+  NormArgs a{scale, eps, post, norm, 1};
+  check_residual_norm(x, residual, a, {gate, post_weight, post_bias, weight, bias});
+  auto [h, y, stats] = norm_outputs(x, residual, a, false);
+  return {h, y};
+}
+NormResult residual_norm_forward_meta(SUPA_NORM_PARAMS) {
+  NormArgs a{scale, eps, post, norm, 1};
+  check_residual_norm(x, residual, a, {gate, post_weight, post_bias, weight, bias});
+  return norm_outputs(x, residual, a, true);
+}
+
+// The inputs' places among the gradients.
+enum NormInput { kX, kResidual, kGate, kPostWeight, kPostBias, kWeight, kBias, kNormInputs };
+using NormGrads = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
+
+// What the backward reads: the gradients of h and y (one of them at least), x and
+// residual or, in their place, h; the forward's statistics; its other arguments.
+#define SUPA_NORM_BACKWARD_PARAMS                                                                                    \
+  const OptTensor &grad_h, const OptTensor &grad_y, const OptTensor &x, const OptTensor &residual,                   \
+      const OptTensor &h, const OptTensor &stats, const OptTensor &gate, double scale, int64_t post,                 \
+      const OptTensor &post_weight, const OptTensor &post_bias, int64_t norm, const OptTensor &weight,               \
+      const OptTensor &bias, double eps, at::ScalarType dtype, at::ScalarType residual_dtype,                        \
+      std::array<bool, 7> wanted
+
+// Checks the arguments and allocates the gradients that are wanted.
+std::array<at::Tensor, kNormInputs> norm_grads(SUPA_NORM_BACKWARD_PARAMS, NormArgs& a) {
+  constexpr const char* op = "residual_norm (backward)";
+  TORCH_CHECK(given(grad_h) || given(grad_y), op, ": expected a gradient of h or y");
+  const at::Tensor& like = given(grad_h) ? *grad_h : *grad_y;
+  TORCH_CHECK(is_supa(like), op, ": expected supa tensors, got a gradient on ", like.device());
+  check_norm(op, like, dtype, residual_dtype, a, {gate, post_weight, post_bias, weight, bias});
+  const int64_t rows[] = {like.numel() / like.size(-1), 4};
+  const auto check = [&](const char* name, const OptTensor& t, at::ScalarType type, c10::IntArrayRef sizes) {
+    if (!given(t)) return;
+    check_on(op, name, *t, like);
+    TORCH_CHECK(t->scalar_type() == type && t->sizes() == sizes, op, ": expected ", name, " of ", type, " and shape ",
+                sizes, ", got ", t->scalar_type(), " of ", t->sizes());
+  };
+  check("grad_h", grad_h, residual_dtype, like.sizes());
+  check("grad_y", grad_y, dtype, like.sizes());
+  check("x", x, dtype, like.sizes());
+  check("residual", residual, residual_dtype, like.sizes());
+  check("h", h, residual_dtype, like.sizes());
+  check("stats", stats, at::kFloat, rows);
+  const OptTensor* params[] = {&gate, &post_weight, &post_bias, &weight, &bias};
+  std::array<at::Tensor, kNormInputs> out;
+  if (wanted[kX]) out[kX] = empty_beside(like, like.sizes(), dtype);
+  if (wanted[kResidual]) out[kResidual] = empty_beside(like, like.sizes(), residual_dtype);
+  for (int i = kGate; i < kNormInputs; ++i)
+    if (const OptTensor& p = *params[i - kGate]; wanted[i] && given(p))
+      out[i] = empty_beside(like, p->sizes(), p->scalar_type());
+  return out;
+}
+
+NormGrads residual_norm_backward(SUPA_NORM_BACKWARD_PARAMS) {
+  NormArgs a{scale, eps, post, norm, 1};
+  const at::Tensor& like = given(grad_h) ? *grad_h : tensor(grad_y);
+  const c10::OptionalDeviceGuard guard(like.defined() ? std::optional(like.device()) : std::nullopt);
+  auto out = norm_grads(grad_h, grad_y, x, residual, h, stats, gate, scale, post, post_weight, post_bias, norm, weight,
+                        bias, eps, dtype, residual_dtype, wanted, a);
+  if (like.numel() == 0) {
+    for (auto& t : out)
+      if (t.defined()) t.zero_();
+    return std::tuple_cat(out);
+  }
+  const OptTensor gh = contiguous(grad_h), gy = contiguous(grad_y), hc = contiguous(h), st = contiguous(stats);
+  const NormParams p = contiguous(NormParams{gate, post_weight, post_bias, weight, bias});
+  supa_amd_residual_norm_desc d = norm_desc(like.numel() / like.size(-1), like.size(-1), dtype, residual_dtype, a, p);
+  Rows xr{}, rr{};  // hold copies until the launch
+  if (given(x)) {
+    xr = rows_of(*x);
+    d.x = xr.t.data_ptr();
+    d.x_stride = xr.stride;
+  }
+  if (given(residual)) {
+    rr = rows_of(*residual);
+    d.residual = rr.t.data_ptr();
+    d.residual_stride = rr.stride;
+  }
+  const int64_t ws_bytes = supa_amd_residual_norm_backward_workspace_bytes(&d);
+  TORCH_CHECK(ws_bytes >= 0, "residual_norm: ", supa_amd_status_string((int)ws_bytes));
+  const auto dev = like.device().index();
+  const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
+  const auto data = [&](int i) -> void* { return out[i].defined() ? out[i].data_ptr() : nullptr; };
+  check_status(supa_amd_residual_norm_backward(&d, ptr(hc), ptr(gh), ptr(gy), static_cast<const float*>(ptr(st)), data(kX),
+                                               data(kResidual), data(kGate), data(kPostWeight), data(kPostBias),
+                                               data(kWeight), data(kBias), ws.data_ptr(), ws_bytes, current_stream(dev)),
+               "residual_norm (backward)");
+  return std::tuple_cat(out);
+}
+NormGrads residual_norm_backward_meta(SUPA_NORM_BACKWARD_PARAMS) {
+  NormArgs a{scale, eps, post, norm, 1};
+  return std::tuple_cat(norm_grads(grad_h, grad_y, x, residual, h, stats, gate, scale, post, post_weight, post_bias, norm,
+                                   weight, bias, eps, dtype, residual_dtype, wanted, a));
 }
 
 // A node of its own, with plain fields, instead of a custom Function: the small
@@ -205,9 +346,6 @@ std::tuple<at::Tensor, at::Tensor> residual_norm(const at::Tensor& x, const at::
 // of theirs); forming it again costs a read ([8192, 4096] bf16, RMS norm, both ways:
 // 118 us, from the rounded h 107; [16384, 8192] 452, 397).
 struct ResidualNormBackward final : public torch::autograd::Node {
-  // the inputs' places, in the order of the edges
-  enum { kX, kResidual, kGate, kPostWeight, kPostBias, kWeight, kBias, kInputs };
-
   std::string name() const override { return "ResidualNormBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
@@ -221,119 +359,99 @@ struct ResidualNormBackward final : public torch::autograd::Node {
   variable_list apply(variable_list&& grads) override {
     TORCH_CHECK(!at::GradMode::is_enabled(),
                 "residual_norm: the gradient has no gradient of its own (create_graph)");
-    variable_list out(kInputs);
-    if (!grads[0].defined() && !(grads.size() > 1 && grads[1].defined())) return out;
+    variable_list out(kNormInputs);
+    const OptTensor gh = maybe(grads[0]), gy = grads.size() > 1 ? maybe(grads[1]) : std::nullopt;
+    if (!gh && !gy) return out;
     std::lock_guard<std::mutex> lock(mutex_);
-    const at::Tensor gh = grads[0].defined() ? grads[0].contiguous() : at::Tensor();
-    const at::Tensor gy = grads.size() > 1 && grads[1].defined() ? grads[1].contiguous() : at::Tensor();
-    const c10::Device device = gh.defined() ? gh.device() : gy.device();
-    const c10::DeviceGuard guard(device);
-    // hooks on saved tensors (offloading, recomputation) may give them back with other strides
-    const auto back = [&](const SavedVariable& v, int32_t dtype, c10::IntArrayRef sizes) {
+    const c10::Device device = gh ? gh->device() : gy->device();
+    // hooks on saved tensors (offloading, recomputation) may give them back otherwise; other strides do no harm
+    const auto back = [&](const SavedVariable& v, std::optional<at::ScalarType> dtype, c10::IntArrayRef sizes) {
       const at::Tensor t = v.unpack(shared_from_this());
-      TORCH_CHECK(!t.defined() || (t.device() == device && dtype_code(t.scalar_type()) == dtype && t.sizes() == sizes),
+      TORCH_CHECK(!t.defined() || (t.device() == device && t.scalar_type() == dtype && t.sizes() == sizes),
                   "residual_norm: a saved tensor came back as ", t.scalar_type(), " of shape ", t.sizes(), " on ",
                   t.device(), ", expected shape ", sizes, " on ", device);
-      return t;
+      return maybe(t);
     };
-    const int64_t width[] = {d.width}, rows[] = {d.rows, 4};
-    at::Tensor xt = back(x, d.dtype, shape), rt = back(residual, d.residual_dtype, shape);
-    for (auto [t, stride] : {std::pair(&xt, &d.x_stride), std::pair(&rt, &d.residual_stride)}) {
-      if (!t->defined() || t->numel() == 0) continue;
-      const Rows r = rows_of(*t);
-      *t = r.t;
-      *stride = r.stride;
+    const int64_t width[] = {shape.back()}, rows[] = {stats_rows, 4};
+    const OptTensor xt = back(x, dtype, shape), rt = back(residual, residual_dtype, shape),
+                    ht = back(h, residual_dtype, shape), st = back(stats, at::kFloat, rows);
+    OptTensor p[kNormInputs];
+    std::array<bool, 7> wanted;
+    for (int i = 0; i < kNormInputs; ++i) {
+      wanted[i] = task_should_compute_output(i);
+      if (i >= kGate) p[i] = back(params[i], param_dtype, i == kGate ? c10::IntArrayRef(gate_shape) : c10::IntArrayRef(width));
     }
-    const auto dense = [](const at::Tensor& t) { return t.defined() ? t.contiguous() : t; };
-    const at::Tensor ht = dense(back(h, d.residual_dtype, shape)), st = dense(back(stats, SUPA_AMD_F32, rows));
-    at::Tensor p[kInputs];
-    for (int i = kGate; i < kInputs; ++i)
-      p[i] = dense(back(params[i], d.param_dtype, i == kGate ? c10::IntArrayRef(gate_shape) : c10::IntArrayRef(width)));
-    const auto dev = device.index();
-    const auto data = [](const at::Tensor& t) -> void* { return t.defined() ? t.data_ptr() : nullptr; };
-
-    d.x = data(xt);
-    d.residual = data(rt);
-    d.gate = data(p[kGate]);
-    d.post_weight = data(p[kPostWeight]);
-    d.post_bias = data(p[kPostBias]);
-    d.weight = data(p[kWeight]);
-    d.bias = data(p[kBias]);
-    if (task_should_compute_output(kX)) out[kX] = empty_supa(shape, (at::ScalarType)d.dtype, dev);
-    if (task_should_compute_output(kResidual)) out[kResidual] = empty_supa(shape, (at::ScalarType)d.residual_dtype, dev);
-    for (int i = kGate; i < kInputs; ++i)
-      if (p[i].defined() && task_should_compute_output(i))
-        out[i] = empty_supa(i == kGate ? c10::IntArrayRef(gate_shape) : p[i].sizes(), p[i].scalar_type(), dev);
-    if (d.rows == 0) {
-      for (auto& t : out)
-        if (t.defined()) t.zero_();
-      return out;
-    }
-    const int64_t ws_bytes = supa_amd_residual_norm_backward_workspace_bytes(&d);
-    TORCH_CHECK(ws_bytes >= 0, "residual_norm: ", supa_amd_status_string((int)ws_bytes));
-    const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
-    check_status(supa_amd_residual_norm_backward(&d, data(ht), data(gh), data(gy),
-                                                 st.defined() ? st.data_ptr<float>() : nullptr, data(out[kX]),
-                                                 data(out[kResidual]), data(out[kGate]), data(out[kPostWeight]),
-                                                 data(out[kPostBias]), data(out[kWeight]), data(out[kBias]),
-                                                 ws.data_ptr(), ws_bytes, current_stream(dev)),
-                 "residual_norm (backward)");
+    static const auto op = find_op<decltype(residual_norm_backward)>("supa::_residual_norm_backward");
+    const at::AutoDispatchBelowAutograd below;
+    std::tie(out[kX], out[kResidual], out[kGate], out[kPostWeight], out[kPostBias], out[kWeight], out[kBias]) =
+        op.call(gh, gy, xt, rt, ht, st, p[kGate], scale, post, p[kPostWeight], p[kPostBias], norm, p[kWeight], p[kBias],
+                eps, dtype, residual_dtype, wanted);
     return out;
   }
 
-  SavedVariable x, residual, h, stats, params[kInputs];
-  supa_amd_residual_norm_desc d{};  // its pointers are set from the saved tensors
+  SavedVariable x, residual, h, stats, params[kNormInputs];
+  at::ScalarType dtype, residual_dtype;
+  std::optional<at::ScalarType> param_dtype;
+  double scale, eps;
+  int64_t post, norm, stats_rows;
   std::vector<int64_t> shape, gate_shape;
 };
 
-std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(const at::Tensor& x, const at::Tensor& residual,
-                                                          const OptTensor& gate, double scale, int64_t post,
-                                                          const OptTensor& post_weight, const OptTensor& post_bias,
-                                                          int64_t norm, const OptTensor& weight, const OptTensor& bias,
-                                                          double eps) {
+std::tuple<at::Tensor, at::Tensor> residual_norm_autograd(c10::DispatchKeySet ks, SUPA_NORM_PARAMS) {
   check_no_tangent("residual_norm", {&x, &residual, &tensor(gate), &tensor(post_weight), &tensor(post_bias),
                                      &tensor(weight), &tensor(bias)});
+  const OptTensor* params[] = {&gate, &post_weight, &post_bias, &weight, &bias};
   bool needs = x.requires_grad() || residual.requires_grad();
-  for (const OptTensor* t : {&gate, &post_weight, &post_bias, &weight, &bias})
-    needs = needs || (given(*t) && (*t)->requires_grad());
+  for (const OptTensor* t : params) needs = needs || (given(*t) && (*t)->requires_grad());
   if (!needs || !at::GradMode::is_enabled()) {
+    static const auto op = find_op<decltype(residual_norm)>("supa::residual_norm");
     const at::AutoDispatchBelowAutograd below;
-    return residual_norm(x, residual, gate, scale, post, post_weight, post_bias, norm, weight, bias, eps);
+    return op.redispatch(ks & c10::after_autograd_keyset, x, residual, gate, scale, post, post_weight, post_bias, norm,
+                         weight, bias, eps);
   }
   NormArgs a{scale, eps, post, norm, 1};
-  check_residual_norm(x, residual, gate, a, post_weight, post_bias, weight, bias);
+  check_residual_norm(x, residual, a, {gate, post_weight, post_bias, weight, bias});
   auto node = std::shared_ptr<ResidualNormBackward>(new ResidualNormBackward(), torch::autograd::deleteNode);
-  using Node = ResidualNormBackward;
   const auto edge = [](const OptTensor& t) {
     return given(t) ? torch::autograd::impl::gradient_edge(*t) : torch::autograd::Edge();
   };
   node->set_next_edges({torch::autograd::impl::gradient_edge(x), torch::autograd::impl::gradient_edge(residual),
                         edge(gate), edge(post_weight), edge(post_bias), edge(weight), edge(bias)});
-  NormResult r;
+  at::Tensor xr, rr, h, y, stats;
+  OptTensor g;
   {
+    static const auto op = find_op<decltype(residual_norm_forward)>("supa::_residual_norm_forward");
     const at::AutoDispatchBelowAutograd below;
-    const c10::DeviceGuard guard(x.device());
-    const Rows xr = rows_of(x), rr = rows_of(residual);
-    const OptTensor g = contiguous(gate), pw = contiguous(post_weight), pb = contiguous(post_bias),
-                    w = contiguous(weight), b = contiguous(bias);
-    r = residual_norm_forward(xr, rr, g, a, pw, pb, w, b, true);
-    node->d = norm_desc(xr, rr, g, a, pw, pb, w, b);
-    const bool from_h = !given(gate) && post == SUPA_AMD_NORM_NONE &&
-                        (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat);
-    const bool needs_h = norm != SUPA_AMD_NORM_NONE;
-    if (!from_h) node->x = SavedVariable(xr.t, false);
-    if (!from_h && needs_h) node->residual = SavedVariable(rr.t, false);
-    if (r.stats.defined()) node->stats = SavedVariable(r.stats, false);
-    const OptTensor* saved[] = {nullptr, nullptr, &g, &pw, &pb, &w, &b};
-    for (int i = Node::kGate; i < Node::kInputs; ++i)
-      if (given(*saved[i])) node->params[i] = SavedVariable(**saved[i], false);
-    node->shape = x.sizes().vec();
-    if (given(gate)) node->gate_shape = gate->sizes().vec();
-    torch::autograd::set_history(r.h, node);
-    if (r.y.defined()) torch::autograd::set_history(r.y, node);
-    if (from_h && needs_h) node->h = SavedVariable(r.h, true);
+    xr = rows_of(x).t;  // a copy is made once, for both ways
+    rr = rows_of(residual).t;
+    g = contiguous(gate);
+    std::tie(h, y, stats) = op.call(xr, rr, g, scale, post, post_weight, post_bias, norm, weight, bias, eps);
   }
-  return {r.h, r.y};
+  node->dtype = x.scalar_type();
+  node->residual_dtype = residual.scalar_type();
+  node->scale = scale;
+  node->eps = eps;
+  node->post = post;
+  node->norm = norm;
+  node->shape = x.sizes().vec();
+  node->stats_rows = x.numel() / x.size(-1);
+  const bool from_h = !given(gate) && post == SUPA_AMD_NORM_NONE &&
+                      (norm == SUPA_AMD_NORM_NONE || residual.scalar_type() == at::kFloat);
+  const bool needs_h = norm != SUPA_AMD_NORM_NONE;
+  if (!from_h) node->x = SavedVariable(xr, false);
+  if (!from_h && needs_h) node->residual = SavedVariable(rr, false);
+  if (stats.defined()) node->stats = SavedVariable(stats, false);
+  for (int i = kGate; i < kNormInputs; ++i) {
+    const OptTensor& p = i == kGate ? g : *params[i - kGate];
+    if (!given(p)) continue;
+    node->params[i] = SavedVariable(*p, false);
+    node->param_dtype = p->scalar_type();
+  }
+  if (given(gate)) node->gate_shape = gate->sizes().vec();
+  torch::autograd::set_history(h, node);
+  if (y.defined()) torch::autograd::set_history(y, node);
+  if (from_h && needs_h) node->h = SavedVariable(h, true);
+  return {h, y};
 }
 
 // --------------------------------------------------------- rotary_embedding
@@ -358,7 +476,7 @@ RotaryShape rotary_shape(const char* op, const char* name, const at::Tensor& t) 
 
 RotaryArgs check_rotary(const char* op, const at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies,
                         const OptTensor& positions, int64_t offset, bool interleaved, double scale, bool inverse) {
-  TORCH_CHECK(q.device().type() == kSupa, op, ": expected supa tensors, got q on ", q.device());
+  TORCH_CHECK(is_supa(q), op, ": expected supa tensors, got q on ", q.device());
   TORCH_CHECK(is_float16_or_32(q.scalar_type()), op, ": expected float32, bfloat16 or float16, got q of ",
               q.scalar_type());
   const RotaryShape s = rotary_shape(op, "q", q);
@@ -453,7 +571,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const O
   const RotaryArgs a = check_rotary(op, q, k, frequencies, positions, offset, interleaved, scale, inverse);
   const at::Tensor qi = heads_contiguous(q), ki = given(k) ? heads_contiguous(*k) : at::Tensor();
   const at::Tensor qo = rotated_like(qi), ko = ki.defined() ? rotated_like(ki) : at::Tensor();
-  launch_rotary(op, qi, qo, ki, ko, a);
+  if (!q.is_meta()) launch_rotary(op, qi, qo, ki, ko, a);
   return {qo, ko};
 }
 
@@ -508,18 +626,18 @@ void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& freq
     TORCH_CHECK(t->stride(-1) == 1, op, ": expected heads whose elements are contiguous");
     TORCH_CHECK(apart(*t, t->dim() - 1, t->size(-1)), op, ": expected a tensor whose heads do not overlap in memory");
   }
+  if (q.is_meta()) return;
   if (given(k) && q.numel() > 0 && k->numel() > 0)
     TORCH_CHECK(beside(q, *k), op, ": q and k overlap in memory");
   launch_rotary(op, q, q, given(k) ? *k : at::Tensor(), given(k) ? *k : at::Tensor(), a);
 }
 
-std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q, const OptTensor& k,
-                                                             const at::Tensor& frequencies, const OptTensor& positions,
-                                                             int64_t offset, bool interleaved, double scale,
-                                                             bool inverse);
+c10::TypedOperatorHandle<decltype(rotary_embedding)> rotary_op() {
+  static const auto op = find_op<decltype(rotary_embedding)>("supa::rotary_embedding");
+  return op;
+}
 
-// The rotation back.  Under create_graph by the same call, which has a gradient
-// of its own.
+// The rotation back, by the same operator, which has a gradient of its own.
 struct RotaryEmbeddingBackward final : public torch::autograd::Node {
   std::string name() const override { return "RotaryEmbeddingBackward"; }
   void release_variables() override {
@@ -538,9 +656,7 @@ struct RotaryEmbeddingBackward final : public torch::autograd::Node {
     const OptTensor second = both ? OptTensor(gk) : std::nullopt;
     const at::Tensor f = frequencies.unpack();
     const OptTensor p = maybe(positions.unpack());
-    auto [a, b] = at::GradMode::is_enabled()
-                      ? rotary_embedding_autograd(first, second, f, p, offset, interleaved, scale, !inverse)
-                      : rotary_embedding(first, second, f, p, offset, interleaved, scale, !inverse);
+    auto [a, b] = rotary_op().call(first, second, f, p, offset, interleaved, scale, !inverse);
     if (gq.defined()) out[0] = a;
     if (gk.defined()) out[1] = both ? b : a;
     return out;
@@ -552,17 +668,19 @@ struct RotaryEmbeddingBackward final : public torch::autograd::Node {
   double scale;
 };
 
-std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q, const OptTensor& k,
-                                                             const at::Tensor& frequencies, const OptTensor& positions,
-                                                             int64_t offset, bool interleaved, double scale,
-                                                             bool inverse) {
+std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(c10::DispatchKeySet ks, const at::Tensor& q,
+                                                             const OptTensor& k, const at::Tensor& frequencies,
+                                                             const OptTensor& positions, int64_t offset,
+                                                             bool interleaved, double scale, bool inverse) {
   check_no_tangent("rotary_embedding", {&q, &tensor(k), &frequencies});
   const bool needs = q.requires_grad() || (given(k) && k->requires_grad());
   TORCH_CHECK(!frequencies.requires_grad(), "rotary_embedding: frequencies have no gradient");
-  if (!needs || !at::GradMode::is_enabled()) {
+  const auto forward = [&] {
     const at::AutoDispatchBelowAutograd below;
-    return rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
-  }
+    return rotary_op().redispatch(ks & c10::after_autograd_keyset, q, k, frequencies, positions, offset, interleaved,
+                                  scale, inverse);
+  };
+  if (!needs || !at::GradMode::is_enabled()) return forward();
   auto node = std::shared_ptr<RotaryEmbeddingBackward>(new RotaryEmbeddingBackward(), torch::autograd::deleteNode);
   torch::autograd::edge_list edges{torch::autograd::impl::gradient_edge(q)};
   if (given(k)) edges.push_back(torch::autograd::impl::gradient_edge(*k));
@@ -572,8 +690,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(const at::Tensor& q
   node->interleaved = interleaved;
   node->inverse = inverse;
   node->scale = scale;
-  const at::AutoDispatchBelowAutograd below;
-  auto [qo, ko] = rotary_embedding(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  auto [qo, ko] = forward();
   node->frequencies = SavedVariable(frequencies, false);
   if (given(positions)) node->positions = SavedVariable(*positions, false);
   torch::autograd::set_history(qo, node);
@@ -585,24 +702,46 @@ void written(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
-void rotary_embedding_autograd_(at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies,
+void rotary_embedding_autograd_(c10::DispatchKeySet ks, at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies,
                                 const OptTensor& positions, int64_t offset, bool interleaved, double scale,
                                 bool inverse) {
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || (given(k) && k->requires_grad())),
               "rotary_embedding_: the call in place has no gradient; use rotary_embedding");
   check_no_tangent("rotary_embedding_", {&q, &tensor(k), &frequencies});
+  static const auto op = find_op<decltype(rotary_embedding_)>("supa::rotary_embedding_");
   const at::AutoDispatchBelowAutograd below;
-  rotary_embedding_(q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  op.redispatch(ks & c10::after_autograd_keyset, q, k, frequencies, positions, offset, interleaved, scale, inverse);
   written(q);
   if (given(k)) written(*k);
 }
 
 // ----------------------------------------------------------- clip_grad_norm_
-at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bool error_if_nonfinite) {
-  constexpr const char* op = "clip_grad_norm_";
+// Checks the arguments; the norm's type.
+at::ScalarType check_clip(const char* op, at::TensorList grads, double max_norm, double ord) {
   TORCH_CHECK(!grads.empty(), op, ": expected at least one tensor");
   TORCH_CHECK(max_norm >= 0, op, ": expected max_norm >= 0, got ", max_norm);
   TORCH_CHECK(ord == 1.0 || ord == 2.0 || ord == HUGE_VAL, op, ": expected the norm 1, 2 or inf, got ", ord);
+  const c10::Device device = grads[0].device();
+  at::ScalarType norm_type = at::kFloat;
+  for (const at::Tensor& g : grads) {
+    TORCH_CHECK(is_supa(g) && g.layout() == at::kStrided, op, ": expected dense supa tensors, got one of layout ",
+                g.layout(), " on ", g.device());
+    TORCH_CHECK(g.device() == device, op, ": the tensors are on ", device, " and ", g.device(), ", expected one device");
+    const at::ScalarType t = g.scalar_type();
+    TORCH_CHECK(is_float16_or_32(t) || t == at::kDouble, op, ": expected floating tensors, got one of ", t);
+    if (t == at::kDouble) norm_type = at::kDouble;
+  }
+  return norm_type;
+}
+
+at::Tensor clip_grad_norm_meta_(at::TensorList grads, double max_norm, double ord, bool /*error_if_nonfinite*/) {
+  const at::ScalarType norm_type = check_clip("clip_grad_norm_", grads, max_norm, ord);
+  return empty_beside(grads[0], {}, norm_type);
+}
+
+at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bool error_if_nonfinite) {
+  constexpr const char* op = "clip_grad_norm_";
+  const at::ScalarType norm_type = check_clip(op, grads, max_norm, ord);
   const c10::Device device = grads[0].device();
   const size_t n = grads.size();
   std::vector<at::Tensor> copies;         // of tensors that are not dense, in the list's order
@@ -612,16 +751,9 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   // the memory from a tensor's first element to behind its last, and the tensor
   std::vector<std::tuple<const char*, const char*, size_t>> spans;
   spans.reserve(n);
-  at::ScalarType norm_type = at::kFloat;
-  const c10::OptionalDeviceGuard guard(device);
+  const c10::DeviceGuard guard(device);
   for (size_t i = 0; i < n; ++i) {
     const at::Tensor& g = grads[i];
-    TORCH_CHECK(g.device().type() == kSupa && g.layout() == at::kStrided, op,
-                ": expected dense supa tensors, got one of layout ", g.layout(), " on ", g.device());
-    TORCH_CHECK(g.device() == device, op, ": the tensors are on ", device, " and ", g.device(), ", expected one device");
-    const at::ScalarType t = g.scalar_type();
-    TORCH_CHECK(is_float16_or_32(t) || t == at::kDouble, op, ": expected floating tensors, got one of ", t);
-    if (t == at::kDouble) norm_type = at::kDouble;
     at::Tensor x = g;
     if (!g.is_non_overlapping_and_dense()) {
       at::assert_no_internal_overlap(g);
@@ -636,7 +768,7 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
     }
     p[i] = x.data_ptr();
     numel[i] = x.numel();
-    dtypes[i] = dtype_code(t);
+    dtypes[i] = dtype_code(g.scalar_type());
   }
   // two that reach over each other have to lie beside each other, as the columns of a matrix do
   std::sort(spans.begin(), spans.end());
@@ -678,9 +810,11 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   return norm;
 }
 
-at::Tensor clip_grad_norm_autograd_(at::TensorList grads, double max_norm, double ord, bool error_if_nonfinite) {
+at::Tensor clip_grad_norm_autograd_(c10::DispatchKeySet ks, at::TensorList grads, double max_norm, double ord,
+                                    bool error_if_nonfinite) {
+  static const auto op = find_op<decltype(clip_grad_norm_)>("supa::clip_grad_norm_");
   const at::AutoDispatchBelowAutograd below;  // the scaling is no part of a graph, as under no_grad
-  at::Tensor norm = clip_grad_norm_(grads, max_norm, ord, error_if_nonfinite);
+  at::Tensor norm = op.redispatch(ks & c10::after_autograd_keyset, grads, max_norm, ord, error_if_nonfinite);
   for (const at::Tensor& g : grads) written(g);
   return norm;
 }
@@ -692,6 +826,15 @@ TORCH_LIBRARY(supa, m) {
   m.def(
       "residual_norm(Tensor x, Tensor residual, Tensor? gate, float residual_scale, int post_norm, Tensor? post_weight, "
       "Tensor? post_bias, int norm, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor)");
+  // its parts for training: the rows' statistics beside h and y; the gradients of the seven tensors
+  m.def(
+      "_residual_norm_forward(Tensor x, Tensor residual, Tensor? gate, float residual_scale, int post_norm, Tensor? "
+      "post_weight, Tensor? post_bias, int norm, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "_residual_norm_backward(Tensor? grad_h, Tensor? grad_y, Tensor? x, Tensor? residual, Tensor? h, Tensor? stats, "
+      "Tensor? gate, float residual_scale, int post_norm, Tensor? post_weight, Tensor? post_bias, int norm, Tensor? weight, "
+      "Tensor? bias, float eps, ScalarType dtype, ScalarType residual_dtype, bool[7] output_mask) -> "
+      "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def(
       "rotary_embedding(Tensor q, Tensor? k, Tensor frequencies, Tensor? positions, int offset, bool interleaved, "
       "float scale, bool inverse) -> (Tensor, Tensor)");
@@ -704,15 +847,32 @@ TORCH_LIBRARY(supa, m) {
 TORCH_LIBRARY_IMPL(supa, PrivateUse1, m) {
   using namespace supa;
   m.impl("residual_norm", TORCH_FN(residual_norm));
+  m.impl("_residual_norm_forward", TORCH_FN(residual_norm_forward));
+  m.impl("_residual_norm_backward", TORCH_FN(residual_norm_backward));
   m.impl("rotary_embedding", TORCH_FN(rotary_embedding));
   m.impl("rotary_embedding_", TORCH_FN(rotary_embedding_));
   m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_));
 }
 
-TORCH_LIBRARY_IMPL(supa, AutogradPrivateUse1, m) {
+TORCH_LIBRARY_IMPL(supa, Meta, m) {
   using namespace supa;
+  m.impl("residual_norm", TORCH_FN(residual_norm_meta));
+  m.impl("_residual_norm_forward", TORCH_FN(residual_norm_forward_meta));
+  m.impl("_residual_norm_backward", TORCH_FN(residual_norm_backward_meta));
+  m.impl("rotary_embedding", TORCH_FN(rotary_embedding));
+  m.impl("rotary_embedding_", TORCH_FN(rotary_embedding_));
+  m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_meta_));
+}
+
+namespace supa {
+namespace {
+void autograd_kernels(torch::Library& m) {
   m.impl("residual_norm", TORCH_FN(residual_norm_autograd));
   m.impl("rotary_embedding", TORCH_FN(rotary_embedding_autograd));
   m.impl("rotary_embedding_", TORCH_FN(rotary_embedding_autograd_));
   m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_autograd_));
 }
+}  // namespace
+}  // namespace supa
+TORCH_LIBRARY_IMPL(supa, AutogradPrivateUse1, m) { supa::autograd_kernels(m); }
+TORCH_LIBRARY_IMPL(supa, Autograd, m) { supa::autograd_kernels(m); }  // meta tensors, and wrappers of any
