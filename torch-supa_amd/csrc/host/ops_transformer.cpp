@@ -698,8 +698,9 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding_autograd(c10::DispatchKeySet
   return {qo, ko};
 }
 
-void written(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+c10::TypedOperatorHandle<decltype(rotary_embedding_)> rotary_op_() {
+  static const auto op = find_op<decltype(rotary_embedding_)>("supa::rotary_embedding_");
+  return op;
 }
 
 void rotary_embedding_autograd_(c10::DispatchKeySet ks, at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies,
@@ -708,9 +709,25 @@ void rotary_embedding_autograd_(c10::DispatchKeySet ks, at::Tensor& q, const Opt
   TORCH_CHECK(!at::GradMode::is_enabled() || !(q.requires_grad() || (given(k) && k->requires_grad())),
               "rotary_embedding_: the call in place has no gradient; use rotary_embedding");
   check_no_tangent("rotary_embedding_", {&q, &tensor(k), &frequencies});
-  static const auto op = find_op<decltype(rotary_embedding_)>("supa::rotary_embedding_");
   const at::AutoDispatchBelowAutograd below;
-  op.redispatch(ks & c10::after_autograd_keyset, q, k, frequencies, positions, offset, interleaved, scale, inverse);
+  rotary_op_().redispatch(ks & c10::after_autograd_keyset, q, k, frequencies, positions, offset, interleaved, scale,
+                          inverse);
+}
+
+// A tensor that was written has a new version, in inference mode too (where autograd's
+// kernels are left out, this key's are not).
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+void rotary_embedding_versions_(c10::DispatchKeySet ks, at::Tensor& q, const OptTensor& k,
+                                const at::Tensor& frequencies, const OptTensor& positions, int64_t offset,
+                                bool interleaved, double scale, bool inverse) {
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    rotary_op_().redispatch(ks & c10::after_ADInplaceOrView_keyset, q, k, frequencies, positions, offset, interleaved,
+                            scale, inverse);
+  }
   written(q);
   if (given(k)) written(*k);
 }
@@ -810,11 +827,24 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   return norm;
 }
 
+c10::TypedOperatorHandle<decltype(clip_grad_norm_)> clip_op() {
+  static const auto op = find_op<decltype(clip_grad_norm_)>("supa::clip_grad_norm_");
+  return op;
+}
+
 at::Tensor clip_grad_norm_autograd_(c10::DispatchKeySet ks, at::TensorList grads, double max_norm, double ord,
                                     bool error_if_nonfinite) {
-  static const auto op = find_op<decltype(clip_grad_norm_)>("supa::clip_grad_norm_");
   const at::AutoDispatchBelowAutograd below;  // the scaling is no part of a graph, as under no_grad
-  at::Tensor norm = op.redispatch(ks & c10::after_autograd_keyset, grads, max_norm, ord, error_if_nonfinite);
+  return clip_op().redispatch(ks & c10::after_autograd_keyset, grads, max_norm, ord, error_if_nonfinite);
+}
+
+at::Tensor clip_grad_norm_versions_(c10::DispatchKeySet ks, at::TensorList grads, double max_norm, double ord,
+                                    bool error_if_nonfinite) {
+  at::Tensor norm;
+  {
+    const at::AutoDispatchBelowADInplaceOrView below;
+    norm = clip_op().redispatch(ks & c10::after_ADInplaceOrView_keyset, grads, max_norm, ord, error_if_nonfinite);
+  }
   for (const at::Tensor& g : grads) written(g);
   return norm;
 }
@@ -875,4 +905,9 @@ void autograd_kernels(torch::Library& m) {
 }  // namespace
 }  // namespace supa
 TORCH_LIBRARY_IMPL(supa, AutogradPrivateUse1, m) { supa::autograd_kernels(m); }
+TORCH_LIBRARY_IMPL(supa, ADInplaceOrView, m) {
+  using namespace supa;
+  m.impl("rotary_embedding_", TORCH_FN(rotary_embedding_versions_));
+  m.impl("clip_grad_norm_", TORCH_FN(clip_grad_norm_versions_));
+}
 TORCH_LIBRARY_IMPL(supa, Autograd, m) { supa::autograd_kernels(m); }  // meta tensors, and wrappers of any
