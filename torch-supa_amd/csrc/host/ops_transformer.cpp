@@ -575,45 +575,67 @@ std::tuple<at::Tensor, at::Tensor> rotary_embedding(const at::Tensor& q, const O
   return {qo, ko};
 }
 
-// Whether blocks of `block` elements, one at every index of the dims before
-// `dims`, keep apart: each dim steps over all that the smaller steps reach.  The
-// dims are as long as t's or, if there is one, the other tensor's, the longer.
-bool apart(const at::Tensor& t, int64_t dims, int64_t block, const at::Tensor& other = {}) {
-  std::vector<std::pair<int64_t, int64_t>> steps;  // stride, size
-  for (int64_t i = 0; i < dims; ++i) {
-    const int64_t size = other.defined() ? std::max(t.size(i), other.size(i)) : t.size(i);
-    if (size > 1) steps.emplace_back(t.stride(i), size);
-  }
-  std::sort(steps.begin(), steps.end());
-  for (const auto& [stride, size] : steps) {
-    if (stride < block) return false;
-    block += (size - 1) * stride;
+// A step through memory, in bytes, and how often the one and the other tensor take it.
+struct Step {
+  int64_t stride, one, other;
+};
+using Steps = c10::SmallVector<Step, 8>;
+
+// The steps of a tensor and, if there is one, of another, from long to short; a
+// step that both take is one step, one that a tensor takes in two dims is two.
+Steps steps_of(const at::Tensor& one, const at::Tensor& other = {}) {
+  Steps steps;
+  const auto add = [&](const at::Tensor& t, int64_t Step::* times) {
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      if (t.size(i) == 1) continue;
+      const int64_t stride = t.stride(i) * (int64_t)t.element_size();
+      auto at = std::find_if(steps.begin(), steps.end(), [&](const Step& s) { return s.stride == stride && s.*times == 0; });
+      if (at == steps.end()) at = steps.insert(at, {stride, 0, 0});
+      (*at).*times = t.size(i) - 1;
+    }
+  };
+  add(one, &Step::one);
+  if (other.defined()) add(other, &Step::other);
+  std::sort(steps.begin(), steps.end(), [](const Step& a, const Step& b) { return a.stride > b.stride; });
+  return steps;
+}
+
+// Whether blocks of `block` bytes, one at every combination of the first n steps
+// (the one tensor's), keep apart: each step goes past all that the smaller ones reach.
+bool apart(const Steps& steps, size_t n, int64_t block) {
+  for (size_t i = n; i-- > 0;) {
+    if (steps[i].stride < block) return false;
+    block += steps[i].one * steps[i].stride;
   }
   return true;
 }
 
-// Whether q and k, of one type and number of dims, share no element: over some of
-// the trailing dims (or none) k lies beside q, and the dims before step alike from
-// one such pair to the next (q and k of a packed projection, token by token or
-// sample by sample).
-bool beside(const at::Tensor& q, const at::Tensor& k) {
-  const int64_t nd = q.dim();
-  // elements from the first to behind the last, over the dims from `from` on
-  const auto extent = [&](const at::Tensor& t, int64_t from) {
-    int64_t e = 1;
-    for (int64_t i = from; i < nd; ++i) e += (t.size(i) - 1) * t.stride(i);
-    return e;
-  };
-  const int64_t shift = (static_cast<const char*>(k.data_ptr()) - static_cast<const char*>(q.data_ptr())) /
-                        (int64_t)q.element_size();
-  const int64_t gap = std::abs(shift);
-  for (int64_t from = 0; from <= nd; ++from) {
-    bool alike = true;
-    for (int64_t i = 0; i < from; ++i) alike = alike && ((q.size(i) == 1 && k.size(i) == 1) || q.stride(i) == k.stride(i));
-    const int64_t first = extent(shift >= 0 ? q : k, from), second = extent(shift >= 0 ? k : q, from);
-    if (alike && first <= gap && apart(q, from, gap + second, k)) return true;
+// Whether two tensors share no memory, of any types and shapes: over their smaller
+// steps (or none, or all) each fills a block, the other's beside the one's, and
+// their larger steps, which both may take, lead from one such pair of blocks to the
+// next (q and k of a packed projection, token by token or sample by sample; the
+// columns of a matrix).
+bool beside(const at::Tensor& a, const at::Tensor& b) {
+  const bool ordered = a.data_ptr() <= b.data_ptr();
+  const at::Tensor &one = ordered ? a : b, &other = ordered ? b : a;
+  const int64_t distance = static_cast<const char*>(other.data_ptr()) - static_cast<const char*>(one.data_ptr());
+  const Steps steps = steps_of(one, other);
+  int64_t first = (int64_t)one.element_size(), second = (int64_t)other.element_size();  // the blocks' bytes
+  for (size_t outer = steps.size();; --outer) {
+    // the other's first block lies so many steps ahead, and `gap` behind the one's block there
+    int64_t gap = distance;
+    Steps joint(steps.begin(), steps.begin() + outer);
+    for (Step& s : joint) {
+      if (s.stride == 0) return false;
+      const int64_t ahead = gap / s.stride;
+      gap -= ahead * s.stride;
+      s.one = std::max(s.one, s.other + ahead);
+    }
+    if (first <= gap && apart(joint, outer, gap + second)) return true;
+    if (outer == 0) return false;
+    first += steps[outer - 1].one * steps[outer - 1].stride;
+    second += steps[outer - 1].other * steps[outer - 1].stride;
   }
-  return false;
 }
 
 void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& frequencies, const OptTensor& positions,
@@ -624,7 +646,9 @@ void rotary_embedding_(at::Tensor& q, const OptTensor& k, const at::Tensor& freq
   for (const at::Tensor* t : {(const at::Tensor*)&q, given(k) ? &*k : nullptr}) {
     if (!t || t->numel() == 0) continue;
     TORCH_CHECK(t->stride(-1) == 1, op, ": expected heads whose elements are contiguous");
-    TORCH_CHECK(apart(*t, t->dim() - 1, t->size(-1)), op, ": expected a tensor whose heads do not overlap in memory");
+    const Steps steps = steps_of(*t);
+    TORCH_CHECK(apart(steps, steps.size(), (int64_t)t->element_size()), op,
+                ": expected a tensor whose heads do not overlap in memory");
   }
   if (q.is_meta()) return;
   if (given(k) && q.numel() > 0 && k->numel() > 0)
@@ -792,9 +816,7 @@ at::Tensor clip_grad_norm_(at::TensorList grads, double max_norm, double ord, bo
   for (size_t i = 0; i < spans.size(); ++i) {
     const auto& [at, end, one] = spans[i];
     for (size_t j = i + 1; j < spans.size() && std::get<0>(spans[j]) < end; ++j) {
-      const at::Tensor &a = grads[one], &b = grads[std::get<2>(spans[j])];
-      TORCH_CHECK(a.scalar_type() == b.scalar_type() && a.dim() == b.dim() && beside(a, b), op,
-                  ": two of the tensors share memory");
+      TORCH_CHECK(beside(grads[one], grads[std::get<2>(spans[j])]), op, ": two of the tensors share memory");
     }
   }
   const auto dev = device.index();

@@ -157,8 +157,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 
     The sum is float64 and does not depend on timing.  The gradients are on one
     device, of float32, bfloat16, float16 or float64 in any mixture, and do not
-    share memory (a parameter listed twice is an error); parameters without a
-    gradient are left out.  A norm that is NaN makes every gradient NaN, one
+    share memory (a parameter listed twice is an error; slices of one buffer may
+    reach over each other); parameters without a gradient are left out.  A norm that is NaN makes every gradient NaN, one
     that is infinite makes them zero; error_if_nonfinite raises instead, before
     anything is scaled, and waits for the norm."""
     if isinstance(parameters, torch.Tensor):
