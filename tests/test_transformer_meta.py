@@ -3,6 +3,7 @@ supa tensors give the results' shapes, types and strides, with gradients, and
 refuse what the device refuses; dispatch modes see every call, forward and
 backward.  No GPU."""
 import math
+import warnings
 
 import pytest
 import torch
@@ -128,3 +129,17 @@ def test_backward_arguments():
     ]:
         with pytest.raises(RuntimeError, match=text):
             op(**{**base, **kw})
+
+
+def test_numbers_that_require_a_gradient():
+    """A learned scale would lose its gradient with its conversion to a number."""
+    x, f, p = meta(4, 8, grad=True), meta(4, dtype=F64), torch.nn.Parameter(torch.tensor(0.5))
+    calls = [lambda s: torch.supa.residual_norm(x, x, residual_scale=s), lambda s: torch.supa.residual_norm(x, x, eps=s),
+             lambda s: torch.supa.rotary_embedding(meta(4, 1, 8, grad=True), None, f, scale=s)]
+    for call in calls:
+        with pytest.raises(TypeError, match="has no gradient"):
+            call(p)
+        assert call(p.detach())[0].requires_grad and call(0.5)[0].requires_grad
+        with torch.no_grad(), warnings.catch_warnings():
+            warnings.simplefilter("ignore")  # torch's own, of the conversion
+            call(p)

@@ -27,6 +27,13 @@ def _norm_kind(name, value):
         raise ValueError(f"residual_norm: expected {name} 'rms', 'layer' or None, got {value!r}") from None
 
 
+def _number(name, value):
+    """value; a tensor whose gradient would be lost with its conversion to a number raises."""
+    if isinstance(value, torch.Tensor) and value.requires_grad and torch.is_grad_enabled():
+        raise TypeError(f"{name} is a number and has no gradient, got a tensor that requires one")
+    return value
+
+
 def residual_norm(x, residual, *, gate=None, residual_scale=1.0, post_norm=None, post_weight=None, post_bias=None,
                   norm="rms", weight=None, bias=None, eps=1e-6):
     """Adds a block's output to the residual stream and normalises the sum for
@@ -50,10 +57,12 @@ def residual_norm(x, residual, *, gate=None, residual_scale=1.0, post_norm=None,
     Statistics, products and the gradients' sums are float32, and y is the norm
     of h before h is rounded.
 
-    Differentiable (once) in every tensor.
+    Differentiable (once) in x, residual, gate, weights and biases;
+    residual_scale and eps are numbers.
     """
-    return _residual_norm(x, residual, gate, residual_scale, _norm_kind("post_norm", post_norm), post_weight, post_bias,
-                          _norm_kind("norm", norm), weight, bias, eps)
+    return _residual_norm(x, residual, gate, _number("residual_norm: residual_scale", residual_scale),
+                          _norm_kind("post_norm", post_norm), post_weight, post_bias, _norm_kind("norm", norm), weight,
+                          bias, _number("residual_norm: eps", eps))
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, original_length=None, slow=1.0,
@@ -137,7 +146,7 @@ def rotary_embedding(q, k, frequencies, positions=0, *, layout="half", scale=1.0
 
     Angles are formed in 64 bits.  Differentiable in q and k.  Returns (q, k)."""
     at, offset, interleaved = _rotary_args("rotary_embedding", positions, layout)
-    return _rotary_embedding(q, k, frequencies, at, offset, interleaved, scale, False)
+    return _rotary_embedding(q, k, frequencies, at, offset, interleaved, _number("rotary_embedding: scale", scale), False)
 
 
 def rotary_embedding_(q, k, frequencies, positions=0, *, layout="half", scale=1.0):
