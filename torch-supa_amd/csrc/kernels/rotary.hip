@@ -9,9 +9,9 @@
 // are on their way.  Where a token's heads are neighbours in memory the tile is
 // all heads of one token (or of a few, if they are small); where a head's tokens
 // are, it is a run of tokens of some heads, so that a workgroup reads and writes
-// long pieces of memory and shares few lines with others.  position * frequency is formed in 64 bits and reduced to a
-// fraction of a turn there: a float32 angle is off by 0.03 rad at position
-// 500 000.  The fraction, its sine and cosine and the rotation are float32.
+// long pieces of memory and shares few lines with others.  position * frequency is formed in 64 bits and reduced there
+// to whole quarter turns and the rest: a float32 angle is off by 0.03 rad at position
+// 500 000.  The rest, its sine and cosine and the rotation are float32.
 //
 // Measured on MI355X: [1, 131072, 20, 128] bf16 206 us (6.5 TB/s; its 350
 // instructions a wavefront and vector would take some 180 alone), [4, 2048, 40, 128]
@@ -188,9 +188,16 @@ __global__ void __launch_bounds__(kRotBlock) k_rotary(RotArgs g) {
         p = g.pos64 ? static_cast<const int64_t*>(g.pos)[at] : (int64_t)static_cast<const int32_t*>(g.pos)[at];
       }
       const double turns = (double)(p + g.offset) * g.freq[i - tk * pairs] * 0.15915494309189533577;
+      // Whole quarter turns are taken off before the rest, at most an eighth of a turn, is
+      // rounded to float32: its sine and cosine keep 24 bits also next to their zeros.
+      const double half = 2.0 * (turns - rint(turns)), quarter = rint(2.0 * half);
+      const int quarters = (int)quarter & 3;
       float s, c;
-      sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
-      cs[i] = make_float2(g.scale * c, g.scale * (g.inverse ? -s : s));
+      sincospif((float)(half - 0.5 * quarter), &s, &c);
+      const float sn = quarters & 1 ? c : s, cn = quarters & 1 ? s : c;
+      s = (quarters & 2) != 0 != (g.inverse != 0) ? -sn : sn;
+      c = (quarters + 1) & 2 ? -cn : cn;
+      cs[i] = make_float2(g.scale * c, g.scale * s);
     }
   }
   __syncthreads();

@@ -144,7 +144,9 @@ def rotary_embedding(q, k, frequencies, positions=0, *, layout="half", scale=1.0
     int64 or int32 tensor ``[seq]`` or ``[batch, seq]``, or the first of
     consecutive positions.
 
-    Angles are formed in 64 bits.  Differentiable in q and k.  Returns (q, k)."""
+    Angles are formed in 64 bits; their sines and cosines are float32, within a
+    few units in the last place, and so is the rotation, before the one rounding
+    to q's dtype.  Differentiable in q and k.  Returns (q, k)."""
     at, offset, interleaved = _rotary_args("rotary_embedding", positions, layout)
     return _rotary_embedding(q, k, frequencies, at, offset, interleaved, _number("rotary_embedding: scale", scale), False)
 
