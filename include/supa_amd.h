@@ -850,7 +850,8 @@ int supa_amd_residual_norm_forward(const supa_amd_residual_norm_desc* d, void* h
  * grad_post_bias, grad_weight and grad_bias of param_dtype in their
  * parameter's shape, summed in float32 in an order that only the sizes fix.
  * h, when given, is the forward's h and takes the place of x and residual
- * (which are then not read): for a call without post norm and gate.  x is read
+ * (which are then not read): for a call without post norm and gate.  A 16-bit
+ * h brings its rounding into the gradients.  x is read
  * for those two, residual only when there is a norm. */
 int64_t supa_amd_residual_norm_backward_workspace_bytes(const supa_amd_residual_norm_desc* d);
 int supa_amd_residual_norm_backward(const supa_amd_residual_norm_desc* d, const void* h, const void* grad_h,

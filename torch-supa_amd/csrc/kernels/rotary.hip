@@ -13,8 +13,8 @@
 // to whole quarter turns and the rest: a float32 angle is off by 0.03 rad at position
 // 500 000.  The rest, its sine and cosine and the rotation are float32.
 //
-// Measured on MI355X: [1, 131072, 20, 128] bf16 206 us (6.5 TB/s; its 350
-// instructions a wavefront and vector would take some 180 alone), [4, 2048, 40, 128]
+// Measured on MI355X: [1, 131072, 20, 128] bf16 206 us (6.5 TB/s; its 271
+// instructions a wavefront and unit would take some 145 alone), [4, 2048, 40, 128]
 // bf16 30 us (5.6 TB/s, launch included), float32 55 us (6.1 TB/s).
 #include "row_group.h"
 
