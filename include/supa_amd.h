@@ -923,6 +923,115 @@ int supa_amd_clip_grad_norm(int32_t ntensors, void* const* tensors, const int64_
                             double ord, double max_norm, void* norm_out, int32_t norm_dtype, void* workspace,
                             int64_t ws_bytes, void* stream);
 
+/* ------------------------------------ distillation from a teacher's top logits
+ * Per row of `vocab` student logits x and `entries` pairs of a token and a
+ * teacher's logit t, with z = x / temperature and q = softmax(z):
+ *   p_k = exp(t_k / temperature - lt),  lt = teacher_lse, or the pairs' own log-sum-exp
+ *   loss = sum_k p_k (log p_k - log q_(token k))
+ * and with teacher_lse (the log-sum-exp of all of the teacher's logits over
+ * temperature) the tokens that are not listed as one more class: r = max(0, 1 - sum p)
+ * against the student's mass outside the list, + r (log r - log q_R).  A pair whose token is
+ * negative, or whose logit is -inf, is not there; a token of vocab and more is
+ * left out too and sets *error_flag (when given).  A token listed twice has the sum of both
+ * p.  A row without a pair has loss 0 and gradient 0 and does not count for the mean.  The
+ * logits are read in float32 and summed in it, what depends on the pairs is float64.
+ * No reference counterpart: a program of the reference writes it as log_softmax, gather and sums. */
+#define SUPA_AMD_DISTILL_MAX_ENTRIES 1024
+
+typedef struct supa_amd_distill_desc {
+  int64_t rows;              /* fewer than 2^31 */
+  int64_t vocab;             /* 1 .. 2^31 - 1 */
+  int64_t entries;           /* 1 .. SUPA_AMD_DISTILL_MAX_ENTRIES */
+  int64_t inner;             /* row r of the logits lies at (r / inner) logits_strides[0] + (r % inner) logits_strides[1] */
+  int64_t logits_strides[2]; /* elements; those of a row are contiguous */
+  int32_t dtype;             /* of the logits: f32, bf16 or f16 */
+  int32_t teacher_dtype;     /* f32, bf16 or f16 */
+  int32_t index_dtype;       /* I64 or I32 */
+  int32_t reduction;         /* SUPA_AMD_REDUCTION_* */
+  double temperature;        /* 1e-30 .. 1e30 */
+  const void* logits;
+  const void* indices;       /* [rows, entries], contiguous */
+  const void* teacher;       /* [rows, entries], contiguous */
+  const float* teacher_lse;  /* [rows], or NULL */
+} supa_amd_distill_desc;
+
+/* loss: [rows] for reduction none, else one float; count (not for none): the rows
+ * that count.  For the backward: stats, 8 floats a row; weights ([rows,
+ * entries], may be NULL without a backward), each pair's p, or -1.  The backward takes the same
+ * descriptor (teacher and teacher_lse are not read) and writes the contiguous gradient of the logits, in their
+ * dtype; it overlaps no input. */
+int64_t supa_amd_distill_workspace_bytes(const supa_amd_distill_desc* d);
+int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, float* weights,
+                             void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream);
+int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_loss, const float* count,
+                              const float* stats, const float* weights, void* grad_logits, void* stream);
+
+/* ------------------------------------------- balance of a router's experts
+ * Of each sequence of `tokens` rows of router logits x, over its n counted tokens (mask,
+ * or all of them):
+ *   p = softmax(x), or sigmoid(x) / sum of them;  c_e = counted tokens' choices of expert e
+ *   loss = mean over sequences with n > 0 of  sum_e (experts c_e / (k n)) (sum_t p_te / n)
+ * (0 where none has a counted token).  Choices below 0 count for no expert; those of `experts` and
+ * more too, and set *error_flag (when given).  The counts are constants for the gradient.
+ * Sums are float32 a workgroup, then float64, in an order that only the sizes fix.
+ * No reference counterpart. */
+#define SUPA_AMD_SCORES_SOFTMAX 0
+#define SUPA_AMD_SCORES_SIGMOID 1
+
+typedef struct supa_amd_balance_desc {
+  int64_t sequences, tokens; /* their product fewer than 2^31 */
+  int64_t experts;           /* 1 .. 1024 */
+  int64_t k;                 /* choices a token: 1 .. experts */
+  int32_t dtype;             /* of the logits: f32, bf16 or f16 */
+  int32_t index_dtype;       /* I64 or I32 */
+  int32_t scores;            /* SUPA_AMD_SCORES_* */
+  int32_t reserved;
+  const void* logits;        /* [sequences, tokens, experts], contiguous */
+  const void* chosen;        /* [sequences, tokens, k], contiguous */
+  const void* mask;          /* [sequences, tokens] bytes, 0: the token does not count; or NULL */
+} supa_amd_balance_desc;
+
+/* counts: [sequences, experts].  For the backward: load ([sequences, experts]) and scale ([sequences + 1]).  The backward reads
+ * neither chosen nor the counts; the gradient is contiguous, in the logits' dtype, and overlaps no input. */
+int64_t supa_amd_balance_workspace_bytes(const supa_amd_balance_desc* d);
+int supa_amd_balance_forward(const supa_amd_balance_desc* d, float* loss, int64_t* counts, float* load, float* scale,
+                             void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream);
+int supa_amd_balance_backward(const supa_amd_balance_desc* d, const float* grad_loss, const float* load,
+                              const float* scale, void* grad_logits, void* stream);
+
+/* ------------------------------------------- logits before a token is drawn
+ * Of each row, in this order, in float32, rounded once:
+ *   x > 0 ? x / repetition : x * repetition   where the token is in the row's history
+ *   x - frequency count - presence (count > 0)    count: its times behind the history's prompt
+ *   x + the sum of the token's biases
+ *   -inf                                      where the token's bit of `allowed` is 0
+ * The history is the first lengths[row] (clamped to [0, history]) of the row's tokens, the
+ * prompt its first prompt_lengths[row].  Tokens outside [0, vocab) are passed over, in the history and
+ * among the biases.  out may be in; otherwise it overlaps no input.  No reference counterpart. */
+typedef struct supa_amd_adjust_desc {
+  int64_t rows, vocab;       /* rows below 2^31, vocab below 2^29 */
+  int64_t history;           /* most tokens a row, 0: no penalties */
+  int64_t biases;            /* entries a row, 0: none */
+  int64_t in_stride, out_stride, tokens_stride, bias_tokens_stride, bias_stride, allowed_stride; /* from row to row */
+  int32_t dtype;             /* of in and out: f32, bf16 or f16 */
+  int32_t token_dtype, length_dtype, prompt_dtype, bias_token_dtype; /* I64 or I32 */
+  int32_t reserved;
+  double repetition_value, presence_value, frequency_value; /* where the pointer is NULL */
+  const void* in;
+  void* out;
+  const void* tokens;
+  const void* lengths;        /* [rows], or NULL: all are `history` long */
+  const void* prompt_lengths; /* [rows], or NULL: no prompt */
+  const float* repetition;    /* [rows], or NULL */
+  const float* presence;
+  const float* frequency;
+  const void* bias_tokens;
+  const float* bias;
+  const uint32_t* allowed;    /* bit v % 32 of word v / 32 of the row; or NULL */
+} supa_amd_adjust_desc;
+
+int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -233,6 +233,8 @@ void check_flags(c10::DeviceIndex d, int first, int n) {
   if (code != 0) {
     TORCH_CHECK_INDEX(code != 2, "supa: a kernel reported an out-of-bounds index (a scatter_ index outside the "
                                  "destination's size along dim)");
+    TORCH_CHECK_INDEX(code != 3, "supa: a kernel reported an out-of-bounds index (a distillation_loss token or a "
+                                 "router_balance_loss expert past the last dim of the logits)");
     TORCH_CHECK_INDEX(false, "supa: a kernel reported an out-of-bounds target index (nll_loss target outside "
                              "[0, n_classes) and not ignore_index)");
   }

@@ -12,6 +12,12 @@ from __future__ import annotations
 import torch
 
 from .. import _C
+from .logits import (  # noqa: F401
+    adjust_logits,
+    adjust_logits_,
+    distillation_loss,
+    router_balance_loss,
+)
 from .transformer import (  # noqa: F401
     clip_grad_norm_,
     residual_norm,
