@@ -956,15 +956,15 @@ typedef struct supa_amd_distill_desc {
 } supa_amd_distill_desc;
 
 /* loss: [rows] for reduction none, else one float; count (not for none): the rows
- * that count.  For the backward: stats, 8 floats a row; weights ([rows,
- * entries], may be NULL without a backward), each pair's p, or -1.  The backward takes the same
- * descriptor (teacher and teacher_lse are not read) and writes the contiguous gradient of the logits, in their
+ * that count.  For the backward: stats, 8 floats a row; pairs ([rows, entries], 8 bytes each and
+ * 8-byte aligned; may be NULL without a backward), a token as int32, or -1, and its p as float32.  The
+ * backward takes the same descriptor (indices, teacher and teacher_lse are not read) and writes the contiguous gradient of the logits, in their
  * dtype; it overlaps no input. */
 int64_t supa_amd_distill_workspace_bytes(const supa_amd_distill_desc* d);
-int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, float* weights,
+int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, void* pairs,
                              void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream);
 int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_loss, const float* count,
-                              const float* stats, const float* weights, void* grad_logits, void* stream);
+                              const float* stats, const void* pairs, void* grad_logits, void* stream);
 
 /* ------------------------------------------- balance of a router's experts
  * Of each sequence of `tokens` rows of router logits x, over its n counted tokens (mask,

@@ -77,7 +77,7 @@ def test_distill_refuses(lib, kw, want):
     d = distill_desc(**kw)
     assert lib.supa_amd_distill_forward(ctypes.byref(d), vp(FAKE), vp(FAKE), vp(FAKE), vp(FAKE), vp(FAKE), i64(1 << 20),
                                         None, None) == want
-    if "teacher" not in kw:  # which the backward does not read
+    if not kw.keys() & {"teacher", "indices"}:  # which the backward does not read
         assert lib.supa_amd_distill_backward(ctypes.byref(d), vp(FAKE), vp(FAKE), vp(FAKE), vp(FAKE), vp(FAKE), None) == want
 
 
@@ -95,11 +95,12 @@ def test_distill_other_refusals(lib):
     assert forward(ws=None) == EWORKSPACE and forward(size=need - 1) == EWORKSPACE and forward(ws=FAKE + 4) == EINVAL
     assert forward(distill_desc(rows=0, reduction=0)) == 0
 
-    def back(d=d, grad=FAKE, count=FAKE, stats=FAKE, weights=FAKE, out=FAKE):
-        return bwd(ctypes.byref(d), vp(grad), vp(count), vp(stats), vp(weights), vp(out), None)
+    def back(d=d, grad=FAKE, count=FAKE, stats=FAKE, pairs=FAKE, out=FAKE):
+        return bwd(ctypes.byref(d), vp(grad), vp(count), vp(stats), vp(pairs), vp(out), None)
 
-    for name in ("grad", "count", "stats", "weights", "out"):
+    for name in ("grad", "count", "stats", "pairs", "out"):
         assert back(**{name: None}) == EINVAL, name
+    assert back(pairs=FAKE + 4) == EINVAL
     assert back(distill_desc(rows=0)) == 0
 
 

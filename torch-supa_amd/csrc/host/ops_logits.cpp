@@ -61,21 +61,13 @@ LogitRows logit_rows(const at::Tensor& t) {
   return {t, std::max<int64_t>(1, size[0]), {stride[1], stride[0]}};
 }
 
-void check_distill_sizes(const char* op, const at::Tensor& logits, const at::Tensor& indices, double temperature,
-                         int64_t reduction) {
+void check_distill_logits(const char* op, const at::Tensor& logits, double temperature, int64_t reduction) {
   TORCH_CHECK(is_supa(logits), op, ": expected supa tensors, got logits on ", logits.device());
   TORCH_CHECK(is_float16_or_32(logits.scalar_type()), op, ": expected float32, bfloat16 or float16, got logits of ",
               logits.scalar_type());
   TORCH_CHECK(logits.dim() >= 1 && logits.size(-1) >= 1 && logits.size(-1) < (int64_t(1) << 31), op,
               ": expected logits with a last dim of 1 to 2^31 - 1 tokens, got shape ", logits.sizes());
   TORCH_CHECK(logits.numel() / logits.size(-1) < (int64_t(1) << 31), op, ": expected fewer than 2^31 rows");
-  check_on(op, "indices", indices, logits);
-  TORCH_CHECK(is_index(indices.scalar_type()), op, ": expected int64 or int32 indices, got ", indices.scalar_type());
-  TORCH_CHECK(indices.dim() == logits.dim() && indices.sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
-              op, ": indices of shape ", indices.sizes(), " do not fit logits of shape ", logits.sizes(),
-              ": they differ in the last dim alone");
-  TORCH_CHECK(indices.size(-1) >= 1 && indices.size(-1) <= SUPA_AMD_DISTILL_MAX_ENTRIES, op, ": expected 1 to ",
-              SUPA_AMD_DISTILL_MAX_ENTRIES, " tokens a row, got ", indices.size(-1));
   TORCH_CHECK(temperature >= 1e-30 && temperature <= 1e30, op, ": expected a temperature of 1e-30 to 1e30, got ", temperature);
   check_reduction(op, reduction);
 }
@@ -83,7 +75,14 @@ void check_distill_sizes(const char* op, const at::Tensor& logits, const at::Ten
 void check_distill(const at::Tensor& logits, const at::Tensor& indices, const at::Tensor& teacher,
                    const OptTensor& teacher_lse, double temperature, int64_t reduction) {
   constexpr const char* op = "distillation_loss";
-  check_distill_sizes(op, logits, indices, temperature, reduction);
+  check_distill_logits(op, logits, temperature, reduction);
+  check_on(op, "indices", indices, logits);
+  TORCH_CHECK(is_index(indices.scalar_type()), op, ": expected int64 or int32 indices, got ", indices.scalar_type());
+  TORCH_CHECK(indices.dim() == logits.dim() && indices.sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+              op, ": indices of shape ", indices.sizes(), " do not fit logits of shape ", logits.sizes(),
+              ": they differ in the last dim alone");
+  TORCH_CHECK(indices.size(-1) >= 1 && indices.size(-1) <= SUPA_AMD_DISTILL_MAX_ENTRIES, op, ": expected 1 to ",
+              SUPA_AMD_DISTILL_MAX_ENTRIES, " tokens a row, got ", indices.size(-1));
   check_on(op, "teacher_logits", teacher, logits);
   TORCH_CHECK(is_float16_or_32(teacher.scalar_type()), op, ": expected teacher_logits of float32, bfloat16 or float16, got ",
               teacher.scalar_type());
@@ -98,48 +97,51 @@ void check_distill(const at::Tensor& logits, const at::Tensor& indices, const at
   }
 }
 
-supa_amd_distill_desc distill_desc(const LogitRows& x, const at::Tensor& indices, double temperature, int64_t reduction) {
+supa_amd_distill_desc distill_desc(const LogitRows& x, int64_t entries, double temperature, int64_t reduction) {
   supa_amd_distill_desc d{};
   d.vocab = x.t.size(-1);
   d.rows = x.t.numel() / d.vocab;
-  d.entries = indices.size(-1);
+  d.entries = entries;
   d.inner = x.inner;
   d.logits_strides[0] = x.stride[0];
   d.logits_strides[1] = x.stride[1];
   d.dtype = dtype_code(x.t.scalar_type());
   d.teacher_dtype = SUPA_AMD_F32;
-  d.index_dtype = dtype_code(indices.scalar_type());
+  d.index_dtype = SUPA_AMD_I64;
   d.reduction = (int32_t)reduction;
   d.temperature = temperature;
   d.logits = x.t.data_ptr();
-  d.indices = indices.data_ptr();
   return d;
 }
 
-// loss, count (undefined without a reduction), the rows' statistics, the pairs' weights (if wanted).
+// loss, count (undefined without a reduction), the rows' statistics, the pairs as the backward reads them (if wanted).
 using DistillResult = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>;
-DistillResult distill_outputs(const at::Tensor& logits, const at::Tensor& indices, int64_t reduction, bool want_weights) {
+DistillResult distill_outputs(const at::Tensor& logits, const at::Tensor& indices, int64_t reduction, bool want_pairs) {
   const auto leading = logits.sizes().slice(0, logits.dim() - 1);
   const int64_t stats[] = {logits.numel() / logits.size(-1), 8};
   const bool none = reduction == SUPA_AMD_REDUCTION_NONE;
+  std::vector<int64_t> pairs = indices.sizes().vec();
+  pairs.push_back(2);
   return {empty_beside(logits, none ? leading : c10::IntArrayRef(), at::kFloat),
           none ? at::Tensor() : empty_beside(logits, {}, at::kFloat), empty_beside(logits, stats, at::kFloat),
-          want_weights ? empty_beside(logits, indices.sizes(), at::kFloat) : at::Tensor()};
+          want_pairs ? empty_beside(logits, pairs, at::kInt) : at::Tensor()};
 }
 
 #define SUPA_DISTILL_PARAMS                                                                                     \
   const at::Tensor &logits, const at::Tensor &indices, const at::Tensor &teacher, const OptTensor &teacher_lse, \
       double temperature, int64_t reduction
 
-DistillResult distill_run(SUPA_DISTILL_PARAMS, bool want_weights) {
+DistillResult distill_run(SUPA_DISTILL_PARAMS, bool want_pairs) {
   check_distill(logits, indices, teacher, teacher_lse, temperature, reduction);
   const c10::DeviceGuard guard(logits.device());
-  const DistillResult r = distill_outputs(logits, indices, reduction, want_weights);
-  const auto& [loss, count, stats, weights] = r;
+  const DistillResult r = distill_outputs(logits, indices, reduction, want_pairs);
+  const auto& [loss, count, stats, pairs] = r;
   const LogitRows x = logit_rows(logits);
   const at::Tensor ids = indices.contiguous(), t = teacher.contiguous();
   const at::Tensor lse = given(teacher_lse) ? teacher_lse->to(at::kFloat).contiguous() : at::Tensor();
-  supa_amd_distill_desc d = distill_desc(x, ids, temperature, reduction);
+  supa_amd_distill_desc d = distill_desc(x, ids.size(-1), temperature, reduction);
+  d.index_dtype = dtype_code(ids.scalar_type());
+  d.indices = ids.data_ptr();
   d.teacher_dtype = dtype_code(t.scalar_type());
   d.teacher = t.data_ptr();
   // an empty tensor has no address, and says "given" all the same: there are no rows then
@@ -149,7 +151,7 @@ DistillResult distill_run(SUPA_DISTILL_PARAMS, bool want_weights) {
   TORCH_CHECK(ws_bytes >= 0, "distillation_loss: ", supa_amd_status_string((int)ws_bytes));
   const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
   check_status(supa_amd_distill_forward(&d, loss.data_ptr<float>(), count.defined() ? count.data_ptr<float>() : nullptr,
-                                        stats.data_ptr<float>(), weights.defined() ? weights.data_ptr<float>() : nullptr,
+                                        stats.data_ptr<float>(), pairs.defined() ? pairs.data_ptr() : nullptr,
                                         ws.data_ptr(), ws_bytes, stream_error_flag(dev), current_stream(dev)),
                "distillation_loss");
   return r;
@@ -171,12 +173,12 @@ DistillResult distillation_loss_forward_meta(SUPA_DISTILL_PARAMS) {
 }
 
 #define SUPA_DISTILL_BACKWARD_PARAMS                                                                             \
-  const at::Tensor &grad_loss, const at::Tensor &logits, const at::Tensor &indices, const OptTensor &count,      \
-      const at::Tensor &stats, const at::Tensor &weights, double temperature, int64_t reduction
+  const at::Tensor &grad_loss, const at::Tensor &logits, const OptTensor &count, const at::Tensor &stats,        \
+      const at::Tensor &pairs, double temperature, int64_t reduction
 
 at::Tensor distill_grad(SUPA_DISTILL_BACKWARD_PARAMS) {
   constexpr const char* op = "distillation_loss (backward)";
-  check_distill_sizes(op, logits, indices, temperature, reduction);
+  check_distill_logits(op, logits, temperature, reduction);
   const int64_t rows[] = {logits.numel() / logits.size(-1), 8};
   const bool none = reduction == SUPA_AMD_REDUCTION_NONE;
   const auto check = [&](const char* name, const at::Tensor& t, c10::IntArrayRef sizes) {
@@ -186,26 +188,29 @@ at::Tensor distill_grad(SUPA_DISTILL_BACKWARD_PARAMS) {
   };
   check("grad_loss", grad_loss, none ? logits.sizes().slice(0, logits.dim() - 1) : c10::IntArrayRef());
   check("stats", stats, rows);
-  check("weights", weights, indices.sizes());
+  check_on(op, "pairs", pairs, logits);
+  TORCH_CHECK(pairs.scalar_type() == at::kInt && pairs.dim() == logits.dim() + 1 && pairs.size(-1) == 2 &&
+                  pairs.sizes().slice(0, logits.dim() - 1) == logits.sizes().slice(0, logits.dim() - 1),
+              op, ": pairs of ", pairs.scalar_type(), " and shape ", pairs.sizes(), " do not fit logits of shape ", logits.sizes());
   TORCH_CHECK(none || given(count), op, ": expected the count of the rows");
   if (!none) check("count", *count, {});
   return empty_beside(logits, logits.sizes(), logits.scalar_type());
 }
 at::Tensor distillation_loss_backward(SUPA_DISTILL_BACKWARD_PARAMS) {
   const c10::OptionalDeviceGuard guard(logits.device());
-  const at::Tensor grad = distill_grad(grad_loss, logits, indices, count, stats, weights, temperature, reduction);
+  const at::Tensor grad = distill_grad(grad_loss, logits, count, stats, pairs, temperature, reduction);
   if (logits.numel() == 0) return grad;
   const LogitRows x = logit_rows(logits);
-  const at::Tensor ids = indices.contiguous(), g = grad_loss.contiguous(), st = stats.contiguous(), w = weights.contiguous();
-  const supa_amd_distill_desc d = distill_desc(x, ids, temperature, reduction);
+  const at::Tensor g = grad_loss.contiguous(), st = stats.contiguous(), p = pairs.contiguous();
+  const supa_amd_distill_desc d = distill_desc(x, p.size(-2), temperature, reduction);
   check_status(supa_amd_distill_backward(&d, g.data_ptr<float>(), static_cast<const float*>(ptr(count)),
-                                         st.data_ptr<float>(), w.data_ptr<float>(), grad.data_ptr(),
+                                         st.data_ptr<float>(), p.data_ptr(), grad.data_ptr(),
                                          current_stream(logits.device().index())),
                "distillation_loss (backward)");
   return grad;
 }
 at::Tensor distillation_loss_backward_meta(SUPA_DISTILL_BACKWARD_PARAMS) {
-  return distill_grad(grad_loss, logits, indices, count, stats, weights, temperature, reduction);
+  return distill_grad(grad_loss, logits, count, stats, pairs, temperature, reduction);
 }
 
 // What a node takes back from its saved tensors: hooks on them (offloading, recomputation) may give back others.
@@ -218,23 +223,22 @@ struct DistillationLossBackward final : public torch::autograd::Node {
   std::string name() const override { return "DistillationLossBackward"; }
   void release_variables() override {
     std::lock_guard<std::mutex> lock(mutex_);
-    for (SavedVariable* v : {&logits, &indices, &count, &stats, &weights}) v->reset_data();
+    for (SavedVariable* v : {&logits, &count, &stats, &pairs}) v->reset_data();
   }
   variable_list apply(variable_list&& grads) override {
     check_once("distillation_loss");
     variable_list out(1);
     if (!grads[0].defined() || !task_should_compute_output(0)) return out;
     std::lock_guard<std::mutex> lock(mutex_);
-    const at::Tensor x = logits.unpack(shared_from_this()), i = indices.unpack(shared_from_this()),
-                     s = stats.unpack(shared_from_this()), w = weights.unpack(shared_from_this()),
-                     c = count.unpack(shared_from_this());
-    for (const at::Tensor* t : {&x, &i, &s, &w}) check_back("distillation_loss", *t, grads[0].device());
+    const at::Tensor x = logits.unpack(shared_from_this()), c = count.unpack(shared_from_this()),
+                     s = stats.unpack(shared_from_this()), p = pairs.unpack(shared_from_this());
+    for (const at::Tensor* t : {&x, &s, &p}) check_back("distillation_loss", *t, grads[0].device());
     static const auto op = find_op<decltype(distillation_loss_backward)>("supa::_distillation_loss_backward");
     const at::AutoDispatchBelowAutograd below;
-    out[0] = op.call(grads[0], x, i, maybe(c), s, w, temperature, reduction);
+    out[0] = op.call(grads[0], x, maybe(c), s, p, temperature, reduction);
     return out;
   }
-  SavedVariable logits, indices, count, stats, weights;
+  SavedVariable logits, count, stats, pairs;
   double temperature;
   int64_t reduction;
 };
@@ -254,19 +258,17 @@ at::Tensor distillation_loss_autograd(c10::DispatchKeySet ks, SUPA_DISTILL_PARAM
   node->set_next_edges({torch::autograd::impl::gradient_edge(logits)});
   node->temperature = temperature;
   node->reduction = reduction;
-  at::Tensor x, ids, loss, count, stats, weights;
+  at::Tensor x, loss, count, stats, pairs;
   {
     static const auto op = find_op<decltype(distillation_loss_forward)>("supa::_distillation_loss_forward");
     const at::AutoDispatchBelowAutograd below;
     x = logit_rows(logits).t;  // a copy is made once, for both ways
-    ids = indices.contiguous();
-    std::tie(loss, count, stats, weights) = op.call(x, ids, teacher, teacher_lse, temperature, reduction);
+    std::tie(loss, count, stats, pairs) = op.call(x, indices, teacher, teacher_lse, temperature, reduction);
   }
   node->logits = SavedVariable(x, false);
-  node->indices = SavedVariable(ids, false);
   if (count.defined()) node->count = SavedVariable(count, false);
   node->stats = SavedVariable(stats, false);
-  node->weights = SavedVariable(weights, false);
+  node->pairs = SavedVariable(pairs, false);
   torch::autograd::set_history(loss, node);
   return loss;
 }
@@ -653,13 +655,13 @@ TORCH_LIBRARY_FRAGMENT(supa, m) {
   m.def(
       "distillation_loss(Tensor logits, Tensor indices, Tensor teacher_logits, Tensor? teacher_lse, float temperature, "
       "int reduction) -> Tensor");
-  // its parts for training: the count, the rows' statistics and the pairs' weights beside the loss
+  // its parts for training: the count, the rows' statistics and the pairs beside the loss
   m.def(
       "_distillation_loss_forward(Tensor logits, Tensor indices, Tensor teacher_logits, Tensor? teacher_lse, float "
       "temperature, int reduction) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def(
-      "_distillation_loss_backward(Tensor grad_loss, Tensor logits, Tensor indices, Tensor? count, Tensor stats, Tensor "
-      "weights, float temperature, int reduction) -> Tensor");
+      "_distillation_loss_backward(Tensor grad_loss, Tensor logits, Tensor? count, Tensor stats, Tensor pairs, "
+      "float temperature, int reduction) -> Tensor");
   m.def(
       "router_balance_loss(Tensor logits, Tensor experts, Tensor? mask, int scores, bool per_sequence) -> (Tensor, Tensor)");
   m.def(

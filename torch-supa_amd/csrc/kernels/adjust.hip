@@ -11,16 +11,21 @@
 // rows.  A workgroup takes a range of a row's columns.  It counts the range's tokens in LDS: it
 // reads the row's whole history (from the L2, which the row's other workgroups
 // share) and keeps what falls into its range, so no counts go through memory and there is
-// one launch; integer counts do not depend on the order of the additions.
-// Biases are put into a second table by one owner per token.  The range's
-// logits are requested before the history is read.
+// one launch; integer counts do not depend on the order of the additions.  Counts
+// are 16 bits where the history is short enough for them, so that a range is long
+// and the history is read few times; what the prompt holds and which tokens have a
+// bias are bits.  The biases are in a hash table of the range's tokens, each put
+// there by the last entry of its token, with the sum in the entries' order.  The range's first logits are requested before
+// the history is read.
 #include "row_group.h"
 
 namespace sa {
 
-constexpr int kAdjVecs = 4;                  // most vectors of logits a thread holds
-constexpr uint32_t kAdjSeen = 0x80000000u;   // in the prompt
+constexpr int kAdjVecs = 4;                  // vectors of logits that a thread has in flight
 constexpr int kAdjUnroll = 4;                // tokens of the history in flight a thread
+constexpr int kAdjMaxRange = 32768;
+constexpr int kAdjHash = 1024;               // most biases whose table is in LDS; of more, a token's are looked for in memory
+constexpr int64_t kAdjNarrow = 65535;        // the longest history that 16 bits count
 
 struct AdjustArgs {
   const void* in;
@@ -36,6 +41,7 @@ struct AdjustArgs {
   int64_t tokens_stride, bias_tokens_stride, bias_stride, allowed_stride;
   int64_t vocab, history;
   int32_t biases, range;
+  int32_t hash;     // slots of the biases' table, a power of two >= 2 biases; 0: no table
   int32_t tok64, len64, prompt64, bias_tok64;
   float repetition_value, presence_value, frequency_value;
 };
@@ -44,30 +50,51 @@ __device__ __forceinline__ int64_t adj_int(const void* p, int is64, int64_t at) 
   return is64 ? static_cast<const int64_t*>(p)[at] : (int64_t)static_cast<const int32_t*>(p)[at];
 }
 
-template <typename T, bool PEN, bool BIAS> __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
+// LDS of a workgroup, in words: counts, bits of the prompt's tokens (PEN), bits of the tokens with a
+// bias, the biases' table: tokens, then owners or values (BIAS).
+inline __host__ __device__ int adj_count_words(int range, bool wide) { return wide ? range : range / 2; }
+inline size_t adj_lds_bytes(int range, bool pen, bool wide, bool biased, int hash) {
+  return (pen ? 4 * (size_t)(adj_count_words(range, wide) + range / 32) : 0) +
+         (biased ? 4 * (size_t)(range / 32) + 8 * (size_t)hash : 0);
+}
+
+// WIDE: counts of 32 bits.
+template <typename T, bool PEN, bool WIDE, bool BIAS>
+__global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
   constexpr int V = VecOf<T>::V;
-  extern __shared__ uint32_t lds[];  // PEN: counts of the range's tokens; BIAS: their biases
+  extern __shared__ uint4 lds[];
   __shared__ int twice;
-  uint32_t* count = lds;
-  float* bias = reinterpret_cast<float*>(lds + (PEN ? g.range : 0));
+  uint32_t* const count = reinterpret_cast<uint32_t*>(lds);
+  uint32_t* const prompt_bits = count + adj_count_words(g.range, WIDE);
+  uint32_t* const bias_bits = PEN ? prompt_bits + g.range / 32 : count;
+  int32_t* const hash_at = reinterpret_cast<int32_t*>(bias_bits + g.range / 32);
+  int32_t* const hash_value = hash_at + g.hash;
   const int64_t row = row0 + blockIdx.x, c0 = (int64_t)blockIdx.y * g.range;
   const int width = (int)(g.vocab - c0 < g.range ? g.vocab - c0 : g.range), nt = blockDim.x;
   const T* in = static_cast<const T*>(g.in) + (row * g.in_stride + c0);
   T* out = static_cast<T*>(g.out) + (row * g.out_stride + c0);
   RowVec<T, V> w[kAdjVecs];
+  auto request = [&](int base) {
 #pragma unroll
-  for (int i = 0; i < kAdjVecs; ++i) {
-    const int col = (threadIdx.x + i * nt) * V;
-    if (col < width) w[i] = row_load<true, V>(in, col, width);
+    for (int i = 0; i < kAdjVecs; ++i) {
+      const int col = base + (threadIdx.x + i * nt) * V;
+      if (col < width) w[i] = row_load<true, V>(in, col, width);
+    }
+  };
+  request(0);
+  if (PEN || BIAS) {
+    const int words = (PEN ? adj_count_words(g.range, WIDE) + g.range / 32 : 0) + (BIAS ? g.range / 32 : 0);
+    for (int i = threadIdx.x; i < words / 4; i += nt) lds[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = words / 4 * 4 + threadIdx.x; i < words; i += nt) count[i] = 0u;
+    if (BIAS) {
+      for (int i = threadIdx.x; i < g.hash; i += nt) {
+        hash_at[i] = -1;
+        hash_value[i] = 0;
+      }
+      if (threadIdx.x == 0) twice = 0;
+    }
+    __syncthreads();
   }
-  if (PEN) {
-    for (int i = threadIdx.x; i < g.range; i += nt) count[i] = 0u;
-  }
-  if (BIAS) {
-    for (int i = threadIdx.x; i < g.range; i += nt) reinterpret_cast<int32_t*>(bias)[i] = 0;
-    if (threadIdx.x == 0) twice = 0;
-  }
-  if (PEN || BIAS) __syncthreads();
   float rho = 1.0f, presence = 0.0f, frequency = 0.0f;
   if constexpr (PEN) {
     rho = g.repetition ? g.repetition[row] : g.repetition_value;
@@ -90,73 +117,118 @@ template <typename T, bool PEN, bool BIAS> __global__ void __launch_bounds__(102
 #pragma unroll
       for (int u = 0; u < kAdjUnroll; ++u) {
         if ((uint64_t)tok[u] >= (uint64_t)width) continue;
-        if (t0 + u * nt < prompt) atomicOr(&count[tok[u]], kAdjSeen);
-        else atomicAdd(&count[tok[u]], 1u);
+        const int c = (int)tok[u];
+        if (t0 + u * nt < prompt) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
+        else if (WIDE) atomicAdd(&count[c], 1u);
+        else atomicAdd(&count[c / 2], c & 1 ? 0x10000u : 1u);
       }
     }
   }
+  // the slot that holds a column, or the free one that it would get: at most half of them are taken
+  auto slot_of = [&](int col, auto&& step) {
+    uint32_t h = ((uint32_t)col * 0x9E3779B1u) >> 16 & (uint32_t)(g.hash - 1);
+    while (!step(h)) h = (h + 1) & (uint32_t)(g.hash - 1);
+    return h;
+  };
+  auto find = [&](int col) { return slot_of(col, [&](uint32_t h) { return hash_at[h] == col; }); };
   if constexpr (BIAS) {
-    // the last entry of a token owns its place: first by number, then with the sum
-    int32_t* owner = reinterpret_cast<int32_t*>(bias);
     const int64_t at = row * g.bias_tokens_stride, bt = row * g.bias_stride;
-    for (int j = threadIdx.x; j < g.biases; j += nt) {
+    auto column = [&](int j) {  // of entry j; -1: elsewhere
       const int64_t tok = adj_int(g.bias_tokens, g.bias_tok64, at + j) - c0;
-      if ((uint64_t)tok < (uint64_t)width) atomicMax(&owner[tok], j + 1);
-    }
-    __syncthreads();
+      return (uint64_t)tok < (uint64_t)width ? (int)tok : -1;
+    };
     for (int j = threadIdx.x; j < g.biases; j += nt) {
-      const int64_t tok = adj_int(g.bias_tokens, g.bias_tok64, at + j) - c0;
-      if ((uint64_t)tok < (uint64_t)width && owner[tok] != j + 1) twice = 1;
+      const int col = column(j);
+      if (col < 0) continue;
+      atomicOr(&bias_bits[col / 32], 1u << (col % 32));
+      if (g.hash == 0) continue;
+      const uint32_t h = slot_of(col, [&](uint32_t h) {
+        const int was = atomicCAS(&hash_at[h], -1, col);
+        return was == -1 || was == col;
+      });
+      atomicMax(&hash_value[h], j + 1);  // the last entry owns the slot
     }
-    __syncthreads();
-    for (int j0 = 0; j0 < g.biases; j0 += nt) {
-      const int j = j0 + threadIdx.x;
-      int64_t tok = -1;
-      float b = 0.0f;
-      bool own = false;
-      if (j < g.biases) {
-        tok = adj_int(g.bias_tokens, g.bias_tok64, at + j) - c0;
-        own = (uint64_t)tok < (uint64_t)width && owner[tok] == j + 1;
-        if (own && twice) {
-          for (int i = 0; i < j; ++i)
-            if (adj_int(g.bias_tokens, g.bias_tok64, at + i) - c0 == tok) b += g.bias[bt + i];
-        }
-        if (own) b += g.bias[bt + j];
+    if (g.hash != 0) {
+      __syncthreads();
+      for (int j = threadIdx.x; j < g.biases; j += nt) {
+        const int col = column(j);
+        if (col >= 0 && hash_value[find(col)] != j + 1) twice = 1;
       }
-      __syncthreads();  // a sum's bits must not pass for an entry's number
-      if (own) bias[tok] = b;
+      __syncthreads();
+      for (int j0 = 0; j0 < g.biases; j0 += nt) {
+        const int j = j0 + threadIdx.x, col = j < g.biases ? column(j) : -1;
+        const uint32_t h = col >= 0 ? find(col) : 0u;
+        const bool own = col >= 0 && hash_value[h] == j + 1;
+        float b = 0.0f;
+        if (own) {
+          if (twice) {
+            for (int i = 0; i < j; ++i)
+              if (column(i) == col) b += g.bias[bt + i];
+          }
+          b += g.bias[bt + j];
+        }
+        __syncthreads();  // a value's bits must not pass for an entry's number
+        if (own) hash_value[h] = __float_as_int(b);
+      }
     }
   }
   if (PEN || BIAS) __syncthreads();
+  auto bias_of = [&](int col) {
+    if (g.hash != 0) return __int_as_float(hash_value[find(col)]);
+    float b = 0.0f;
+    for (int j = 0; j < g.biases; ++j)
+      if (adj_int(g.bias_tokens, g.bias_tok64, row * g.bias_tokens_stride + j) - c0 == col) b += g.bias[row * g.bias_stride + j];
+    return b;
+  };
   const uint32_t* allowed = g.allowed ? g.allowed + row * g.allowed_stride : nullptr;
+  for (int base = 0; base < width; base += nt * V * kAdjVecs) {
+    if (base > 0) request(base);
 #pragma unroll
-  for (int i = 0; i < kAdjVecs; ++i) {
-    const int col = (threadIdx.x + i * nt) * V;
-    if (col >= width) continue;
-    float f[V];
+    for (int i = 0; i < kAdjVecs; ++i) {
+      const int col = base + (threadIdx.x + i * nt) * V;  // the tables reach to the range's end, which is whole vectors
+      if (col >= width) continue;
+      float f[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      f[k] = row_elem<T, V>(w[i], k);
-      const int at = col + k;  // tables reach to the end of the range, which is whole vectors
+      for (int k = 0; k < V; ++k) f[k] = row_elem<T, V>(w[i], k);
+      constexpr uint32_t all = (1u << V) - 1u;
       if constexpr (PEN) {
-        const uint32_t c = count[at];
-        if (c) {
-          f[k] = f[k] > 0.0f ? f[k] / rho : f[k] * rho;
-          const float times = (float)(c & ~kAdjSeen);
-          f[k] = f[k] - frequency * times;
-          f[k] = f[k] - (times > 0.0f ? presence : 0.0f);
+        uint32_t c[WIDE ? V : V / 2], any = 0u;
+        __builtin_memcpy(c, count + (WIDE ? col : col / 2), sizeof(c));
+#pragma unroll
+        for (int k = 0; k < (WIDE ? V : V / 2); ++k) any |= c[k];
+        const uint32_t said = prompt_bits[col / 32] >> (col % 32) & all;
+        if (any | said) {
+#pragma unroll
+          for (int k = 0; k < V; ++k) {
+            const uint32_t n = WIDE ? c[k] : (c[k / 2] >> (k % 2 * 16) & 0xffffu);
+            if (n == 0u && !(said >> k & 1u)) continue;
+            f[k] = f[k] > 0.0f ? f[k] / rho : f[k] * rho;
+            f[k] = f[k] - frequency * (float)n;
+            f[k] = f[k] - (n > 0u ? presence : 0.0f);
+          }
         }
       }
-      if constexpr (BIAS) f[k] = f[k] + bias[at];
-    }
-    if (allowed) {
-      const int64_t v = c0 + col;
-      const uint32_t bits = allowed[v / 32] >> (v % 32);
+      if constexpr (BIAS) {
+        const uint32_t biased = bias_bits[col / 32] >> (col % 32) & all;
+        if (biased) {
+#pragma unroll 1
+          for (int k = 0; k < V; ++k)
+            if (biased >> k & 1u) {
+              const float b = bias_of(col + k);
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (!(bits >> k & 1u)) f[k] = -__builtin_inff();
+              for (int e = 0; e < V; ++e) f[e] = e == k ? f[e] + b : f[e];
+            }
+        }
+      }
+      if (allowed) {
+        const int64_t v = c0 + col;
+        const uint32_t bits = allowed[v / 32] >> (v % 32);
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+          if (!(bits >> k & 1u)) f[k] = -__builtin_inff();
+      }
+      row_store<T, V>(out, col, width, f);
     }
-    row_store<T, V>(out, col, width, f);
   }
 }
 
@@ -210,20 +282,33 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
   return with_float_storage(d->dtype, [&](auto* tag) -> int {
     using T = std::remove_pointer_t<decltype(tag)>;
     constexpr int V = VecOf<T>::V;
-    // a thread holds up to kAdjVecs vectors; 8192 columns' two tables are 64 KiB of LDS
-    const int block = 1024;
-    a.range = 8192;
+    const bool wide = pen && d->history > kAdjNarrow;
+    // 512 workgroups, two a CU, if the rows are long enough for them; no shorter ranges than 1024
+    // columns, and none whose counts pass 64 KiB of LDS: two workgroups a CU
+    if (biased && a.biases <= kAdjHash) {
+      a.hash = 64;
+      while (a.hash < 2 * a.biases) a.hash *= 2;
+    }
+    a.range = 1024;
+    while (a.range < (wide || a.hash > 512 ? 16384 : kAdjMaxRange) && (a.vocab + a.range - 1) / a.range * d->rows > 512) a.range *= 2;
+    const int block = std::min(1024, a.range / V);
     const unsigned ranges = (unsigned)((a.vocab + a.range - 1) / a.range);
-    static_assert(1024 * kAdjVecs * V >= 8192);
-    const size_t lds = (size_t)a.range * 4 * ((pen ? 1 : 0) + (biased ? 1 : 0));
+    const size_t lds = adj_lds_bytes(a.range, pen, wide, biased, a.hash);
     const int64_t slab = std::max<int64_t>(1, ((int64_t(1) << 32) - 1) / block / ranges);
     for (int64_t r0 = 0; r0 < d->rows; r0 += slab) {
       const dim3 grid((unsigned)std::min(slab, d->rows - r0), ranges);
-      if (pen && biased) k_adjust<T, true, true><<<grid, block, lds, st>>>(a, r0);
-      else if (pen) k_adjust<T, true, false><<<grid, block, lds, st>>>(a, r0);
-      else if (biased) k_adjust<T, false, true><<<grid, block, lds, st>>>(a, r0);
-      else k_adjust<T, false, false><<<grid, block, lds, st>>>(a, r0);
-      const int rc = launch_status();
+      auto go = [&](auto p, auto w, auto b) {
+        auto kernel = k_adjust<T, p.value, w.value, b.value>;
+        if (lds > 65536) {
+          const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+          if (e != hipSuccess) return (int)e;
+        }
+        kernel<<<grid, block, lds, st>>>(a, r0);
+        return launch_status();
+      };
+      auto with_bias = [&](auto p, auto w) { return biased ? go(p, w, std::true_type{}) : go(p, w, std::false_type{}); };
+      const int rc = !pen ? with_bias(std::false_type{}, std::false_type{})
+                          : (wide ? with_bias(std::true_type{}, std::true_type{}) : with_bias(std::true_type{}, std::false_type{}));
       if (rc) return rc;
     }
     return SUPA_AMD_OK;

@@ -28,31 +28,31 @@ struct BalanceArgs {
   const void* chosen;
   const uint8_t* mask;
   int64_t tokens;          // of a sequence
-  int32_t experts, k, idx64, blocks;  // blocks: workgroups a sequence
+  int32_t experts, k, idx64;
+  int32_t blocks;          // workgroups a sequence
   int64_t sequences;
 };
 
-__device__ __forceinline__ float max16(float v) {
+// Maximum or sum over the G threads of a token (4, 8, 16 or 64), in every one of them.
+template <int G, typename F> __device__ __forceinline__ float token_join(float v, F&& f) {
   auto perm = [](float x, auto ctrl) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), decltype(ctrl)::value, 0xf, 0xf, true));
   };
-  v = fmaxf(v, perm(v, std::integral_constant<int, 0xB1>{}));
-  v = fmaxf(v, perm(v, std::integral_constant<int, 0x4E>{}));
-  v = fmaxf(v, perm(v, std::integral_constant<int, 0x141>{}));
-  v = fmaxf(v, perm(v, std::integral_constant<int, 0x140>{}));
-  return v;
-}
-template <int G> __device__ __forceinline__ float token_max(float v) {
-  v = max16(v);
+  v = f(v, perm(v, std::integral_constant<int, 0xB1>{}));                           // quad_perm [1, 0, 3, 2]
+  v = f(v, perm(v, std::integral_constant<int, 0x4E>{}));                           // quad_perm [2, 3, 0, 1]
+  if constexpr (G >= 8) v = f(v, perm(v, std::integral_constant<int, 0x141>{}));    // row_half_mirror
+  if constexpr (G >= 16) v = f(v, perm(v, std::integral_constant<int, 0x140>{}));   // row_mirror
   if constexpr (G == 64) {
     auto lane = [&](int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), l)); };
-    return fmaxf(fmaxf(lane(0), lane(16)), fmaxf(lane(32), lane(48)));
+    v = f(f(lane(0), lane(16)), f(lane(32), lane(48)));
   }
   return v;
 }
+template <int G> __device__ __forceinline__ float token_max(float v) {
+  return token_join<G>(v, [](float a, float b) { return fmaxf(a, b); });
+}
 template <int G> __device__ __forceinline__ float token_sum(float v) {
-  if constexpr (G == 64) return sum64(v);
-  else return sum16(v);
+  return token_join<G>(v, [](float a, float b) { return a + b; });
 }
 
 // The thread's columns of a token: NV vectors of V, the one that would run past the
@@ -179,12 +179,10 @@ k_balance_fwd(BalanceArgs g, int64_t seq0, float* __restrict__ part_p, int32_t* 
     }
   }
   // the groups of a wavefront, then the wavefronts
-  if constexpr (G == 16) {
 #pragma unroll
-    for (int i = 0; i < NV * V; ++i) {
-      acc[i] += __shfl_xor(acc[i], 16, 64);
-      acc[i] += __shfl_xor(acc[i], 32, 64);
-    }
+  for (int off = G; off < 64; off *= 2) {
+#pragma unroll
+    for (int i = 0; i < NV * V; ++i) acc[i] += __shfl_xor(acc[i], off, 64);
   }
   const int wave = threadIdx.x >> 6;
   if ((threadIdx.x & 63) < G) {
@@ -365,12 +363,44 @@ int balance_args(const supa_amd_balance_desc* d, BalanceArgs& g) {
   g.experts = (int32_t)d->experts;
   g.k = (int32_t)d->k;
   g.idx64 = d->index_dtype == SUPA_AMD_I64;
-  // up to 512 workgroups in all, each with some rounds of its groups
-  const int64_t round = 4 * kBalUnroll;
-  const int64_t want = (d->tokens + round - 1) / round;
-  g.blocks = (int32_t)std::max<int64_t>(1, std::min<int64_t>(want, std::max<int64_t>(1, 512 / std::max<int64_t>(1, d->sequences))));
   return SUPA_AMD_OK;
 }
+
+// f(type, threads a token, vectors a thread).  Few threads with up to 16 elements each: what a token's threads
+// exchange, its maximum and sum, is then a few steps for many tokens at once.
+template <typename F> int with_balance(const supa_amd_balance_desc* d, F&& f) {
+  return with_float_storage(d->dtype, [&](auto* tag) -> int {
+    using T = std::remove_pointer_t<decltype(tag)>;
+    constexpr int V = 16 / (int)sizeof(T), N = 16 / V;
+    auto scores = [&](auto threads, auto vecs) -> int {
+      return d->scores == SUPA_AMD_SCORES_SIGMOID ? f(tag, threads, vecs, std::true_type{})
+                                                  : f(tag, threads, vecs, std::false_type{});
+    };
+    using std::integral_constant;
+    const int64_t vecs = (d->experts + V - 1) / V;
+    if (vecs <= 4) return scores(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    if (vecs <= 4 * N) return scores(integral_constant<int, 4>{}, integral_constant<int, N>{});
+    if (vecs <= 8 * N) return scores(integral_constant<int, 8>{}, integral_constant<int, N>{});
+    if (vecs <= 16 * N) return scores(integral_constant<int, 16>{}, integral_constant<int, N>{});
+    return scores(integral_constant<int, 64>{}, integral_constant<int, N>{});
+  });
+}
+
+// Threads that share a token, as with_balance chooses them.
+int balance_threads(int64_t experts, int dtype) {
+  const int64_t vecs = (experts * dtype_size(dtype) + 15) / 16;
+  const int n = dtype == SUPA_AMD_F32 ? 4 : 2;
+  return vecs <= 4 * n ? 4 : (vecs <= 8 * n ? 8 : (vecs <= 16 * n ? 16 : 64));
+}
+
+// Workgroups a sequence: `most` in all, each with a round of its groups at least.
+int32_t balance_blocks(const supa_amd_balance_desc* d, int64_t most) {
+  const int64_t round = kBalBlock / balance_threads(d->experts, d->dtype) * kBalUnroll;
+  const int64_t want = (d->tokens + round - 1) / round, each = std::max<int64_t>(1, most / std::max<int64_t>(1, d->sequences));
+  return (int32_t)std::max<int64_t>(1, std::min(want, each));
+}
+constexpr int64_t kBalFwdBlocks = 1024;  // whose partials the second launch adds
+constexpr int64_t kBalBwdBlocks = 1 << 14;
 
 // Workspace: the shares of the loss, then the partials: sums, counts, tokens; the arrivals.
 struct BalanceSpace {
@@ -387,25 +417,6 @@ BalanceSpace balance_space(const BalanceArgs& g) {
   return s;
 }
 
-// f(type, threads a token, vectors a thread): the fewest registers that hold the experts.
-template <typename F> int with_balance(const supa_amd_balance_desc* d, F&& f) {
-  return with_float_storage(d->dtype, [&](auto* tag) -> int {
-    using T = std::remove_pointer_t<decltype(tag)>;
-    constexpr int V = 16 / (int)sizeof(T);
-    auto scores = [&](auto threads, auto vecs) -> int {
-      return d->scores == SUPA_AMD_SCORES_SIGMOID ? f(tag, threads, vecs, std::true_type{})
-                                                  : f(tag, threads, vecs, std::false_type{});
-    };
-    using std::integral_constant;
-    if (d->experts <= 16 * V) return scores(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    if (d->experts <= 64 * V) return scores(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    if constexpr (V == 4) {
-      if (d->experts > 128 * V) return scores(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    }
-    return scores(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  });
-}
-
 }  // namespace sa
 
 using namespace sa;
@@ -415,7 +426,9 @@ extern "C" {
 int64_t supa_amd_balance_workspace_bytes(const supa_amd_balance_desc* d) {
   BalanceArgs g;
   const int rc = balance_args(d, g);
-  return rc ? rc : balance_space(g).bytes;
+  if (rc) return rc;
+  g.blocks = balance_blocks(d, kBalFwdBlocks);
+  return balance_space(g).bytes;
 }
 
 int supa_amd_balance_forward(const supa_amd_balance_desc* d, float* loss, int64_t* counts, float* load, float* scale,
@@ -425,6 +438,7 @@ int supa_amd_balance_forward(const supa_amd_balance_desc* d, float* loss, int64_
   if (rc) return rc;
   if (d->sequences == 0) return SUPA_AMD_EINVAL;
   if (!loss || !counts || !load || !scale || (d->tokens > 0 && (!d->logits || !d->chosen))) return SUPA_AMD_EINVAL;
+  g.blocks = balance_blocks(d, kBalFwdBlocks);
   const BalanceSpace s = balance_space(g);
   if (!workspace || ws_bytes < s.bytes) return SUPA_AMD_EWORKSPACE;
   if (!aligned(workspace, 8)) return SUPA_AMD_EINVAL;
@@ -463,6 +477,7 @@ int supa_amd_balance_backward(const supa_amd_balance_desc* d, const float* grad_
   if (rc) return rc;
   if (d->sequences == 0 || d->tokens == 0) return SUPA_AMD_OK;
   if (!grad_loss || !load || !scale || !grad_logits || !d->logits) return SUPA_AMD_EINVAL;
+  g.blocks = balance_blocks(d, kBalBwdBlocks);
   hipStream_t st = static_cast<hipStream_t>(stream);
   for (int64_t s0 = 0; s0 < g.sequences; s0 += 65535) {
     const unsigned n = (unsigned)std::min<int64_t>(65535, g.sequences - s0);
