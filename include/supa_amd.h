@@ -943,15 +943,16 @@ typedef struct supa_amd_distill_desc {
   int64_t vocab;             /* 1 .. 2^31 - 1 */
   int64_t entries;           /* 1 .. SUPA_AMD_DISTILL_MAX_ENTRIES */
   int64_t inner;             /* row r of the logits lies at (r / inner) logits_strides[0] + (r % inner) logits_strides[1] */
-  int64_t logits_strides[2]; /* elements; those of a row are contiguous */
+  int64_t logits_strides[2]; /* elements; those of a row are contiguous.  So for the others' rows: */
+  int64_t indices_strides[2], teacher_strides[2], lse_strides[2];
   int32_t dtype;             /* of the logits: f32, bf16 or f16 */
   int32_t teacher_dtype;     /* f32, bf16 or f16 */
   int32_t index_dtype;       /* I64 or I32 */
   int32_t reduction;         /* SUPA_AMD_REDUCTION_* */
   double temperature;        /* 1e-30 .. 1e30 */
   const void* logits;
-  const void* indices;       /* [rows, entries], contiguous */
-  const void* teacher;       /* [rows, entries], contiguous */
+  const void* indices;       /* [rows, entries] */
+  const void* teacher;       /* [rows, entries] */
   const float* teacher_lse;  /* [rows], or NULL */
 } supa_amd_distill_desc;
 

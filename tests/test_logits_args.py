@@ -16,7 +16,8 @@ FAKE = 256  # never dereferenced: the checks come first
 
 
 class DistillDesc(ctypes.Structure):
-    _fields_ = [(n, i64) for n in ("rows", "vocab", "entries", "inner")] + [("logits_strides", i64 * 2)] + [
+    _fields_ = [(n, i64) for n in ("rows", "vocab", "entries", "inner")] + [
+        (n + "_strides", i64 * 2) for n in ("logits", "indices", "teacher", "lse")] + [
         (n, i32) for n in ("dtype", "teacher_dtype", "index_dtype", "reduction")] + [("temperature", dbl)] + [
         (n, vp) for n in ("logits", "indices", "teacher", "teacher_lse")]
 

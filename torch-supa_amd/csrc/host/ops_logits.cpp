@@ -61,6 +61,24 @@ LogitRows logit_rows(const at::Tensor& t) {
   return {t, std::max<int64_t>(1, size[0]), {stride[1], stride[0]}};
 }
 
+// Rows of another tensor of the logits' leading dims, split into outer and inner ones as the
+// logits' are; `width` elements each, contiguous (has_row: in a last dim of its own).  A copy where a view
+// has no such form.
+LogitRows rows_beside(const at::Tensor& t, int64_t inner, bool has_row) {
+  const int64_t leading = t.dim() - (has_row ? 1 : 0), width = has_row ? t.size(-1) : 1;
+  bool ok = !has_row || width == 1 || t.stride(-1) == 1;
+  int64_t size[2] = {1, 1}, stride[2] = {0, 0};  // inner, outer
+  for (int64_t i = leading - 1; i >= 0 && ok; --i) {
+    if (t.size(i) == 1) continue;
+    const int level = size[0] == inner ? 1 : 0;
+    if (size[level] == 1) stride[level] = t.stride(i);
+    else ok = t.stride(i) == stride[level] * size[level];
+    size[level] *= t.size(i);
+  }
+  if (!ok || (size[0] != inner && t.numel() > 0)) return {t.contiguous(), inner, {inner * width, width}};
+  return {t, inner, {stride[1], stride[0]}};
+}
+
 void check_distill_logits(const char* op, const at::Tensor& logits, double temperature, int64_t reduction) {
   TORCH_CHECK(is_supa(logits), op, ": expected supa tensors, got logits on ", logits.device());
   TORCH_CHECK(is_float16_or_32(logits.scalar_type()), op, ": expected float32, bfloat16 or float16, got logits of ",
@@ -137,15 +155,21 @@ DistillResult distill_run(SUPA_DISTILL_PARAMS, bool want_pairs) {
   const DistillResult r = distill_outputs(logits, indices, reduction, want_pairs);
   const auto& [loss, count, stats, pairs] = r;
   const LogitRows x = logit_rows(logits);
-  const at::Tensor ids = indices.contiguous(), t = teacher.contiguous();
-  const at::Tensor lse = given(teacher_lse) ? teacher_lse->to(at::kFloat).contiguous() : at::Tensor();
-  supa_amd_distill_desc d = distill_desc(x, ids.size(-1), temperature, reduction);
-  d.index_dtype = dtype_code(ids.scalar_type());
-  d.indices = ids.data_ptr();
-  d.teacher_dtype = dtype_code(t.scalar_type());
-  d.teacher = t.data_ptr();
+  const LogitRows ids = rows_beside(indices, x.inner, true), t = rows_beside(teacher, x.inner, true);
+  supa_amd_distill_desc d = distill_desc(x, indices.size(-1), temperature, reduction);
+  d.index_dtype = dtype_code(indices.scalar_type());
+  d.indices = ids.t.data_ptr();
+  d.teacher_dtype = dtype_code(teacher.scalar_type());
+  d.teacher = t.t.data_ptr();
+  LogitRows lse{};
+  if (given(teacher_lse)) lse = rows_beside(teacher_lse->to(at::kFloat), x.inner, false);
+  for (int i = 0; i < 2; ++i) {
+    d.indices_strides[i] = ids.stride[i];
+    d.teacher_strides[i] = t.stride[i];
+    d.lse_strides[i] = lse.stride[i];
+  }
   // an empty tensor has no address, and says "given" all the same: there are no rows then
-  d.teacher_lse = lse.defined() ? lse.data_ptr<float>() : nullptr;
+  d.teacher_lse = lse.t.defined() ? lse.t.data_ptr<float>() : nullptr;
   const auto dev = logits.device().index();
   const int64_t ws_bytes = supa_amd_distill_workspace_bytes(&d);
   TORCH_CHECK(ws_bytes >= 0, "distillation_loss: ", supa_amd_status_string((int)ws_bytes));

@@ -58,6 +58,11 @@ inline size_t adj_lds_bytes(int range, bool pen, bool wide, bool biased, int has
          (biased ? 4 * (size_t)(range / 32) + 8 * (size_t)hash : 0);
 }
 
+// A token's column from c0 on; one far outside is not in any range.
+__device__ __forceinline__ int64_t adj_column(const void* p, int is64, int64_t at, int64_t c0) {
+  return (int64_t)((uint64_t)adj_int(p, is64, at) - (uint64_t)c0);
+}
+
 // WIDE: counts of 32 bits.
 template <typename T, bool PEN, bool WIDE, bool BIAS>
 __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
@@ -82,6 +87,42 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     }
   };
   request(0);
+  // the first tokens of the history too, also where they turn out to lie behind its length
+  int64_t tok[kAdjUnroll];
+  const int64_t tokens_at = row * g.tokens_stride;
+  auto history = [&](int64_t t0, int64_t n) {
+#pragma unroll
+    for (int u = 0; u < kAdjUnroll; ++u) {
+      const int64_t t = t0 + u * nt;
+      tok[u] = t < n ? adj_column(g.tokens, g.tok64, tokens_at + t, c0) : -1;
+    }
+  };
+  float rho = 1.0f, presence = 0.0f, frequency = 0.0f;
+  int64_t n = g.history, prompt = 0;
+  if constexpr (PEN) {
+    history(threadIdx.x, n);
+    rho = g.repetition ? g.repetition[row] : g.repetition_value;
+    presence = g.presence ? g.presence[row] : g.presence_value;
+    frequency = g.frequency ? g.frequency[row] : g.frequency_value;
+    if (g.lengths) {
+      const int64_t v = adj_int(g.lengths, g.len64, row);
+      n = v < 0 ? 0 : (v < n ? v : n);
+    }
+    if (g.prompts) prompt = adj_int(g.prompts, g.prompt64, row);
+  }
+  const int64_t bias_tokens_at = row * g.bias_tokens_stride, bias_at = row * g.bias_stride;
+  auto column = [&](int j) {  // of bias j; -1: elsewhere
+    const int64_t t = adj_column(g.bias_tokens, g.bias_tok64, bias_tokens_at + j, c0);
+    return (uint64_t)t < (uint64_t)width ? (int)t : -1;
+  };
+  int first_column = -1;  // of the thread's first bias, and the bias
+  float first_bias = 0.0f;
+  if constexpr (BIAS) {
+    if ((int)threadIdx.x < g.biases) {
+      first_column = column(threadIdx.x);
+      first_bias = g.bias[bias_at + threadIdx.x];
+    }
+  }
   if (PEN || BIAS) {
     const int words = (PEN ? adj_count_words(g.range, WIDE) + g.range / 32 : 0) + (BIAS ? g.range / 32 : 0);
     for (int i = threadIdx.x; i < words / 4; i += nt) lds[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -95,33 +136,19 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     }
     __syncthreads();
   }
-  float rho = 1.0f, presence = 0.0f, frequency = 0.0f;
   if constexpr (PEN) {
-    rho = g.repetition ? g.repetition[row] : g.repetition_value;
-    presence = g.presence ? g.presence[row] : g.presence_value;
-    frequency = g.frequency ? g.frequency[row] : g.frequency_value;
-    int64_t n = g.history, prompt = 0;
-    if (g.lengths) {
-      const int64_t v = adj_int(g.lengths, g.len64, row);
-      n = v < 0 ? 0 : (v < n ? v : n);
-    }
-    if (g.prompts) prompt = adj_int(g.prompts, g.prompt64, row);
-    const int64_t at = row * g.tokens_stride;
-    for (int64_t t0 = threadIdx.x; t0 < n; t0 += (int64_t)nt * kAdjUnroll) {
-      int64_t tok[kAdjUnroll];
+    for (int64_t t0 = threadIdx.x; t0 < n;) {
 #pragma unroll
       for (int u = 0; u < kAdjUnroll; ++u) {
         const int64_t t = t0 + u * nt;
-        tok[u] = t < n ? adj_int(g.tokens, g.tok64, at + t) - c0 : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < kAdjUnroll; ++u) {
-        if ((uint64_t)tok[u] >= (uint64_t)width) continue;
+        if ((uint64_t)tok[u] >= (uint64_t)width || t >= n) continue;
         const int c = (int)tok[u];
-        if (t0 + u * nt < prompt) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
+        if (t < prompt) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
         else if (WIDE) atomicAdd(&count[c], 1u);
         else atomicAdd(&count[c / 2], c & 1 ? 0x10000u : 1u);
       }
+      t0 += (int64_t)nt * kAdjUnroll;
+      if (t0 < n) history(t0, n);
     }
   }
   // the slot that holds a column, or the free one that it would get: at most half of them are taken
@@ -132,13 +159,9 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
   };
   auto find = [&](int col) { return slot_of(col, [&](uint32_t h) { return hash_at[h] == col; }); };
   if constexpr (BIAS) {
-    const int64_t at = row * g.bias_tokens_stride, bt = row * g.bias_stride;
-    auto column = [&](int j) {  // of entry j; -1: elsewhere
-      const int64_t tok = adj_int(g.bias_tokens, g.bias_tok64, at + j) - c0;
-      return (uint64_t)tok < (uint64_t)width ? (int)tok : -1;
-    };
+    auto column_of = [&](int j) { return j == (int)threadIdx.x ? first_column : column(j); };
     for (int j = threadIdx.x; j < g.biases; j += nt) {
-      const int col = column(j);
+      const int col = column_of(j);
       if (col < 0) continue;
       atomicOr(&bias_bits[col / 32], 1u << (col % 32));
       if (g.hash == 0) continue;
@@ -151,21 +174,21 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     if (g.hash != 0) {
       __syncthreads();
       for (int j = threadIdx.x; j < g.biases; j += nt) {
-        const int col = column(j);
+        const int col = column_of(j);
         if (col >= 0 && hash_value[find(col)] != j + 1) twice = 1;
       }
       __syncthreads();
       for (int j0 = 0; j0 < g.biases; j0 += nt) {
-        const int j = j0 + threadIdx.x, col = j < g.biases ? column(j) : -1;
+        const int j = j0 + threadIdx.x, col = j < g.biases ? column_of(j) : -1;
         const uint32_t h = col >= 0 ? find(col) : 0u;
         const bool own = col >= 0 && hash_value[h] == j + 1;
         float b = 0.0f;
         if (own) {
           if (twice) {
             for (int i = 0; i < j; ++i)
-              if (column(i) == col) b += g.bias[bt + i];
+              if (column(i) == col) b += g.bias[bias_at + i];
           }
-          b += g.bias[bt + j];
+          b += j == (int)threadIdx.x ? first_bias : g.bias[bias_at + j];
         }
         __syncthreads();  // a value's bits must not pass for an entry's number
         if (own) hash_value[h] = __float_as_int(b);
@@ -177,7 +200,7 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     if (g.hash != 0) return __int_as_float(hash_value[find(col)]);
     float b = 0.0f;
     for (int j = 0; j < g.biases; ++j)
-      if (adj_int(g.bias_tokens, g.bias_tok64, row * g.bias_tokens_stride + j) - c0 == col) b += g.bias[row * g.bias_stride + j];
+      if (column(j) == col) b += g.bias[bias_at + j];
     return b;
   };
   const uint32_t* allowed = g.allowed ? g.allowed + row * g.allowed_stride : nullptr;
@@ -291,7 +314,9 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
     }
     a.range = 1024;
     while (a.range < (wide || a.hash > 512 ? 16384 : kAdjMaxRange) && (a.vocab + a.range - 1) / a.range * d->rows > 512) a.range *= 2;
-    const int block = std::min(1024, a.range / V);
+    // a vector of the range for each thread, and of a history 8 tokens at most, up to 1024 threads
+    const int64_t threads = std::max<int64_t>(a.range / V, pen ? (d->history / 8 + 63) / 64 * 64 : 0);
+    const int block = (int)std::min<int64_t>(1024, threads);
     const unsigned ranges = (unsigned)((a.vocab + a.range - 1) / a.range);
     const size_t lds = adj_lds_bytes(a.range, pen, wide, biased, a.hash);
     const int64_t slab = std::max<int64_t>(1, ((int64_t(1) << 32) - 1) / block / ranges);

@@ -20,17 +20,14 @@
 // A token listed twice has the sum of its p: the row's first such pair carries it.
 // Twice-listed tokens are found by a hash table in LDS; only rows that have one
 // compare all pairs.
-#include <cmath>
-
-#include "softmax_common.h"
+#include "row_group.h"
 
 namespace sa {
 
 constexpr int kDisBlock = 256;
-constexpr int kDisEntries = 4;            // pairs a thread holds in the forward
-constexpr int kDisMaxEntries = kDisBlock * kDisEntries;
+constexpr int kDisMaxEntries = 1024;
 static_assert(kDisMaxEntries == SUPA_AMD_DISTILL_MAX_ENTRIES);
-constexpr int kDisUnroll = 4;             // 16-byte vectors in flight per thread
+constexpr int kDisUnroll = 2;             // 16-byte vectors in flight per thread
 constexpr int kDisWaveVecs = 2048;        // most vectors of a row that a wavefront takes alone
 constexpr int kDisSegment = 1 << 17;      // columns whose bitmap is in LDS at a time: 16 KiB
 constexpr int kDisStats = 8;              // floats a row keeps for the backward
@@ -42,15 +39,14 @@ struct DistillArgs {
   const void* idx;
   const void* teacher;
   const float* teacher_lse;
-  int64_t xs[2];     // distance of rows: outer, inner
+  int64_t xs[2], is[2], ts[2], ls[2];  // distances of rows, outer and inner: of logits, indices, teacher, teacher_lse
   FastDiv inner;     // row -> (outer, inner)
   int64_t vocab;
   int32_t entries, hash;  // pairs a row; slots of its hash table, a power of two >= 2 entries
   int32_t idx64, teacher_dtype;
   int32_t segment;   // columns of a bitmap
-  double c;          // log2(e) / temperature
-  float c_near;      // c rounded
-  float c_hi, c_lo;  // c in two parts, both above 0: -inf stays -inf through their products
+  double teacher_c;  // log2(e) / temperature
+  float c;           // that rounded, for all that is the student's: a temperature off by 2^-25 of itself
   double inv_t;
 };
 
@@ -59,67 +55,48 @@ template <typename T> __device__ __forceinline__ const T* dis_row(const DistillA
   g.inner.divmod((uint32_t)row, o, i);
   return static_cast<const T*>(g.x) + ((int64_t)o * g.xs[0] + (int64_t)i * g.xs[1]);
 }
+// Where a row of one of the others starts.
+__device__ __forceinline__ int64_t dis_at(const DistillArgs& g, int64_t row, const int64_t (&strides)[2]) {
+  uint32_t o, i;
+  g.inner.divmod((uint32_t)row, o, i);
+  return (int64_t)o * strides[0] + (int64_t)i * strides[1];
+}
 __device__ __forceinline__ int64_t dis_index(const DistillArgs& g, int64_t at) {
   return g.idx64 ? static_cast<const int64_t*>(g.idx)[at] : (int64_t)static_cast<const int32_t*>(g.idx)[at];
 }
 
-// Exchange among the G threads of a row through LDS.
-template <int G> __device__ __forceinline__ void team_sync() {
-  if constexpr (G == 64) {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-  } else {
-    __syncthreads();
-  }
+// Exchange among the threads of a wavefront through LDS.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
-// Maxima / sums of N values over the G threads, in every one of them, in a fixed order.  lds: N values
-// a wavefront of the row, used by no other exchange.
-template <int G, int N> __device__ __forceinline__ void team_max(float (&v)[N], float* lds) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v[i] = fmaxf(v[i], __shfl_xor(v[i], off, 64));
-  }
-  if constexpr (G > 64) {
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) lds[wave * N + i] = v[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-#pragma unroll
-      for (int w = 0; w < G / 64; ++w) v[i] = fmaxf(v[i], lds[w * N + i]);
-    }
-  }
+  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
+  return v;
 }
-template <int G, int N> __device__ __forceinline__ void team_sum(double (&v)[N], double* lds) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v[i] += __shfl_xor(v[i], off, 64);
-  }
-  if constexpr (G > 64) {
-    const int wave = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) lds[wave * N + i] = v[i];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      v[i] = lds[i];
-#pragma unroll
-      for (int w = 1; w < G / 64; ++w) v[i] += lds[w * N + i];
-    }
-  }
+// The sum of a wavefront, in every lane: four lane permutations within 16 lanes, then the four rows of 16.
+__device__ __forceinline__ double wave_sum(double v) {
+  auto halves = [](double x, auto&& f) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)f((int)(uint32_t)u), hi = (uint32_t)f((int)(uint32_t)(u >> 32));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  auto perm = [&](double x, auto ctrl) {
+    return halves(x, [](int h) { return __builtin_amdgcn_update_dpp(0, h, decltype(ctrl)::value, 0xf, 0xf, true); });
+  };
+  v += perm(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1, 0, 3, 2]
+  v += perm(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2, 3, 0, 1]
+  v += perm(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
+  v += perm(v, std::integral_constant<int, 0x140>{});  // row_mirror
+  auto lane = [&](int l) { return halves(v, [&](int h) { return __builtin_amdgcn_readlane(h, l); }); };
+  return (lane(0) + lane(16)) + (lane(32) + lane(48));
 }
 
-// A row's pairs: thread l of G holds pairs l, l + G, ...
-struct DistillEntries {
-  int32_t at[kDisEntries];  // token, or -1: none there
-  float t[kDisEntries], x[kDisEntries];  // teacher's and student's logits
+// A row's pairs in a wavefront: lane l holds pairs l, l + 64, ... NE of them.
+template <int NE> struct DistillEntries {
+  int32_t at[NE];          // token, or -1: none there
+  float t[NE], x[NE];      // teacher's and student's logits
 };
 
 // A pair as the backward reads it: the token, or -1 where another pair carries it or none is there, and the bits of its p.
@@ -135,8 +112,10 @@ struct DistillLds {
   int32_t* hash;
   uint32_t* bits;
 };
-inline __host__ __device__ size_t dis_lds_bytes(int entries, int hash, int64_t segment) {
-  return (size_t)((entries + 1) / 2 * 2) * 12 + (size_t)hash * 4 + (size_t)((segment + 63) / 64) * 8;
+// Words of a bitmap: a segment, which may begin some places into a vector and end in one.
+inline __host__ __device__ int dis_bit_words(int segment) { return (segment + 16 + 63) / 64 * 2; }
+inline __host__ __device__ size_t dis_lds_bytes(int entries, int hash, int segment) {
+  return (size_t)((entries + 1) / 2 * 2) * 12 + (size_t)hash * 4 + (segment > 0 ? 4 * (size_t)dis_bit_words(segment) : 0);
 }
 __device__ __forceinline__ DistillLds dis_lds(char* p, int entries, int hash) {
   const int n = (entries + 1) / 2 * 2;
@@ -148,39 +127,55 @@ __device__ __forceinline__ DistillLds dis_lds(char* p, int entries, int hash) {
   return s;
 }
 
-// Loads a row's pairs, and finds tokens that are listed twice (*dup, zero before).  A pair is there if its
-// token is in [0, vocab) and its teacher logit is not -inf.  Not HASH: the tokens alone.  Ends without an exchange.
-template <typename T, int G, bool HASH>
-__device__ __forceinline__ DistillEntries dis_entries(const DistillArgs& g, const T* xr, int64_t row, int l,
-                                                      const DistillLds& s, int* dup, int32_t* error_flag) {
-  DistillEntries e;
+// The token of pair k of a row, or -1: a pair is there if its token is in [0, vocab) and its teacher logit is not -inf.
+__device__ __forceinline__ int32_t dis_token(const DistillArgs& g, int64_t indices, int64_t teacher, int k, float* t,
+                                             int32_t* error_flag) {
+  const int64_t at = dis_index(g, indices + k);
+  *t = load_dyn<float>(g.teacher, teacher + k, g.teacher_dtype);
+  if (at >= g.vocab && error_flag) *error_flag = 3;
+  return at >= 0 && at < g.vocab && *t != -__builtin_inff() ? (int32_t)at : -1;
+}
+
+// Loads a row's pairs; whether any is there, in every lane.
+template <int NE>
+__device__ __forceinline__ bool dis_entries(const DistillArgs& g, int64_t row, int lane, DistillEntries<NE>& e,
+                                            int32_t* error_flag) {
+  const int64_t indices = dis_at(g, row, g.is), teacher = dis_at(g, row, g.ts);
+  bool any = false;
 #pragma unroll
-  for (int i = 0; i < kDisEntries; ++i) {
+  for (int i = 0; i < NE; ++i) {
+    const int k = lane + i * 64;
     e.at[i] = -1;
     e.t[i] = -__builtin_inff();
-    e.x[i] = -__builtin_inff();
-    const int k = l + i * G;
-    if (k >= g.entries) continue;
-    const int64_t at = dis_index(g, row * g.entries + k);
-    e.t[i] = load_dyn<float>(g.teacher, row * g.entries + k, g.teacher_dtype);
-    if (HASH && at >= g.vocab && error_flag) *error_flag = 3;
-    if (at >= 0 && at < g.vocab && e.t[i] != -__builtin_inff()) e.at[i] = (int32_t)at;
-    if (!HASH) continue;
-    if (e.at[i] >= 0) e.x[i] = (float)to_arith(xr[at]);
-    s.at[k] = e.at[i];
-    if (e.at[i] >= 0) {  // at most half of the slots are taken: the search ends
-      uint32_t h = ((uint32_t)at * 0x9E3779B1u) >> 16;
-      for (;; ++h) {
-        const int old = atomicCAS(&s.hash[h & (uint32_t)(g.hash - 1)], -1, e.at[i]);
-        if (old == -1) break;
-        if (old == e.at[i]) {
-          *dup = 1;
-          break;
-        }
-      }
+    if (k < g.entries) e.at[i] = dis_token(g, indices, teacher, k, &e.t[i], error_flag);
+    any = any || e.at[i] >= 0;
+  }
+  return __any(any);
+}
+
+// The student's logits of the pairs, and whether a token is listed twice, in every lane.  One wavefront a row.
+template <typename T, int NE>
+__device__ __forceinline__ bool dis_listed(const DistillArgs& g, const T* xr, int lane, DistillEntries<NE>& e,
+                                           const DistillLds& s) {
+#pragma unroll
+  for (int i = 0; i < NE; ++i) e.x[i] = e.at[i] >= 0 ? (float)to_arith(xr[e.at[i]]) : -__builtin_inff();
+  for (int i = lane; i < g.hash; i += 64) s.hash[i] = -1;
+  wave_sync();
+  bool twice = false;
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    const int k = lane + i * 64;
+    if (k < g.entries) s.at[k] = e.at[i];
+    if (e.at[i] < 0) continue;
+    uint32_t h = ((uint32_t)e.at[i] * 0x9E3779B1u) >> 16;
+    for (;; ++h) {  // at most half of the slots are taken: the search ends
+      const int old = atomicCAS(&s.hash[h & (uint32_t)(g.hash - 1)], -1, e.at[i]);
+      twice = twice || old == e.at[i];
+      if (old == -1 || old == e.at[i]) break;
     }
   }
-  return e;
+  wave_sync();
+  return __any(twice);
 }
 
 __device__ __forceinline__ void dis_split(double v, float* out) {
@@ -200,95 +195,101 @@ struct DistillOut {
   }
 };
 
-// A row without a pair: nothing is read of its logits.
-template <int G>
-__device__ __forceinline__ void dis_nothing(const DistillArgs& g, int64_t row, int l, const DistillOut& out) {
+// A row without a pair: nothing is read of its logits.  One wavefront.
+__device__ __forceinline__ void dis_nothing(const DistillArgs& g, int64_t row, int lane, const DistillOut& out) {
   if (out.pairs) {
-    for (int k = l; k < g.entries; k += G) out.pairs[row * g.entries + k] = DistillPair{-1, 0.0f};
+    for (int k = lane; k < g.entries; k += 64) out.pairs[row * g.entries + k] = DistillPair{-1, 0.0f};
   }
-  if (l < kDisStats) out.stats[row * kDisStats + l] = 0.0f;
-  if (l == 0) out.row(row, 0.0f, false);
+  if (lane < kDisStats) out.stats[row * kDisStats + lane] = 0.0f;
+  if (lane == 0) out.row(row, 0.0f, false);
 }
 
-// From the stream's pair (m, s) -- the largest of its raw logits and the sum of exp2((x - m) c) -- and
-// the row's pairs to the row's loss, its statistics and the pairs' weights.  Every thread of the row; exchanged before.
-template <int G, bool REST>
-__device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, int l, float m, float s,
-                                           const DistillEntries& e, const DistillLds& lds, const int* dup, float* lds_f,
-                                           double* lds_d, const DistillOut& out) {
-  float top[2] = {-__builtin_inff(), m};
+// From the stream's pair (m, s) -- a base next to the largest x c, and the sum of exp2(x c - m) -- and
+// the row's pairs to the row's loss, its statistics and the pairs' weights.  One wavefront.
+template <int NE, bool REST>
+__device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, int lane, float m, float s,
+                                           const DistillEntries<NE>& e, float teacher_lse, bool twice,
+                                           const DistillLds& lds, const DistillOut& out) {
+  float top_t = -__builtin_inff(), top = m;
 #pragma unroll
-  for (int i = 0; i < kDisEntries; ++i) {
+  for (int i = 0; i < NE; ++i) {
     if (e.at[i] < 0) continue;
-    top[0] = fmaxf(top[0], e.t[i]);
-    if (REST) top[1] = fmaxf(top[1], e.x[i]);
+    top_t = fmaxf(top_t, e.t[i]);
+    if (REST) top = fmaxf(top, e.x[i] * g.c);
   }
-  team_max<G, 2>(top, lds_f);
-  const bool twice = *dup != 0;
-  const double M = top[1] == -__builtin_inff() ? 0.0 : (double)top[1];
-  const double lt = REST ? (double)g.teacher_lse[row] * kLog2eD : (double)top[0] * g.c;
-  double p[kDisEntries];
-  bool first[kDisEntries];  // no pair before lists the token
-  double sum[5] = {0.0, 0.0, 0.0, 0.0, 0.0};  // p, p log2 p, p (z - M), listed tokens' exp2(z - M) and their number
+  if (REST) top = wave_max(top);
+  else top_t = wave_max(top_t);
+  const float M = top == -__builtin_inff() ? 0.0f : top;
+  const double lt = REST ? (double)teacher_lse * kLog2eD : (double)top_t * g.teacher_c;
+  double p[NE];
+  bool first[NE];  // no pair before lists the token
+  double sum[3] = {0.0, 0.0, 0.0};  // p, p log2 p, p (z - M)
+  float mass = 0.0f;                // the listed tokens' exp2(z - M)
+  int distinct = 0;
 #pragma unroll
-  for (int i = 0; i < kDisEntries; ++i) {
+  for (int i = 0; i < NE; ++i) {
     p[i] = 0.0;
     first[i] = e.at[i] >= 0;
     if (e.at[i] < 0) continue;
-    const double log_p = (double)e.t[i] * g.c - lt;
+    const double log_p = (double)e.t[i] * g.teacher_c - lt, z = (double)e.x[i] * (double)g.c - (double)M;
     p[i] = exp2(log_p);
     if (p[i] != 0.0) {
       sum[0] += p[i];
       sum[1] += p[i] * log_p;
-      sum[2] += p[i] * (((double)e.x[i] - M) * g.c);
+      sum[2] += p[i] * z;
     }
     if (twice) {
-      const int k = l + i * G;
+      const int k = lane + i * 64;
       for (int j = 0; j < k && first[i]; ++j) first[i] = lds.at[j] != e.at[i];
       lds.p[k] = p[i];
     }
     if (REST && first[i]) {
-      sum[3] += exp2(((double)e.x[i] - M) * g.c);
-      sum[4] += 1.0;
+      mass += __builtin_amdgcn_exp2f((float)z);
+      ++distinct;
     }
   }
-  team_sum<G, 5>(sum, lds_d);
-  if (twice) {
-    if constexpr (G == 64) team_sync<G>();  // the sums have exchanged otherwise
 #pragma unroll
-    for (int i = 0; i < kDisEntries; ++i) {
-      const int k = l + i * G;
+  for (int i = 0; i < 3; ++i) sum[i] = wave_sum(sum[i]);
+  if (REST) {
+    mass = sum64(mass);
+    distinct = (int)sum64((float)distinct);  // at most 1024
+  }
+  if (twice) {
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
       if (!first[i]) continue;
-      for (int j = k + 1; j < g.entries; ++j)
+      for (int j = lane + i * 64 + 1; j < g.entries; ++j)
         if (lds.at[j] == e.at[i]) p[i] += lds.p[j];
     }
   }
   const double norm = REST ? 1.0 : 1.0 / sum[0];
+  if (out.pairs) {
 #pragma unroll
-  for (int i = 0; i < kDisEntries; ++i) {
-    const int k = l + i * G;
-    if (out.pairs && k < g.entries)
-      out.pairs[row * g.entries + k] = DistillPair{first[i] ? e.at[i] : -1, (float)(p[i] * norm)};
+    for (int i = 0; i < NE; ++i) {
+      const int k = lane + i * 64;
+      if (k < g.entries) out.pairs[row * g.entries + k] = DistillPair{first[i] ? e.at[i] : -1, (float)(p[i] * norm)};
+    }
   }
-  if (l != 0) return;
+  if (lane != 0) return;
   float st[kDisStats] = {};
   double total = (double)s;  // of exp2(z - M)
-  if (REST) total = (s != 0.0f ? (double)s * exp2(((double)m - M) * g.c) : 0.0) + sum[3];
-  const double lse = M * g.c + log2(total);
+  if (REST) total = (s != 0.0f ? (double)s * exp2((double)m - (double)M) : 0.0) + (double)mass;
+  const double log_total = log2(total), lse = (double)M + log_total;
   double weight = 1.0, L;
   if constexpr (REST) {
     weight = sum[0];
-    L = sum[1] - sum[2] + weight * log2(total);
-    const bool empty = sum[4] == (double)g.vocab;  // every token is listed
+    L = sum[1] - sum[2] + weight * log_total;
+    const bool empty = (int64_t)distinct == g.vocab;  // every token is listed
     const double r = empty ? 0.0 : fmax(0.0, 1.0 - sum[0]);
-    const double rest = (m == -__builtin_inff() ? 0.0 : (double)m * g.c) + log2((double)s);  // -inf: no mass outside
+    const double rest = (m == -__builtin_inff() ? 0.0 : (double)m) + log2((double)s);  // -inf: no mass outside
     if (r > 0.0) L += r * (log2(r) - (rest - lse));
     weight += r;
-    const bool mass = rest != -__builtin_inf() && !empty;
-    dis_split(mass ? rest : 0.0, st);
-    st[2] = mass ? (float)(weight * exp2(rest - lse) - r) : 0.0f;
+    const bool some = rest != -__builtin_inf() && !empty;
+    dis_split(some ? rest : 0.0, st);
+    st[2] = some ? (float)(weight * exp2(rest - lse) - r) : 0.0f;
   } else {
-    L = (sum[1] - sum[2]) * norm - log2(sum[0]) + log2(total);
+    L = (sum[1] - sum[2]) * norm - log2(sum[0]) + log_total;
     dis_split(lse, st);
     st[2] = 1.0f;
   }
@@ -300,186 +301,208 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   for (int i = 0; i < kDisStats; ++i) out.stats[row * kDisStats + i] = st[i];
 }
 
-// One online step over a batch of values: (m, s) with those of f.
+// One online step over a batch of logits: (m, s) with those of f.  m is the largest x c, rounded, and as such the
+// exact base of the sum.
 template <int N> __device__ __forceinline__ void dis_online(float& m, float& s, const float (&f)[N], float c) {
   float mb = f[0];
 #pragma unroll
   for (int k = 1; k < N; ++k) mb = fmaxf(mb, f[k]);
   // fmaxf passes over a NaN, so M says nothing of them: the sum is always taken, and is then NaN
-  const float M = fmaxf(m, mb), base = M == -__builtin_inff() ? 0.0f : M;
+  const float M = fmaxf(m, mb * c), base = M == -__builtin_inff() ? 0.0f : M;
   float sb = 0.0f;
 #pragma unroll
-  for (int k = 0; k < N; ++k) sb += __builtin_amdgcn_exp2f((f[k] - base) * c);
-  s = (M != -__builtin_inff() ? s * __builtin_amdgcn_exp2f((m - M) * c) : s) + sb;
+  for (int k = 0; k < N; ++k) sb += __builtin_amdgcn_exp2f(fmaf(f[k], c, -base));
+  s = (M != -__builtin_inff() ? s * __builtin_amdgcn_exp2f(m - M) : s) + sb;
   m = M;
 }
 
-// (m, s) of the columns [c0, c1) of a row for one of G threads; c0 is a multiple of a vector.  REST: the
-// listed tokens, whose bits are set from column c0 on, count as -inf.
-template <typename T, int G, bool REST>
-__device__ __forceinline__ void dis_stream(const T* xr, int64_t c0, int64_t c1, int l, float c, const uint32_t* bits,
-                                           float& m, float& s) {
-  constexpr int V = VecOf<T>::V;
-  const T* p = xr + c0;
-  const int n = (int)(c1 - c0), nvec = n / V;
-  for (int v0 = l; v0 < nvec; v0 += G * kDisUnroll) {
-    uint4 w[kDisUnroll];
+// The columns [c0, c1) of a row for one of G threads, in vectors at multiples of 16 bytes, whatever the row's
+// address; the few elements before and behind them go one to a thread.  The first batch is requested when it
+// is made.
+template <typename T, int G, bool REST> struct DistillStream {
+  static constexpr int V = VecOf<T>::V, U = kDisUnroll;
+  const T* p;        // the first whole vector
+  int head, tail;    // elements before and behind the vectors
+  int nvec, l;
+  uint4 w[U];
+  T edge;
+
+  __device__ __forceinline__ DistillStream(const T* xr, int64_t c0, int64_t c1, int thread) : l(thread) {
+    const int n = (int)(c1 - c0), at = (int)(reinterpret_cast<uintptr_t>(xr + c0) % 16 / sizeof(T));
+    head = at == 0 ? 0 : (V - at < n ? V - at : n);
+    p = xr + c0 + head;
+    nvec = (n - head) / V;
+    tail = n - head - nvec * V;
+    request(l);
+    if (l < head + tail) edge = p[edge_at()];
+  }
+  __device__ __forceinline__ int64_t edge_at() const { return l < head ? l - head : (int64_t)nvec * V + (l - head); }
+  // Where the bitmap has column c0: the first vector's bits begin at bit V.
+  __device__ __forceinline__ int shift() const { return V - head; }
+  __device__ __forceinline__ void request(int v0) {
 #pragma unroll
-    for (int u = 0; u < kDisUnroll; ++u)
+    for (int u = 0; u < U; ++u)
       if (v0 + u * G < nvec) w[u] = ld_any_stream(p + (int64_t)(v0 + u * G) * V);
-    float f[kDisUnroll * V];
+  }
+  // Adds them to (m, s).  REST: the listed tokens, whose bits are set, count as -inf.
+  __device__ __forceinline__ void run(float c, const uint32_t* bits, float& m, float& s) {
+    for (int v0 = l; v0 < nvec; v0 += G * U) {
+      float f[U * V];
 #pragma unroll
-    for (int u = 0; u < kDisUnroll; ++u) {
-      const int v = v0 + u * G;
-      if (v < nvec) {
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * G;
+        if (v < nvec) {
 #pragma unroll
-        for (int k = 0; k < V; ++k) f[u * V + k] = elem_f<T>(w[u], k);
-        if constexpr (REST) {
-          const uint32_t b = bits[v * V / 32] >> (v * V % 32) & ((1u << V) - 1u);
-          if (b) {
+          for (int k = 0; k < V; ++k) f[u * V + k] = elem_f<T>(w[u], k);
+          if constexpr (REST) {
+            const int bit = (v + 1) * V;
+            const uint32_t b = bits[bit / 32] >> (bit % 32) & ((1u << V) - 1u);
+            if (b) {
 #pragma unroll
-            for (int k = 0; k < V; ++k)
-              if (b >> k & 1u) f[u * V + k] = -__builtin_inff();
+              for (int k = 0; k < V; ++k)
+                if (b >> k & 1u) f[u * V + k] = -__builtin_inff();
+            }
           }
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k) f[u * V + k] = -__builtin_inff();
         }
-      } else {
-#pragma unroll
-        for (int k = 0; k < V; ++k) f[u * V + k] = -__builtin_inff();
       }
+      request(v0 + G * U);
+      dis_online(m, s, f, c);
     }
-    dis_online(m, s, f, c);
+    if (l < head + tail) {
+      float f[1] = {(float)to_arith(edge)};
+      if constexpr (REST) {
+        const int bit = (int)edge_at() + V;
+        if (bits[bit / 32] >> (bit % 32) & 1u) f[0] = -__builtin_inff();
+      }
+      dis_online(m, s, f, c);
+    }
   }
-  for (int j = nvec * V + l; j < n; j += G) {  // after the whole vectors
-    float f[1] = {(float)to_arith(p[j])};
-    if (REST && (bits[j / 32] >> (j % 32) & 1u)) f[0] = -__builtin_inff();
-    dis_online(m, s, f, c);
-  }
-}
-
-// (m, s) of all G threads, in every one of them.
-template <int G> __device__ __forceinline__ void dis_join(float& m, float& s, float c, float* lds_m, float* lds_s) {
-  float M = m;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
-  if constexpr (G > 64) {
-    if ((threadIdx.x & 63) == 0) lds_m[threadIdx.x >> 6] = M;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < G / 64; ++w) M = fmaxf(M, lds_m[w]);
-  }
-  if (M != -__builtin_inff()) s *= __builtin_amdgcn_exp2f((m - M) * c);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-  if constexpr (G > 64) {
-    if ((threadIdx.x & 63) == 0) lds_s[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = lds_s[0];
-#pragma unroll
-    for (int w = 1; w < G / 64; ++w) s += lds_s[w];
-  }
-  m = M;
-}
-
-// Sets the bits of the listed tokens in [c0, c0 + segment); exchanges before and after.
-template <int G>
-__device__ __forceinline__ void dis_mark(const DistillArgs& g, const DistillEntries& e, int64_t c0, int l, uint32_t* bits) {
-  team_sync<G>();
-  for (int i = l; i < (g.segment + 31) / 32; i += G) bits[i] = 0u;
-  team_sync<G>();
-#pragma unroll
-  for (int i = 0; i < kDisEntries; ++i) {
-    const int64_t at = (int64_t)e.at[i] - c0;
-    if (e.at[i] >= 0 && at >= 0 && at < g.segment) atomicOr(&bits[at / 32], 1u << (at % 32));
-  }
-  team_sync<G>();
-}
-
-// Whether any of the row's pairs is there, in every thread of the row.
-template <int G> __device__ __forceinline__ bool dis_any(const DistillEntries& e) {
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < kDisEntries; ++i) any = any || e.at[i] >= 0;
-  if constexpr (G == 64) {
-    team_sync<G>();
-    return __any(any);
-  } else {
-    return __syncthreads_or(any);
-  }
-}
-
-// Exchanges of a row's finish.
-template <int G> struct DistillJoin {
-  float f[2 * G / 64], m[G / 64], s[G / 64];
-  double d[5 * G / 64];
-  int dup;
 };
 
-// G threads a row.
-template <typename T, int G, bool REST>
-__global__ void __launch_bounds__(kDisBlock)
+// (m, s) of a wavefront, in every lane.
+__device__ __forceinline__ void dis_join(float& m, float& s) {
+  const float M = wave_max(m);
+  if (M != -__builtin_inff()) s *= __builtin_amdgcn_exp2f(m - M);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
+  m = M;
+}
+
+// Sets the bits of the listed tokens in [c0, c0 + segment), `shift` places on, by all G threads of a row; exchanged at its end.
+template <int G>
+__device__ __forceinline__ void dis_mark(const DistillArgs& g, int64_t row, int64_t c0, int shift, int l, uint32_t* bits) {
+  auto sync = [] {
+    if constexpr (G == 64) wave_sync();
+    else __syncthreads();
+  };
+  sync();
+  for (int i = l; i < dis_bit_words(g.segment); i += G) bits[i] = 0u;
+  sync();
+  const int64_t indices = dis_at(g, row, g.is), teacher = dis_at(g, row, g.ts);
+  for (int k = l; k < g.entries; k += G) {
+    float t;
+    const int32_t token = dis_token(g, indices, teacher, k, &t, nullptr);
+    const int64_t at = token - c0;
+    if (token < 0 || at < 0 || at >= g.segment) continue;
+    const int bit = (int)at + shift;
+    atomicOr(&bits[bit / 32], 1u << (bit % 32));
+  }
+  sync();
+}
+
+// G threads a row; the first wavefront knows the pairs and finishes the row.  Short rows: several to a workgroup.
+template <typename T, int G, int NE, bool REST>
+__global__ void __launch_bounds__(G < kDisBlock ? kDisBlock : G)
 k_distill_fwd(DistillArgs g, int64_t row0, int64_t rows, DistillOut out, int32_t* error_flag) {
-  constexpr int TEAMS = kDisBlock / G;
+  constexpr int TEAMS = G < kDisBlock ? kDisBlock / G : 1, W = G / 64;
   extern __shared__ double lds_dyn[];
-  __shared__ DistillJoin<G> join[TEAMS];
-  const int team = threadIdx.x / G, l = threadIdx.x % G;
+  __shared__ float2 lds_join[W];
+  // the same in a wavefront, and known to be: a row's addresses are scalar then
+  const int team = TEAMS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / G);
+  const int l = TEAMS == 1 ? threadIdx.x : threadIdx.x & 63, lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(l >> 6);
   const int64_t row = row0 + (int64_t)blockIdx.x * TEAMS + team;
   if (row >= row0 + rows) return;  // whole rows: no exchange is left waiting
-  DistillJoin<G>& j = join[team];
   const T* xr = dis_row<T>(g, row);
   const DistillLds s = dis_lds(
       reinterpret_cast<char*>(lds_dyn) + team * dis_lds_bytes(g.entries, g.hash, REST ? g.segment : 0), g.entries, g.hash);
-  for (int i = l; i < g.hash; i += G) s.hash[i] = -1;
-  if (l == 0) j.dup = 0;
-  team_sync<G>();
-  const DistillEntries e = dis_entries<T, G, true>(g, xr, row, l, s, &j.dup, error_flag);
-  if (!dis_any<G>(e)) return dis_nothing<G>(g, row, l, out);
-  float m = -__builtin_inff(), sum = 0.0f;
-  for (int64_t c0 = 0; c0 < g.vocab; c0 += g.segment) {
-    if (REST) dis_mark<G>(g, e, c0, l, s.bits);
-    dis_stream<T, G, REST>(xr, c0, c0 + g.segment < g.vocab ? c0 + g.segment : g.vocab, l, g.c_near, s.bits, m, sum);
+  auto end = [&](int64_t c0) { return c0 + g.segment < g.vocab ? c0 + g.segment : g.vocab; };
+  DistillStream<T, G, REST> first(xr, 0, end(0), l);
+  DistillEntries<NE> e;
+  const float teacher_lse = REST ? g.teacher_lse[dis_at(g, row, g.ls)] : 0.0f;
+  const bool any = dis_entries(g, row, lane, e, wave == 0 ? error_flag : nullptr);  // in every wavefront: all know without a barrier
+  if (!any) {
+    if (wave == 0) dis_nothing(g, row, lane, out);
+    return;
   }
-  dis_join<G>(m, sum, g.c_near, j.m, j.s);
-  dis_finish<G, REST>(g, row, l, m, sum, e, s, &j.dup, j.f, j.d, out);
+  bool twice = false;
+  if (wave == 0) twice = dis_listed(g, xr, lane, e, s);
+  float m = -__builtin_inff(), sum = 0.0f;
+  if (REST) dis_mark<G>(g, row, 0, first.shift(), l, s.bits);
+  first.run(g.c, s.bits, m, sum);
+  for (int64_t c0 = g.segment; c0 < g.vocab; c0 += g.segment) {
+    DistillStream<T, G, REST> next(xr, c0, end(c0), l);
+    if (REST) dis_mark<G>(g, row, c0, next.shift(), l, s.bits);
+    next.run(g.c, s.bits, m, sum);
+  }
+  dis_join(m, sum);
+  if constexpr (W > 1) {
+    if (lane == 0) lds_join[wave] = make_float2(m, sum);
+    __syncthreads();
+    if (wave != 0) return;
+    const float2 part = lane < W ? lds_join[lane] : make_float2(-__builtin_inff(), 0.0f);
+    m = part.x;
+    sum = part.y;
+    dis_join(m, sum);
+  }
+  dis_finish<NE, REST>(g, row, lane, m, sum, e, teacher_lse, twice, s, out);
 }
 
 // Few rows: parts of a row (of `columns` columns, a multiple of 32) to a workgroup each; (m, s) of each part ...
 template <typename T, bool REST>
 __global__ void __launch_bounds__(kDisBlock)
 k_distill_part(DistillArgs g, int64_t columns, float2* __restrict__ parts) {
-  constexpr int G = kDisBlock;
+  constexpr int G = kDisBlock, W = G / 64;
   extern __shared__ double lds_dyn[];
-  __shared__ float lds_m[G / 64], lds_s[G / 64];
+  __shared__ float2 lds_join[W];
   const int64_t row = blockIdx.y, c0 = blockIdx.x * columns, c1 = c0 + columns < g.vocab ? c0 + columns : g.vocab;
   const T* xr = dis_row<T>(g, row);
   uint32_t* bits = reinterpret_cast<uint32_t*>(lds_dyn);
-  DistillEntries e;
-  if constexpr (REST) e = dis_entries<T, G, false>(g, xr, row, threadIdx.x, DistillLds{}, nullptr, nullptr);
   float m = -__builtin_inff(), sum = 0.0f;
   for (int64_t s0 = c0; s0 < c1; s0 += g.segment) {
-    if (REST) dis_mark<G>(g, e, s0, threadIdx.x, bits);
-    dis_stream<T, G, REST>(xr, s0, s0 + g.segment < c1 ? s0 + g.segment : c1, threadIdx.x, g.c_near, bits, m, sum);
+    DistillStream<T, G, REST> stream(xr, s0, s0 + g.segment < c1 ? s0 + g.segment : c1, threadIdx.x);
+    if (REST) dis_mark<G>(g, row, s0, stream.shift(), threadIdx.x, bits);
+    stream.run(g.c, bits, m, sum);
   }
-  dis_join<G>(m, sum, g.c_near, lds_m, lds_s);
+  dis_join(m, sum);
+  if ((threadIdx.x & 63) == 0) lds_join[threadIdx.x >> 6] = make_float2(m, sum);
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  const float2 part = threadIdx.x < W ? lds_join[threadIdx.x] : make_float2(-__builtin_inff(), 0.0f);
+  m = part.x;
+  sum = part.y;
+  dis_join(m, sum);
   if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float2(m, sum);
 }
-// ... and the rows from their parts, G threads a row.
-template <typename T, int G, bool REST>
-__global__ void __launch_bounds__(G)
+// ... and the rows from their parts, a wavefront each.
+template <typename T, int NE, bool REST>
+__global__ void __launch_bounds__(64)
 k_distill_rows(DistillArgs g, int nparts, const float2* __restrict__ parts, DistillOut out, int32_t* error_flag) {
   extern __shared__ double lds_dyn[];
-  __shared__ DistillJoin<G> j;
   const int64_t row = blockIdx.x;
-  const int l = threadIdx.x;
+  const int lane = threadIdx.x;
+  const float2 part = lane < nparts ? parts[row * nparts + lane] : make_float2(-__builtin_inff(), 0.0f);
   const DistillLds s = dis_lds(reinterpret_cast<char*>(lds_dyn), g.entries, g.hash);
-  for (int i = l; i < g.hash; i += G) s.hash[i] = -1;
-  if (l == 0) j.dup = 0;
-  team_sync<G>();
-  const DistillEntries e = dis_entries<T, G, true>(g, dis_row<T>(g, row), row, l, s, &j.dup, error_flag);
-  if (!dis_any<G>(e)) return dis_nothing<G>(g, row, l, out);
-  const float2 part = l < nparts ? parts[row * nparts + l] : make_float2(-__builtin_inff(), 0.0f);
+  DistillEntries<NE> e;
+  const float teacher_lse = REST ? g.teacher_lse[dis_at(g, row, g.ls)] : 0.0f;
+  if (!dis_entries(g, row, lane, e, error_flag)) return dis_nothing(g, row, lane, out);
+  const bool twice = dis_listed(g, dis_row<T>(g, row), lane, e, s);
   float m = part.x, sum = part.y;
-  dis_join<G>(m, sum, g.c_near, j.m, j.s);
-  dis_finish<G, REST>(g, row, l, m, sum, e, s, &j.dup, j.f, j.d, out);
+  dis_join(m, sum);
+  dis_finish<NE, REST>(g, row, lane, m, sum, e, teacher_lse, twice, s, out);
 }
 
 // The sum (or mean) of the rows' losses and the number of rows that count, in float64 and a fixed order.  More
@@ -491,7 +514,7 @@ template <bool PART>
 __global__ void __launch_bounds__(kDisSumBlock)
 k_distill_total(const float2* __restrict__ rows, const double* __restrict__ parts, int64_t n, int mean,
                 double* __restrict__ parts_out, float* __restrict__ loss, float* __restrict__ count) {
-  __shared__ double lds[2 * kDisSumBlock / 64];
+  __shared__ double lds[2][kDisSumBlock / 64];
   double v[2] = {0.0, 0.0};
   if (parts) {
     for (int64_t i = threadIdx.x; i < n; i += kDisSumBlock) {
@@ -510,7 +533,15 @@ k_distill_total(const float2* __restrict__ rows, const double* __restrict__ part
       v[1] += (double)r[u].y;
     }
   }
-  team_sum<kDisSumBlock, 2>(v, lds);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    v[i] = wave_sum(v[i]);
+    if ((threadIdx.x & 63) == 0) lds[i][threadIdx.x >> 6] = v[i];
+  }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) v[i] = wave_sum(threadIdx.x < kDisSumBlock / 64 ? lds[i][threadIdx.x] : 0.0);
   if (threadIdx.x != 0) return;
   if constexpr (PART) {
     parts_out[2 * blockIdx.x] = v[0];
@@ -521,96 +552,85 @@ k_distill_total(const float2* __restrict__ rows, const double* __restrict__ part
   }
 }
 
-// Vectors per thread of a backward workgroup.
-constexpr int kDisBwdUnroll = 4;
-
-// grad[row, columns of the workgroup].  The exponent x c - base is formed with c and base in two
-// floats each: next to 0, where the probabilities are large, it has 24 bits.
-template <typename T>
-__global__ void __launch_bounds__(kDisBlock)
-k_distill_bwd(DistillArgs g, int64_t row0, const float* __restrict__ stats, const DistillPair* __restrict__ pairs,
-              const float* __restrict__ count, const float* __restrict__ grad_out, int reduction, T* __restrict__ grad) {
-  constexpr int V = VecOf<T>::V, U = kDisBwdUnroll;
-  extern __shared__ float listed[];  // p of the row's pairs
-  __shared__ uint32_t bits[kDisBlock * U * V / 32];
-  __shared__ uint16_t number[kDisBlock * U * V];  // of a column's pair, where its bit is set
-  const int64_t row = row0 + blockIdx.y;
+// grad[row, columns of the G threads]: one vector a thread, as memory takes a read and a
+// write stream best ([3700, 128256] bf16, reading and writing alone: 287 us so, 310 to 335 with four
+// vectors a thread, 64 to 1024 threads).  Everything is requested before anything is waited for.
+// The exponent x c - base is formed with a base of two floats: next to 0, where the
+// probabilities are large, it has 24 bits.
+template <typename T, int G>
+__global__ void __launch_bounds__(G < kDisBlock ? kDisBlock : G)
+k_distill_bwd(DistillArgs g, int64_t row0, int64_t rows, const float* __restrict__ stats,
+              const DistillPair* __restrict__ pairs, const float* __restrict__ count,
+              const float* __restrict__ grad_out, int reduction, T* __restrict__ grad) {
+  constexpr int V = VecOf<T>::V, TEAMS = G < kDisBlock ? kDisBlock / G : 1, reach = G * V;
+  __shared__ uint32_t lds_bits[TEAMS][reach / 32];
+  __shared__ float lds_p[TEAMS][reach];
+  const int team = TEAMS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / G);  // scalar, as the row's addresses then
+  const int l = TEAMS == 1 ? threadIdx.x : threadIdx.x & 63;
+  uint32_t* bits = lds_bits[team];
+  float* listed = lds_p[team];  // p of a column whose bit is set
+  const int64_t row = row0 + (int64_t)blockIdx.y * TEAMS + team;
+  if (row >= row0 + rows) return;  // whole rows: no exchange is left waiting
   const T* xr = dis_row<T>(g, row);
   T* dst = grad + row * g.vocab;
-  const int64_t off = grid_off<T, V>(dst, g.vocab);
-  const int64_t c0 = (int64_t)blockIdx.x * blockDim.x * U * V - off;
+  const int64_t c0 = (int64_t)blockIdx.x * reach - grid_off<T, V>(dst, g.vocab), col = c0 + l * V;
+  const bool whole = col >= 0 && col + V <= g.vocab;
+  uint4 w;
+  if (whole) {
+    w = ld_any_stream(xr + col);
+  } else {
+    T e[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) e[k] = col + k >= 0 && col + k < g.vocab ? xr[col + k] : T{};
+    __builtin_memcpy(&w, e, 16);
+  }
+  const DistillPair* pr = pairs + row * g.entries;
+  DistillPair pair{-1, 0.0f};
+  if (l < g.entries) pair = pr[l];
   const float* st = stats + row * kDisStats;
+  const float base_hi = st[0], base_lo = st[1], lse_hi = st[4], lse_lo = st[5], weight = st[3], rest = st[2];
   const bool counted = st[6] != 0.0f;
-  auto at = [&](int u) { return (int)(threadIdx.x + u * blockDim.x) * V; };  // a vector's first column from c0 on
-  if (!counted) {
-    float zero[V] = {};
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t col = c0 + at(u);
-      if (col >= 0 && col + V <= g.vocab) {
-        store_any<T, V>(dst + col, zero);
-      } else {
-        for (int k = col < 0 ? (int)-col : 0; k < V && col + k < g.vocab; ++k) dst[col + k] = from_arith<T>(0.0f);
-      }
-    }
-    return;
-  }
-  uint4 w[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t col = c0 + at(u);
-    if (col >= 0 && col + V <= g.vocab) {
-      w[u] = ld_any_stream(xr + col);
-    } else {
-      T e[V];
-#pragma unroll
-      for (int k = 0; k < V; ++k) e[k] = col + k >= 0 && col + k < g.vocab ? xr[col + k] : T{};
-      __builtin_memcpy(&w[u], e, 16);
-    }
-  }
-  const int reach = (int)blockDim.x * U * V;
-  for (int i = threadIdx.x; i < reach / 32; i += blockDim.x) bits[i] = 0u;
-  __syncthreads();
-  for (int k = threadIdx.x; k < g.entries; k += blockDim.x) {
-    const DistillPair e = pairs[row * g.entries + k];
-    const int64_t col = e.at - c0;
-    if (e.at < 0 || col < 0 || col >= reach) continue;
-    atomicOr(&bits[col / 32], 1u << (col % 32));
-    number[col] = (uint16_t)k;  // the one pair that carries the token
-    listed[k] = e.p;
-  }
-  const float base_hi = st[0], base_lo = st[1], lse_hi = st[4], lse_lo = st[5], weight = st[3];
   float gs = reduction == SUPA_AMD_REDUCTION_NONE ? grad_out[row] : grad_out[0];
   if (reduction == SUPA_AMD_REDUCTION_MEAN) gs /= count[0];
   gs = (float)((double)gs * g.inv_t);
-  const float k0 = st[2] * gs;
-  __syncthreads();
+  for (int i = l; i < reach / 32; i += G) bits[i] = 0u;
+  auto sync = [] {
+    if constexpr (G == 64) wave_sync();
+    else __syncthreads();
+  };
+  sync();
+  for (int k = l; k < g.entries; k += G) {
+    if (k != l) pair = pr[k];
+    const int64_t at = pair.at - c0;
+    if (pair.at < 0 || at < 0 || at >= reach) continue;
+    atomicOr(&bits[at / 32], 1u << (at % 32));
+    listed[at] = pair.p;  // the one pair that carries the token
+  }
+  const float k0 = rest * gs;
+  sync();
+  float f[V];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t col = c0 + at(u);
-    float f[V];
+  for (int k = 0; k < V; ++k) {
+    const float x = elem_f<T>(w, k);
+    const float v = __builtin_amdgcn_exp2f(fmaf(x, g.c, -base_hi) - base_lo) * k0;
+    f[k] = counted ? v : 0.0f;
+  }
+  const uint32_t here = bits[l * V / 32] >> (l * V % 32) & ((1u << V) - 1u);
+  if (here) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float x = elem_f<T>(w[u], k);
-      f[k] = __builtin_amdgcn_exp2f(fmaf(x, g.c_hi, -base_hi) + fmaf(x, g.c_lo, -base_lo)) * k0;
+      if (!(here >> k & 1u)) continue;
+      const float x = elem_f<T>(w, k);
+      const float q = __builtin_amdgcn_exp2f(fmaf(x, g.c, -lse_hi) - lse_lo);
+      f[k] = (q * weight - listed[l * V + k]) * gs;
     }
-    const uint32_t here = bits[at(u) / 32] >> (at(u) % 32) & ((1u << V) - 1u);
-    if (here) {
+  }
+  if (whole) {
+    store_any<T, V>(dst + col, f);
+  } else {
 #pragma unroll
-      for (int k = 0; k < V; ++k) {
-        if (!(here >> k & 1u)) continue;
-        const float x = elem_f<T>(w[u], k);
-        const float q = __builtin_amdgcn_exp2f(fmaf(x, g.c_hi, -lse_hi) + fmaf(x, g.c_lo, -lse_lo));
-        f[k] = (q * weight - listed[number[at(u) + k]]) * gs;
-      }
-    }
-    if (col >= 0 && col + V <= g.vocab) {
-      store_any<T, V>(dst + col, f);
-    } else {
-#pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (col + k >= 0 && col + k < g.vocab) dst[col + k] = from_arith<T>(f[k]);
-    }
+    for (int k = 0; k < V; ++k)
+      if (col + k >= 0 && col + k < g.vocab) dst[col + k] = from_arith<T>(f[k]);
   }
 }
 
@@ -634,8 +654,12 @@ int dis_args(const supa_amd_distill_desc* d, DistillArgs& g) {
   g.idx = d->indices;
   g.teacher = d->teacher;
   g.teacher_lse = d->teacher_lse;
-  g.xs[0] = d->logits_strides[0];
-  g.xs[1] = d->logits_strides[1];
+  for (int i = 0; i < 2; ++i) {
+    g.xs[i] = d->logits_strides[i];
+    g.is[i] = d->indices_strides[i];
+    g.ts[i] = d->teacher_strides[i];
+    g.ls[i] = d->lse_strides[i];
+  }
   g.inner = FastDiv((uint32_t)d->inner);
   g.vocab = d->vocab;
   g.entries = (int32_t)d->entries;
@@ -644,21 +668,22 @@ int dis_args(const supa_amd_distill_desc* d, DistillArgs& g) {
   g.idx64 = d->index_dtype == SUPA_AMD_I64;
   g.teacher_dtype = d->teacher_dtype;
   g.segment = (int32_t)std::min<int64_t>(kDisSegment, (d->vocab + 31) / 32 * 32);
-  g.c = kLog2eD / d->temperature;
-  g.c_near = (float)g.c;
-  g.c_hi = (double)g.c_near < g.c ? g.c_near : std::nextafterf(g.c_near, 0.0f);
-  g.c_lo = std::max((float)(g.c - (double)g.c_hi), 1.2e-38f);
+  g.teacher_c = kLog2eD / d->temperature;
+  g.c = (float)g.teacher_c;
   g.inv_t = 1.0 / d->temperature;
   return SUPA_AMD_OK;
 }
 
-// Parts of a row's columns for each of `rows` rows; 1: whole rows.
+// Parts of a row's columns for each of `rows` rows; 1: whole rows.  With two launches more than 500 rows
+// gain nothing ([700, 128256] bf16 35 us whole, 39 in parts), nor do parts of under 32 KiB ([500, 32000] bf16 13
+// and 15); few long rows do ([100, 128256] bf16 22 us whole, 14 in parts; [16, 262144] float32 32 and 11).
 int64_t dis_splits(int64_t rows, int64_t vocab, int dtype) {
   const int64_t vecs = vocab * dtype_size(dtype) / 16;
-  return std::max<int64_t>(1, std::min<int64_t>({64, 768 / std::max<int64_t>(1, rows), vecs / (2 * kDisBlock * kDisUnroll)}));
+  if (rows >= 512) return 1;
+  return std::max<int64_t>(1, std::min<int64_t>({64, 1536 / std::max<int64_t>(1, rows), vecs / 2048}));
 }
 
-template <typename T, bool REST>
+template <typename T, int NE, bool REST>
 int dis_forward(const DistillArgs& g, int64_t rows, int dtype, const DistillOut& out, float2* parts, int32_t* error_flag,
                 hipStream_t st) {
   const int64_t splits = dis_splits(rows, g.vocab, dtype);
@@ -667,32 +692,28 @@ int dis_forward(const DistillArgs& g, int64_t rows, int dtype, const DistillOut&
     const int64_t columns = ((g.vocab + splits - 1) / splits + 255) / 256 * 256;
     const int64_t n = (g.vocab + columns - 1) / columns;
     p.segment = (int32_t)std::min<int64_t>(columns, kDisSegment);
-    const size_t bitmap = REST ? (size_t)p.segment / 8 : 0;
+    const size_t bitmap = REST ? 4 * (size_t)dis_bit_words(p.segment) : 0;
     k_distill_part<T, REST><<<dim3((unsigned)n, (unsigned)rows), kDisBlock, bitmap, st>>>(p, columns, parts);
     const int rc = launch_status();
     if (rc) return rc;
     const size_t lds = dis_lds_bytes(g.entries, g.hash, 0);
-    if (g.entries <= 64 * kDisEntries)
-      k_distill_rows<T, 64, REST><<<(unsigned)rows, 64, lds, st>>>(g, (int)n, parts, out, error_flag);
-    else
-      k_distill_rows<T, kDisBlock, REST><<<(unsigned)rows, kDisBlock, lds, st>>>(g, (int)n, parts, out, error_flag);
+    k_distill_rows<T, NE, REST><<<(unsigned)rows, 64, lds, st>>>(g, (int)n, parts, out, error_flag);
     return launch_status();
   }
   auto go = [&](auto threads) -> int {
-    constexpr int G = decltype(threads)::value, per = kDisBlock / G;
+    constexpr int G = decltype(threads)::value, block = G < kDisBlock ? kDisBlock : G, per = block / G;
     const size_t lds = per * dis_lds_bytes(g.entries, g.hash, REST ? g.segment : 0);
-    const int64_t slab = ((int64_t(1) << 32) - 1) / kDisBlock * per;  // HIP: fewer than 2^32 threads a launch
+    const int64_t slab = ((int64_t(1) << 32) - 1) / block * per;  // HIP: fewer than 2^32 threads a launch
     for (int64_t r0 = 0; r0 < rows; r0 += slab) {
       const int64_t n = std::min(slab, rows - r0);
-      k_distill_fwd<T, G, REST><<<(unsigned)((n + per - 1) / per), kDisBlock, lds, st>>>(g, r0, n, out, error_flag);
+      k_distill_fwd<T, G, NE, REST><<<(unsigned)((n + per - 1) / per), block, lds, st>>>(g, r0, n, out, error_flag);
       const int rc = launch_status();
       if (rc) return rc;
     }
     return SUPA_AMD_OK;
   };
-  // a wavefront a row where rows are short
-  if (g.entries <= 64 * kDisEntries && g.vocab * dtype_size(dtype) <= 16 * kDisWaveVecs)
-    return go(std::integral_constant<int, 64>{});
+  // a wavefront a row where rows are short and its bitmaps, of which there are four, small
+  if (NE == 4 && g.vocab * dtype_size(dtype) <= 16 * kDisWaveVecs) return go(std::integral_constant<int, 64>{});
   return go(std::integral_constant<int, kDisBlock>{});
 }
 
@@ -743,8 +764,14 @@ int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float*
   if (d->rows > 0) {
     rc = with_float_storage(d->dtype, [&](auto* tag) -> int {
       using T = std::remove_pointer_t<decltype(tag)>;
-      return d->teacher_lse ? dis_forward<T, true>(g, d->rows, d->dtype, out, parts, error_flag, st)
-                            : dis_forward<T, false>(g, d->rows, d->dtype, out, parts, error_flag, st);
+      auto forward = [&](auto entries, auto rest) {
+        return dis_forward<T, entries.value, rest.value>(g, d->rows, d->dtype, out, parts, error_flag, st);
+      };
+      auto lists = [&](auto rest) {
+        return g.entries <= 256 ? forward(std::integral_constant<int, 4>{}, rest)
+                                : forward(std::integral_constant<int, kDisMaxEntries / 64>{}, rest);
+      };
+      return d->teacher_lse ? lists(std::true_type{}) : lists(std::false_type{});
     });
   }
   if (rc || !total) return rc;
@@ -773,19 +800,23 @@ int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_
     constexpr int V = VecOf<T>::V;
     T* gx = static_cast<T*>(grad_logits);
     const int64_t vecs = grid_vecs<T, V>(gx, g.vocab);
-    // rows shorter than a workgroup's reach get fewer threads
-    const int64_t each = (vecs + kDisBwdUnroll - 1) / kDisBwdUnroll;
-    const int block = (int)std::min<int64_t>(kDisBlock, (each + 63) / 64 * 64);
-    const unsigned blocks = (unsigned)((each + block - 1) / block);
-    const int64_t slab = std::min<int64_t>(65535, ((int64_t(1) << 32) - 1) / block / blocks);
-    for (int64_t r0 = 0; r0 < d->rows; r0 += slab) {
-      const unsigned n = (unsigned)std::min(slab, d->rows - r0);
-      k_distill_bwd<T><<<dim3(blocks, n), block, sizeof(float) * g.entries, st>>>(
-          g, r0, stats, static_cast<const DistillPair*>(pairs), count, grad_loss, d->reduction, gx);
-      const int rc = launch_status();
-      if (rc) return rc;
-    }
-    return SUPA_AMD_OK;
+    auto go = [&](auto threads) -> int {
+      constexpr int G = decltype(threads)::value, block = G < kDisBlock ? kDisBlock : G, teams = block / G;
+      const unsigned blocks = (unsigned)((vecs + G - 1) / G);
+      const int64_t slab = teams * std::max<int64_t>(1, std::min<int64_t>(65535, ((int64_t(1) << 32) - 1) / block / blocks));
+      for (int64_t r0 = 0; r0 < d->rows; r0 += slab) {
+        const int64_t n = std::min(slab, d->rows - r0);
+        k_distill_bwd<T, G><<<dim3(blocks, (unsigned)((n + teams - 1) / teams)), block, 0, st>>>(
+            g, r0, n, stats, static_cast<const DistillPair*>(pairs), count, grad_loss, d->reduction, gx);
+        const int rc = launch_status();
+        if (rc) return rc;
+      }
+      return SUPA_AMD_OK;
+    };
+    // every workgroup looks all pairs through: more of them, and more columns a workgroup
+    if (vecs <= 128) return go(std::integral_constant<int, 64>{});
+    if (g.entries <= 256 || vecs <= 256) return go(std::integral_constant<int, 256>{});
+    return go(std::integral_constant<int, 1024>{});
   });
 }
 
