@@ -21,6 +21,7 @@
 
 namespace sa {
 
+constexpr int kAdjApart = 8;                 // XCDs
 constexpr int kAdjVecs = 4;                  // vectors of logits that a thread has in flight
 constexpr int kAdjUnroll = 4;                // tokens of the history in flight a thread
 constexpr int kAdjMaxRange = 32768;
@@ -41,6 +42,8 @@ struct AdjustArgs {
   int64_t tokens_stride, bias_tokens_stride, bias_stride, allowed_stride;
   int64_t vocab, history;
   int32_t biases, range;
+  FastDiv ranges;   // of a row
+  int32_t apart;    // a row's workgroups are kAdjApart of the launch apart; else `rows` of it
   int32_t hash;     // slots of the biases' table, a power of two >= 2 biases; 0: no table
   int32_t tok64, len64, prompt64, bias_tok64;
   float repetition_value, presence_value, frequency_value;
@@ -65,7 +68,7 @@ __device__ __forceinline__ int64_t adj_column(const void* p, int is64, int64_t a
 
 // WIDE: counts of 32 bits.
 template <typename T, bool PEN, bool WIDE, bool BIAS>
-__global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
+__global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int64_t rows) {
   constexpr int V = VecOf<T>::V;
   extern __shared__ uint4 lds[];
   __shared__ int twice;
@@ -74,7 +77,14 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
   uint32_t* const bias_bits = PEN ? prompt_bits + g.range / 32 : count;
   int32_t* const hash_at = reinterpret_cast<int32_t*>(bias_bits + g.range / 32);
   int32_t* const hash_value = hash_at + g.hash;
-  const int64_t row = row0 + blockIdx.x, c0 = (int64_t)blockIdx.y * g.range;
+  uint32_t row_at = blockIdx.x, range = blockIdx.y;
+  if (g.apart) {  // in runs of as many rows with all their ranges
+    uint32_t run;
+    g.ranges.divmod(blockIdx.x / (uint32_t)kAdjApart, run, range);
+    row_at = run * kAdjApart + blockIdx.x % (uint32_t)kAdjApart;
+    if (row_at >= rows) return;
+  }
+  const int64_t row = row0 + row_at, c0 = (int64_t)range * g.range;
   const int width = (int)(g.vocab - c0 < g.range ? g.vocab - c0 : g.range), nt = blockDim.x;
   const T* in = static_cast<const T*>(g.in) + (row * g.in_stride + c0);
   T* out = static_cast<T*>(g.out) + (row * g.out_stride + c0);
@@ -87,42 +97,6 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     }
   };
   request(0);
-  // the first tokens of the history too, also where they turn out to lie behind its length
-  int64_t tok[kAdjUnroll];
-  const int64_t tokens_at = row * g.tokens_stride;
-  auto history = [&](int64_t t0, int64_t n) {
-#pragma unroll
-    for (int u = 0; u < kAdjUnroll; ++u) {
-      const int64_t t = t0 + u * nt;
-      tok[u] = t < n ? adj_column(g.tokens, g.tok64, tokens_at + t, c0) : -1;
-    }
-  };
-  float rho = 1.0f, presence = 0.0f, frequency = 0.0f;
-  int64_t n = g.history, prompt = 0;
-  if constexpr (PEN) {
-    history(threadIdx.x, n);
-    rho = g.repetition ? g.repetition[row] : g.repetition_value;
-    presence = g.presence ? g.presence[row] : g.presence_value;
-    frequency = g.frequency ? g.frequency[row] : g.frequency_value;
-    if (g.lengths) {
-      const int64_t v = adj_int(g.lengths, g.len64, row);
-      n = v < 0 ? 0 : (v < n ? v : n);
-    }
-    if (g.prompts) prompt = adj_int(g.prompts, g.prompt64, row);
-  }
-  const int64_t bias_tokens_at = row * g.bias_tokens_stride, bias_at = row * g.bias_stride;
-  auto column = [&](int j) {  // of bias j; -1: elsewhere
-    const int64_t t = adj_column(g.bias_tokens, g.bias_tok64, bias_tokens_at + j, c0);
-    return (uint64_t)t < (uint64_t)width ? (int)t : -1;
-  };
-  int first_column = -1;  // of the thread's first bias, and the bias
-  float first_bias = 0.0f;
-  if constexpr (BIAS) {
-    if ((int)threadIdx.x < g.biases) {
-      first_column = column(threadIdx.x);
-      first_bias = g.bias[bias_at + threadIdx.x];
-    }
-  }
   if (PEN || BIAS) {
     const int words = (PEN ? adj_count_words(g.range, WIDE) + g.range / 32 : 0) + (BIAS ? g.range / 32 : 0);
     for (int i = threadIdx.x; i < words / 4; i += nt) lds[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -136,19 +110,33 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     }
     __syncthreads();
   }
+  float rho = 1.0f, presence = 0.0f, frequency = 0.0f;
   if constexpr (PEN) {
-    for (int64_t t0 = threadIdx.x; t0 < n;) {
+    rho = g.repetition ? g.repetition[row] : g.repetition_value;
+    presence = g.presence ? g.presence[row] : g.presence_value;
+    frequency = g.frequency ? g.frequency[row] : g.frequency_value;
+    int64_t n = g.history, prompt = 0;
+    if (g.lengths) {
+      const int64_t v = adj_int(g.lengths, g.len64, row);
+      n = v < 0 ? 0 : (v < n ? v : n);
+    }
+    if (g.prompts) prompt = adj_int(g.prompts, g.prompt64, row);
+    const int64_t at = row * g.tokens_stride;
+    for (int64_t t0 = threadIdx.x; t0 < n; t0 += (int64_t)nt * kAdjUnroll) {
+      int64_t tok[kAdjUnroll];
 #pragma unroll
       for (int u = 0; u < kAdjUnroll; ++u) {
         const int64_t t = t0 + u * nt;
-        if ((uint64_t)tok[u] >= (uint64_t)width || t >= n) continue;
+        tok[u] = t < n ? adj_column(g.tokens, g.tok64, at + t, c0) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kAdjUnroll; ++u) {
+        if ((uint64_t)tok[u] >= (uint64_t)width) continue;
         const int c = (int)tok[u];
-        if (t < prompt) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
+        if (t0 + u * nt < prompt) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
         else if (WIDE) atomicAdd(&count[c], 1u);
         else atomicAdd(&count[c / 2], c & 1 ? 0x10000u : 1u);
       }
-      t0 += (int64_t)nt * kAdjUnroll;
-      if (t0 < n) history(t0, n);
     }
   }
   // the slot that holds a column, or the free one that it would get: at most half of them are taken
@@ -159,9 +147,13 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
   };
   auto find = [&](int col) { return slot_of(col, [&](uint32_t h) { return hash_at[h] == col; }); };
   if constexpr (BIAS) {
-    auto column_of = [&](int j) { return j == (int)threadIdx.x ? first_column : column(j); };
+    const int64_t at = row * g.bias_tokens_stride, bt = row * g.bias_stride;
+    auto column = [&](int j) {  // of entry j; -1: elsewhere
+      const int64_t tok = adj_column(g.bias_tokens, g.bias_tok64, at + j, c0);
+      return (uint64_t)tok < (uint64_t)width ? (int)tok : -1;
+    };
     for (int j = threadIdx.x; j < g.biases; j += nt) {
-      const int col = column_of(j);
+      const int col = column(j);
       if (col < 0) continue;
       atomicOr(&bias_bits[col / 32], 1u << (col % 32));
       if (g.hash == 0) continue;
@@ -174,21 +166,21 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     if (g.hash != 0) {
       __syncthreads();
       for (int j = threadIdx.x; j < g.biases; j += nt) {
-        const int col = column_of(j);
+        const int col = column(j);
         if (col >= 0 && hash_value[find(col)] != j + 1) twice = 1;
       }
       __syncthreads();
       for (int j0 = 0; j0 < g.biases; j0 += nt) {
-        const int j = j0 + threadIdx.x, col = j < g.biases ? column_of(j) : -1;
+        const int j = j0 + threadIdx.x, col = j < g.biases ? column(j) : -1;
         const uint32_t h = col >= 0 ? find(col) : 0u;
         const bool own = col >= 0 && hash_value[h] == j + 1;
         float b = 0.0f;
         if (own) {
           if (twice) {
             for (int i = 0; i < j; ++i)
-              if (column(i) == col) b += g.bias[bias_at + i];
+              if (column(i) == col) b += g.bias[bt + i];
           }
-          b += j == (int)threadIdx.x ? first_bias : g.bias[bias_at + j];
+          b += g.bias[bt + j];
         }
         __syncthreads();  // a value's bits must not pass for an entry's number
         if (own) hash_value[h] = __float_as_int(b);
@@ -200,7 +192,7 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0) {
     if (g.hash != 0) return __int_as_float(hash_value[find(col)]);
     float b = 0.0f;
     for (int j = 0; j < g.biases; ++j)
-      if (column(j) == col) b += g.bias[bias_at + j];
+      if (adj_column(g.bias_tokens, g.bias_tok64, row * g.bias_tokens_stride + j, c0) == col) b += g.bias[row * g.bias_stride + j];
     return b;
   };
   const uint32_t* allowed = g.allowed ? g.allowed + row * g.allowed_stride : nullptr;
@@ -314,21 +306,30 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
     }
     a.range = 1024;
     while (a.range < (wide || a.hash > 512 ? 16384 : kAdjMaxRange) && (a.vocab + a.range - 1) / a.range * d->rows > 512) a.range *= 2;
-    // a vector of the range for each thread, and of a history 8 tokens at most, up to 1024 threads
-    const int64_t threads = std::max<int64_t>(a.range / V, pen ? (d->history / 8 + 63) / 64 * 64 : 0);
-    const int block = (int)std::min<int64_t>(1024, threads);
     const unsigned ranges = (unsigned)((a.vocab + a.range - 1) / a.range);
+    a.range = (int32_t)(((a.vocab + ranges - 1) / ranges + 255) / 256 * 256);  // evenly
+    // a vector of the range for each thread, and of a history 8 tokens at most, up to 1024 threads
+    const int64_t threads = std::max<int64_t>(a.range / V, pen ? d->history / 8 : 0);
+    const int block = (int)std::min<int64_t>(1024, (threads + 63) / 64 * 64);
     const size_t lds = adj_lds_bytes(a.range, pen, wide, biased, a.hash);
-    const int64_t slab = std::max<int64_t>(1, ((int64_t(1) << 32) - 1) / block / ranges);
+    // Workgroups go to the eight XCDs in turn.  Where the histories pass what the eight L2s hold, those of a row are
+    // eight apart and next to each other in time, so that its history comes from memory once and from one XCD's L2 for
+    // the others ([512, 128256] float32, histories of 32768: 153 us with all rows' first ranges first, 142 so); else
+    // rows come first, which spreads a number of rows that is no multiple of eight evenly ([37, 50257]: 6.7 and 9.2).
+    a.ranges = FastDiv(ranges);
+    a.apart = pen && d->rows >= 64 && d->rows * d->history * 8 > (int64_t(32) << 20);
+    const int64_t most = ((int64_t(1) << 32) - 1) / block / ranges;  // HIP: fewer than 2^32 threads a launch
+    const int64_t slab = std::max<int64_t>(kAdjApart, most / kAdjApart * kAdjApart);
     for (int64_t r0 = 0; r0 < d->rows; r0 += slab) {
-      const dim3 grid((unsigned)std::min(slab, d->rows - r0), ranges);
+      const int64_t n = std::min(slab, d->rows - r0);
+      const dim3 grid = a.apart ? dim3((unsigned)((n + kAdjApart - 1) / kAdjApart * kAdjApart * ranges)) : dim3((unsigned)n, ranges);
       auto go = [&](auto p, auto w, auto b) {
         auto kernel = k_adjust<T, p.value, w.value, b.value>;
         if (lds > 65536) {
           const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
           if (e != hipSuccess) return (int)e;
         }
-        kernel<<<grid, block, lds, st>>>(a, r0);
+        kernel<<<grid, block, lds, st>>>(a, r0, n);
         return launch_status();
       };
       auto with_bias = [&](auto p, auto w) { return biased ? go(p, w, std::true_type{}) : go(p, w, std::false_type{}); };

@@ -557,7 +557,9 @@ k_distill_total(const float2* __restrict__ rows, const double* __restrict__ part
 // vectors a thread, 64 to 1024 threads).  Everything is requested before anything is waited for.
 // The exponent x c - base is formed with a base of two floats: next to 0, where the
 // probabilities are large, it has 24 bits.
-template <typename T, int G>
+// EDGES: rows that do not consist of whole vectors at multiples of 16 bytes.  The elements before a row's first and
+// behind its last then go one to a thread.
+template <typename T, int G, bool EDGES>
 __global__ void __launch_bounds__(G < kDisBlock ? kDisBlock : G)
 k_distill_bwd(DistillArgs g, int64_t row0, int64_t rows, const float* __restrict__ stats,
               const DistillPair* __restrict__ pairs, const float* __restrict__ count,
@@ -573,16 +575,20 @@ k_distill_bwd(DistillArgs g, int64_t row0, int64_t rows, const float* __restrict
   if (row >= row0 + rows) return;  // whole rows: no exchange is left waiting
   const T* xr = dis_row<T>(g, row);
   T* dst = grad + row * g.vocab;
-  const int64_t c0 = (int64_t)blockIdx.x * reach - grid_off<T, V>(dst, g.vocab), col = c0 + l * V;
-  const bool whole = col >= 0 && col + V <= g.vocab;
-  uint4 w;
-  if (whole) {
-    w = ld_any_stream(xr + col);
-  } else {
-    T e[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) e[k] = col + k >= 0 && col + k < g.vocab ? xr[col + k] : T{};
-    __builtin_memcpy(&w, e, 16);
+  const int shift = EDGES ? grid_off<T, V>(dst, g.vocab) : 0;
+  const int64_t c0 = (int64_t)blockIdx.x * reach - shift, col = c0 + l * V;
+  const bool whole = (!EDGES || col >= 0) && col + V <= g.vocab;
+  uint4 w{};
+  if (whole) w = ld_any_stream(xr + col);
+  int64_t lone = 0;
+  bool edge = false;
+  T alone{};
+  if constexpr (EDGES) {
+    const int head = (V - shift % V) % V;
+    const int64_t tail = head < g.vocab ? g.vocab - (g.vocab - head) % V : g.vocab;
+    lone = l < V ? l : tail + (l - V);
+    edge = lone >= c0 && lone < c0 + reach && (l < V ? l < head && lone < g.vocab : lone < g.vocab);
+    if (edge) alone = xr[lone];
   }
   const DistillPair* pr = pairs + row * g.entries;
   DistillPair pair{-1, 0.0f};
@@ -608,29 +614,29 @@ k_distill_bwd(DistillArgs g, int64_t row0, int64_t rows, const float* __restrict
   }
   const float k0 = rest * gs;
   sync();
-  float f[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const float x = elem_f<T>(w, k);
+  auto other = [&](float x) {  // the gradient at a token that is not listed, and at one that is
     const float v = __builtin_amdgcn_exp2f(fmaf(x, g.c, -base_hi) - base_lo) * k0;
-    f[k] = counted ? v : 0.0f;
-  }
-  const uint32_t here = bits[l * V / 32] >> (l * V % 32) & ((1u << V) - 1u);
-  if (here) {
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      if (!(here >> k & 1u)) continue;
-      const float x = elem_f<T>(w, k);
-      const float q = __builtin_amdgcn_exp2f(fmaf(x, g.c, -lse_hi) - lse_lo);
-      f[k] = (q * weight - listed[l * V + k]) * gs;
-    }
-  }
+    return counted ? v : 0.0f;
+  };
+  auto of_listed = [&](float x, float p) {
+    return (__builtin_amdgcn_exp2f(fmaf(x, g.c, -lse_hi) - lse_lo) * weight - p) * gs;
+  };
   if (whole) {
-    store_any<T, V>(dst + col, f);
-  } else {
+    float f[V];
 #pragma unroll
-    for (int k = 0; k < V; ++k)
-      if (col + k >= 0 && col + k < g.vocab) dst[col + k] = from_arith<T>(f[k]);
+    for (int k = 0; k < V; ++k) f[k] = other(elem_f<T>(w, k));
+    const uint32_t here = bits[l * V / 32] >> (l * V % 32) & ((1u << V) - 1u);
+    if (here) {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (here >> k & 1u) f[k] = of_listed(elem_f<T>(w, k), listed[l * V + k]);
+    }
+    store_any<T, V>(dst + col, f);
+  }
+  if (edge) {
+    const int at = (int)(lone - c0);
+    const float x = (float)to_arith(alone);
+    dst[lone] = from_arith<T>(bits[at / 32] >> (at % 32) & 1u ? of_listed(x, listed[at]) : other(x));
   }
 }
 
@@ -800,23 +806,29 @@ int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_
     constexpr int V = VecOf<T>::V;
     T* gx = static_cast<T*>(grad_logits);
     const int64_t vecs = grid_vecs<T, V>(gx, g.vocab);
-    auto go = [&](auto threads) -> int {
+    const bool edges = g.vocab % V != 0 || !aligned(gx, 16);
+    auto go = [&](auto threads, auto with_edges) -> int {
       constexpr int G = decltype(threads)::value, block = G < kDisBlock ? kDisBlock : G, teams = block / G;
-      const unsigned blocks = (unsigned)((vecs + G - 1) / G);
+      unsigned blocks = (unsigned)((vecs + G - 1) / G);
+      // Workgroups go to the eight XCDs in turn.  Where a row takes a multiple of eight, its first and last one, which have
+      // the lone elements, would fall to the same two throughout; one more, which has nothing to do, moves them on from
+      // row to row ([2047, 64001] float16, 32 a row: 100 us, with 33 87).
+      if (decltype(with_edges)::value && blocks % 8 == 0) ++blocks;
       const int64_t slab = teams * std::max<int64_t>(1, std::min<int64_t>(65535, ((int64_t(1) << 32) - 1) / block / blocks));
       for (int64_t r0 = 0; r0 < d->rows; r0 += slab) {
         const int64_t n = std::min(slab, d->rows - r0);
-        k_distill_bwd<T, G><<<dim3(blocks, (unsigned)((n + teams - 1) / teams)), block, 0, st>>>(
+        k_distill_bwd<T, G, decltype(with_edges)::value><<<dim3(blocks, (unsigned)((n + teams - 1) / teams)), block, 0, st>>>(
             g, r0, n, stats, static_cast<const DistillPair*>(pairs), count, grad_loss, d->reduction, gx);
         const int rc = launch_status();
         if (rc) return rc;
       }
       return SUPA_AMD_OK;
     };
+    auto size = [&](auto threads) { return edges ? go(threads, std::true_type{}) : go(threads, std::false_type{}); };
     // every workgroup looks all pairs through: more of them, and more columns a workgroup
-    if (vecs <= 128) return go(std::integral_constant<int, 64>{});
-    if (g.entries <= 256 || vecs <= 256) return go(std::integral_constant<int, 256>{});
-    return go(std::integral_constant<int, 1024>{});
+    if (vecs <= 128) return size(std::integral_constant<int, 64>{});
+    if (g.entries <= 256 || vecs <= 256) return size(std::integral_constant<int, 256>{});
+    return size(std::integral_constant<int, 1024>{});
   });
 }
 
