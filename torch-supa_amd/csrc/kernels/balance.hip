@@ -18,7 +18,7 @@
 
 namespace sa {
 
-constexpr int kBalBlock = 256;
+constexpr int kBalFwdBlock = 512, kBalBwdBlock = 256;
 constexpr int kBalMaxExperts = 1024;
 constexpr int kBalCols = 16;      // columns a workgroup of the second launch adds
 constexpr int kBalSumBlock = 1024;
@@ -55,14 +55,17 @@ template <int G> __device__ __forceinline__ float token_sum(float v) {
   return token_join<G>(v, [](float a, float b) { return a + b; });
 }
 
-// The thread's columns of a token: NV vectors of V, the one that would run past the
-// end moved back to it.  Element k of vector j is its own where bit j V + k of `own` is set.
+// The thread's columns of a token: NV vectors of V, the one that would run past the end moved back to
+// it.  Its first elements are another vector's too: they have the same values, and are left out of sums.
+// Element k of vector j is the thread's own where bit j V + k of `own` is set.  Fewer than V experts go element
+// by element.
 template <typename T, int G, int NV> struct BalCols {
   static constexpr int V = 16 / (int)sizeof(T);
   int col[NV];
   uint32_t own;
   int experts;
-  __device__ __forceinline__ BalCols(int l, int e) : own(0u), experts(e) {
+  bool ragged;  // some vector is not all its thread's own
+  __device__ __forceinline__ BalCols(int l, int e) : own(0u), experts(e), ragged(e % V != 0) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (l + j * G) * V;
@@ -72,68 +75,82 @@ template <typename T, int G, int NV> struct BalCols {
         if (col[j] + k >= c && col[j] + k < e) own |= 1u << (j * V + k);
     }
   }
-  __device__ __forceinline__ bool is_own(int j, int k) const { return own >> (j * V + k) & 1u; }
+  __device__ __forceinline__ bool is_own(int i) const { return own >> i & 1u; }
   __device__ __forceinline__ bool live(int j) const { return own >> (j * V) & ((1u << V) - 1u); }
-  __device__ __forceinline__ RowVec<T, V> load(const T* row, int j) const {
-    RowVec<T, V> r{};
-    if (!live(j)) return r;
+  // Vector j of a token; -inf in the vectors that are not there, zeros for a token that does not count.
+  __device__ __forceinline__ RowVec<T, V> load(const T* row, int j, bool on) const {
+    constexpr uint32_t ninf = std::is_same<T, float>::value ? 0xff800000u : (std::is_same<T, bf16>::value ? 0xff80ff80u : 0xfc00fc00u);
+    RowVec<T, V> r;
+    const uint32_t fill = live(j) ? 0u : ninf;
+    r.q[0] = make_uint4(fill, fill, fill, fill);
+    if (!on || !live(j)) return r;
     if (experts >= V) {
       r.q[0] = ld_any_stream(row + col[j]);
     } else {
+      const uint16_t half = (uint16_t)(ninf & 0xffffu);
       T e[V];
 #pragma unroll
-      for (int k = 0; k < V; ++k) e[k] = k < experts ? row[k] : T{};
+      for (int k = 0; k < V; ++k) {
+        if constexpr (std::is_same<T, float>::value) e[k] = k < experts ? row[k] : -__builtin_inff();
+        else e[k] = k < experts ? row[k] : __builtin_bit_cast(T, half);
+      }
       __builtin_memcpy(&r, e, sizeof(r));
     }
     return r;
   }
-  // The shares p of the token; 1 - sigmoid in `rest` (SIG).  -inf in the places that are not its own.
+  // The sum of f(i) over the thread's own elements.
+  template <typename F> __device__ __forceinline__ float own_sum(F&& f) const {
+    float s = 0.0f;
+    if (!ragged) {  // the whole launch's threads
+#pragma unroll
+      for (int i = 0; i < NV * V; ++i) s += f(i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NV * V; ++i) s += is_own(i) ? f(i) : 0.0f;
+    }
+    return s;
+  }
+  // e of a token's shares e / (sum of e): the reciprocal of the sum; 1 - sigmoid in `rest` (SIG).
   template <bool SIG>
-  __device__ __forceinline__ void shares(const RowVec<T, V> (&w)[NV], float (&p)[NV * V], float (&rest)[NV * V]) const {
+  __device__ __forceinline__ float shares(const RowVec<T, V> (&w)[NV], float (&e)[NV * V], float (&rest)[NV * V]) const {
     float m = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
-      const float x = row_elem<T, V>(w[i / V], i % V);
-      p[i] = is_own(i / V, i % V) ? x : -__builtin_inff();
+      e[i] = row_elem<T, V>(w[i / V], i % V);
       // sigmoid(x) = e^min(x, 0) / (1 + e^-|x|): the largest is scaled to at least 1/2, so none is lost to underflow
-      m = fmaxf(m, SIG ? fminf(p[i], 0.0f) : p[i]);
+      m = fmaxf(m, SIG ? fminf(e[i], 0.0f) : e[i]);
     }
-    m = token_max<G>(m);
-    float s = 0.0f;
+    const float base = token_max<G>(m) * kLog2e;  // rounded, but the same for all of the token
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
       if constexpr (SIG) {
-        const float e = __builtin_amdgcn_exp2f(-fabsf(p[i]) * kLog2e), r = 1.0f / (1.0f + e);
-        rest[i] = p[i] > 0.0f ? e * r : r;
-        p[i] = __builtin_amdgcn_exp2f((fminf(p[i], 0.0f) - m) * kLog2e) * r;  // a NaN is in r
+        const float x = e[i], u = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e), r = 1.0f / (1.0f + u);
+        rest[i] = x > 0.0f ? u * r : r;
+        e[i] = __builtin_amdgcn_exp2f(fmaf(fminf(x, 0.0f), kLog2e, -base)) * r;  // a NaN is in r
       } else {
-        p[i] = __builtin_amdgcn_exp2f((p[i] - m) * kLog2e);
+        e[i] = __builtin_amdgcn_exp2f(fmaf(e[i], kLog2e, -base));
       }
-      s += p[i];
     }
-    s = token_sum<G>(s);
-    const float inv = 1.0f / s;
-#pragma unroll
-    for (int i = 0; i < NV * V; ++i) p[i] *= inv;
+    return 1.0f / token_sum<G>(own_sum([&](int i) { return e[i]; }));
   }
 };
 
-// Tokens a thread's group has on their way at once.
+// Tokens that a thread's group has on their way at once in the backward.
 constexpr int kBalUnroll = 2;
 
 template <typename T, int G, int NV, bool SIG>
-__global__ void __launch_bounds__(kBalBlock)
+__global__ void __launch_bounds__(kBalFwdBlock)
 k_balance_fwd(BalanceArgs g, int64_t seq0, float* __restrict__ part_p, int32_t* __restrict__ part_c,
               int32_t* __restrict__ part_n, int32_t* __restrict__ arrived, int32_t* error_flag) {
   using Cols = BalCols<T, G, NV>;
-  constexpr int V = Cols::V, TEAMS = kBalBlock / G, U = kBalUnroll, WAVES = kBalBlock / 64;
+  constexpr int V = Cols::V, TEAMS = kBalFwdBlock / G, WAVES = kBalFwdBlock / 64;
   extern __shared__ float lds[];  // [WAVES][experts] sums, then [experts] counts
   int32_t* hist = reinterpret_cast<int32_t*>(lds + WAVES * g.experts);
   __shared__ int32_t lds_n;
   const int team = threadIdx.x / G, l = threadIdx.x % G;
   const int64_t seq = seq0 + blockIdx.y;
   if (seq0 == 0 && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *arrived = 0;  // for the second launch
-  for (int i = threadIdx.x; i < g.experts; i += kBalBlock) hist[i] = 0;
+  for (int i = threadIdx.x; i < g.experts; i += kBalFwdBlock) hist[i] = 0;
   if (threadIdx.x == 0) lds_n = 0;
   __syncthreads();
   const Cols cols(l, g.experts);
@@ -143,40 +160,24 @@ k_balance_fwd(BalanceArgs g, int64_t seq0, float* __restrict__ part_p, int32_t* 
   int32_t n = 0;
   const int64_t step = (int64_t)g.blocks * TEAMS;
   // the same number of rounds for every group: exchanges among threads of a wavefront need all of them
-  for (int64_t t0 = (int64_t)blockIdx.x * TEAMS; t0 < g.tokens; t0 += step * U) {
-    RowVec<T, V> w[U][NV];
-    bool on[U];
-    int32_t pick[U];  // the thread's choice, -1: none
+  for (int64_t t0 = (int64_t)blockIdx.x * TEAMS; t0 < g.tokens; t0 += step) {
+    const int64_t t = t0 + team, row = seq * g.tokens + t;
+    const bool on = t < g.tokens && (!g.mask || g.mask[row]);
+    RowVec<T, V> w[NV];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t t = t0 + u * step + team;
-      on[u] = t < g.tokens && (!g.mask || g.mask[seq * g.tokens + t]);
-      pick[u] = -1;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) w[u][j] = RowVec<T, V>{};
-      if (!on[u]) continue;
-      const int64_t row = seq * g.tokens + t;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) w[u][j] = cols.load(static_cast<const T*>(g.x) + row * g.experts, j);
-      for (int i = l; i < g.k; i += G) {
-        const int64_t at = row * g.k + i;
-        const int64_t e = g.idx64 ? static_cast<const int64_t*>(g.chosen)[at]
-                                  : (int64_t)static_cast<const int32_t*>(g.chosen)[at];
-        if (e >= g.experts && error_flag) *error_flag = 3;
-        if (e < 0 || e >= g.experts) continue;
-        if (i < G) pick[u] = (int32_t)e;
-        else atomicAdd(&hist[e], 1);
-      }
+    for (int j = 0; j < NV; ++j) w[j] = cols.load(static_cast<const T*>(g.x) + row * g.experts, j, on);
+    for (int i = l; on && i < g.k; i += G) {
+      const int64_t at = row * g.k + i;
+      const int64_t e = g.idx64 ? static_cast<const int64_t*>(g.chosen)[at]
+                                : (int64_t)static_cast<const int32_t*>(g.chosen)[at];
+      if (e >= g.experts && error_flag) *error_flag = 3;
+      if (e >= 0 && e < g.experts) atomicAdd(&hist[e], 1);
     }
+    float e[NV * V], rest[NV * V];
+    const float inv = cols.template shares<SIG>(w, e, rest), scale = on ? inv : 0.0f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (pick[u] >= 0) atomicAdd(&hist[pick[u]], 1);
-      float p[NV * V], rest[NV * V];
-      cols.template shares<SIG>(w[u], p, rest);
-#pragma unroll
-      for (int i = 0; i < NV * V; ++i) acc[i] += on[u] ? p[i] : 0.0f;
-      n += on[u] && l == 0 ? 1 : 0;
-    }
+    for (int i = 0; i < NV * V; ++i) acc[i] = fmaf(e[i], scale, acc[i]);
+    n += on && l == 0 ? 1 : 0;
   }
   // the groups of a wavefront, then the wavefronts
 #pragma unroll
@@ -188,12 +189,12 @@ k_balance_fwd(BalanceArgs g, int64_t seq0, float* __restrict__ part_p, int32_t* 
   if ((threadIdx.x & 63) < G) {
 #pragma unroll
     for (int i = 0; i < NV * V; ++i)
-      if (cols.is_own(i / V, i % V)) lds[wave * g.experts + cols.col[i / V] + i % V] = acc[i];
+      if (cols.is_own(i)) lds[wave * g.experts + cols.col[i / V] + i % V] = acc[i];
   }
   if (n > 0) atomicAdd(&lds_n, n);
   __syncthreads();
   const int64_t at = seq * g.blocks + blockIdx.x;
-  for (int i = threadIdx.x; i < g.experts; i += kBalBlock) {
+  for (int i = threadIdx.x; i < g.experts; i += kBalFwdBlock) {
     float s = lds[i];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) s += lds[v * g.experts + i];
@@ -210,45 +211,65 @@ k_balance_sum(BalanceArgs g, int64_t seq0, int64_t all_blocks, const float* __re
               const int32_t* __restrict__ part_c, const int32_t* __restrict__ part_n, int32_t* arrived,
               double* shares, int64_t* __restrict__ counts, float* __restrict__ load, float* scale,
               float* __restrict__ loss) {
-  constexpr int SLICES = kBalSumBlock / kBalCols;
-  __shared__ double lds_p[SLICES][kBalCols];
-  __shared__ int64_t lds_c[SLICES][kBalCols];
-  __shared__ int64_t lds_n;
+  constexpr int SLICES = kBalSumBlock / kBalCols, WAVES = kBalSumBlock / 64;
+  __shared__ double lds_p[WAVES][kBalCols];
+  __shared__ int64_t lds_c[WAVES][kBalCols], lds_n[WAVES];
   __shared__ int last;
-  __shared__ double lds_t[2][kBalSumBlock / 64];
+  __shared__ double lds_t[2][WAVES];
   const int64_t seq = seq0 + blockIdx.y;
-  const int c = threadIdx.x % kBalCols, slice = threadIdx.x / kBalCols;
+  const int c = threadIdx.x % kBalCols, slice = threadIdx.x / kBalCols, wave = threadIdx.x >> 6;
   const int e = blockIdx.x * kBalCols + c;
-  if (threadIdx.x == 0) lds_n = 0;
   double p = 0.0;
-  int64_t count = 0;
+  int64_t count = 0, tokens = 0;
   if (e < g.experts) {
-    for (int b = slice; b < g.blocks; b += SLICES) {
-      const int64_t at = (seq * g.blocks + b) * g.experts + e;
-      p += (double)part_p[at];
-      count += part_c[at];
+    constexpr int U = 4;
+    for (int b0 = slice; b0 < g.blocks; b0 += SLICES * U) {
+      float v[U];
+      int32_t k[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const bool on = b0 + u * SLICES < g.blocks;
+        const int64_t at = (seq * g.blocks + b0 + u * SLICES) * g.experts + e;
+        v[u] = on ? part_p[at] : 0.0f;
+        k[u] = on ? part_c[at] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        p += (double)v[u];
+        count += k[u];
+      }
     }
   }
-  lds_p[slice][c] = p;
-  lds_c[slice][c] = count;
-  int64_t tokens = 0;
   for (int b = threadIdx.x; b < g.blocks; b += kBalSumBlock) tokens += part_n[seq * g.blocks + b];
-  __syncthreads();
-  if (tokens > 0) atomicAdd(reinterpret_cast<unsigned long long*>(&lds_n), (unsigned long long)tokens);
-  for (int half = SLICES / 2; half > 0; half /= 2) {
-    if (slice < half) {
-      lds_p[slice][c] += lds_p[slice + half][c];
-      lds_c[slice][c] += lds_c[slice + half][c];
-    }
-    __syncthreads();
+#pragma unroll
+  for (int off = 32; off >= kBalCols; off >>= 1) {  // the wavefront's slices
+    p += __shfl_xor(p, off, 64);
+    count += __shfl_xor(count, off, 64);
   }
-  const int64_t n = lds_n;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) tokens += __shfl_xor(tokens, off, 64);
+  if ((threadIdx.x & 63) < kBalCols) {
+    lds_p[wave][c] = p;
+    lds_c[wave][c] = count;
+  }
+  if ((threadIdx.x & 63) == 0) lds_n[wave] = tokens;
+  __syncthreads();
+  int64_t n = 0;
+  p = 0.0;
+  count = 0;
+  if (threadIdx.x < kBalCols) {
+    for (int w = 0; w < WAVES; ++w) {
+      p += lds_p[w][c];
+      count += lds_c[w][c];
+      n += lds_n[w];
+    }
+  }
   double share = 0.0;
   if (threadIdx.x < kBalCols && e < g.experts) {
-    const double a = n > 0 ? (double)g.experts * (double)lds_c[0][c] / ((double)g.k * (double)n) : 0.0;
-    counts[seq * g.experts + e] = lds_c[0][c];
+    const double a = n > 0 ? (double)g.experts * (double)count / ((double)g.k * (double)n) : 0.0;
+    counts[seq * g.experts + e] = count;
     load[seq * g.experts + e] = (float)(a - 1.0);
-    share = n > 0 ? a * lds_p[0][c] / (double)n : 0.0;
+    share = n > 0 ? a * p / (double)n : 0.0;
   }
 #pragma unroll
   for (int off = kBalCols / 2; off > 0; off >>= 1) share += __shfl_xor(share, off, 64);
@@ -284,18 +305,18 @@ k_balance_sum(BalanceArgs g, int64_t seq0, int64_t all_blocks, const float* __re
 }
 
 template <typename T, int G, int NV, bool SIG>
-__global__ void __launch_bounds__(kBalBlock)
+__global__ void __launch_bounds__(kBalBwdBlock)
 k_balance_bwd(BalanceArgs g, int64_t seq0, const float* __restrict__ load, const float* __restrict__ scale,
               const float* __restrict__ grad_out, T* __restrict__ grad) {
   using Cols = BalCols<T, G, NV>;
-  constexpr int V = Cols::V, TEAMS = kBalBlock / G, U = kBalUnroll;
+  constexpr int V = Cols::V, TEAMS = kBalBwdBlock / G, U = kBalUnroll;
   const int team = threadIdx.x / G, l = threadIdx.x % G;
   const int64_t seq = seq0 + blockIdx.y;
   const Cols cols(l, g.experts);
   float a[NV * V];
 #pragma unroll
   for (int i = 0; i < NV * V; ++i)
-    a[i] = cols.is_own(i / V, i % V) ? load[seq * g.experts + cols.col[i / V] + i % V] : 0.0f;
+    a[i] = cols.live(i / V) && cols.col[i / V] + i % V < g.experts ? load[seq * g.experts + cols.col[i / V] + i % V] : 0.0f;
   const float gs = grad_out[0] * scale[seq] * scale[g.sequences];
   const int64_t step = (int64_t)g.blocks * TEAMS;
   for (int64_t t0 = (int64_t)blockIdx.x * TEAMS; t0 < g.tokens; t0 += step * U) {
@@ -306,40 +327,34 @@ k_balance_bwd(BalanceArgs g, int64_t seq0, const float* __restrict__ load, const
       const int64_t t = t0 + u * step + team;
       on[u] = t < g.tokens && (!g.mask || g.mask[seq * g.tokens + t]);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) w[u][j] = RowVec<T, V>{};
-      if (!on[u]) continue;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) w[u][j] = cols.load(static_cast<const T*>(g.x) + (seq * g.tokens + t) * g.experts, j);
+      for (int j = 0; j < NV; ++j) w[u][j] = cols.load(static_cast<const T*>(g.x) + (seq * g.tokens + t) * g.experts, j, on[u]);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t t = t0 + u * step + team;
-      float p[NV * V], rest[NV * V];
-      cols.template shares<SIG>(w[u], p, rest);
-      float d = 0.0f;
-#pragma unroll
-      for (int i = 0; i < NV * V; ++i) d = fmaf(p[i], a[i], d);
-      d = token_sum<G>(d);
+      float e[NV * V], rest[NV * V];
+      const float inv = cols.template shares<SIG>(w[u], e, rest);
+      const float d = token_sum<G>(cols.own_sum([&](int i) { return e[i] * a[i]; })) * inv;
       if (t >= g.tokens) continue;
+      const float k0 = on[u] ? inv * gs : 0.0f;
       T* dst = grad + (seq * g.tokens + t) * g.experts;
 #pragma unroll
       for (int i = 0; i < NV * V; ++i) {
-        p[i] = p[i] * (a[i] - d) * gs;
-        if (SIG) p[i] *= rest[i];
-        p[i] = on[u] ? p[i] : 0.0f;
+        e[i] = e[i] * (a[i] - d) * k0;
+        if (SIG) e[i] *= rest[i];
       }
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (!cols.live(j)) continue;
         float f[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) f[k] = p[j * V + k];
-        if ((cols.own >> (j * V) & ((1u << V) - 1u)) == (1u << V) - 1u) {
+        for (int k = 0; k < V; ++k) f[k] = e[j * V + k];
+        if (g.experts >= V) {
           store_any<T, V>(dst + cols.col[j], f);
         } else {
 #pragma unroll
           for (int k = 0; k < V; ++k)
-            if (cols.is_own(j, k)) dst[cols.col[j] + k] = from_arith<T>(f[k]);
+            if (k < g.experts) dst[k] = from_arith<T>(f[k]);
         }
       }
     }
@@ -366,7 +381,7 @@ int balance_args(const supa_amd_balance_desc* d, BalanceArgs& g) {
   return SUPA_AMD_OK;
 }
 
-// f(type, threads a token, vectors a thread).  Few threads with up to 16 elements each: what a token's threads
+// f(type, threads a token, vectors a thread).  Few threads with up to 16 elements each (32, to avoid idle ones): what a token's threads
 // exchange, its maximum and sum, is then a few steps for many tokens at once.
 template <typename F> int with_balance(const supa_amd_balance_desc* d, F&& f) {
   return with_float_storage(d->dtype, [&](auto* tag) -> int {
@@ -382,7 +397,10 @@ template <typename F> int with_balance(const supa_amd_balance_desc* d, F&& f) {
     if (vecs <= 4 * N) return scores(integral_constant<int, 4>{}, integral_constant<int, N>{});
     if (vecs <= 8 * N) return scores(integral_constant<int, 8>{}, integral_constant<int, N>{});
     if (vecs <= 16 * N) return scores(integral_constant<int, 16>{}, integral_constant<int, N>{});
-    return scores(integral_constant<int, 64>{}, integral_constant<int, N>{});
+    if (N == 2 && vecs <= 64) return scores(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    if (vecs <= 128) return scores(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    if constexpr (N == 4) return scores(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    return SUPA_AMD_ELAYOUT;
   });
 }
 
@@ -390,16 +408,18 @@ template <typename F> int with_balance(const supa_amd_balance_desc* d, F&& f) {
 int balance_threads(int64_t experts, int dtype) {
   const int64_t vecs = (experts * dtype_size(dtype) + 15) / 16;
   const int n = dtype == SUPA_AMD_F32 ? 4 : 2;
-  return vecs <= 4 * n ? 4 : (vecs <= 8 * n ? 8 : (vecs <= 16 * n ? 16 : 64));
+  return vecs <= 4 * n ? 4 : (vecs <= 8 * n ? 8 : (vecs <= 64 ? 16 : 64));
 }
 
 // Workgroups a sequence: `most` in all, each with a round of its groups at least.
-int32_t balance_blocks(const supa_amd_balance_desc* d, int64_t most) {
-  const int64_t round = kBalBlock / balance_threads(d->experts, d->dtype) * kBalUnroll;
+int32_t balance_blocks(const supa_amd_balance_desc* d, int64_t most, int threads) {
+  const int64_t round = threads / balance_threads(d->experts, d->dtype);
   const int64_t want = (d->tokens + round - 1) / round, each = std::max<int64_t>(1, most / std::max<int64_t>(1, d->sequences));
   return (int32_t)std::max<int64_t>(1, std::min(want, each));
 }
-constexpr int64_t kBalFwdBlocks = 1024;  // whose partials the second launch adds
+// Two workgroups of 512 threads a CU for the forward: more have more partials, which the second launch adds
+// ([262144, 256] float32, both launches: 68 us; 1024 of 256 threads 73, 2048 84; [262144, 64] bf16 24, 28 and 40).
+constexpr int64_t kBalFwdBlocks = 512;
 constexpr int64_t kBalBwdBlocks = 1 << 14;
 
 // Workspace: the shares of the loss, then the partials: sums, counts, tokens; the arrivals.
@@ -427,7 +447,7 @@ int64_t supa_amd_balance_workspace_bytes(const supa_amd_balance_desc* d) {
   BalanceArgs g;
   const int rc = balance_args(d, g);
   if (rc) return rc;
-  g.blocks = balance_blocks(d, kBalFwdBlocks);
+  g.blocks = balance_blocks(d, kBalFwdBlocks, kBalFwdBlock);
   return balance_space(g).bytes;
 }
 
@@ -438,7 +458,7 @@ int supa_amd_balance_forward(const supa_amd_balance_desc* d, float* loss, int64_
   if (rc) return rc;
   if (d->sequences == 0) return SUPA_AMD_EINVAL;
   if (!loss || !counts || !load || !scale || (d->tokens > 0 && (!d->logits || !d->chosen))) return SUPA_AMD_EINVAL;
-  g.blocks = balance_blocks(d, kBalFwdBlocks);
+  g.blocks = balance_blocks(d, kBalFwdBlocks, kBalFwdBlock);
   const BalanceSpace s = balance_space(g);
   if (!workspace || ws_bytes < s.bytes) return SUPA_AMD_EWORKSPACE;
   if (!aligned(workspace, 8)) return SUPA_AMD_EINVAL;
@@ -448,12 +468,12 @@ int supa_amd_balance_forward(const supa_amd_balance_desc* d, float* loss, int64_
   int32_t *part_c = reinterpret_cast<int32_t*>(ws + s.c), *part_n = reinterpret_cast<int32_t*>(ws + s.n),
           *arrived = reinterpret_cast<int32_t*>(ws + s.arrived);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const size_t lds = (size_t)g.experts * 4 * (kBalBlock / 64 + 1);
+  const size_t lds = (size_t)g.experts * 4 * (kBalFwdBlock / 64 + 1);
   for (int64_t s0 = 0; s0 < g.sequences; s0 += 65535) {
     const unsigned n = (unsigned)std::min<int64_t>(65535, g.sequences - s0);
     const int rc = with_balance(d, [&](auto* tag, auto threads, auto vecs, auto sig) -> int {
       using T = std::remove_pointer_t<decltype(tag)>;
-      k_balance_fwd<T, threads.value, vecs.value, sig.value><<<dim3(g.blocks, n), kBalBlock, lds, st>>>(
+      k_balance_fwd<T, threads.value, vecs.value, sig.value><<<dim3(g.blocks, n), kBalFwdBlock, lds, st>>>(
           g, s0, part_p, part_c, part_n, arrived, error_flag);
       return launch_status();
     });
@@ -477,13 +497,13 @@ int supa_amd_balance_backward(const supa_amd_balance_desc* d, const float* grad_
   if (rc) return rc;
   if (d->sequences == 0 || d->tokens == 0) return SUPA_AMD_OK;
   if (!grad_loss || !load || !scale || !grad_logits || !d->logits) return SUPA_AMD_EINVAL;
-  g.blocks = balance_blocks(d, kBalBwdBlocks);
+  g.blocks = balance_blocks(d, kBalBwdBlocks, kBalBwdBlock * kBalUnroll);
   hipStream_t st = static_cast<hipStream_t>(stream);
   for (int64_t s0 = 0; s0 < g.sequences; s0 += 65535) {
     const unsigned n = (unsigned)std::min<int64_t>(65535, g.sequences - s0);
     const int rc = with_balance(d, [&](auto* tag, auto threads, auto vecs, auto sig) -> int {
       using T = std::remove_pointer_t<decltype(tag)>;
-      k_balance_bwd<T, threads.value, vecs.value, sig.value><<<dim3(g.blocks, n), kBalBlock, 0, st>>>(
+      k_balance_bwd<T, threads.value, vecs.value, sig.value><<<dim3(g.blocks, n), kBalBwdBlock, 0, st>>>(
           g, s0, load, scale, grad_loss, static_cast<T*>(grad_logits));
       return launch_status();
     });
