@@ -119,7 +119,7 @@ def test_masked_tokens_say_nothing(no_fallback):
         dx = logits.to("supa").requires_grad_()
         other, c2 = torch.supa.router_balance_loss(dx, experts.to("supa"), mask=mask.to("supa"), scores=scores)
         (g2,) = torch.autograd.grad(other, dx)
-        assert float(other) == float(loss) and torch.equal(c2.cpu(), c.cpu()) and torch.equal(g2.cpu(), g.cpu())
+        assert float(other.detach()) == float(loss.detach()) and torch.equal(c2.cpu(), c.cpu()) and torch.equal(g2.cpu(), g.cpu())
         assert not g2.cpu()[~mask].any()
 
 
@@ -128,13 +128,13 @@ def test_nothing_counts(no_fallback):
     none = torch.zeros(3, 4, dtype=torch.bool)
     for per_sequence in (False, True):
         loss, c, g = check(logits, experts, none, per_sequence=per_sequence)
-        assert float(loss) == 0 and not c.cpu().any() and not g.cpu().any()
+        assert float(loss.detach()) == 0 and not c.cpu().any() and not g.cpu().any()
     for shape in ((0, 6), (2, 0, 6), (0, 4, 6)):
         dx = torch.empty(shape, device="supa", requires_grad=True)
         loss, c = torch.supa.router_balance_loss(dx, torch.empty(shape[:-1] + (2,), dtype=torch.int64, device="supa"),
                                                  per_sequence=len(shape) == 3)
         (g,) = torch.autograd.grad(loss, dx)
-        assert float(loss) == 0 and g.shape == shape and not c.cpu().any() and c.shape == ((shape[0], 6) if len(shape) == 3 else (6,))
+        assert float(loss.detach()) == 0 and g.shape == shape and not c.cpu().any() and c.shape == ((shape[0], 6) if len(shape) == 3 else (6,))
 
 
 def test_dropped_choices(no_fallback):
@@ -165,7 +165,7 @@ def test_extreme_logits(no_fallback):
     for scores in ("softmax", "sigmoid"):
         loss, _ = torch.supa.router_balance_loss(logits.to("supa").requires_grad_(), experts.to("supa"), scores=scores)
         want = definition(logits.double(), experts, None, scores, False)[0]
-        assert abs(float(loss) - float(want)) <= (K + 97 * U) * float(want)
+        assert abs(float(loss.detach()) - float(want)) <= (K + 97 * U) * float(want)
     logits, experts, _ = make((30, 12), 2)
     for shift in (-200.0, 200.0):  # sigmoids that float32 does not hold, and ones
         check(logits + shift, experts, None, "sigmoid")
@@ -205,7 +205,7 @@ def test_differences(no_fallback):
         (g,) = torch.autograd.grad(loss, dx)
         h = 2.0 ** -5
         # third derivatives are under 2 max load / tokens < 2; the losses' own roundings on both sides
-        tol = 2 * h * h / 6 + 2 * (K + 97 * U) * float(loss) / (2 * h)
+        tol = 2 * h * h / 6 + 2 * (K + 97 * U) * float(loss.detach()) / (2 * h)
         for r, c in ((0, 0), (1, 3), (2, 5)):
             v = [logits.clone(), logits.clone()]
             v[0][r, c] += h
