@@ -255,6 +255,32 @@ def test_excluded_tokens_at_any_temperature(temperature, no_fallback):
               temperature, "none")
 
 
+@pytest.mark.parametrize("x", T)
+@pytest.mark.parametrize("temperature", [1.0, 0.25, 1e-3])
+def test_lowest_values(x, temperature, no_fallback):
+    """Rows that a mask of the type's lowest value leaves nothing of are even, in part or whole; the largest value too."""
+    logits, i, t, lse = make(7, 530, 6, x, "f32", True, 31, temperature)
+    fi = torch.finfo(T[x])
+    logits[0] = fi.min
+    logits[1] = fi.min
+    logits[1, i[1]] = 0.0
+    logits[2] = fi.min
+    logits[2, ::2] = -math.inf
+    logits[2, i[2]] = fi.min
+    logits[3] = fi.max
+    logits[4] = torch.where(torch.arange(530) % 3 == 0, fi.max, fi.min).to(T[x])
+    logits[4, i[4]] = fi.max
+    logits[5] = fi.min
+    logits[5, i[5, :3]] = fi.max
+    t[5, 3:] = -math.inf
+    # a teacher without a rest where the student's would cost (largest - lowest) / temperature: no float32
+    lse[1], lse[5] = torch.logsumexp(t[1].double() / temperature, 0) - 0.1, torch.logsumexp(t[5].double() / temperature, 0) - 0.1
+    for v in (None, lse):
+        for reduction in ("none", "sum"):
+            rows = slice(0, 5) if reduction == "sum" else slice(0, 7)
+            check(logits[rows], i[rows], t[rows], v if v is None else v[rows], temperature, reduction)
+
+
 def test_infinite_losses_and_nans(no_fallback):
     x, i, t, lse = make(5, 400, 4, "f32", "f32", True, 6)
     x[0, i[0, 0]] = -math.inf  # a listed token that the student excludes
@@ -352,6 +378,16 @@ def test_past_the_end(supa):
     i[2, 1] = -1
     want, _, _ = definition(x.double(), i, t, None, 1.0, "none")
     assert torch.allclose(loss.detach().double().cpu(), want, atol=S(50) + 1e-5, rtol=0)
+
+
+def test_past_the_end_but_not_there(no_fallback):
+    """Padding by a teacher's logit of -inf may list any token."""
+    x, i, t, _ = make(4, 50, 6)
+    i[1, 2:], t[1, 2:] = 50, -math.inf
+    i[2], t[2] = 2 ** 31 - 1, -math.inf
+    check(x, i, t)
+    check(x, i.int(), t)
+    torch.supa.synchronize()
 
 
 def test_many_rows(no_fallback):

@@ -176,6 +176,21 @@ def test_extreme_logits(no_fallback):
     assert loss.isnan() and g[4].isnan().all() and g[:4].cpu().isfinite().all() and g[5:].cpu().isfinite().all()
 
 
+@pytest.mark.parametrize("x", T)
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_lowest_values(x, scores, no_fallback):
+    """Tokens that a mask of the type's lowest value leaves no expert are spread evenly."""
+    logits, experts, _ = make((30, 20), 2, x)
+    logits[::3] = torch.finfo(T[x]).min
+    logits[1::3, 4:] = torch.finfo(T[x]).min
+    logits[6, 1::2] = -math.inf
+    loss, _ = torch.supa.router_balance_loss(logits.to("supa"), experts.to("supa"), scores=scores)
+    want = definition(logits.double(), experts, None, scores, False)[0]
+    assert abs(float(loss.detach()) - float(want)) <= (K + 97 * U) * float(want)
+    logits[6] = torch.finfo(T[x]).min
+    check(logits, experts, None, scores, upstream=256.0)
+
+
 def test_even_loads(no_fallback):
     """Loads next to 1: the gradient is a small difference."""
     g = torch.Generator().manual_seed(3)

@@ -200,6 +200,9 @@ def test_router_balance_loss_arguments(kw, match):
     (dict(tokens=meta(3, 5, dtype=LONG)), "tokens of shape"), (dict(tokens=meta(5, dtype=LONG)), "tokens of shape"),
     (dict(tokens=meta(2, 5, dtype=LONG), repetition=0.0), "repetition > 0"),
     (dict(tokens=meta(2, 5, dtype=LONG), repetition=math.nan), "repetition > 0"),
+    (dict(tokens=meta(2, 5, dtype=LONG), repetition=1e-60), "repetition > 0"),  # as float32
+    (dict(tokens=meta(2, 5, dtype=LONG), repetition=1e39), "repetition > 0"),
+    (dict(tokens=meta(2, 5, dtype=LONG), presence=1e39), "finite penalties"),
     (dict(tokens=meta(2, 5, dtype=LONG), presence=math.inf), "finite"),
     (dict(tokens=meta(2, 5, dtype=LONG), lengths=meta(2)), "lengths of int64"),
     (dict(tokens=meta(2, 5, dtype=LONG), lengths=meta(3, dtype=LONG)), "lengths of shape"),

@@ -537,8 +537,9 @@ void check_adjust(const char* op, const at::Tensor& logits, SUPA_ADJUST_PARAMS) 
   check_value("repetition", repetition, false);
   check_value("presence", presence, false);
   check_value("frequency", frequency, false);
-  TORCH_CHECK(std::isfinite(repetition_value) && repetition_value > 0, op, ": expected repetition > 0, got ", repetition_value);
-  TORCH_CHECK(std::isfinite(presence_value) && std::isfinite(frequency_value), op, ": expected finite penalties, got ",
+  // as float32, which the kernel takes them in
+  TORCH_CHECK(std::isfinite((float)repetition_value) && (float)repetition_value > 0, op, ": expected repetition > 0, got ", repetition_value);
+  TORCH_CHECK(std::isfinite((float)presence_value) && std::isfinite((float)frequency_value), op, ": expected finite penalties, got ",
               presence_value, " and ", frequency_value);
   const bool penalties = given(repetition) || given(presence) || given(frequency) || repetition_value != 1.0 ||
                          presence_value != 0.0 || frequency_value != 0.0;

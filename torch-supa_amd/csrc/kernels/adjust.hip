@@ -141,13 +141,13 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int
       }
     }
   }
-  // the slot that holds a column, or the free one that it would get: at most half of them are taken
+  // the slot that holds a column, or the free one that it would get: at most half of them are taken, so one is met
   auto slot_of = [&](int col, auto&& step) {
     uint32_t h = ((uint32_t)col * 0x9E3779B1u) >> 16 & (uint32_t)(g.hash - 1);
     while (!step(h)) h = (h + 1) & (uint32_t)(g.hash - 1);
     return h;
   };
-  auto find = [&](int col) { return slot_of(col, [&](uint32_t h) { return hash_at[h] == col; }); };
+  auto find = [&](int col) { return slot_of(col, [&](uint32_t h) { return hash_at[h] == col || hash_at[h] == -1; }); };
   if constexpr (BIAS) {
     const int64_t at = row * g.bias_tokens_stride, bt = row * g.bias_stride;
     auto column = [&](int j) {  // of entry j; -1: elsewhere

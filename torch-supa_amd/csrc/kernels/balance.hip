@@ -120,15 +120,15 @@ template <typename T, int G, int NV> struct BalCols {
       // sigmoid(x) = e^min(x, 0) / (1 + e^-|x|): the largest is scaled to at least 1/2, so none is lost to underflow
       m = fmaxf(m, SIG ? fminf(e[i], 0.0f) : e[i]);
     }
-    const float base = token_max<G>(m) * kLog2e;  // rounded, but the same for all of the token
+    m = token_max<G>(m);  // subtracted before the scale: the type's lowest value times log2(e) is no float
 #pragma unroll
     for (int i = 0; i < NV * V; ++i) {
       if constexpr (SIG) {
         const float x = e[i], u = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e), r = 1.0f / (1.0f + u);
         rest[i] = x > 0.0f ? u * r : r;
-        e[i] = __builtin_amdgcn_exp2f(fmaf(fminf(x, 0.0f), kLog2e, -base)) * r;  // a NaN is in r
+        e[i] = __builtin_amdgcn_exp2f((fminf(x, 0.0f) - m) * kLog2e) * r;  // a NaN is in r
       } else {
-        e[i] = __builtin_amdgcn_exp2f(fmaf(e[i], kLog2e, -base));
+        e[i] = __builtin_amdgcn_exp2f((e[i] - m) * kLog2e);
       }
     }
     return 1.0f / token_sum<G>(own_sum([&](int i) { return e[i]; }));
@@ -364,7 +364,7 @@ k_balance_bwd(BalanceArgs g, int64_t seq0, const float* __restrict__ load, const
 int balance_args(const supa_amd_balance_desc* d, BalanceArgs& g) {
   if (!d || d->sequences < 0 || d->tokens < 0 || d->experts < 1 || d->k < 1) return SUPA_AMD_EINVAL;
   if (d->experts > kBalMaxExperts || d->k > d->experts || d->sequences >= (int64_t(1) << 31) ||
-      d->tokens >= (int64_t(1) << 31) || (d->sequences > 0 && d->tokens >= (int64_t(1) << 31) / d->sequences))
+      d->tokens >= (int64_t(1) << 31) || (d->sequences > 0 && d->tokens > ((int64_t(1) << 31) - 1) / d->sequences))
     return SUPA_AMD_ELAYOUT;
   if (d->scores != SUPA_AMD_SCORES_SOFTMAX && d->scores != SUPA_AMD_SCORES_SIGMOID) return SUPA_AMD_EINVAL;
   if (d->dtype != SUPA_AMD_F32 && d->dtype != SUPA_AMD_BF16 && d->dtype != SUPA_AMD_F16) return SUPA_AMD_EDTYPE;

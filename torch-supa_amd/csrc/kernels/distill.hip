@@ -127,13 +127,16 @@ __device__ __forceinline__ DistillLds dis_lds(char* p, int entries, int hash) {
   return s;
 }
 
-// The token of pair k of a row, or -1: a pair is there if its token is in [0, vocab) and its teacher logit is not -inf.
+// The token of pair k of a row, or -1: a pair is there if its token is not negative and its teacher logit is not -inf.
+// One that is there and lists a token of vocab or more is an error.
 __device__ __forceinline__ int32_t dis_token(const DistillArgs& g, int64_t indices, int64_t teacher, int k, float* t,
                                              int32_t* error_flag) {
   const int64_t at = dis_index(g, indices + k);
   *t = load_dyn<float>(g.teacher, teacher + k, g.teacher_dtype);
-  if (at >= g.vocab && error_flag) *error_flag = 3;
-  return at >= 0 && at < g.vocab && *t != -__builtin_inff() ? (int32_t)at : -1;
+  if (at < 0 || *t == -__builtin_inff()) return -1;
+  if (at < g.vocab) return (int32_t)at;
+  if (error_flag) *error_flag = 3;
+  return -1;
 }
 
 // Loads a row's pairs; whether any is there, in every lane.
@@ -178,11 +181,6 @@ __device__ __forceinline__ bool dis_listed(const DistillArgs& g, const T* xr, in
   return __any(twice);
 }
 
-__device__ __forceinline__ void dis_split(double v, float* out) {
-  out[0] = (float)v;
-  out[1] = (float)(v - (double)out[0]);
-}
-
 // What a row's finish writes: its loss, alone or with whether it counts, its statistics and its pairs (may be null).
 struct DistillOut {
   float* loss;
@@ -204,7 +202,10 @@ __device__ __forceinline__ void dis_nothing(const DistillArgs& g, int64_t row, i
   if (lane == 0) out.row(row, 0.0f, false);
 }
 
-// From the stream's pair (m, s) -- a base next to the largest x c, and the sum of exp2(x c - m) -- and
+// What a row keeps for the backward, as floats in this order.
+enum { kStatRestMax, kStatRest, kStatMax, kStatListed, kStatCounts };
+
+// From the stream's pair (m, s) -- the largest x, and the sum of exp2((x - m) c) -- and
 // the row's pairs to the row's loss, its statistics and the pairs' weights.  One wavefront.
 template <int NE, bool REST>
 __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, int lane, float m, float s,
@@ -215,7 +216,7 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   for (int i = 0; i < NE; ++i) {
     if (e.at[i] < 0) continue;
     top_t = fmaxf(top_t, e.t[i]);
-    if (REST) top = fmaxf(top, e.x[i] * g.c);
+    if (REST) top = fmaxf(top, e.x[i]);
   }
   if (REST) top = wave_max(top);
   else top_t = wave_max(top_t);
@@ -223,15 +224,15 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   const double lt = REST ? (double)teacher_lse * kLog2eD : (double)top_t * g.teacher_c;
   double p[NE];
   bool first[NE];  // no pair before lists the token
-  double sum[3] = {0.0, 0.0, 0.0};  // p, p log2 p, p (z - M)
-  float mass = 0.0f;                // the listed tokens' exp2(z - M)
+  double sum[3] = {0.0, 0.0, 0.0};  // p, p log2 p, p z with z = (x - M) c
+  float mass = 0.0f;                // the listed tokens' exp2(z)
   int distinct = 0;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
     p[i] = 0.0;
     first[i] = e.at[i] >= 0;
     if (e.at[i] < 0) continue;
-    const double log_p = (double)e.t[i] * g.teacher_c - lt, z = (double)e.x[i] * (double)g.c - (double)M;
+    const double log_p = (double)e.t[i] * g.teacher_c - lt, z = ((double)e.x[i] - (double)M) * (double)g.c;
     p[i] = exp2(log_p);
     if (p[i] != 0.0) {
       sum[0] += p[i];
@@ -273,46 +274,44 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   }
   if (lane != 0) return;
   float st[kDisStats] = {};
-  double total = (double)s;  // of exp2(z - M)
-  if (REST) total = (s != 0.0f ? (double)s * exp2((double)m - (double)M) : 0.0) + (double)mass;
-  const double log_total = log2(total), lse = (double)M + log_total;
-  double weight = 1.0, L;
+  double total = (double)s;  // of exp2((x - M) c) over the row
+  if (REST) total = (double)s * exp2(((double)m - (double)M) * (double)g.c) + (double)mass;
+  const double log_total = log2(total);
+  double L;
   if constexpr (REST) {
-    weight = sum[0];
+    double weight = sum[0];
     L = sum[1] - sum[2] + weight * log_total;
     const bool empty = (int64_t)distinct == g.vocab;  // every token is listed
     const double r = empty ? 0.0 : fmax(0.0, 1.0 - sum[0]);
-    const double rest = (m == -__builtin_inff() ? 0.0 : (double)m) + log2((double)s);  // -inf: no mass outside
-    if (r > 0.0) L += r * (log2(r) - (rest - lse));
+    const double rest = ((double)m - (double)M) * (double)g.c + log2((double)s) - log_total;  // log2 of q_R; -inf: no mass outside
+    if (r > 0.0) L += r * (log2(r) - rest);
     weight += r;
-    const bool some = rest != -__builtin_inf() && !empty;
-    dis_split(some ? rest : 0.0, st);
-    st[2] = some ? (float)(weight * exp2(rest - lse) - r) : 0.0f;
+    st[kStatRest] = s == 0.0f || empty ? 0.0f : (float)((weight * exp2(rest) - r) / (double)s);
+    st[kStatListed] = (float)(weight / total);
   } else {
     L = (sum[1] - sum[2]) * norm - log2(sum[0]) + log_total;
-    dis_split(lse, st);
-    st[2] = 1.0f;
+    st[kStatRest] = st[kStatListed] = (float)(1.0 / total);
   }
-  st[3] = (float)weight;
-  dis_split(lse, st + 4);
-  st[6] = 1.0f;  // the row counts
+  st[kStatRestMax] = s == 0.0f ? 0.0f : m;  // no mass: of logits of -inf, whose gradient is 0, not -inf - -inf
+  st[kStatMax] = top;
+  st[kStatCounts] = 1.0f;
   out.row(row, (float)(L * kLn2), true);
 #pragma unroll
   for (int i = 0; i < kDisStats; ++i) out.stats[row * kDisStats + i] = st[i];
 }
 
-// One online step over a batch of logits: (m, s) with those of f.  m is the largest x c, rounded, and as such the
-// exact base of the sum.
+// One online step over a batch of logits: (m, s) with those of f.  m is the largest x itself, subtracted before the scale:
+// a row whose logits are all the type's lowest value, whose product with c is no float, is as even as any other.
 template <int N> __device__ __forceinline__ void dis_online(float& m, float& s, const float (&f)[N], float c) {
-  float mb = f[0];
+  float M = m;
 #pragma unroll
-  for (int k = 1; k < N; ++k) mb = fmaxf(mb, f[k]);
+  for (int k = 0; k < N; ++k) M = fmaxf(M, f[k]);
   // fmaxf passes over a NaN, so M says nothing of them: the sum is always taken, and is then NaN
-  const float M = fmaxf(m, mb * c), base = M == -__builtin_inff() ? 0.0f : M;
+  const float base = M == -__builtin_inff() ? 0.0f : M;
   float sb = 0.0f;
 #pragma unroll
-  for (int k = 0; k < N; ++k) sb += __builtin_amdgcn_exp2f(fmaf(f[k], c, -base));
-  s = (M != -__builtin_inff() ? s * __builtin_amdgcn_exp2f(m - M) : s) + sb;
+  for (int k = 0; k < N; ++k) sb += __builtin_amdgcn_exp2f((f[k] - base) * c);
+  s = s * __builtin_amdgcn_exp2f((m - base) * c) + sb;
   m = M;
 }
 
@@ -383,9 +382,9 @@ template <typename T, int G, bool REST> struct DistillStream {
 };
 
 // (m, s) of a wavefront, in every lane.
-__device__ __forceinline__ void dis_join(float& m, float& s) {
+__device__ __forceinline__ void dis_join(float& m, float& s, float c) {
   const float M = wave_max(m);
-  if (M != -__builtin_inff()) s *= __builtin_amdgcn_exp2f(m - M);
+  if (M != -__builtin_inff()) s *= __builtin_amdgcn_exp2f((m - M) * c);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   m = M;
@@ -448,7 +447,7 @@ k_distill_fwd(DistillArgs g, int64_t row0, int64_t rows, DistillOut out, int32_t
     if (REST) dis_mark<G>(g, row, c0, next.shift(), l, s.bits);
     next.run(g.c, s.bits, m, sum);
   }
-  dis_join(m, sum);
+  dis_join(m, sum, g.c);
   if constexpr (W > 1) {
     if (lane == 0) lds_join[wave] = make_float2(m, sum);
     __syncthreads();
@@ -456,7 +455,7 @@ k_distill_fwd(DistillArgs g, int64_t row0, int64_t rows, DistillOut out, int32_t
     const float2 part = lane < W ? lds_join[lane] : make_float2(-__builtin_inff(), 0.0f);
     m = part.x;
     sum = part.y;
-    dis_join(m, sum);
+    dis_join(m, sum, g.c);
   }
   dis_finish<NE, REST>(g, row, lane, m, sum, e, teacher_lse, twice, s, out);
 }
@@ -477,14 +476,14 @@ k_distill_part(DistillArgs g, int64_t columns, float2* __restrict__ parts) {
     if (REST) dis_mark<G>(g, row, s0, stream.shift(), threadIdx.x, bits);
     stream.run(g.c, bits, m, sum);
   }
-  dis_join(m, sum);
+  dis_join(m, sum, g.c);
   if ((threadIdx.x & 63) == 0) lds_join[threadIdx.x >> 6] = make_float2(m, sum);
   __syncthreads();
   if (threadIdx.x >= 64) return;
   const float2 part = threadIdx.x < W ? lds_join[threadIdx.x] : make_float2(-__builtin_inff(), 0.0f);
   m = part.x;
   sum = part.y;
-  dis_join(m, sum);
+  dis_join(m, sum, g.c);
   if (threadIdx.x == 0) parts[row * gridDim.x + blockIdx.x] = make_float2(m, sum);
 }
 // ... and the rows from their parts, a wavefront each.
@@ -501,7 +500,7 @@ k_distill_rows(DistillArgs g, int nparts, const float2* __restrict__ parts, Dist
   if (!dis_entries(g, row, lane, e, error_flag)) return dis_nothing(g, row, lane, out);
   const bool twice = dis_listed(g, dis_row<T>(g, row), lane, e, s);
   float m = part.x, sum = part.y;
-  dis_join(m, sum);
+  dis_join(m, sum, g.c);
   dis_finish<NE, REST>(g, row, lane, m, sum, e, teacher_lse, twice, s, out);
 }
 
@@ -555,8 +554,8 @@ k_distill_total(const float2* __restrict__ rows, const double* __restrict__ part
 // grad[row, columns of the G threads]: one vector a thread, as memory takes a read and a
 // write stream best ([3700, 128256] bf16, reading and writing alone: 287 us so, 310 to 335 with four
 // vectors a thread, 64 to 1024 threads).  Everything is requested before anything is waited for.
-// The exponent x c - base is formed with a base of two floats: next to 0, where the
-// probabilities are large, it has 24 bits.
+// The probabilities are exp2((x - largest x) c) times a factor of the row: the exponent is exact next to 0, where
+// they are large.
 // EDGES: rows that do not consist of whole vectors at multiples of 16 bytes.  The elements before a row's first and
 // behind its last then go one to a thread.
 template <typename T, int G, bool EDGES>
@@ -594,8 +593,8 @@ k_distill_bwd(DistillArgs g, int64_t row0, int64_t rows, const float* __restrict
   DistillPair pair{-1, 0.0f};
   if (l < g.entries) pair = pr[l];
   const float* st = stats + row * kDisStats;
-  const float base_hi = st[0], base_lo = st[1], lse_hi = st[4], lse_lo = st[5], weight = st[3], rest = st[2];
-  const bool counted = st[6] != 0.0f;
+  const float rest_max = st[kStatRestMax], rest = st[kStatRest], max = st[kStatMax], mass = st[kStatListed];
+  const bool counted = st[kStatCounts] != 0.0f;
   float gs = reduction == SUPA_AMD_REDUCTION_NONE ? grad_out[row] : grad_out[0];
   if (reduction == SUPA_AMD_REDUCTION_MEAN) gs /= count[0];
   gs = (float)((double)gs * g.inv_t);
@@ -615,11 +614,11 @@ k_distill_bwd(DistillArgs g, int64_t row0, int64_t rows, const float* __restrict
   const float k0 = rest * gs;
   sync();
   auto other = [&](float x) {  // the gradient at a token that is not listed, and at one that is
-    const float v = __builtin_amdgcn_exp2f(fmaf(x, g.c, -base_hi) - base_lo) * k0;
+    const float v = __builtin_amdgcn_exp2f((x - rest_max) * g.c) * k0;
     return counted ? v : 0.0f;
   };
   auto of_listed = [&](float x, float p) {
-    return (__builtin_amdgcn_exp2f(fmaf(x, g.c, -lse_hi) - lse_lo) * weight - p) * gs;
+    return (__builtin_amdgcn_exp2f((x - max) * g.c) * mass - p) * gs;
   };
   if (whole) {
     float f[V];
