@@ -143,6 +143,22 @@ def test_numbers_and_defaults(no_fallback):
     check(tokens | {"lengths": torch.tensor([0, 1000, -5, 60]), "prompt_lengths": torch.tensor([3, 2000, -4, 60]), "repetition": 2.0, "presence": 1.0})
 
 
+@pytest.mark.parametrize("rows, vocab, length", [(3, 20011, 0), (2, 20011, 300), (2, 9000, 70000), (300, 2500, 40)], ids=str)
+def test_a_bias_of_every_token(rows, vocab, length, no_fallback):
+    """More biases than the hash table takes, each token once, in any order, or again and again."""
+    d = make(rows, vocab, length, vocab, False, "bf16", 17)
+    g = torch.Generator().manual_seed(1)
+    d["bias_tokens"][0] = torch.randperm(vocab, generator=g)
+    d["bias_tokens"][1, ::2] = d["bias_tokens"][1, 1::2][: (vocab + 1) // 2].repeat(2)[: (vocab + 1) // 2]
+    got = check(d)
+    s = to_supa(d)
+    x = s.pop("logits")
+    for _ in range(3):
+        assert torch.equal(torch.supa.adjust_logits(x, **s).cpu(), got)
+    d["bias_tokens"][-1] = vocab - 1
+    check(d | {"bias_tokens": d["bias_tokens"].int()})
+
+
 def test_tokens_outside_are_passed_over(no_fallback):
     d = make(5, 200, 50, 20, False)
     d["tokens"][:, ::3] = -1

@@ -14,8 +14,9 @@
 // one launch; integer counts do not depend on the order of the additions.  Counts
 // are 16 bits where the history is short enough for them, so that a range is long
 // and the history is read few times; what the prompt holds and which tokens have a
-// bias are bits.  The biases are in a hash table of the range's tokens, each put
-// there by the last entry of its token, with the sum in the entries' order.  The range's first logits are requested before
+// bias are bits.  The biases' sums are in LDS, in a hash table of the range's tokens or, of many, one for each
+// of its columns; the entries of a token add theirs in turn, in their order, so that the sum does not
+// depend on which thread comes first.  The range's first logits are requested before
 // the history is read.
 #include "row_group.h"
 
@@ -25,8 +26,11 @@ constexpr int kAdjApart = 8;                 // XCDs
 constexpr int kAdjVecs = 4;                  // vectors of logits that a thread has in flight
 constexpr int kAdjUnroll = 2;               // tokens of the history in flight a thread: with 4 and 8 the long histories took 162 and 233 us, with 2 152
 constexpr int kAdjMaxRange = 32768;
-constexpr int kAdjHash = 1024;               // most biases whose table is in LDS; of more, a token's are looked for in memory
+constexpr int kAdjHash = 1024;               // most biases that go into a hash table
+constexpr int kAdjDense = 8192;              // columns of a range where there are more: 64 KiB of sums and turns
 constexpr int64_t kAdjNarrow = 65535;        // the longest history that 16 bits count
+
+constexpr int kAdjNobody = 0x7fffffff;
 
 struct AdjustArgs {
   const void* in;
@@ -44,7 +48,7 @@ struct AdjustArgs {
   int32_t biases, range;
   FastDiv ranges;   // of a row
   int32_t apart;    // a row's workgroups are kAdjApart of the launch apart; else `rows` of it
-  int32_t hash;     // slots of the biases' table, a power of two >= 2 biases; 0: no table
+  int32_t hash;     // slots of the biases' hash table, a power of two >= 2 biases; 0: a slot for each column
   int32_t tok64, len64, prompt64, bias_tok64;
   float repetition_value, presence_value, frequency_value;
 };
@@ -54,11 +58,11 @@ __device__ __forceinline__ int64_t adj_int(const void* p, int is64, int64_t at) 
 }
 
 // LDS of a workgroup, in words: counts, bits of the prompt's tokens (PEN), bits of the tokens with a
-// bias, the biases' table: tokens, then owners or values (BIAS).
+// bias, and of each slot of the biases' table its column (of a hash table), sum and whose turn it is (BIAS).
 inline __host__ __device__ int adj_count_words(int range, bool wide) { return wide ? range : range / 2; }
 inline size_t adj_lds_bytes(int range, bool pen, bool wide, bool biased, int hash) {
   return (pen ? 4 * (size_t)(adj_count_words(range, wide) + range / 32) : 0) +
-         (biased ? 4 * (size_t)(range / 32) + 8 * (size_t)hash : 0);
+         (biased ? 4 * (size_t)(range / 32) + (hash != 0 ? 12 * (size_t)hash : 8 * (size_t)range) : 0);
 }
 
 // A token's column from c0 on; one far outside is not in any range.
@@ -71,12 +75,13 @@ template <typename T, bool PEN, bool WIDE, bool BIAS>
 __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int64_t rows) {
   constexpr int V = VecOf<T>::V;
   extern __shared__ uint4 lds[];
-  __shared__ int twice;
   uint32_t* const count = reinterpret_cast<uint32_t*>(lds);
   uint32_t* const prompt_bits = count + adj_count_words(g.range, WIDE);
   uint32_t* const bias_bits = PEN ? prompt_bits + g.range / 32 : count;
   int32_t* const hash_at = reinterpret_cast<int32_t*>(bias_bits + g.range / 32);
-  int32_t* const hash_value = hash_at + g.hash;
+  const int slots = g.hash != 0 ? g.hash : g.range;
+  float* const slot_sum = reinterpret_cast<float*>(hash_at + g.hash);
+  int32_t* const turn = hash_at + g.hash + slots;
   uint32_t row_at = blockIdx.x, range = blockIdx.y;
   if (g.apart) {  // in runs of as many rows with all their ranges
     uint32_t run;
@@ -114,11 +119,11 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int
     for (int i = threadIdx.x; i < words / 4; i += nt) lds[i] = make_uint4(0u, 0u, 0u, 0u);
     for (int i = words / 4 * 4 + threadIdx.x; i < words; i += nt) count[i] = 0u;
     if (BIAS) {
-      for (int i = threadIdx.x; i < g.hash; i += nt) {
-        hash_at[i] = -1;
-        hash_value[i] = 0;
+      for (int i = threadIdx.x; i < g.hash; i += nt) hash_at[i] = -1;
+      for (int i = threadIdx.x; i < slots; i += nt) {
+        slot_sum[i] = 0.0f;
+        turn[i] = kAdjNobody;
       }
-      if (threadIdx.x == 0) twice = 0;
     }
     __syncthreads();
   }
@@ -145,57 +150,39 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int
   auto slot_of = [&](int col, auto&& step) {
     uint32_t h = ((uint32_t)col * 0x9E3779B1u) >> 16 & (uint32_t)(g.hash - 1);
     while (!step(h)) h = (h + 1) & (uint32_t)(g.hash - 1);
-    return h;
+    return (int)h;
   };
-  auto find = [&](int col) { return slot_of(col, [&](uint32_t h) { return hash_at[h] == col || hash_at[h] == -1; }); };
   if constexpr (BIAS) {
     const int64_t at = row * g.bias_tokens_stride, bt = row * g.bias_stride;
-    auto column = [&](int j) {  // of entry j; -1: elsewhere
-      const int64_t tok = adj_column(g.bias_tokens, g.bias_tok64, at + j, c0);
-      return (uint64_t)tok < (uint64_t)width ? (int)tok : -1;
-    };
-    for (int j = threadIdx.x; j < g.biases; j += nt) {
-      const int col = column(j);
-      if (col < 0) continue;
-      atomicOr(&bias_bits[col / 32], 1u << (col % 32));
-      if (g.hash == 0) continue;
-      const uint32_t h = slot_of(col, [&](uint32_t h) {
-        const int was = atomicCAS(&hash_at[h], -1, col);
-        return was == -1 || was == col;
-      });
-      atomicMax(&hash_value[h], j + 1);  // the last entry owns the slot
-    }
-    if (g.hash != 0) {
-      __syncthreads();
-      for (int j = threadIdx.x; j < g.biases; j += nt) {
-        const int col = column(j);
-        if (col >= 0 && hash_value[find(col)] != j + 1) twice = 1;
+    for (int64_t j0 = 0; j0 < g.biases; j0 += nt) {
+      const int64_t j = j0 + threadIdx.x, col = j < g.biases ? adj_column(g.bias_tokens, g.bias_tok64, at + j, c0) : -1;
+      bool waits = (uint64_t)col < (uint64_t)width;
+      int slot = (int)col;
+      float b = 0.0f;
+      if (waits) {
+        b = g.bias[bt + j];
+        atomicOr(&bias_bits[col / 32], 1u << (col % 32));
+        if (g.hash != 0) slot = slot_of((int)col, [&](uint32_t h) {
+          const int was = atomicCAS(&hash_at[h], -1, (int)col);
+          return was == -1 || was == (int)col;
+        });
       }
-      __syncthreads();
-      for (int j0 = 0; j0 < g.biases; j0 += nt) {
-        const int j = j0 + threadIdx.x, col = j < g.biases ? column(j) : -1;
-        const uint32_t h = col >= 0 ? find(col) : 0u;
-        const bool own = col >= 0 && hash_value[h] == j + 1;
-        float b = 0.0f;
-        if (own) {
-          if (twice) {
-            for (int i = 0; i < j; ++i)
-              if (column(i) == col) b += g.bias[bt + i];
-          }
-          b += g.bias[bt + j];
+      do {  // the first of a slot's entries that wait takes its turn: each round ends with fewer
+        if (waits) atomicMin(&turn[slot], (int)j);
+        __syncthreads();
+        const bool now = waits && turn[slot] == (int)j;
+        __syncthreads();
+        if (now) {
+          slot_sum[slot] += b;
+          turn[slot] = kAdjNobody;
+          waits = false;
         }
-        __syncthreads();  // a value's bits must not pass for an entry's number
-        if (own) hash_value[h] = __float_as_int(b);
-      }
+      } while (__syncthreads_or(waits));
     }
   }
   if (PEN || BIAS) __syncthreads();
   auto bias_of = [&](int col) {
-    if (g.hash != 0) return __int_as_float(hash_value[find(col)]);
-    float b = 0.0f;
-    for (int j = 0; j < g.biases; ++j)
-      if (adj_column(g.bias_tokens, g.bias_tok64, row * g.bias_tokens_stride + j, c0) == col) b += g.bias[row * g.bias_stride + j];
-    return b;
+    return slot_sum[g.hash != 0 ? slot_of(col, [&](uint32_t h) { return hash_at[h] == col || hash_at[h] == -1; }) : col];
   };
   const uint32_t* allowed = g.allowed ? g.allowed + row * g.allowed_stride : nullptr;
   for (int base = 0; base < width; base += nt * V * kAdjVecs) {
@@ -306,8 +293,9 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
       a.hash = 64;
       while (a.hash < 2 * a.biases) a.hash *= 2;
     }
+    const int most_range = biased && a.hash == 0 ? kAdjDense : (wide || a.hash > 512 ? 16384 : kAdjMaxRange);
     a.range = 1024;
-    while (a.range < (wide || a.hash > 512 ? 16384 : kAdjMaxRange) && (a.vocab + a.range - 1) / a.range * d->rows > 512) a.range *= 2;
+    while (a.range < most_range && (a.vocab + a.range - 1) / a.range * d->rows > 512) a.range *= 2;
     const unsigned ranges = (unsigned)((a.vocab + a.range - 1) / a.range);
     a.range = (int32_t)(((a.vocab + ranges - 1) / ranges + 255) / 256 * 256);  // evenly
     // a vector of the range for each thread, and of a history 8 tokens at most, up to 1024 threads
@@ -319,7 +307,7 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
     // the others ([512, 128256] float32, histories of 32768: 153 us with all rows' first ranges first, 142 so); else
     // rows come first, which spreads a number of rows that is no multiple of eight evenly ([37, 50257]: 6.7 and 9.2).
     a.ranges = FastDiv(ranges);
-    a.apart = pen && d->rows >= 64 && d->rows * d->history * 8 > (int64_t(32) << 20);
+    a.apart = (pen && d->rows >= 64 && d->rows * d->history * 8 > (int64_t(32) << 20)) || ranges > 65535;
     const int64_t most = ((int64_t(1) << 32) - 1) / block / ranges;  // HIP: fewer than 2^32 threads a launch
     const int64_t slab = std::max<int64_t>(kAdjApart, most / kAdjApart * kAdjApart);
     for (int64_t r0 = 0; r0 < d->rows; r0 += slab) {
