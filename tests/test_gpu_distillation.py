@@ -209,6 +209,23 @@ def test_a_token_listed_twice(k, rest, no_fallback):
     check(x, i, t, lse)
 
 
+@pytest.mark.parametrize("k", [64, 256, 1000])
+@pytest.mark.parametrize("rest", [False, True], ids=["listed", "rest"])
+def test_tokens_listed_many_times(k, rest, no_fallback):
+    """All, in pairs, far apart and at random: the same bits each time."""
+    for vocab in (40, 1500, 70001):
+        x, i, t, lse = make(6, max(vocab, k), k, "f32", "f32", rest, vocab)
+        i[0] = i[0, 3]
+        i[1] = (torch.arange(k) // 2) % vocab
+        i[2] = torch.arange(k) % (k // 2 + 1) % vocab
+        i[3] = torch.randint(0, min(vocab, 90), (k,), generator=torch.Generator().manual_seed(k))
+        i[4] = (torch.arange(k) * 65536) % max(vocab, k)
+        i[4, ::3] = -1
+        loss, g = check(x, i, t, lse, reduction="none")
+        again, g2 = check(x, i, t, lse, reduction="none")
+        assert torch.equal(loss.detach().cpu(), again.detach().cpu()) and torch.equal(g.cpu(), g2.cpu())
+
+
 def test_every_token_listed(no_fallback):
     """No rest: what the teacher's lse leaves over has nowhere to go."""
     for vocab in (1, 5, 300):

@@ -18,8 +18,8 @@
 // element whose bit is set takes its p from there.
 //
 // A token listed twice has the sum of its p: the row's first such pair carries it.
-// Twice-listed tokens are found by a hash table in LDS; only rows that have one
-// compare all pairs.
+// Such tokens, and their first pairs, are found by a hash table in LDS; the others add their p to the
+// first's in turn, in the order of the pairs.
 #include "row_group.h"
 
 namespace sa {
@@ -105,25 +105,26 @@ struct DistillPair {
   float p;
 };
 
-// LDS of a row, in this order: the slow path's p (float64), the pairs' tokens, the hash table, the bitmap.
+// LDS of a row, in this order: the pairs' p (float64) and whose turn it is to add to it, both of rows that list a token
+// twice alone; the hash table's tokens and their first pairs; the bitmap.
 struct DistillLds {
   double* p;
-  int32_t* at;
-  int32_t* hash;
+  int32_t *turn, *hash, *first;
   uint32_t* bits;
 };
 // Words of a bitmap: a segment, which may begin some places into a vector and end in one.
 inline __host__ __device__ int dis_bit_words(int segment) { return (segment + 16 + 63) / 64 * 2; }
 inline __host__ __device__ size_t dis_lds_bytes(int entries, int hash, int segment) {
-  return (size_t)((entries + 1) / 2 * 2) * 12 + (size_t)hash * 4 + (segment > 0 ? 4 * (size_t)dis_bit_words(segment) : 0);
+  return (size_t)((entries + 1) / 2 * 2) * 12 + (size_t)hash * 8 + (segment > 0 ? 4 * (size_t)dis_bit_words(segment) : 0);
 }
 __device__ __forceinline__ DistillLds dis_lds(char* p, int entries, int hash) {
   const int n = (entries + 1) / 2 * 2;
   DistillLds s;
   s.p = reinterpret_cast<double*>(p);
-  s.at = reinterpret_cast<int32_t*>(s.p + n);
-  s.hash = s.at + n;
-  s.bits = reinterpret_cast<uint32_t*>(s.hash + hash);
+  s.turn = reinterpret_cast<int32_t*>(s.p + n);
+  s.hash = s.turn + n;
+  s.first = s.hash + hash;
+  s.bits = reinterpret_cast<uint32_t*>(s.first + hash);
   return s;
 }
 
@@ -156,29 +157,72 @@ __device__ __forceinline__ bool dis_entries(const DistillArgs& g, int64_t row, i
   return __any(any);
 }
 
+// The slot of a token in the hash table, of which at most half are taken: step says whether this is it.
+template <typename F> __device__ __forceinline__ int dis_slot(const DistillArgs& g, int32_t token, F&& step) {
+  uint32_t h = ((uint32_t)token * 0x9E3779B1u) >> 16 & (uint32_t)(g.hash - 1);
+  while (!step(h)) h = (h + 1) & (uint32_t)(g.hash - 1);
+  return (int)h;
+}
+
 // The student's logits of the pairs, and whether a token is listed twice, in every lane.  One wavefront a row.
 template <typename T, int NE>
 __device__ __forceinline__ bool dis_listed(const DistillArgs& g, const T* xr, int lane, DistillEntries<NE>& e,
                                            const DistillLds& s) {
 #pragma unroll
   for (int i = 0; i < NE; ++i) e.x[i] = e.at[i] >= 0 ? (float)to_arith(xr[e.at[i]]) : -__builtin_inff();
-  for (int i = lane; i < g.hash; i += 64) s.hash[i] = -1;
+  for (int i = lane; i < g.hash; i += 64) {
+    s.hash[i] = -1;
+    s.first[i] = kDisMaxEntries;
+  }
   wave_sync();
   bool twice = false;
 #pragma unroll
   for (int i = 0; i < NE; ++i) {
-    const int k = lane + i * 64;
-    if (k < g.entries) s.at[k] = e.at[i];
     if (e.at[i] < 0) continue;
-    uint32_t h = ((uint32_t)e.at[i] * 0x9E3779B1u) >> 16;
-    for (;; ++h) {  // at most half of the slots are taken: the search ends
-      const int old = atomicCAS(&s.hash[h & (uint32_t)(g.hash - 1)], -1, e.at[i]);
+    const int h = dis_slot(g, e.at[i], [&](uint32_t h) {
+      const int old = atomicCAS(&s.hash[h], -1, e.at[i]);
       twice = twice || old == e.at[i];
-      if (old == -1 || old == e.at[i]) break;
-    }
+      return old == -1 || old == e.at[i];
+    });
+    atomicMin(&s.first[h], lane + i * 64);
   }
   wave_sync();
   return __any(twice);
+}
+
+// Gives the p of pairs whose token an earlier one lists to the first that does; `first` says which pairs are.
+template <int NE>
+__device__ __forceinline__ void dis_share(const DistillArgs& g, int lane, const DistillEntries<NE>& e, double (&p)[NE],
+                                          bool (&first)[NE], const DistillLds& s) {
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    if (e.at[i] < 0) continue;
+    s.p[lane + i * 64] = p[i];
+    s.turn[lane + i * 64] = 64;
+  }
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    int to = lane + i * 64;
+    if (e.at[i] >= 0) to = s.first[dis_slot(g, e.at[i], [&](uint32_t h) { return s.hash[h] == e.at[i]; })];
+    bool waits = to != lane + i * 64;
+    first[i] = first[i] && !waits;
+    while (__any(waits)) {  // the lowest lane that waits for a pair takes its turn: each round ends with fewer
+      if (waits) atomicMin(&s.turn[to], lane);
+      wave_sync();
+      const bool now = waits && s.turn[to] == lane;
+      wave_sync();
+      if (now) {
+        s.p[to] += p[i];
+        s.turn[to] = 64;
+        waits = false;
+      }
+      wave_sync();
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NE; ++i)
+    if (first[i]) p[i] = s.p[lane + i * 64];
 }
 
 // What a row's finish writes: its loss, alone or with whether it counts, its statistics and its pairs (may be null).
@@ -231,7 +275,7 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   for (int i = 0; i < NE; ++i) {
     p[i] = 0.0;
     first[i] = e.at[i] >= 0;
-    if (e.at[i] < 0) continue;
+    if (!first[i]) continue;
     const double log_p = (double)e.t[i] * g.teacher_c - lt, z = ((double)e.x[i] - (double)M) * (double)g.c;
     p[i] = exp2(log_p);
     if (p[i] != 0.0) {
@@ -239,13 +283,13 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
       sum[1] += p[i] * log_p;
       sum[2] += p[i] * z;
     }
-    if (twice) {
-      const int k = lane + i * 64;
-      for (int j = 0; j < k && first[i]; ++j) first[i] = lds.at[j] != e.at[i];
-      lds.p[k] = p[i];
-    }
-    if (REST && first[i]) {
-      mass += __builtin_amdgcn_exp2f((float)z);
+  }
+  if (twice) dis_share(g, lane, e, p, first, lds);
+  if (REST) {
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      if (!first[i]) continue;
+      mass += __builtin_amdgcn_exp2f((e.x[i] - M) * g.c);
       ++distinct;
     }
   }
@@ -254,15 +298,6 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   if (REST) {
     mass = sum64(mass);
     distinct = (int)sum64((float)distinct);  // at most 1024
-  }
-  if (twice) {
-    wave_sync();
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-      if (!first[i]) continue;
-      for (int j = lane + i * 64 + 1; j < g.entries; ++j)
-        if (lds.at[j] == e.at[i]) p[i] += lds.p[j];
-    }
   }
   const double norm = REST ? 1.0 : 1.0 / sum[0];
   if (out.pairs) {
