@@ -75,22 +75,25 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
   return v;
 }
+template <typename F> __device__ __forceinline__ double wave_halves(double x, F&& f) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)f((int)(uint32_t)u), hi = (uint32_t)f((int)(uint32_t)(u >> 32));
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// The value of one lane.
+__device__ __forceinline__ double wave_lane(double v, int l) {
+  return wave_halves(v, [&](int h) { return __builtin_amdgcn_readlane(h, l); });
+}
 // The sum of a wavefront, in every lane: four lane permutations within 16 lanes, then the four rows of 16.
 __device__ __forceinline__ double wave_sum(double v) {
-  auto halves = [](double x, auto&& f) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = (uint32_t)f((int)(uint32_t)u), hi = (uint32_t)f((int)(uint32_t)(u >> 32));
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-  };
   auto perm = [&](double x, auto ctrl) {
-    return halves(x, [](int h) { return __builtin_amdgcn_update_dpp(0, h, decltype(ctrl)::value, 0xf, 0xf, true); });
+    return wave_halves(x, [](int h) { return __builtin_amdgcn_update_dpp(0, h, decltype(ctrl)::value, 0xf, 0xf, true); });
   };
   v += perm(v, std::integral_constant<int, 0xB1>{});   // quad_perm [1, 0, 3, 2]
   v += perm(v, std::integral_constant<int, 0x4E>{});   // quad_perm [2, 3, 0, 1]
   v += perm(v, std::integral_constant<int, 0x141>{});  // row_half_mirror
   v += perm(v, std::integral_constant<int, 0x140>{});  // row_mirror
-  auto lane = [&](int l) { return halves(v, [&](int h) { return __builtin_amdgcn_readlane(h, l); }); };
-  return (lane(0) + lane(16)) + (lane(32) + lane(48));
+  return (wave_lane(v, 0) + wave_lane(v, 16)) + (wave_lane(v, 32) + wave_lane(v, 48));
 }
 
 // A row's pairs in a wavefront: lane l holds pairs l, l + 64, ... NE of them.
@@ -307,28 +310,35 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
       if (k < g.entries) out.pairs[row * g.entries + k] = DistillPair{first[i] ? e.at[i] : -1, (float)(p[i] * norm)};
     }
   }
-  if (lane != 0) return;
-  float st[kDisStats] = {};
-  double total = (double)s;  // of exp2((x - M) c) over the row
-  if (REST) total = (double)s * exp2(((double)m - (double)M) * (double)g.c) + (double)mass;
-  const double log_total = log2(total);
+  // the same in all lanes from here on, but for the logarithms: a float64 one costs about 60 instructions, so each
+  // lane takes one
+  double weight = 1.0, r = 0.0, total = (double)s, rest_scale = 1.0;  // total: of exp2((x - M) c) over the row
+  bool rest = true;
+  const double down = ((double)m - (double)M) * (double)g.c;
+  if constexpr (REST) {
+    rest = (int64_t)distinct != g.vocab && s != 0.0f;  // some token is not listed, and has mass
+    r = (int64_t)distinct == g.vocab ? 0.0 : fmax(0.0, 1.0 - sum[0]);
+    weight = sum[0] + r;
+    const double whole = rint(fmax(down, -2000.0));
+    rest_scale = ldexp((double)__builtin_amdgcn_exp2f((float)(fmax(down, -2000.0) - whole)), (int)whole);
+    total = (double)s * rest_scale + (double)mass;
+  }
+  const double lg = log2(lane == 0 ? total : (lane == 1 ? (REST ? (double)s : sum[0]) : r));
+  const double log_total = wave_lane(lg, 0);
   double L;
   if constexpr (REST) {
-    double weight = sum[0];
-    L = sum[1] - sum[2] + weight * log_total;
-    const bool empty = (int64_t)distinct == g.vocab;  // every token is listed
-    const double r = empty ? 0.0 : fmax(0.0, 1.0 - sum[0]);
-    const double rest = ((double)m - (double)M) * (double)g.c + log2((double)s) - log_total;  // log2 of q_R; -inf: no mass outside
-    if (r > 0.0) L += r * (log2(r) - rest);
-    weight += r;
-    st[kStatRest] = s == 0.0f || empty ? 0.0f : (float)((weight * exp2(rest) - r) / (double)s);
-    st[kStatListed] = (float)(weight / total);
+    L = sum[1] - sum[2] + sum[0] * log_total;
+    if (r > 0.0) L += r * (wave_lane(lg, 2) - (down + wave_lane(lg, 1) - log_total));  // log2 of r and of q_R
   } else {
-    L = (sum[1] - sum[2]) * norm - log2(sum[0]) + log_total;
-    st[kStatRest] = st[kStatListed] = (float)(1.0 / total);
+    L = (sum[1] - sum[2]) * norm - wave_lane(lg, 1) + log_total;
   }
+  if (lane != 0) return;
+  const double scale = weight / total;
+  float st[kDisStats] = {};
   st[kStatRestMax] = s == 0.0f ? 0.0f : m;  // no mass: of logits of -inf, whose gradient is 0, not -inf - -inf
+  st[kStatRest] = !rest ? 0.0f : (float)(scale * rest_scale - (REST ? r / (double)s : 0.0));
   st[kStatMax] = top;
+  st[kStatListed] = (float)scale;
   st[kStatCounts] = 1.0f;
   out.row(row, (float)(L * kLn2), true);
 #pragma unroll
