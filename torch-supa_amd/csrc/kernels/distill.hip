@@ -8,7 +8,9 @@
 // (w q_R - r) exp(z_j - lse_R) elsewhere (w = sum p + r; without rest: q_j).
 //
 // HBM-bound: the forward reads the logits once, the backward reads them and
-// writes the gradient; the pairs are a few hundred bytes a row.  The forward
+// writes the gradient; the pairs are a few hundred bytes a row.  [3700, 128256] bf16 with 64 pairs: forward 155 us
+// (6.1 TB/s of a read stream's 6.8), backward 304 (6.2 of 6.7).  Rows of a few hundred tokens are bound by the instructions of a
+// row's finish ([65536, 256]: 99 us, 781 a row).  The forward
 // keeps an online (max, sum of exp2) pair a thread, float32; what depends on the
 // pairs alone (K exponentials, their sums, logarithms) is float64: r and small
 // losses are differences of near values.  q_R is summed over its own elements,
@@ -24,11 +26,10 @@
 
 namespace sa {
 
-constexpr int kDisBlock = 256;
+constexpr int kDisBlock = 256;  // threads a row; 512 and 1024 gained 1 to 4 us below 256 rows, and lost 12 to 45 % with the rest or many pairs
 constexpr int kDisMaxEntries = 1024;
 static_assert(kDisMaxEntries == SUPA_AMD_DISTILL_MAX_ENTRIES);
-constexpr int kDisUnroll = 2;             // 16-byte vectors in flight per thread
-constexpr int kDisWaveVecs = 2048;        // most vectors of a row that a wavefront takes alone
+constexpr int kDisUnroll = 2;             // 16-byte vectors in flight per thread; 4 and 8 cost registers, and so rows on a CU
 constexpr int kDisSegment = 1 << 17;      // columns whose bitmap is in LDS at a time: 16 KiB
 constexpr int kDisStats = 8;              // floats a row keeps for the backward
 constexpr double kLn2 = 0.69314718055994530942;
@@ -762,8 +763,11 @@ int dis_forward(const DistillArgs& g, int64_t rows, int dtype, const DistillOut&
     }
     return SUPA_AMD_OK;
   };
-  // a wavefront a row where rows are short and its bitmaps, of which there are four, small
-  if (NE == 4 && g.vocab * dtype_size(dtype) <= 16 * kDisWaveVecs) return go(std::integral_constant<int, 64>{});
+  // A wavefront a row, where there are enough for four a SIMD, up to 16 KiB a row ([65536, 1000] bf16 76 us, 149 with 256
+  // threads; [16384, 8192] 63 and 65; [8192, 12000] 51 and 46), with the rest, whose bitmap then needs no barrier, up to 64 KiB
+  // ([5000, 20000] 46 and 55); of fewer rows, up to 8 KiB ([600, 4000] 8.2 and 8.5, [600, 8000] 9.8 and 8.7).
+  const int64_t wave_bytes = rows >= 4096 ? (REST ? 64 << 10 : 16 << 10) : 8 << 10;
+  if (NE == 4 && g.vocab * dtype_size(dtype) <= wave_bytes) return go(std::integral_constant<int, 64>{});
   return go(std::integral_constant<int, kDisBlock>{});
 }
 
@@ -869,7 +873,8 @@ int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_
       return SUPA_AMD_OK;
     };
     auto size = [&](auto threads) { return edges ? go(threads, std::true_type{}) : go(threads, std::false_type{}); };
-    // every workgroup looks all pairs through: more of them, and more columns a workgroup
+    // Every workgroup looks all pairs through: more of them, and more columns a workgroup ([2000, 50257] bf16 with 1000 pairs
+    // 92 us, 109 with 256 threads).  Short rows: a wavefront each ([65536, 1024] bf16 49 us, 63 with 256 threads).
     if (vecs <= 128) return size(std::integral_constant<int, 64>{});
     if (g.entries <= 256 || vecs <= 256) return size(std::integral_constant<int, 256>{});
     return size(std::integral_constant<int, 1024>{});
