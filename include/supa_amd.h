@@ -931,8 +931,8 @@ int supa_amd_clip_grad_norm(int32_t ntensors, void* const* tensors, const int64_
  * and with teacher_lse (the log-sum-exp of all of the teacher's logits over
  * temperature) the tokens that are not listed as one more class: r = max(0, 1 - sum p)
  * against the student's mass outside the list, + r (log r - log q_R).  A pair whose token is
- * negative, or whose logit is -inf, is not there; a token of vocab and more is
- * left out too and sets *error_flag (when given).  A token listed twice has the sum of both
+ * negative, or whose logit is -inf, is not there; one that is there with a token of vocab
+ * and more is left out too and sets *error_flag (when given).  A token listed twice has the sum of both
  * p.  A row without a pair has loss 0 and gradient 0 and does not count for the mean.  The
  * logits are read in float32 and summed in it, what depends on the pairs is float64.
  * No reference counterpart: a program of the reference writes it as log_softmax, gather and sums. */
@@ -957,10 +957,10 @@ typedef struct supa_amd_distill_desc {
 } supa_amd_distill_desc;
 
 /* loss: [rows] for reduction none, else one float; count (not for none): the rows
- * that count.  For the backward: stats, 8 floats a row; pairs ([rows, entries], 8 bytes each and
- * 8-byte aligned; may be NULL without a backward), a token as int32, or -1, and its p as float32.  The
- * backward takes the same descriptor (indices, teacher and teacher_lse are not read) and writes the contiguous gradient of the logits, in their
- * dtype; it overlaps no input. */
+ * that count.  What the backward takes: stats, 8 floats a row, written in any case; pairs ([rows, entries], 8 bytes
+ * each and 8-byte aligned; may be NULL without a backward), a token as int32, or -1, and its p as float32.  The
+ * backward takes the same descriptor (indices, teacher and teacher_lse are not read) and writes the contiguous
+ * gradient of the logits, in their dtype; it overlaps no input. */
 int64_t supa_amd_distill_workspace_bytes(const supa_amd_distill_desc* d);
 int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, void* pairs,
                              void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream);

@@ -117,6 +117,13 @@ def test_balance_refuses(lib, kw, want):
     assert lib.supa_amd_balance_backward(ctypes.byref(d), vp(FAKE), vp(FAKE), vp(FAKE), vp(FAKE), None) == want
 
 
+def test_balance_takes_any_product_below_the_limit(lib):
+    for sequences, tokens in ((3, (2 ** 31 - 1) // 3), (1, 2 ** 31 - 1), (2 ** 31 - 1, 1)):
+        d = balance_desc(sequences=sequences, tokens=tokens)
+        assert lib.supa_amd_balance_workspace_bytes(ctypes.byref(d)) > 0
+        assert lib.supa_amd_balance_workspace_bytes(ctypes.byref(balance_desc(sequences=sequences, tokens=tokens + 1))) == ELAYOUT
+
+
 def test_balance_other_refusals(lib):
     fwd, bwd = lib.supa_amd_balance_forward, lib.supa_amd_balance_backward
     d = balance_desc()
@@ -246,3 +253,14 @@ def test_operators_are_registered():
     for op in ("distillation_loss", "router_balance_loss", "adjust_logits", "adjust_logits_"):
         for key in ("PrivateUse1", "AutogradPrivateUse1", "Meta"):
             assert torch._C._dispatch_has_kernel_for_dispatch_key("supa::" + op, key), (op, key)
+
+
+def test_a_learned_temperature_is_refused():
+    """It would get no gradient."""
+    x, i, t = meta(4, 50), meta(4, 3, dtype=LONG), meta(4, 3)
+    learned = torch.tensor(2.0, requires_grad=True)
+    with pytest.raises(TypeError, match="temperature is a number"):
+        torch.supa.distillation_loss(x, i, t, temperature=learned)
+    with torch.no_grad():
+        torch.supa.distillation_loss(x, i, t, temperature=learned)
+    torch.supa.distillation_loss(x, i, t, temperature=torch.tensor(2.0))

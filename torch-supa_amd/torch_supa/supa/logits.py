@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import torch
 
+from .transformer import _number
+
 _distillation_loss = torch.ops.supa.distillation_loss.default
 _router_balance_loss = torch.ops.supa.router_balance_loss.default
 _adjust_logits = torch.ops.supa.adjust_logits.default
@@ -34,7 +36,7 @@ def distillation_loss(logits, indices, teacher_logits, *, teacher_lse=None, temp
         p = exp(teacher_logits / temperature - lse)
         loss = sum(p * (log(p) - log(q[indices])))
 
-    logits are ``[..., vocab]`` of float32, bfloat16 or float16, indices (int64 or
+    temperature is a number.  logits are ``[..., vocab]`` of float32, bfloat16 or float16, indices (int64 or
     int32) and teacher_logits (any of the three types) ``[..., k]`` with k up to 1024;
     their order does not matter.  A pair with a negative index, or a teacher's
     logit of -inf, is not there: rows may store fewer than k.  A row without any has
@@ -52,8 +54,10 @@ def distillation_loss(logits, indices, teacher_logits, *, teacher_lse=None, temp
     ``"sum"``, ``[...]`` for ``"none"``.  It is not multiplied by temperature ** 2.
     Exponentials of the logits are summed in float32, what depends on the listed pairs is
     float64.  Differentiable (once) in logits; the teacher is a constant.  An index of vocab
-    and more raises an IndexError when the stream is next waited for, as cross_entropy's targets do."""
-    return _distillation_loss(logits, indices, teacher_logits, teacher_lse, temperature,
+    and more, in a pair that is there, raises an IndexError when the stream is next waited for, as cross_entropy's
+    targets do."""
+    return _distillation_loss(logits, indices, teacher_logits, teacher_lse,
+                              _number("distillation_loss: temperature", temperature),
                               _choice("distillation_loss: reduction", reduction, _REDUCTIONS))
 
 
