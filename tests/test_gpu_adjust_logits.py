@@ -159,6 +159,30 @@ def test_a_bias_of_every_token(rows, vocab, length, no_fallback):
     check(d | {"bias_tokens": d["bias_tokens"].int()})
 
 
+@pytest.mark.parametrize("index", [torch.int64, torch.int32])
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+def test_histories_end_anywhere(index, shift, no_fallback):
+    """Every length about whole loads and whole rounds of them, rows at any alignment, tokens behind a row's length
+    that would count."""
+    near = [0, 1, 2, 3, 4, 5, 7, 8, 9, 255, 256, 257, 259, 511, 513, 1023, 1025, 2047, 2049, 4095, 4097, 4103]
+    rows, vocab = len(near), 777
+    d = make(rows, vocab, 4103 + shift, 0, False, seed=shift)
+    d["lengths"] = torch.tensor(near)
+    d["tokens"] = d["tokens"].to(index)
+    if index == torch.int64:  # their lower halves are tokens
+        d["tokens"][:, ::5] += 2 ** 32
+        d["tokens"][:, 1::7] -= 2 ** 32
+    check(d)
+    d["prompt_lengths"] = (torch.tensor(near) - 2).clamp(min=0)
+    d["tokens"] = torch.full_like(d["tokens"], 776)
+    check(d)
+    s = to_supa(d)
+    x, history = s.pop("logits"), s.pop("tokens")
+    wide = torch.full((rows, history.shape[1] + 3), 5, dtype=index, device="supa")
+    wide[:, shift : shift + history.shape[1]] = history
+    assert torch.equal(torch.supa.adjust_logits(x, tokens=wide[:, shift : shift + history.shape[1]], **s).cpu(), check(d))
+
+
 def test_tokens_outside_are_passed_over(no_fallback):
     d = make(5, 200, 50, 20, False)
     d["tokens"][:, ::3] = -1

@@ -9,7 +9,7 @@
 //
 // HBM-bound for batches (a row is read and written once: [512, 65536] bf16 under a grammar 26 us, 5.1 TB/s), latency for single
 // rows ([1, 32000], a history of 700: 4.7 us), and with long histories bound by reading them ([512, 128256] float32,
-// histories of 32768: 153 us, of which 85 are instructions).  A workgroup takes a range of a row's columns.  It counts the range's tokens in LDS: it
+// histories of 32768: 135 us).  A workgroup takes a range of a row's columns.  It counts the range's tokens in LDS: it
 // reads the row's whole history (from the L2, which the row's other workgroups
 // share) and keeps what falls into its range, so no counts go through memory and there is
 // one launch; integer counts do not depend on the order of the additions.  Counts
@@ -25,8 +25,8 @@ namespace sa {
 
 constexpr int kAdjApart = 8;                 // XCDs
 constexpr int kAdjVecs = 4;                  // vectors of logits that a thread has in flight
-constexpr int kAdjUnroll = 2;                // tokens of the history in flight a thread: with 4 and 8 the long histories took 162 and 233 us, with 2 152
-constexpr int kAdjMaxRange = 32768;          // with 65536 the history is read half as often, but one workgroup fills a CU: 170 us for 153
+constexpr int kAdjUnroll = 2;                // 16-byte loads of the history in flight a thread: with 1 the long histories took 149 us, with 2 135
+constexpr int kAdjMaxRange = 32768;          // with 65536 the history is read half as often, but one workgroup fills a CU (170 us for 153, when the scan was slower)
 constexpr int kAdjHash = 1024;               // most biases that go into a hash table
 constexpr int kAdjDense = 8192;              // columns of a range where there are more: 64 KiB of sums and turns
 constexpr int64_t kAdjNarrow = 65535;        // the longest history that 16 bits count
@@ -129,23 +129,41 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int
     __syncthreads();
   }
   if constexpr (PEN) {
-    const int64_t at = row * g.tokens_stride;
-    for (int64_t t0 = threadIdx.x; t0 < n; t0 += (int64_t)nt * kAdjUnroll) {
-      int64_t tok[kAdjUnroll];
-#pragma unroll
-      for (int u = 0; u < kAdjUnroll; ++u) {
-        const int64_t t = t0 + u * nt;
-        tok[u] = t < n ? adj_column(g.tokens, g.tok64, at + t, c0) : -1;
-      }
-#pragma unroll
-      for (int u = 0; u < kAdjUnroll; ++u) {
-        if ((uint64_t)tok[u] >= (uint64_t)width) continue;
-        const int c = (int)tok[u];
-        if (t0 + u * nt < prompt) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
+    // n is below 2^31, and so are tokens that count: those with a higher half are in no range.  Whole loads need no check
+    // of each token's place: one token a load, each checked, took 152 us for 135.
+    auto scan = [&](auto* history) {
+      using Token = std::remove_cv_t<std::remove_pointer_t<decltype(history)>>;
+      const Token* at = history + row * g.tokens_stride;
+      const uint32_t end = (uint32_t)n, start = prompt < 0 ? 0u : (uint32_t)(prompt < n ? prompt : n), base = (uint32_t)c0;
+      auto take = [&](Token token, uint32_t t) {
+        const uint32_t c = (uint32_t)token - base;
+        if (c >= (uint32_t)width || (sizeof(Token) == 8 && (uint64_t)token >> 32 != 0)) return;
+        if (t < start) atomicOr(&prompt_bits[c / 32], 1u << (c % 32));
         else if (WIDE) atomicAdd(&count[c], 1u);
         else atomicAdd(&count[c / 2], c & 1 ? 0x10000u : 1u);
-      }
-    }
+      };
+      constexpr int N = 16 / (int)sizeof(Token);  // tokens of a load; it needs their alignment alone
+      struct alignas(sizeof(Token)) Tokens { Token v[N]; };
+      const uint32_t step = (uint32_t)nt * N;
+      uint32_t t = threadIdx.x * N;
+      auto batch = [&](auto size) {
+        constexpr int U = decltype(size)::value;
+        Tokens tokens[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) __builtin_memcpy(&tokens[u], at + t + u * step, sizeof(Tokens));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) take(tokens[u].v[k], t + u * step + k);
+        }
+        t += step * U;
+      };
+      while (t + step * (kAdjUnroll - 1) + N <= end) batch(std::integral_constant<int, kAdjUnroll>{});
+      while (t + N <= end) batch(std::integral_constant<int, 1>{});
+      for (; t < end; ++t) take(at[t], t);  // fewer than N, of one thread
+    };
+    if (g.tok64) scan(static_cast<const int64_t*>(g.tokens));
+    else scan(static_cast<const int32_t*>(g.tokens));
   }
   // the slot that holds a column, or the free one that it would get: at most half of them are taken, so one is met
   auto slot_of = [&](int col, auto&& step) {
