@@ -26,7 +26,7 @@ namespace sa {
 constexpr int kAdjApart = 8;                 // XCDs
 constexpr int kAdjVecs = 4;                  // vectors of logits that a thread has in flight
 constexpr int kAdjUnroll = 2;                // 16-byte loads of the history in flight a thread: with 1 the long histories took 149 us, with 2 135
-constexpr int kAdjMaxRange = 32768;          // with 65536 the history is read half as often, but one workgroup fills a CU (170 us for 153, when the scan was slower)
+constexpr int kAdjMaxRange = 32768;          // histories of 32768 tokens: 137 us, with 16384 168, with 65536, one workgroup a CU, 153
 constexpr int kAdjHash = 1024;               // most biases that go into a hash table
 constexpr int kAdjDense = 8192;              // columns of a range where there are more: 64 KiB of sums and turns
 constexpr int64_t kAdjNarrow = 65535;        // the longest history that 16 bits count
@@ -323,7 +323,7 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
     const size_t lds = adj_lds_bytes(a.range, pen, wide, biased, a.hash);
     // Workgroups go to the eight XCDs in turn.  Where the histories pass what the eight L2s hold, those of a row are
     // eight apart and next to each other in time, so that its history comes from memory once and from one XCD's L2 for
-    // the others ([512, 128256] float32, histories of 32768: 153 us with all rows' first ranges first, 142 so, inputs partly in the caches); else
+    // the others ([512, 128256] float32, histories of 32768: 148 us with all rows' first ranges first, 137 so); else
     // rows come first, which spreads a number of rows that is no multiple of eight evenly ([37, 50257]: 6.7 and 9.2).
     a.ranges = FastDiv(ranges);
     a.apart = (pen && d->rows >= 64 && d->rows * d->history * 8 > (int64_t(32) << 20)) || ranges > 65535;
