@@ -418,6 +418,34 @@ def test_many_rows(no_fallback):
     check(x, i, torch.randn(rows, 2, generator=g), reduction="mean")
 
 
+@pytest.mark.parametrize("x, vocab", [("bf16", 5003), ("f16", 20001), ("f32", 15999), ("bf16", 33001)])
+@pytest.mark.parametrize("rest", [False, True], ids=["listed", "rest"])
+def test_many_long_rows(x, vocab, rest, no_fallback):
+    """Enough rows for a wavefront each: copies of a few, which are checked, have their losses and gradients
+    but for the order of the sums."""
+    few, k = 41, 30
+    logits, i, t, lse = make(few, vocab, k, x, "f32", rest, 5, 0.8)
+    i[3] = -1
+    i[4, 20:] = i[4, 0]
+    loss, g = check(logits, i, t, lse, 0.8, "none", torch.full((few,), 64.0))
+    copies = lambda v: v.repeat((101,) + (1,) * (v.dim() - 1)).to("supa")  # noqa: E731
+    dx = copies(logits).requires_grad_()
+    many = torch.supa.distillation_loss(dx, copies(i), copies(t), temperature=0.8, reduction="none",
+                                        teacher_lse=None if lse is None else copies(lse))
+    (gm,) = torch.autograd.grad(many, dx, torch.full((101 * few,), 64.0, device="supa"))
+    many, gm = many.detach().cpu().view(101, few), gm.cpu().view(101, few, vocab)
+    # Copies are not the same bits: vectors lie at multiples of 16 bytes, so a row's address decides which element falls to
+    # which thread, and a float32 sum depends on that order.  Each order's sum is within S of the exact one, relative, so two
+    # are within 2 S, and the losses, logarithms of them, absolutely; a gradient off by at most `off` each way and rounded once
+    # (half an eps of a value that is |g| + off at most) is within 2 off + eps (|g| + off) of the other.
+    assert ((many - loss.detach().cpu()).abs() <= 2 * S(vocab) + 4 * U * many.abs()).all()
+    off = (3 * S(vocab) + 300 * U) * magnitude(logits, i, t, lse, 0.8) * 64 / 0.8
+    fi, g = torch.finfo(T[x]), g.double().cpu()
+    far = 2 * off + fi.eps * (g.abs() + off) + fi.tiny * fi.eps
+    for each in gm:
+        assert ((each.double() - g).abs() <= far).all()
+
+
 def test_saved_tensors(no_fallback):
     """Twice through the graph; a write to the logits in between is noticed; a hook's copies do."""
     x, i, t, _ = make(5, 600, 4)

@@ -52,8 +52,8 @@ def distillation_loss(logits, indices, teacher_logits, *, teacher_lse=None, temp
 
     The loss is float32: a scalar for reduction ``"mean"`` (over the rows that count) or
     ``"sum"``, ``[...]`` for ``"none"``.  It is not multiplied by temperature ** 2.
-    Exponentials of the logits are summed in float32, what depends on the listed pairs is
-    float64.  Differentiable (once) in logits; the teacher is a constant.  An index of vocab
+    Exponentials of the logits are summed in float32, in an order that the sizes and the alignment of a row fix, what depends on
+    the listed pairs is float64.  Differentiable (once) in logits; the teacher is a constant.  An index of vocab
     and more, in a pair that is there, raises an IndexError when the stream is next waited for, as cross_entropy's
     targets do."""
     return _distillation_loss(logits, indices, teacher_logits, teacher_lse,
