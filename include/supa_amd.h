@@ -964,6 +964,11 @@ typedef struct supa_amd_distill_desc {
 int64_t supa_amd_distill_workspace_bytes(const supa_amd_distill_desc* d);
 int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, void* pairs,
                              void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream);
+/* The same with teacher_lse ([rows]; lse_strides) in float64, in place of the descriptor's, which is not read: what the teacher
+ * leaves to the rest, 1 - sum p, is a difference of near values. */
+int supa_amd_distill_forward_lse64(const supa_amd_distill_desc* d, const double* teacher_lse, float* loss, float* count,
+                                   float* stats, void* pairs, void* workspace, int64_t ws_bytes, int32_t* error_flag,
+                                   void* stream);
 int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_loss, const float* count,
                               const float* stats, const void* pairs, void* grad_logits, void* stream);
 

@@ -162,21 +162,26 @@ DistillResult distill_run(SUPA_DISTILL_PARAMS, bool want_pairs) {
   d.teacher_dtype = dtype_code(teacher.scalar_type());
   d.teacher = t.t.data_ptr();
   LogitRows lse{};
-  if (given(teacher_lse)) lse = rows_beside(teacher_lse->to(at::kFloat), x.inner, false);
+  const bool lse64 = given(teacher_lse) && teacher_lse->scalar_type() == at::kDouble;
+  if (given(teacher_lse)) lse = rows_beside(lse64 ? *teacher_lse : teacher_lse->to(at::kFloat), x.inner, false);
   for (int i = 0; i < 2; ++i) {
     d.indices_strides[i] = ids.stride[i];
     d.teacher_strides[i] = t.stride[i];
     d.lse_strides[i] = lse.stride[i];
   }
   // an empty tensor has no address, and says "given" all the same: there are no rows then
-  d.teacher_lse = lse.t.defined() ? lse.t.data_ptr<float>() : nullptr;
+  if (lse.t.defined() && !lse64) d.teacher_lse = lse.t.data_ptr<float>();
   const auto dev = logits.device().index();
   const int64_t ws_bytes = supa_amd_distill_workspace_bytes(&d);
   TORCH_CHECK(ws_bytes >= 0, "distillation_loss: ", supa_amd_status_string((int)ws_bytes));
   const at::Tensor ws = empty_supa({ws_bytes}, at::kByte, dev);
-  check_status(supa_amd_distill_forward(&d, loss.data_ptr<float>(), count.defined() ? count.data_ptr<float>() : nullptr,
-                                        stats.data_ptr<float>(), pairs.defined() ? pairs.data_ptr() : nullptr,
-                                        ws.data_ptr(), ws_bytes, stream_error_flag(dev), current_stream(dev)),
+  float* const counts = count.defined() ? count.data_ptr<float>() : nullptr;
+  void* const kept = pairs.defined() ? pairs.data_ptr() : nullptr;
+  check_status(lse64 ? supa_amd_distill_forward_lse64(&d, lse.t.data_ptr<double>(), loss.data_ptr<float>(), counts,
+                                                      stats.data_ptr<float>(), kept, ws.data_ptr(), ws_bytes,
+                                                      stream_error_flag(dev), current_stream(dev))
+                     : supa_amd_distill_forward(&d, loss.data_ptr<float>(), counts, stats.data_ptr<float>(), kept,
+                                                ws.data_ptr(), ws_bytes, stream_error_flag(dev), current_stream(dev)),
                "distillation_loss");
   return r;
 }

@@ -39,12 +39,12 @@ struct DistillArgs {
   const void* x;
   const void* idx;
   const void* teacher;
-  const float* teacher_lse;
+  const void* teacher_lse;  // float32, or float64 (lse64)
   int64_t xs[2], is[2], ts[2], ls[2];  // distances of rows, outer and inner: of logits, indices, teacher, teacher_lse
   FastDiv inner;     // row -> (outer, inner)
   int64_t vocab;
   int32_t entries, hash;  // pairs a row; slots of its hash table, a power of two >= 2 entries
-  int32_t idx64, teacher_dtype;
+  int32_t idx64, lse64, teacher_dtype;
   int32_t segment;   // columns of a bitmap
   double teacher_c;  // log2(e) / temperature
   float c;           // that rounded, for all that is the student's: a temperature off by 2^-25 of itself
@@ -64,6 +64,13 @@ __device__ __forceinline__ int64_t dis_at(const DistillArgs& g, int64_t row, con
 }
 __device__ __forceinline__ int64_t dis_index(const DistillArgs& g, int64_t at) {
   return g.idx64 ? static_cast<const int64_t*>(g.idx)[at] : (int64_t)static_cast<const int32_t*>(g.idx)[at];
+}
+
+// A row's teacher_lse.  A float64 one stays so: r = 1 - sum p is a difference of near values, and of a log-sum-exp of 20 float32
+// leaves out up to 1e-6.
+__device__ __forceinline__ double dis_lse(const DistillArgs& g, int64_t row) {
+  const int64_t at = dis_at(g, row, g.ls);
+  return g.lse64 ? static_cast<const double*>(g.teacher_lse)[at] : (double)static_cast<const float*>(g.teacher_lse)[at];
 }
 
 // Exchange among the threads of a wavefront through LDS.
@@ -257,7 +264,7 @@ enum { kStatRestMax, kStatRest, kStatMax, kStatListed, kStatCounts };
 // the row's pairs to the row's loss, its statistics and the pairs' weights.  One wavefront.
 template <int NE, bool REST>
 __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, int lane, float m, float s,
-                                           const DistillEntries<NE>& e, float teacher_lse, bool twice,
+                                           const DistillEntries<NE>& e, double teacher_lse, bool twice,
                                            const DistillLds& lds, const DistillOut& out) {
   float top_t = -__builtin_inff(), top = m;
 #pragma unroll
@@ -269,7 +276,7 @@ __device__ __forceinline__ void dis_finish(const DistillArgs& g, int64_t row, in
   if (REST) top = wave_max(top);
   else top_t = wave_max(top_t);
   const float M = top == -__builtin_inff() ? 0.0f : top;
-  const double lt = REST ? (double)teacher_lse * kLog2eD : (double)top_t * g.teacher_c;
+  const double lt = REST ? teacher_lse * kLog2eD : (double)top_t * g.teacher_c;
   double p[NE];
   bool first[NE];  // no pair before lists the token
   double sum[3] = {0.0, 0.0, 0.0};  // p, p log2 p, p z with z = (x - M) c
@@ -477,7 +484,7 @@ k_distill_fwd(DistillArgs g, int64_t row0, int64_t rows, DistillOut out, int32_t
   auto end = [&](int64_t c0) { return c0 + g.segment < g.vocab ? c0 + g.segment : g.vocab; };
   DistillStream<T, G, REST> first(xr, 0, end(0), l);
   DistillEntries<NE> e;
-  const float teacher_lse = REST ? g.teacher_lse[dis_at(g, row, g.ls)] : 0.0f;
+  const double teacher_lse = REST ? dis_lse(g, row) : 0.0;
   const bool any = dis_entries(g, row, lane, e, wave == 0 ? error_flag : nullptr);  // in every wavefront: all know without a barrier
   if (!any) {
     if (wave == 0) dis_nothing(g, row, lane, out);
@@ -542,7 +549,7 @@ k_distill_rows(DistillArgs g, int nparts, const float2* __restrict__ parts, Dist
   const float2 part = lane < nparts ? parts[row * nparts + lane] : make_float2(-__builtin_inff(), 0.0f);
   const DistillLds s = dis_lds(reinterpret_cast<char*>(lds_dyn), g.entries, g.hash);
   DistillEntries<NE> e;
-  const float teacher_lse = REST ? g.teacher_lse[dis_at(g, row, g.ls)] : 0.0f;
+  const double teacher_lse = REST ? dis_lse(g, row) : 0.0;
   if (!dis_entries(g, row, lane, e, error_flag)) return dis_nothing(g, row, lane, out);
   const bool twice = dis_listed(g, dis_row<T>(g, row), lane, e, s);
   float m = part.x, sum = part.y;
@@ -784,24 +791,10 @@ DistillSpace distill_space(const supa_amd_distill_desc* d) {
   return s;
 }
 
-}  // namespace sa
-
-using namespace sa;
-
-extern "C" {
-
-int64_t supa_amd_distill_workspace_bytes(const supa_amd_distill_desc* d) {
-  DistillArgs g;
-  const int rc = dis_args(d, g);
-  if (rc) return rc;
-  return distill_space(d).bytes;
-}
-
-int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, void* pairs,
-                             void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream) {
-  DistillArgs g;
-  int rc = dis_args(d, g);
-  if (rc) return rc;
+// g: what dis_args made of d, with the teacher_lse that counts.
+int distill_forward(const supa_amd_distill_desc* d, const DistillArgs& g, float* loss, float* count, float* stats, void* pairs,
+                    void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream) {
+  int rc = SUPA_AMD_OK;
   const bool total = d->reduction != SUPA_AMD_REDUCTION_NONE;
   if (d->rows == 0 && !total) return SUPA_AMD_OK;
   if (!loss || (total && !count)) return SUPA_AMD_EINVAL;
@@ -825,7 +818,7 @@ int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float*
         return g.entries <= 256 ? forward(std::integral_constant<int, 4>{}, rest)
                                 : forward(std::integral_constant<int, kDisMaxEntries / 64>{}, rest);
       };
-      return d->teacher_lse ? lists(std::true_type{}) : lists(std::false_type{});
+      return g.teacher_lse ? lists(std::true_type{}) : lists(std::false_type{});
     });
   }
   if (rc || !total) return rc;
@@ -837,6 +830,38 @@ int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float*
   k_distill_total<false><<<1, kDisSumBlock, 0, st>>>(rows, nparts > 0 ? sums : nullptr, nparts > 0 ? nparts : d->rows,
                                                     d->reduction == SUPA_AMD_REDUCTION_MEAN, nullptr, loss, count);
   return launch_status();
+}
+
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" {
+
+int64_t supa_amd_distill_workspace_bytes(const supa_amd_distill_desc* d) {
+  DistillArgs g;
+  const int rc = dis_args(d, g);
+  if (rc) return rc;
+  return distill_space(d).bytes;
+}
+
+int supa_amd_distill_forward(const supa_amd_distill_desc* d, float* loss, float* count, float* stats, void* pairs,
+                             void* workspace, int64_t ws_bytes, int32_t* error_flag, void* stream) {
+  DistillArgs g;
+  const int rc = dis_args(d, g);
+  return rc ? rc : distill_forward(d, g, loss, count, stats, pairs, workspace, ws_bytes, error_flag, stream);
+}
+
+int supa_amd_distill_forward_lse64(const supa_amd_distill_desc* d, const double* teacher_lse, float* loss, float* count,
+                                   float* stats, void* pairs, void* workspace, int64_t ws_bytes, int32_t* error_flag,
+                                   void* stream) {
+  DistillArgs g;
+  const int rc = dis_args(d, g);
+  if (rc) return rc;
+  if (d->rows > 0 && !teacher_lse) return SUPA_AMD_EINVAL;
+  g.teacher_lse = teacher_lse;
+  g.lse64 = 1;
+  return distill_forward(d, g, loss, count, stats, pairs, workspace, ws_bytes, error_flag, stream);
 }
 
 int supa_amd_distill_backward(const supa_amd_distill_desc* d, const float* grad_loss, const float* count,

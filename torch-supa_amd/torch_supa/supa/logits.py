@@ -44,8 +44,8 @@ def distillation_loss(logits, indices, teacher_logits, *, teacher_lse=None, temp
     counts.  A token that is listed twice has the sum of its p.
 
     Without teacher_lse, lse is that of the row's own teacher_logits: p sums to 1 over
-    the listed tokens.  teacher_lse (floats ``[...]``) is the log-sum-exp of all of the
-    teacher's logits over temperature; the tokens that are not listed then are one more
+    the listed tokens.  teacher_lse (floats ``[...]``; float64 is taken as it is) is the
+    log-sum-exp of all of the teacher's logits over temperature; the tokens that are not listed then are one more
     class, with r = 1 - sum(p) of the teacher's mass (at least 0)::
 
         loss += r * (log(r) - log(sum of q over the tokens that are not listed))
