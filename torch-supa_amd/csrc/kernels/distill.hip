@@ -19,9 +19,10 @@
 // (a bit, and the pair's number in a table by column) while its logits are on their way; an
 // element whose bit is set takes its p from there.
 //
-// A token listed twice has the sum of its p: the row's first such pair carries it.
-// Such tokens, and their first pairs, are found by a hash table in LDS; the others add their p to the
-// first's in turn, in the order of the pairs.
+// A token listed twice has the sum of its p in the gradient, and counts once for the listed tokens' mass: the row's first
+// such pair carries it.  The loss is the sum over the pairs as they are, each with its own log p; merged they would have
+// p1 log(P / p1) + p2 log(P / p2) more, P = p1 + p2, which does not depend on the student.  Such tokens,
+// and their first pairs, are found by a hash table in LDS; the others add their p to the first's in turn, in the order of the pairs.
 #include "row_group.h"
 
 namespace sa {

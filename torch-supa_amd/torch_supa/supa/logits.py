@@ -41,7 +41,9 @@ def distillation_loss(logits, indices, teacher_logits, *, teacher_lse=None, temp
     their order does not matter.  A pair with a negative index, or a teacher's
     logit of -inf, is not there: rows may store fewer than k.  A row without any has
     loss 0 and gradient 0, and does not count for the mean, which is NaN where no row
-    counts.  A token that is listed twice has the sum of its p.
+    counts.  A token that is listed twice is listed once for the student, and its gradient has the
+    sum of its p; the loss adds up the pairs, each with its own log(p): it is less by p1 log(P / p1) + p2 log(P / p2)
+    than that of one pair with P = p1 + p2.
 
     Without teacher_lse, lse is that of the row's own teacher_logits: p sums to 1 over
     the listed tokens.  teacher_lse (floats ``[...]``; float64 is taken as it is) is the
