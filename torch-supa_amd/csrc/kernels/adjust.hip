@@ -7,9 +7,10 @@
 //   -inf                                      where the token is not allowed
 // in float32, rounded once.
 //
-// HBM-bound for batches (a row is read and written once: [512, 65536] bf16 under a grammar 26 us, 5.1 TB/s), latency for single
-// rows ([1, 32000], a history of 700: 4.7 us), and with long histories bound by reading them ([512, 128256] float32,
-// histories of 32768: 135 us).  A workgroup takes a range of a row's columns.  It counts the range's tokens in LDS: it
+// HBM-bound for batches (a row is read and written once: [512, 65536] bf16 under a grammar 27 us, 5.0 TB/s), latency for single
+// rows ([1, 32000], a history of 700: 4.3 us), and with long histories bound by reading them ([512, 128256] float32,
+// histories of 32768: 136 us).  All figures here are of launches in a row, three sets of
+// inputs in turn.  A workgroup takes a range of a row's columns.  It counts the range's tokens in LDS: it
 // reads the row's whole history (from the L2, which the row's other workgroups
 // share) and keeps what falls into its range, so no counts go through memory and there is
 // one launch; integer counts do not depend on the order of the additions.  Counts
@@ -25,8 +26,8 @@ namespace sa {
 
 constexpr int kAdjApart = 8;                 // XCDs
 constexpr int kAdjVecs = 4;                  // vectors of logits that a thread has in flight
-constexpr int kAdjUnroll = 2;                // 16-byte loads of the history in flight a thread: with 1 the long histories took 149 us, with 2 135
-constexpr int kAdjMaxRange = 32768;          // histories of 32768 tokens: 137 us, with 16384 168, with 65536, one workgroup a CU, 153
+constexpr int kAdjUnroll = 2;                // 16-byte loads of the history in flight a thread: with 1 the long histories took 146 us, with 2 136
+constexpr int kAdjMaxRange = 32768;          // histories of 32768 tokens: 136 us, with 16384 166, with 65536, one workgroup a CU, 150
 constexpr int kAdjHash = 1024;               // most biases that go into a hash table
 constexpr int kAdjDense = 8192;              // columns of a range where there are more: 64 KiB of sums and turns
 constexpr int64_t kAdjNarrow = 65535;        // the longest history that 16 bits count
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(1024) k_adjust(AdjustArgs g, int64_t row0, int
   }
   if constexpr (PEN) {
     // n is below 2^31, and so are tokens that count: those with a higher half are in no range.  Whole loads need no check
-    // of each token's place: one token a load, each checked, took 152 us for 135.
+    // of each token's place: one token a load, each checked, took 152 us for 136.
     auto scan = [&](auto* history) {
       using Token = std::remove_cv_t<std::remove_pointer_t<decltype(history)>>;
       const Token* at = history + row * g.tokens_stride;
@@ -323,8 +324,8 @@ extern "C" int supa_amd_adjust_logits(const supa_amd_adjust_desc* d, void* strea
     const size_t lds = adj_lds_bytes(a.range, pen, wide, biased, a.hash);
     // Workgroups go to the eight XCDs in turn.  Where the histories pass what the eight L2s hold, those of a row are
     // eight apart and next to each other in time, so that its history comes from memory once and from one XCD's L2 for
-    // the others ([512, 128256] float32, histories of 32768: 148 us with all rows' first ranges first, 137 so); else
-    // rows come first, which spreads a number of rows that is no multiple of eight evenly ([37, 50257]: 6.7 and 9.2).
+    // the others ([512, 128256] float32, histories of 32768: 147 us with all rows' first ranges first, 136 so); else
+    // rows come first, which spreads a number of rows that is no multiple of eight evenly ([37, 50257]: 6.8 and 9.1).
     a.ranges = FastDiv(ranges);
     a.apart = (pen && d->rows >= 64 && d->rows * d->history * 8 > (int64_t(32) << 20)) || ranges > 65535;
     const int64_t most = ((int64_t(1) << 32) - 1) / block / ranges;  // HIP: fewer than 2^32 threads a launch

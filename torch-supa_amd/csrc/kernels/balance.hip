@@ -5,6 +5,8 @@
 //   c_e  = counted tokens' choices of expert e,  a_e = E c_e / (k n) - 1
 //   loss = sum_e (a_e + 1) sum_t p_te / n,  the mean of it over sequences with n > 0
 //   dloss/dx_te = p_te (a_e - sum_e p_te a_e) / n    (sigmoid: times 1 - sigmoid(x_te))
+// Exponents are (x - max) log2(e) in float32, as in this library's softmax: the product's rounding adds |x - max| 2^-24 of
+// itself to a share's error, as much as the difference's own.
 // The - 1 changes nothing, as the shares of a token sum to 1; near balance it keeps
 // the difference in the last line from cancelling.
 //

@@ -11,7 +11,8 @@
 // writes the gradient; the pairs are a few hundred bytes a row.  [3700, 128256] bf16 with 64 pairs: forward 155 us
 // (6.1 TB/s of a read stream's 6.8), backward 304 (6.2 of 6.7).  Rows of a few hundred tokens are bound by the instructions of a
 // row's finish ([65536, 256]: 99 us, 781 a row).  The forward
-// keeps an online (max, sum of exp2) pair a thread, float32; what depends on the
+// keeps an online (max, sum of exp2) pair a thread, float32 (the exponent (x - max) c too, whose product is off by 2^-24 of
+// itself, as in this library's softmax); what depends on the
 // pairs alone (K exponentials, their sums, logarithms) is float64: r and small
 // losses are differences of near values.  q_R is summed over its own elements,
 // not as 1 minus the listed ones: a bitmap of the listed tokens, in LDS, tells
