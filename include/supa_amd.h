@@ -934,7 +934,8 @@ int supa_amd_clip_grad_norm(int32_t ntensors, void* const* tensors, const int64_
  * negative, or whose logit is -inf, is not there; one that is there with a token of vocab
  * and more is left out too and sets *error_flag (when given).  A token listed twice is listed once for
  * q_R, and has the sum of both p in the gradient; the loss is the sum over the pairs, each with its own log p.  A row
- * without a pair has loss 0 and gradient 0 and does not count for the mean.  The logits are read in float32 and summed in it, what depends on the pairs is float64.
+ * without a pair has loss 0 and gradient 0 and does not count for the mean.  The logits are read in
+ * float32 and summed in it, what depends on the pairs is float64.
  * No reference counterpart: a program of the reference writes it as log_softmax, gather and sums. */
 #define SUPA_AMD_DISTILL_MAX_ENTRIES 1024
 
